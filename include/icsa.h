@@ -59,6 +59,7 @@ extern "C" {
 
 #define ICSA_BF16 0
 #define ICSA_F32 1
+#define ICSA_MXFP4 2 /* icsa_mx_linear alone: e2m1 codes and block scales (see icsa_mx_quantize) */
 
 #define ICSA_OK 0
 #define ICSA_EINVAL (-1)       /* invalid argument (null pointer, bad shape/stride/dtype) */
@@ -361,6 +362,68 @@ int icsa_wan_ln_modulate(const void* x, int x_dtype, int64_t x_sb, int64_t x_ss,
                          const float* lw, const float* lb,
                          const float* shift, const float* scale, int64_t mod_sb, float eps,
                          int B, int S, int dim, void* out, int64_t o_sb, int64_t o_ss, void* stream);
+
+/* Workspace bytes of icsa_masked_attn (partials of keys split over workgroups; 0 for most sizes). */
+int64_t icsa_masked_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D);
+
+/* Attention under masks: out_i = sum_j softmax_j(s_ij) v_j over the keys that query i sees,
+ *   s_ij = cap tanh(scale q_i.k_j / cap) + bias[h][clamp(j - p_i, -radius, radius) + radius]
+ * (softcap 0: no cap; bias NULL: none).  q, out [B, Sq, H, D], k, v [B, Sk, Hk, D] bf16 (out bf16 or
+ * f32), D 64 or 128, H a multiple of Hk: heads h H / Hk .. share key head h.
+ * q_starts, k_starts: device int32 [B, docs + 1], not decreasing: document n of batch row b has queries
+ * q_starts[b][n] .. q_starts[b][n + 1] - 1 and keys likewise, and sees its own keys alone; queries
+ * outside every document see nothing.  NULL: one document of everything.  Values past the lengths
+ * are clamped.  causal: query i of a document of Lq queries and Lk keys stands at its key
+ * p_i = i + Lk - Lq and sees keys up to it; prefix (device int32 [B, docs], with causal): the document's
+ * first keys that all of its queries see.  A query that sees nothing gets zeros.  NaN and infinities in
+ * keys and values reach only the queries that see them.
+ * (The reference's own attention wrapper for ragged lengths: wanx/attention.py:18-85.) */
+int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                     const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                     const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                     int B, int Sq, int Sk, int H, int Hk, int D,
+                     const int32_t* q_starts, const int32_t* k_starts, int docs, int causal, const int32_t* prefix,
+                     float scale, float softcap, const float* bias, int radius,
+                     void* out, int out_dtype, int64_t o_sb, int64_t o_ss, int64_t o_sh,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- Microscaled 4-bit floating point (OCP MXFP4) ----
+ * A row of K values is padded with zeros to Kp = K rounded up to 256 and cut into blocks of 32.
+ * A block has a scale byte s, 2^(s - 127), and 32 e2m1 codes (0, .5, 1, 1.5, 2, 3, 4, 6 and
+ * their negatives; bit 3 is the sign):
+ *   codes   u8 [rows, Kp / 2]        the even k in a byte's low nibble
+ *   scales  u8 [Kp / 256, rows, 8]   the 8 blocks of a row's group of 256 side by side
+ * s = 127 + floor(log2 max|x|) - 2, at least 0; codes are round to nearest (ties to the even
+ * code) of x 2^(127 - s), magnitudes over 6 become 6.  A block that holds a NaN or an infinity
+ * has s = 255 and reads as NaN.  Both arrays 16-byte aligned.  (No counterpart in the reference,
+ * whose Linear layers run in bf16: model.py:133-137, 243-245.) */
+#define ICSA_MX_MAX_ROWS (1LL << 30)
+#define ICSA_MX_MAX_K (1 << 22)
+#define ICSA_ACT_NONE 0
+#define ICSA_ACT_GELU_TANH 1
+
+/* Bytes of the two arrays (-1: invalid sizes). */
+int64_t icsa_mx_codes_size(int64_t M, int K);
+int64_t icsa_mx_scales_size(int64_t M, int K);
+
+/* x [M, K] bf16 or f32 (row stride x_ss elements, any alignment) to codes and scales. */
+int icsa_mx_quantize(const void* x, int x_dtype, int64_t x_ss, int64_t M, int K, void* codes, void* scales, void* stream);
+
+/* The values of codes and scales, bf16 (which holds each of them) or f32 [M, K]. */
+int icsa_mx_dequantize(const void* codes, const void* scales, int64_t M, int K, void* out, int out_dtype, int64_t o_ss,
+                       void* stream);
+
+/* Workspace bytes of icsa_mx_linear (0 for an x in 4 bits). */
+int64_t icsa_mx_linear_workspace_size(int64_t M, int N, int K, int x_dtype);
+
+/* out = act(x w^T + bias), f32 accumulation and one rounding at the end: x [M, K] bf16 or f32 (row
+ * stride x_ss; quantised in the call) or ICSA_MXFP4 (codes x, x_scales); w [N, K] in 4 bits;
+ * bias bf16 or f32 [N] or NULL; activation ICSA_ACT_NONE or ICSA_ACT_GELU_TANH; out [M, N]
+ * bf16 or f32 (row stride o_ss), or ICSA_MXFP4: out the codes of the result quantised along N
+ * from f32, out_scales its scales. */
+int icsa_mx_linear(const void* x, const void* x_scales, int x_dtype, int64_t x_ss, const void* w, const void* w_scales,
+                   const void* bias, int bias_dtype, int activation, int64_t M, int N, int K, void* out, void* out_scales,
+                   int out_dtype, int64_t o_ss, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Last error message of the calling thread ("" if none). */
 const char* icsa_last_error(void);

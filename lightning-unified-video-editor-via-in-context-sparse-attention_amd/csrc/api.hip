@@ -11,6 +11,7 @@
 
 #include "flash_plan.h"
 #include "icsa_kernels.h"
+#include "mx_common.h"
 #include "../../include/icsa.h"
 
 namespace {
@@ -561,6 +562,155 @@ int icsa_wan_ln_modulate(const void* x, int x_dtype, int64_t x_sb, int64_t x_ss,
   p.out = reinterpret_cast<bf16*>(out); p.o_sb = o_sb; p.o_ss = o_ss;
   p.B = B; p.S = S; p.dim = dim; p.eps = eps;
   ICSA_HIP_TRY(launch_ln_mod(p, reinterpret_cast<hipStream_t>(stream_)), "layer norm / modulate");
+  return ICSA_OK;
+}
+
+// ---- attention under masks ----
+static int check_masked_sizes(int B, int Sq, int Sk, int H, int Hk, int D) {
+  if (B <= 0 || Sq < 0 || Sk < 0 || H <= 0 || Hk <= 0 || H % Hk != 0)
+    return fail(ICSA_EINVAL, "bad sizes B=%d Sq=%d Sk=%d H=%d Hk=%d (H must be a multiple of Hk)", B, Sq, Sk, H, Hk);
+  if (D != 64 && D != 128) return fail(ICSA_EUNSUPPORTED, "D=%d: head dims are 64 and 128", D);
+  const int64_t rows = (int64_t)Sq * (H / Hk);
+  if (Sk > (1 << 30) || rows > (1 << 30) || (int64_t)B * Hk * ((rows + MA_ROWS - 1) / MA_ROWS) > (1 << 20))
+    return fail(ICSA_EUNSUPPORTED, "too many rows or keys");
+  return ICSA_OK;
+}
+
+int64_t icsa_masked_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D) {
+  if (check_masked_sizes(B, Sq, Sk, H, Hk, D)) return -1;
+  return align256(masked_attn_part_floats(B, Sq, H, Hk, D, masked_attn_splits(B, Sq, Sk, H, Hk)) * 4);
+}
+
+int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                     const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                     const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                     int B, int Sq, int Sk, int H, int Hk, int D,
+                     const int32_t* q_starts, const int32_t* k_starts, int docs, int causal, const int32_t* prefix,
+                     float scale, float softcap, const float* bias, int radius,
+                     void* out, int out_dtype, int64_t o_sb, int64_t o_ss, int64_t o_sh,
+                     void* workspace, int64_t workspace_bytes, void* stream_) {
+  int rc = check_masked_sizes(B, Sq, Sk, H, Hk, D);
+  if (rc || (rc = check_dtype(out_dtype, "out"))) return rc;
+  if (!q_starts != !k_starts) return fail(ICSA_EINVAL, "q_starts and k_starts must be both given or both NULL");
+  if (docs < 1 || (!q_starts && docs != 1)) return fail(ICSA_EINVAL, "docs=%d without document starts", docs);
+  if (prefix && !causal) return fail(ICSA_EINVAL, "a prefix needs the causal mask");
+  if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.f)
+    return fail(ICSA_EINVAL, "scale and softcap must be finite, softcap not negative");
+  if (bias && (radius < 0 || !masked_attn_bias_fits(H, Hk, D, radius)))
+    return fail(ICSA_EUNSUPPORTED, "bias of radius %d for %d heads a key head does not fit the LDS", radius, H / Hk);
+  if (Sq == 0) return ICSA_OK;
+  if (!q || !out || (Sk > 0 && (!k || !v))) return fail(ICSA_EINVAL, "null pointer argument");
+  if (!row_ok(q, ICSA_BF16, q_sb, q_ss, q_sh) || !row_ok(out, out_dtype, o_sb, o_ss, o_sh) ||
+      (Sk > 0 && (!row_ok(k, ICSA_BF16, k_sb, k_ss, k_sh) || !row_ok(v, ICSA_BF16, v_sb, v_ss, v_sh))))
+    return fail(ICSA_EINVAL, "rows must be 16-byte aligned (pointers and strides)");
+  if (k_ss < 0 || v_ss < 0) return fail(ICSA_EINVAL, "negative key stride");
+  MaskedAttnParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = reinterpret_cast<const bf16*>(q); p.q_sb = q_sb; p.q_ss = q_ss; p.q_sh = q_sh;
+  p.k = reinterpret_cast<const bf16*>(k); p.k_sb = k_sb; p.k_ss = k_ss; p.k_sh = k_sh;
+  p.v = reinterpret_cast<const bf16*>(v); p.v_sb = v_sb; p.v_ss = v_ss; p.v_sh = v_sh;
+  p.B = B; p.Sq = Sq; p.Sk = Sk; p.H = H; p.Hk = Hk; p.D = D;
+  p.q_starts = q_starts; p.k_starts = k_starts; p.docs = docs; p.causal = causal != 0; p.prefix = prefix;
+  p.scale = scale; p.softcap = softcap; p.bias = bias; p.radius = radius;
+  p.out = OutView{out, o_sb, o_ss, o_sh, out_dtype};
+  p.n_split = masked_attn_splits(B, Sq, Sk, H, Hk);
+  const int64_t need = icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(ICSA_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  p.part = reinterpret_cast<float*>(workspace);
+  ICSA_HIP_TRY(launch_masked_attn(p, reinterpret_cast<hipStream_t>(stream_)), "masked attention");
+  return ICSA_OK;
+}
+
+// ---- 4-bit floating point ----
+int64_t icsa_mx_codes_size(int64_t M, int K) { return M < 0 || K <= 0 ? -1 : M * (mx_padded(K) / 2); }
+int64_t icsa_mx_scales_size(int64_t M, int K) { return M < 0 || K <= 0 ? -1 : M * (mx_padded(K) / MX_BLOCK); }
+
+static int check_mx_operand(const void* codes, const void* scales, const char* name) {
+  if (!codes || !scales) return fail(ICSA_EINVAL, "%s: codes or scales are NULL", name);
+  if (!aligned16(codes) || !aligned16(scales)) return fail(ICSA_EINVAL, "%s: codes and scales must be 16-byte aligned", name);
+  return ICSA_OK;
+}
+
+static int check_mx_rows(int64_t M, int K, const char* name) {
+  if (M < 0 || K <= 0) return fail(ICSA_EINVAL, "%s: rows %lld and length %d must be positive", name, (long long)M, K);
+  if (M > ICSA_MX_MAX_ROWS || K > ICSA_MX_MAX_K)
+    return fail(ICSA_EUNSUPPORTED, "%s: rows %lld or length %d over the limits", name, (long long)M, K);
+  return ICSA_OK;
+}
+
+int icsa_mx_quantize(const void* x, int x_dtype, int64_t x_ss, int64_t M, int K, void* codes, void* scales, void* stream_) {
+  int rc = check_dtype(x_dtype, "x");
+  if (rc || (rc = check_mx_rows(M, K, "x"))) return rc;
+  if (M == 0) return ICSA_OK;
+  if (!x) return fail(ICSA_EINVAL, "x is NULL");
+  if ((rc = check_mx_operand(codes, scales, "out"))) return rc;
+  MxQuantParams p;
+  p.x = x; p.x_dtype = x_dtype; p.x_ss = x_ss; p.M = M; p.K = K;
+  p.codes = reinterpret_cast<unsigned char*>(codes); p.scales = reinterpret_cast<unsigned char*>(scales);
+  ICSA_HIP_TRY(launch_mx_quantize(p, reinterpret_cast<hipStream_t>(stream_)), "mx quantise");
+  return ICSA_OK;
+}
+
+int icsa_mx_dequantize(const void* codes, const void* scales, int64_t M, int K, void* out, int out_dtype, int64_t o_ss,
+                       void* stream_) {
+  int rc = check_dtype(out_dtype, "out");
+  if (rc || (rc = check_mx_rows(M, K, "codes"))) return rc;
+  if (M == 0) return ICSA_OK;
+  if ((rc = check_mx_operand(codes, scales, "codes"))) return rc;
+  if (!out || (M > 1 && o_ss < K)) return fail(ICSA_EINVAL, "out is NULL or its rows overlap");
+  MxDequantParams p;
+  p.codes = reinterpret_cast<const unsigned char*>(codes); p.scales = reinterpret_cast<const unsigned char*>(scales);
+  p.M = M; p.K = K; p.out = out; p.out_dtype = out_dtype; p.o_ss = o_ss;
+  ICSA_HIP_TRY(launch_mx_dequantize(p, reinterpret_cast<hipStream_t>(stream_)), "mx dequantise");
+  return ICSA_OK;
+}
+
+int64_t icsa_mx_linear_workspace_size(int64_t M, int N, int K, int x_dtype) {
+  if (M < 0 || N <= 0 || K <= 0) return -1;
+  if (x_dtype == ICSA_MXFP4) return 0;
+  return align256(icsa_mx_codes_size(M, K)) + align256(icsa_mx_scales_size(M, K));
+}
+
+int icsa_mx_linear(const void* x, const void* x_scales, int x_dtype, int64_t x_ss, const void* w, const void* w_scales,
+                   const void* bias, int bias_dtype, int activation, int64_t M, int N, int K, void* out, void* out_scales,
+                   int out_dtype, int64_t o_ss, void* workspace, int64_t workspace_bytes, void* stream_) {
+  int rc = check_mx_rows(M, K, "x");
+  if (rc || (rc = check_mx_rows(N, K, "w"))) return rc;
+  if (N == 0) return fail(ICSA_EINVAL, "w has no rows");
+  if (x_dtype != ICSA_MXFP4 && (rc = check_dtype(x_dtype, "x"))) return rc;
+  if (out_dtype != ICSA_MXFP4 && (rc = check_dtype(out_dtype, "out"))) return rc;
+  if (bias && (rc = check_dtype(bias_dtype, "bias"))) return rc;
+  if (activation != ICSA_ACT_NONE && activation != ICSA_ACT_GELU_TANH) return fail(ICSA_EINVAL, "activation %d", activation);
+  if ((rc = check_mx_operand(w, w_scales, "w"))) return rc;
+  if (M == 0) return ICSA_OK;
+  if (!x || !out) return fail(ICSA_EINVAL, "x or out is NULL");
+  if (x_dtype == ICSA_MXFP4 && (rc = check_mx_operand(x, x_scales, "x"))) return rc;
+  if (out_dtype == ICSA_MXFP4) {
+    if ((rc = check_mx_operand(out, out_scales, "out"))) return rc;
+    if (N > ICSA_MX_MAX_K) return fail(ICSA_EUNSUPPORTED, "rows of %d outputs in 4 bits", N);
+  } else if (!aligned16(out) || (M > 1 && o_ss < N)) {
+    return fail(ICSA_EINVAL, "out must be 16-byte aligned and its rows apart");
+  }
+  const int64_t need = icsa_mx_linear_workspace_size(M, N, K, x_dtype);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(ICSA_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  MxGemmParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.x = reinterpret_cast<const unsigned char*>(x); p.x_scales = reinterpret_cast<const unsigned char*>(x_scales);
+  p.w = reinterpret_cast<const unsigned char*>(w); p.w_scales = reinterpret_cast<const unsigned char*>(w_scales);
+  p.M = (int)M; p.N = N; p.groups = mx_padded(K) / MX_GROUP;
+  p.bias = bias; p.bias_dtype = bias_dtype; p.gelu = activation == ICSA_ACT_GELU_TANH;
+  p.out = out; p.out_scales = reinterpret_cast<unsigned char*>(out_scales);
+  p.out_kind = out_dtype == ICSA_MXFP4 ? MX_OUT_MXFP4 : out_dtype == ICSA_F32 ? MX_OUT_F32 : MX_OUT_BF16;
+  p.o_ss = out_dtype == ICSA_MXFP4 ? mx_padded(N) / 2 : o_ss;
+  if (x_dtype != ICSA_MXFP4) {
+    unsigned char* codes = reinterpret_cast<unsigned char*>(workspace);
+    unsigned char* scales = codes + align256(icsa_mx_codes_size(M, K));
+    if ((rc = icsa_mx_quantize(x, x_dtype, x_ss, M, K, codes, scales, stream_))) return rc;
+    p.x = codes; p.x_scales = scales;
+  }
+  ICSA_HIP_TRY(launch_mx_gemm(p, reinterpret_cast<hipStream_t>(stream_)), "mx product");
   return ICSA_OK;
 }
 

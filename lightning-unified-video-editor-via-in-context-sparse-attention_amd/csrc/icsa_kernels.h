@@ -219,3 +219,52 @@ struct SparseBwdParams {
   OutView dq, dk, dv;                // (sb, token stride, sh, dtype)
 };
 hipError_t launch_sparse_bwd(const SparseBwdParams& p, hipStream_t stream);
+
+// ---------------------------------------------------- 4-bit floating point (mx_quant.hip, mx_gemm.hip)
+struct MxQuantParams {
+  const void* x; int x_dtype; int64_t x_ss;       // [M, K] element row stride
+  int64_t M; int K;
+  unsigned char* codes;                           // [M, Kp / 2]
+  unsigned char* scales;                          // [Kp / 256, M, 8]
+};
+hipError_t launch_mx_quantize(const MxQuantParams& p, hipStream_t stream);
+
+struct MxDequantParams {
+  const unsigned char* codes;
+  const unsigned char* scales;
+  int64_t M; int K;
+  void* out; int out_dtype; int64_t o_ss;
+};
+hipError_t launch_mx_dequantize(const MxDequantParams& p, hipStream_t stream);
+
+enum MxOut { MX_OUT_BF16 = 0, MX_OUT_F32 = 1, MX_OUT_MXFP4 = 2 };
+
+struct MxGemmParams {
+  const unsigned char* x; const unsigned char* x_scales;   // [M, Kp / 2], [Kp / 256, M, 8]
+  const unsigned char* w; const unsigned char* w_scales;   // [N, Kp / 2], [Kp / 256, N, 8]
+  int M, N, groups;                                        // groups = Kp / 256
+  const void* bias; int bias_dtype;                        // [N] or null
+  int gelu;
+  void* out; int out_kind; int64_t o_ss;                   // MxOut; o_ss: element row stride (codes: Np / 2)
+  unsigned char* out_scales;                               // [Np / 256, M, 8]
+};
+hipError_t launch_mx_gemm(const MxGemmParams& p, hipStream_t stream);
+
+// ---------------------------------------------------------------- attention under masks (masked_attn.hip)
+#define MA_ROWS 128                  // rows (query, head of the group) of a workgroup
+struct MaskedAttnParams {
+  const bf16* q; int64_t q_sb, q_ss, q_sh;        // [B, Sq, H, D]
+  const bf16* k; int64_t k_sb, k_ss, k_sh;        // [B, Sk, Hk, D]
+  const bf16* v; int64_t v_sb, v_ss, v_sh;
+  int B, Sq, Sk, H, Hk, D;
+  const int* q_starts; const int* k_starts; int docs;   // [B, docs + 1] or null (docs = 1)
+  int causal; const int* prefix;                  // [B, docs] or null
+  float scale, softcap;                           // softcap 0: none
+  const float* bias; int radius;                  // [H, 2 radius + 1] or null
+  OutView out;
+  int n_split; float* part;                       // key ranges an item is split into; their partials
+};
+int masked_attn_splits(int B, int Sq, int Sk, int H, int Hk);
+int64_t masked_attn_part_floats(int B, int Sq, int H, int Hk, int D, int n_split);
+bool masked_attn_bias_fits(int H, int Hk, int D, int radius);
+hipError_t launch_masked_attn(const MaskedAttnParams& p, hipStream_t stream);

@@ -1,0 +1,518 @@
+// Attention under masks: softmax over the visible keys of cap tanh(scale q.k / cap) + bias(distance).
+//
+// Which keys a query sees is one range [lo, hi) of the sequence: its document's keys, cut at the
+// query's own position (causal, aligned at the document's end) or at the document's prefix, whichever is
+// further.  A row of work is a (query, head) pair; the H / Hk heads that share a key head are consecutive rows, so
+// a tile of keys serves them all (one query token of a group is one tile of rows).
+//
+// A workgroup of 4 waves takes 128 rows of one (batch, key head) over the 64-key tiles of the union of
+// their ranges, or over one of n_split equal parts of it where rows are few (icsa_masked_combine_kernel joins
+// the parts).  Only tiles that some row sees in part are masked.  Scores are computed transposed, S^T = K Q^T: a lane
+// holds one row and 32 of a tile's 64 keys, the other 32 are in lane ^ 32 (attn_tile.h).  P goes to
+// the second product from its registers; V is read transposed from its row-major tile.
+//
+// K and V tiles arrive by direct global->LDS loads, two buffers, one barrier a tile: the tile after next is
+// requested when everybody has passed the barrier behind the last use of its buffer.  Two
+// workgroups share a CU: one's exponentials run beside the other's products.
+//
+// Values in masked places: scores are replaced, not added to, so a NaN of a masked key does not
+// matter; V rows that no row of the workgroup sees are cleared in LDS; and where a partly visible tile holds
+// a V that is not finite, 0 * V would reach rows that do not see it, so that tile is added key by
+// key to the rows that do (add_tile_by_key).
+#include "attn_tile.h"
+#include "icsa_kernels.h"
+
+#define MA_THREADS 256
+#define MA_WAVES 4
+#define MA_SCRATCH_WAVE 2048                          // per wave: staged output rows, or half a tile's P
+#define MA_CTL_BYTES 256                              // per-wave ranges, flags
+#define MA_PSUM_MAX 18446744073709551616.0f           // as in the dense kernel: the reference max is raised past it
+#define MA_M_NONE (-3.4028234663852886e38f)           // finite: a tile without visible keys leaves O = l = 0
+#define MA_LOG2E 1.4426950408889634f
+#define MA_TARGET_WG 512                              // two workgroups a CU
+#define MA_MIN_SPLIT_TILES 4                          // key tiles a split part is worth
+#define MA_LDS_MAX (160 * 1024)
+
+namespace {
+
+template <int D> struct Tile {
+  static constexpr int kRow = D * 2, kBytes = ATT_BN * kRow, kChunks = D / 8;
+  static constexpr int kRowsPerLoad = 1024 / kRow, kLoads = 16 / kRowsPerLoad;   // of a wave's 16 rows
+  // 16-byte chunk c of row r sits at c ^ kswz(r) in a K tile: 16 rows' reads of one chunk touch
+  // every bank once; at c ^ vswz(r) in a V tile, for the transposing reads
+  static __device__ __forceinline__ int kswz(int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); }
+  static __device__ __forceinline__ int vswz(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
+};
+
+__host__ __device__ __forceinline__ int ma_fixed_lds(int D) { return 4 * ATT_BN * D * 2 + MA_WAVES * MA_SCRATCH_WAVE + MA_CTL_BYTES; }
+
+// What a row sees: keys [lo, hi); at: the key position its own query is aligned with.
+struct RowRange { int lo, hi, at; };
+
+__device__ __forceinline__ RowRange row_range(const MaskedAttnParams& p, int b, int i) {
+  RowRange r = {0, 0, 0};
+  int q1 = p.Sq, k0 = 0, k1 = p.Sk, n = 0;
+  if (p.q_starts != nullptr) {
+    const int* qs = p.q_starts + (int64_t)b * (p.docs + 1);
+    int lo = 0, hi = p.docs + 1;                      // the count of starts <= i
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (qs[mid] <= i) lo = mid + 1; else hi = mid;
+    }
+    n = lo - 1;
+    if (n < 0 || n >= p.docs) return r;               // in front of the first document, or behind the last
+    q1 = qs[n + 1];
+    const int* ks = p.k_starts + (int64_t)b * (p.docs + 1);
+    k0 = min(max(ks[n], 0), p.Sk);
+    k1 = min(max(ks[n + 1], 0), p.Sk);
+  }
+  const int64_t at = (int64_t)i + k1 - q1;
+  r.at = (int)max((int64_t)-0x40000000, min((int64_t)0x40000000, at));
+  int64_t end = k1;
+  if (p.causal) {
+    end = min(end, max(at + 1, p.prefix ? (int64_t)k0 + p.prefix[(int64_t)b * p.docs + n] : (int64_t)k0));
+  }
+  if (end > k0) { r.lo = k0; r.hi = (int)end; }
+  return r;
+}
+
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x = min(x, __shfl_xor(x, o, 64));
+  return x;
+}
+__device__ __forceinline__ int wave_max(int x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
+  return x;
+}
+
+// One wave's 32 rows of 32 dims to the output: through 2 KB of the wave's LDS, so that bf16
+// stores are 64-byte segments.  v: this lane's 16 values (dims 8 (e / 4) + 4 hl + e % 4 of row li).
+template <int kB16>
+__device__ __forceinline__ void store_dims32(unsigned char* stage, const float v[16], int rows_valid, int64_t row_off[2],
+                                             int64_t own_off, void* out, int d0) {
+  const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5;
+  if constexpr (kB16) {
+    const int wx = (li >> 2) & 3;
+#pragma unroll
+    for (int pr = 0; pr < 2; ++pr) {
+      bf16x4 lo, hi;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { lo[e] = (bf16)v[8 * pr + e]; hi[e] = (bf16)v[8 * pr + 4 + e]; }
+      const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+      const auto w0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+      const auto w1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+      *reinterpret_cast<u32x4*>(stage + li * 64 + (((2 * pr + hl) ^ wx) << 4)) = u32x4{w0[0], w1[0], w0[1], w1[1]};
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 16 * i + (lane >> 2);
+      const u32x4 x = *reinterpret_cast<const u32x4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 2) & 3)) << 4));
+      if (r < rows_valid) *reinterpret_cast<u32x4*>(reinterpret_cast<bf16*>(out) + row_off[i] + d0 + 8 * (lane & 3)) = x;
+    }
+  } else if (li < rows_valid) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(out) + own_off + d0 + 8 * g + 4 * hl) =
+          floatx4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+  }
+}
+
+// element offset of row r (query r / G, head hk G + r % G) in a [B, S, H, D] tensor
+__device__ __forceinline__ int64_t row_at(int64_t sb, int64_t ss, int64_t sh, int b, int hk, int G, int r) {
+  return (int64_t)b * sb + (int64_t)(r / G) * ss + (int64_t)(hk * G + r % G) * sh;
+}
+
+template <int D>
+__device__ __forceinline__ void store_wave(const MaskedAttnParams& p, unsigned char* stage, const floatx16 o[D / 32],
+                                           float inv_l, int b, int hk, int r0, int rows_valid) {
+  const int lane = threadIdx.x & 63, li = lane & 31, G = p.H / p.Hk;
+  int64_t off[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) off[i] = row_at(p.out.sb, p.out.ss, p.out.sh, b, hk, G, r0 + 16 * i + (lane >> 2));
+  const int64_t own = row_at(p.out.sb, p.out.ss, p.out.sh, b, hk, G, r0 + li);
+#pragma unroll
+  for (int ds = 0; ds < D / 32; ++ds) {
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = o[ds][e] * inv_l;
+    if (p.out.dtype == ICSA_DT_BF16) store_dims32<1>(stage, v, rows_valid, off, own, p.out.p, 32 * ds);
+    else store_dims32<0>(stage, v, rows_valid, off, own, p.out.p, 32 * ds);
+  }
+}
+
+}  // namespace
+
+template <int D, bool kCap, bool kBias>
+__global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedAttnParams p) {
+  typedef Tile<D> T;
+  constexpr int kSteps = D / 16, kSub = D / 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* const scratch_all = smem + 4 * T::kBytes;
+  int* const ctl = reinterpret_cast<int*>(scratch_all + MA_WAVES * MA_SCRATCH_WAVE);   // ranges of the 4 waves, 2 flags
+  float* const bias_lds = reinterpret_cast<float*>(scratch_all + MA_WAVES * MA_SCRATCH_WAVE + MA_CTL_BYTES);
+  const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS;
+  const int64_t items = (int64_t)p.B * p.Hk * n_blk * p.n_split;
+  const int w = xcd_remap(blockIdx.x, (int)items);
+  if (w < 0) return;
+  // last row blocks first: under a causal mask they are the longest
+  const int split = w % p.n_split, blk = n_blk - 1 - w / p.n_split % n_blk, bh = w / p.n_split / n_blk;
+  const int b = bh / p.Hk, hk = bh % p.Hk;
+  const int r0 = blk * MA_ROWS + 32 * wave;
+  const int rows_valid = min(32, n_rows - r0);
+
+  // ---- what the rows see ----
+  RowRange rr = {0, 0, 0};
+  if (li < rows_valid) rr = row_range(p, b, (r0 + li) / G);
+  {
+    const bool any = rr.hi > rr.lo;
+    const int lo = wave_min(any ? rr.lo : 0x7fffffff), hi = wave_max(any ? rr.hi : 0);
+    const int in_lo = wave_max(any ? rr.lo : 0), in_hi = wave_min(any ? rr.hi : 0x7fffffff);
+    if (lane == 0) { ctl[wave] = lo; ctl[4 + wave] = hi; ctl[8 + wave] = in_lo; ctl[12 + wave] = in_hi; }
+    if (threadIdx.x < 2) ctl[16 + threadIdx.x] = 0;
+  }
+  const float c = p.scale * MA_LOG2E;
+  if constexpr (kBias) {
+    const int width = 2 * p.radius + 1;
+    const float* src = p.bias + (int64_t)hk * G * width;                 // the group's heads
+    for (int x = threadIdx.x; x < G * width; x += MA_THREADS) {
+      const float f = src[x];            // a type's lowest value stays finite in units of log2, an infinity does not
+      bias_lds[x] = __builtin_isinf(f) ? f : fminf(fmaxf(f * MA_LOG2E, -3.4028234663852886e38f), 3.4028234663852886e38f);
+    }
+  }
+  __syncthreads();
+  // keys that some row sees, [u_lo, u_hi), and keys that every row (that sees any) sees, [a_lo, a_hi)
+  auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  const int u_lo = uni(min(min(ctl[0], ctl[1]), min(ctl[2], ctl[3]))), u_hi = uni(max(max(ctl[4], ctl[5]), max(ctl[6], ctl[7])));
+  const int a_lo = uni(max(max(ctl[8], ctl[9]), max(ctl[10], ctl[11]))), a_hi = uni(min(min(ctl[12], ctl[13]), min(ctl[14], ctl[15])));
+  int t0 = 0, t1 = 0;
+  if (u_hi > u_lo) {
+    const int first = u_lo / ATT_BN, n = (u_hi + ATT_BN - 1) / ATT_BN - first;
+    t0 = first + (int)((int64_t)n * split / p.n_split);
+    t1 = first + (int)((int64_t)n * (split + 1) / p.n_split);
+  }
+
+  // ---- loads ----
+  const bf16* kb = p.k + (int64_t)b * p.k_sb + (int64_t)hk * p.k_sh;
+  const bf16* vb = p.v + (int64_t)b * p.v_sb + (int64_t)hk * p.v_sh;
+  int kofs[T::kLoads], vofs[T::kLoads];
+#pragma unroll
+  for (int i = 0; i < T::kLoads; ++i) {
+    const int r = 16 * wave + T::kRowsPerLoad * i + lane / T::kChunks, ch = lane % T::kChunks;
+    kofs[i] = (int)((r * p.k_ss + 8 * (ch ^ T::kswz(r))) * 2);
+    vofs[i] = (int)((r * p.v_ss + 8 * (ch ^ T::vswz(r))) * 2);
+  }
+  const unsigned lds0 = lds_u32(smem);
+  auto kbuf = [&](int t) { return smem + (t & 1) * T::kBytes; };
+  auto vbuf = [&](int t) { return smem + (2 + (t & 1)) * T::kBytes; };
+  auto load_tile = [&](int t) __attribute__((always_inline)) {
+    const int rows = min(ATT_BN, p.Sk - t * ATT_BN);
+    const u32x4 krs = dma_rsrc(kb + (int64_t)t * ATT_BN * p.k_ss, ((rows - 1) * p.k_ss + D) * 2);
+    const u32x4 vrs = dma_rsrc(vb + (int64_t)t * ATT_BN * p.v_ss, ((rows - 1) * p.v_ss + D) * 2);
+    const unsigned at = lds0 + (t & 1) * T::kBytes + wave * 16 * T::kRow;
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) lds_dma16(at + 1024 * i, kofs[i], krs);
+#pragma unroll
+    for (int i = 0; i < T::kLoads; ++i) lds_dma16(at + 2 * T::kBytes + 1024 * i, vofs[i], vrs);
+  };
+  if (t0 < t1) load_tile(t0);
+
+  bf16x8 qf[kSteps];
+  {
+    const bf16* src = p.q + row_at(p.q_sb, p.q_ss, p.q_sh, b, hk, G, min(r0 + li, n_rows - 1)) + 8 * hl;
+#pragma unroll
+    for (int kk = 0; kk < kSteps; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(src + 16 * kk);
+  }
+  int kro[kSteps], vro[kSub];                        // operand read offsets (bytes); + 32 rows a sub-tile
+#pragma unroll
+  for (int kk = 0; kk < kSteps; ++kk) kro[kk] = li * T::kRow + (((2 * kk + hl) ^ T::kswz(li)) << 4);
+#pragma unroll
+  for (int ds = 0; ds < kSub; ++ds) {
+    const int g = lane >> 4, s = lane & 15, row = 4 * (g >> 1) + (s >> 2), col = 32 * ds + 16 * (g & 1) + 4 * (s & 3);
+    vro[ds] = row * T::kRow + (((col >> 3) ^ T::vswz(row)) << 4) + (col & 7) * 2;
+  }
+  unsigned char* const scratch = scratch_all + wave * MA_SCRATCH_WAVE;
+  const float* const my_bias = kBias ? bias_lds + ((r0 + li) % G) * (2 * p.radius + 1) + p.radius : nullptr;
+
+  floatx16 o[kSub] = {};
+  float m_ref = MA_M_NONE, l_run = 0.f;
+  bool first = true;
+  // a row that sees nothing, or does not exist, asks for no mask of its own: its scores are masked
+  // whenever the others' are, and what it holds is not used
+  const bool some = rr.hi > rr.lo;
+  const int see_lo = some ? rr.lo : 0, see_hi = some ? rr.hi : 0x7fffffff;
+
+  for (int t = t0; t < t1; ++t) {
+    const int j0 = t * ATT_BN;
+    unsigned char* const ks = kbuf(t);
+    unsigned char* const vs = vbuf(t);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const bool wg_partial = j0 < a_lo || j0 + ATT_BN > a_hi;            // for some row of the workgroup
+    if (wg_partial) {
+      // this wave's 16 V rows: those that no row sees cleared, the others looked at
+      const int row = 16 * wave + (lane >> 2), key = j0 + row;
+      u32x4* own = reinterpret_cast<u32x4*>(vs + row * T::kRow + (lane & 3) * (T::kRow / 4));
+      bool bad = false;
+      if (key < u_lo || key >= u_hi) {
+#pragma unroll
+        for (int e = 0; e < T::kRow / 64; ++e) own[e] = u32x4{0u, 0u, 0u, 0u};
+      } else {
+#pragma unroll
+        for (int e = 0; e < T::kRow / 64; ++e) {
+          const u32x4 x = own[e];
+#pragma unroll
+          for (int f = 0; f < 4; ++f) bad |= (x[f] & 0x7f80u) == 0x7f80u || (x[f] & 0x7f800000u) == 0x7f800000u;
+        }
+      }
+      if (__ballot(bad) != 0ull && lane == 0) ctl[16 + (t & 1)] = t + 1;
+    }
+    ATT_BARRIER();
+    if (t + 1 < t1) load_tile(t + 1);
+    if (rows_valid <= 0) continue;                                     // a wave without rows moves tiles only
+    const bool partial = wg_partial && __ballot(j0 < see_lo || j0 + ATT_BN > see_hi) != 0ull;   // for some row of the wave
+
+    floatx16 s[2] = {};
+#pragma unroll
+    for (int kk = 0; kk < kSteps; ++kk) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+        s[sub] = mfma32x32x16(*reinterpret_cast<const bf16x8*>(ks + kro[kk] + sub * 32 * T::kRow), qf[kk], s[sub]);
+    }
+    // scores in units of log2
+    if constexpr (kCap) {
+      const float in = 2.f * MA_LOG2E * p.scale / p.softcap, top = p.softcap * MA_LOG2E;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {               // cap tanh(x) = cap - 2 cap / (1 + exp(2 x))
+          const float e = __builtin_amdgcn_exp2f(s[sub][i] * in);
+          s[sub][i] = fmaf(-2.f * top, __builtin_amdgcn_rcpf(1.f + e), top);
+        }
+    }
+    if constexpr (kBias) {
+      const int d0 = j0 - rr.at + 4 * hl, R = p.radius;
+      if (__ballot(!(d0 >= R || d0 + ATT_BN <= -R)) == 0ull) {           // the whole tile past the table's ends
+        const float x = my_bias[d0 > 0 ? R : -R];
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[sub][i] = kCap ? s[sub][i] + x : fmaf(s[sub][i], c, x);
+      } else {
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float x = my_bias[min(max(d0 + 32 * sub + 8 * (i >> 2) + (i & 3), -R), R)];
+            s[sub][i] = kCap ? s[sub][i] + x : fmaf(s[sub][i], c, x);
+          }
+      }
+    }
+    constexpr bool kScaled = kCap || kBias;            // s already in log2 units
+    const float cs = kScaled ? 1.f : c;
+    if (partial) {
+      // keys outside [lo, hi) as one 64-bit word: element i of sub-tile sub is key 32 sub + 8 (i / 4) + 4 hl + i % 4
+      const int a = min(max(rr.lo - j0, 0), 64), z = min(max(rr.hi - j0, 0), 64);
+      const unsigned long long below_a = a >= 64 ? ~0ull : (1ull << a) - 1, below_z = z >= 64 ? ~0ull : (1ull << z) - 1;
+      const unsigned long long mw = ~(below_z & ~below_a) >> (4 * hl);
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const unsigned wd = (unsigned)(mw >> (32 * sub));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int kbit = 8 * (i >> 2) + (i & 3);
+          const unsigned all = (unsigned)((int)(wd << (31 - kbit)) >> 31);
+          s[sub][i] = __uint_as_float((all & 0xff800000u) | (__float_as_uint(s[sub][i]) & ~all));
+        }
+      }
+    }
+    bf16x8 pf[4];
+    float rs = 0.f;
+    if (!first) {
+      float rsv[4] = {};
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[sub][i], cs, -m_ref));
+          rsv[i & 3] += e;
+          pf[2 * sub + (i >> 3)][i & 7] = (bf16)e;
+        }
+      rs = (rsv[0] + rsv[1]) + (rsv[2] + rsv[3]);
+    }
+    if (first || __ballot(!(rs <= MA_PSUM_MAX)) != 0ull) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[sub][i]);
+      mx = xhalf_max(mx) * cs;
+      const float mn = mx > m_ref ? mx : m_ref;
+      const float al = __builtin_amdgcn_exp2f(m_ref - mn);
+#pragma unroll
+      for (int ds = 0; ds < kSub; ++ds)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[ds][i] *= al;
+      l_run *= al;
+      m_ref = mn;
+      rs = 0.f;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[sub][i], cs, -m_ref));
+          rs += e;
+          pf[2 * sub + (i >> 3)][i & 7] = (bf16)e;
+        }
+      first = false;
+    }
+    l_run += rs;
+
+    if (!(partial && uni(ctl[16 + (t & 1)]) == t + 1)) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int ds = 0; ds < kSub; ++ds) {
+          const rt_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rt_lds_v4s)(vs + vro[ds] + m * 16 * T::kRow));
+          const rt_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rt_lds_v4s)(vs + vro[ds] + (m * 16 + 8) * T::kRow));
+          const short __attribute__((ext_vector_type(8))) a8 = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          o[ds] = mfma32x32x16(__builtin_bit_cast(bf16x8, a8), pf[m], o[ds]);
+        }
+    } else {
+      // key by key, to the rows that see it: P through the wave's scratch, 32 keys at a time
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        bf16* const ps = reinterpret_cast<bf16*>(scratch);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ps[(8 * (i >> 2) + 4 * hl + (i & 3)) * 32 + li] = pf[2 * sub + (i >> 3)][i & 7];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 1
+        for (int x = 0; x < 32; ++x) {
+          const int row = 32 * sub + x, key = j0 + row;
+          const float pv = (float)ps[x * 32 + li];
+          const bool vis = key >= rr.lo && key < rr.hi;
+#pragma unroll
+          for (int ds = 0; ds < kSub; ++ds)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int col = 32 * ds + 8 * g + 4 * hl;
+              const bf16x4 v4 = *reinterpret_cast<const bf16x4*>(vs + row * T::kRow + (((col >> 3) ^ T::vswz(row)) << 4) + (col & 7) * 2);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                o[ds][4 * g + e] = vis ? fmaf(pv, (float)v4[e], o[ds][4 * g + e]) : o[ds][4 * g + e];
+            }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+    }
+  }
+
+  if (rows_valid <= 0) return;
+  if (p.n_split > 1) {
+    // raw O, reference max and the two halves' sums: [item][wave][ds][g][lane][4], [2][64]
+    float* dst = p.part + ((int64_t)((bh * (int64_t)n_blk + blk) * p.n_split + split) * MA_WAVES + wave) * (D * 32 + 128);
+#pragma unroll
+    for (int ds = 0; ds < kSub; ++ds)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<floatx4*>(dst + ((ds * 4 + g) * 64 + lane) * 4) =
+            some ? floatx4{o[ds][4 * g], o[ds][4 * g + 1], o[ds][4 * g + 2], o[ds][4 * g + 3]} : floatx4{};
+    dst[D * 32 + lane] = some ? m_ref : MA_M_NONE;
+    dst[D * 32 + 64 + lane] = some ? l_run : 0.f;
+    return;
+  }
+  if (!some) {                                         // whatever it holds of tiles that others see whole
+#pragma unroll
+    for (int ds = 0; ds < kSub; ++ds) o[ds] = floatx16{};
+  }
+  const float l = xhalf_sum(l_run);
+  store_wave<D>(p, scratch, o, !some || l == 0.f ? 0.f : 1.f / l, b, hk, r0, rows_valid);
+}
+
+// Joins the parts of every item in order (bitwise reproducible): one wave for 32 rows.
+template <int D>
+__global__ void __launch_bounds__(64) icsa_masked_combine_kernel(MaskedAttnParams p) {
+  __shared__ __attribute__((aligned(16))) unsigned char stage[MA_SCRATCH_WAVE];
+  constexpr int kSub = D / 32, kPart = D * 32 + 128;
+  const int lane = threadIdx.x & 63;
+  const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS;
+  const int item = blockIdx.x / MA_WAVES, w = blockIdx.x % MA_WAVES, blk = item % n_blk, bh = item / n_blk;
+  const int r0 = blk * MA_ROWS + 32 * w, rows_valid = min(32, n_rows - r0);
+  if (rows_valid <= 0) return;
+  floatx16 o[kSub] = {};
+  float m = MA_M_NONE, l = 0.f;
+  const float* src = p.part + ((int64_t)item * p.n_split * MA_WAVES + w) * kPart;
+  for (int s = 0; s < p.n_split; ++s, src += (int64_t)MA_WAVES * kPart) {
+    const float ms = src[D * 32 + lane], ls = src[D * 32 + 64 + lane];
+    const float mn = ms > m ? ms : m;
+    const float fo = __builtin_amdgcn_exp2f(m - mn), fn = __builtin_amdgcn_exp2f(ms - mn);
+#pragma unroll
+    for (int ds = 0; ds < kSub; ++ds)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const floatx4 x = *reinterpret_cast<const floatx4*>(src + ((ds * 4 + g) * 64 + lane) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[ds][4 * g + e] = fmaf(x[e], fn, o[ds][4 * g + e] * fo);
+      }
+    l = fmaf(ls, fn, l * fo);
+    m = mn;
+  }
+  l = xhalf_sum(l);
+  store_wave<D>(p, stage, o, l == 0.f ? 0.f : 1.f / l, bh / p.Hk, bh % p.Hk, r0, rows_valid);
+}
+
+// Parts that an item's keys are cut into: enough workgroups for two a CU, each with a few tiles.
+int masked_attn_splits(int B, int Sq, int Sk, int H, int Hk) {
+  const int64_t rows = (int64_t)Sq * (H / Hk), items = (int64_t)B * Hk * ((rows + MA_ROWS - 1) / MA_ROWS);
+  const int tiles = (Sk + ATT_BN - 1) / ATT_BN;
+  if (items <= 0 || items * 2 > MA_TARGET_WG) return 1;
+  int64_t n = (MA_TARGET_WG + items - 1) / items;
+  n = n < tiles / MA_MIN_SPLIT_TILES ? n : tiles / MA_MIN_SPLIT_TILES;
+  return n < 1 ? 1 : (int)n;
+}
+
+int64_t masked_attn_part_floats(int B, int Sq, int H, int Hk, int D, int n_split) {
+  if (n_split <= 1) return 0;
+  const int64_t rows = (int64_t)Sq * (H / Hk);
+  return (int64_t)B * Hk * ((rows + MA_ROWS - 1) / MA_ROWS) * n_split * MA_WAVES * (D * 32 + 128);
+}
+
+bool masked_attn_bias_fits(int H, int Hk, int D, int radius) {
+  return (int64_t)(H / Hk) * (2 * (int64_t)radius + 1) * 4 <= MA_LDS_MAX - ma_fixed_lds(D);
+}
+
+namespace {
+
+template <int D, bool kCap, bool kBias>
+hipError_t run_masked(const MaskedAttnParams& p, hipStream_t stream) {
+  static std::atomic<unsigned> lds_set{0u};
+  const int G = p.H / p.Hk;
+  const int lds = ma_fixed_lds(D) + (kBias ? G * (2 * p.radius + 1) * 4 : 0);
+  const hipError_t a = ensure_lds_limit(reinterpret_cast<const void*>(icsa_masked_attn_kernel<D, kCap, kBias>), MA_LDS_MAX, &lds_set);
+  if (a != hipSuccess) return a;
+  const int64_t blocks = (int64_t)p.B * p.Hk * (((int64_t)p.Sq * G + MA_ROWS - 1) / MA_ROWS);
+  if (blocks * p.n_split > 0x3fffffffLL) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((icsa_masked_attn_kernel<D, kCap, kBias>), dim3(xcd_grid((int)(blocks * p.n_split))), dim3(MA_THREADS), lds,
+                     stream, p);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.n_split == 1) return e;
+  hipLaunchKernelGGL(icsa_masked_combine_kernel<D>, dim3((unsigned)(blocks * MA_WAVES)), dim3(64), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <int D>
+hipError_t pick_masked(const MaskedAttnParams& p, hipStream_t stream) {
+  const bool cap = p.softcap > 0.f, bias = p.bias != nullptr;
+  if (cap) return bias ? run_masked<D, true, true>(p, stream) : run_masked<D, true, false>(p, stream);
+  return bias ? run_masked<D, false, true>(p, stream) : run_masked<D, false, false>(p, stream);
+}
+
+}  // namespace
+
+hipError_t launch_masked_attn(const MaskedAttnParams& p, hipStream_t stream) {
+  // a tile's rows must be addressable with 32-bit offsets
+  if (p.k_ss * 2 * ATT_BN > 0x7fffffffLL || p.v_ss * 2 * ATT_BN > 0x7fffffffLL) return hipErrorInvalidValue;
+  return p.D == 128 ? pick_masked<128>(p, stream) : pick_masked<64>(p, stream);
+}

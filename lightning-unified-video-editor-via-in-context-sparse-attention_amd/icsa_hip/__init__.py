@@ -18,6 +18,7 @@ from .hip_host import (  # noqa: F401
     IcsaArgumentError,
     flash_attn_func,
     gather_kv,
+    masked_attn_func,
     pool,
     SparsePiecewiseAttn1stIntervalsFunction,
     sparse_piecewise_attn_1st_intervals,
@@ -26,6 +27,7 @@ from .hip_host import (  # noqa: F401
     sparse_piecewise_attn_1st_intervals_hip,
     sparse_piecewise_attn_tilelang_hosttopk_hip,
 )
+from .mx import MXFP4Tensor, MXLinear, mx_linear, mx_quantize  # noqa: F401
 
 __all__ = [
     'Backend',
@@ -38,6 +40,11 @@ __all__ = [
     'sparse_piecewise_attn_1st_intervals_fwd_hip',
     'sparse_piecewise_attn_1st_intervals_bwd_hip',
     'flash_attn_func',
+    'masked_attn_func',
+    'MXFP4Tensor',
+    'MXLinear',
+    'mx_quantize',
+    'mx_linear',
     'derived_sizes',
     'IcsaArgumentError',
 ]

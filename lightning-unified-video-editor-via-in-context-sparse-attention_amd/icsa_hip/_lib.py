@@ -18,6 +18,7 @@ _lib = None
 
 BF16 = 0
 F32 = 1
+MXFP4 = 2          # icsa_mx_linear
 
 OK = 0
 EINVAL = -1
@@ -47,6 +48,9 @@ EXPORTS = [
     "icsa_editing_sparse_attention_presummed", "icsa_wan_ln_modulate", "icsa_last_error",
     "icsa_version", "icsa_sparse_piecewise_attn_fwd", "icsa_sparse_piecewise_attn_bwd_workspace_size",
     "icsa_sparse_piecewise_attn_bwd", "icsa_sparse_piecewise_attn_hosttopk",
+    "icsa_mx_codes_size", "icsa_mx_scales_size", "icsa_mx_quantize", "icsa_mx_dequantize",
+    "icsa_mx_linear_workspace_size", "icsa_mx_linear",
+    "icsa_masked_attn_workspace_size", "icsa_masked_attn",
 ]
 
 _p = ctypes.c_void_p
@@ -170,6 +174,25 @@ _SIGNATURES = {
         _p, _p,
         _p, _p, _l, _f,
         _i, _i, _i, _p, _l, _l, _p]),
+    "icsa_mx_codes_size": (_l, [_l, _i]),
+    "icsa_mx_scales_size": (_l, [_l, _i]),
+    "icsa_mx_quantize": (_i, [_p, _i, _l, _l, _i, _p, _p, _p]),
+    "icsa_mx_dequantize": (_i, [_p, _p, _l, _i, _p, _i, _l, _p]),
+    "icsa_mx_linear_workspace_size": (_l, [_l, _i, _i, _i]),
+    "icsa_mx_linear": (_i, [
+        _p, _p, _i, _l, _p, _p,
+        _p, _i, _i, _l, _i, _i, _p, _p,
+        _i, _l, _p, _l, _p]),
+    "icsa_masked_attn_workspace_size": (_l, [_i, _i, _i, _i, _i, _i]),
+    "icsa_masked_attn": (_i, [
+        _p, _l, _l, _l,
+        _p, _l, _l, _l,
+        _p, _l, _l, _l,
+        _i, _i, _i, _i, _i, _i,
+        _p, _p, _i, _i, _p,
+        _f, _f, _p, _i,
+        _p, _i, _l, _l, _l,
+        _p, _l, _p]),
     "icsa_last_error": (ctypes.c_char_p, []),
     "icsa_version": (_i, []),
 }

@@ -19,7 +19,8 @@ BUILD_DIR = os.path.join(CSRC_DIR, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libicsa.so")
 
 SOURCES = ["pool.hip", "compressed.hip", "newkv.hip", "gather.hip", "flash_attn.hip", "sparse_attn.hip", "sparse_bwd.hip",
-           "wan_qk.hip", "wan_block.hip", "api.hip"]
+           "wan_qk.hip", "wan_block.hip", "mx_quant.hip", "mx_gemm.hip", "masked_attn.hip",
+           "api.hip"]
 
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",

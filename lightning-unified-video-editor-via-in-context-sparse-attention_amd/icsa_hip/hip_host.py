@@ -10,6 +10,8 @@
   TKV // 64, keys past TKV masked out of the exact part (triton_kernels.py:185, 489-539).
 * :func:`flash_attn_func` mirrors the call made at editing_sparse_attention.py:211-215
   (flash-attn's ``flash_attn_func(q, k, v)``, dense non-causal, default scale).
+* :func:`masked_attn_func`: dense attention under document, causal and prefix masks, with capped
+  scores, a bias by distance and grouped heads.
 * :func:`pool` and :func:`gather_kv` expose stage 1 and the new-KV gather.
 
 Work is enqueued on ``torch.cuda.current_stream()``; scratch memory comes from torch's
@@ -369,6 +371,87 @@ def flash_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dropout_p
             ptr(out), dtype_code(out), *out.stride()[:3],
             ptr(ws), ws_bytes, stream_ptr(q.device))
     _lib.check("icsa_flash_attn", rc)
+    return out
+
+
+def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_starts: torch.Tensor = None,
+                     k_starts: torch.Tensor = None, causal: bool = False, prefix: torch.Tensor = None,
+                     softcap: float = 0.0, bias: torch.Tensor = None, softmax_scale: float = None,
+                     out_dtype: torch.dtype = None) -> torch.Tensor:
+    """Dense attention under masks: q [B, Sq, H, D], k / v [B, Sk, Hk, D] bfloat16, D 64 or 128, H a
+    multiple of Hk (the H / Hk heads of a group share a key head).  Returns [B, Sq, H, D], bfloat16
+    unless ``out_dtype=torch.float32``.
+
+    Args:
+        q_starts, k_starts: int32 [B, N + 1], not decreasing.  Document n of batch row b has
+            queries ``q_starts[b, n] .. q_starts[b, n + 1] - 1`` and the keys of ``k_starts`` likewise,
+            and sees its own keys alone.  Rows in front of the first and behind the last document see
+            nothing.  Without them everything is one document.  Values past the lengths are clamped on the
+            GPU (no host check: they may change under a captured graph).
+        causal: query i of a document of Lq queries and Lk keys stands at key ``p_i = i + Lk - Lq`` and
+            sees the keys up to it.
+        prefix: int32 [B, N] ([B] without documents), with ``causal``: a document's first
+            keys that all of its queries see.
+        softcap: scores become ``softcap * tanh(score / softcap)``; 0 leaves them.
+        bias: float32 [H, 2 R + 1], added to the (capped) scores: ``bias[h, clamp(j - p_i, -R, R) + R]``.
+        softmax_scale: default ``D ** -0.5``.
+
+    A query that sees nothing gets zeros; NaN and infinities in keys and values reach only the
+    queries that see them.  An inference operator: under an enabled grad mode an input that requires a
+    gradient is refused."""
+    _require(all(isinstance(t, torch.Tensor) and t.dtype == torch.bfloat16 for t in (q, k, v)), "q, k, v must be bfloat16")
+    _require(q.is_cuda and k.device == q.device and v.device == q.device, "q, k, v must be on the same GPU")
+    _require(q.ndim == 4 and k.ndim == 4 and k.shape == v.shape and q.shape[0] == k.shape[0] and
+             q.shape[3] == k.shape[3], "q [B, Sq, H, D], k/v [B, Sk, Hk, D] expected")
+    B, Sq, H, D = q.shape
+    Sk, Hk = k.shape[1:3]
+    _require(D in (64, 128), "D must be 64 or 128")
+    _require(B > 0 and Hk > 0 and H > 0 and H % Hk == 0, "H must be a multiple of Hk")
+    _require(not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (q, k, v, bias)),
+             "masked_attn_func has no backward: call it under torch.no_grad()")
+    _require((q_starts is None) == (k_starts is None), "q_starts and k_starts must be given together")
+    docs = 1
+    if q_starts is not None:
+        _require(q_starts.ndim == 2 and q_starts.shape[0] == B and q_starts.shape[1] >= 2 and
+                 q_starts.shape == k_starts.shape, "q_starts and k_starts must be [B, N + 1]")
+        docs = q_starts.shape[1] - 1
+    _require(prefix is None or causal, "prefix needs causal=True")
+    if prefix is not None:
+        _require(tuple(prefix.shape) == (B, docs) or (docs == 1 and tuple(prefix.shape) == (B,)),
+                 f"prefix must be [{B}, {docs}]")
+    ints = []
+    for name, t in (("q_starts", q_starts), ("k_starts", k_starts), ("prefix", prefix)):
+        if t is not None:
+            _require(t.dtype == torch.int32 and t.device == q.device, f"{name} must be int32 on the GPU of q")
+            t = t.contiguous()
+        ints.append(t)
+    _require(softcap >= 0, "softcap must not be negative")
+    radius = 0
+    if bias is not None:
+        _require(bias.dtype == torch.float32 and bias.device == q.device and bias.ndim == 2 and bias.shape[0] == H and
+                 bias.shape[1] % 2 == 1, f"bias must be float32 [{H}, 2 R + 1] on the GPU of q")
+        radius = bias.shape[1] // 2
+        bias = bias.contiguous()
+    out_dtype = out_dtype or torch.bfloat16
+    _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be bfloat16 or float32")
+    q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in map(inner_contiguous, (q, k, v)))
+    out = torch.empty(B, Sq, H, D, dtype=out_dtype, device=q.device)
+    L = _lib.lib()
+    ws_bytes = L.icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D)
+    if ws_bytes < 0:
+        raise _lib.IcsaError("icsa_masked_attn_workspace_size", int(ws_bytes))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    with on_device(q.device):
+        rc = L.icsa_masked_attn(
+            ptr(q), *q.stride()[:3],
+            ptr(k), *k.stride()[:3],
+            ptr(v), *v.stride()[:3],
+            B, Sq, Sk, H, Hk, D,
+            ptr(ints[0]), ptr(ints[1]), docs, int(causal), ptr(ints[2]),
+            float(D ** -0.5 if softmax_scale is None else softmax_scale), float(softcap), ptr(bias), radius,
+            ptr(out), dtype_code(out), *out.stride()[:3],
+            ptr(ws), ws_bytes, stream_ptr(q.device))
+    _lib.check("icsa_masked_attn", rc)
     return out
 
 
