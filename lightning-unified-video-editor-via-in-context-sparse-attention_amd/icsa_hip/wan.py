@@ -22,7 +22,9 @@ import torch.nn as nn
 
 from . import _lib
 from .editing_sparse_attention import Backend, _editing_sparse_attention_hip, derived_sizes
-from .hip_host import _require, dtype_code, on_device, ptr, stream_ptr
+from .hip_host import (_require, dtype_code, flash_attn_func, masked_attn_func, on_device, ptr,
+                       stream_ptr)
+from .mx import MXLinear, mx_quantize
 
 _rope_cache: dict = {}
 
@@ -263,9 +265,9 @@ class WanSelfAttention(nn.Module):
     capture = None    # a dict here receives the workspace views (decisions) of the next call
 
     def forward(self, x, seq_lens, grid_sizes, source_video_grid_sizes, TAG, freqs):
-        b, s = x.shape[:2]
+        xm = _linear_input(x, self.q, self.k, self.v)
         res = wan_self_attention_core(
-            self.q(x), self.k(x), self.v(x), self.alpha_1(x), self.norm_q.weight,
+            self.q(xm), self.k(xm), self.v(xm), self.alpha_1(x), self.norm_q.weight,
             self.norm_k.weight, grid_sizes, source_video_grid_sizes, TAG, freqs,
             self.num_heads, self.eps, out_dtype=x.dtype, keep_workspace=self.capture is not None)
         if self.capture is not None:
@@ -273,6 +275,11 @@ class WanSelfAttention(nn.Module):
         # the kernels add the residual in f32 and round once at the store, which equals the
         # reference's f32 result cast to the projection's dtype
         return self.o(res.flatten(2))
+
+
+def _linear_input(x, *layers):
+    """x, in 4 bits where all of the layers that read it are MXLinear: quantised once for them."""
+    return mx_quantize(x) if all(isinstance(m, MXLinear) for m in layers) else x
 
 
 class WanLayerNorm(nn.LayerNorm):
@@ -286,7 +293,9 @@ class WanLayerNorm(nn.LayerNorm):
 class WanT2VCrossAttention(nn.Module):
     """WanT2VCrossAttention (model.py:180-188): q / k RMSNorm through the producer in its
     single-tensor, unrotated mode, dense attention over the text tokens through
-    ``icsa_flash_attn``.  Same parameters as the reference class."""
+    ``icsa_flash_attn``, or with ``context_lens`` (int [B]: each batch row's real text tokens; a
+    row of length 0 gets zeros) through ``icsa_masked_attn``.  Same parameters as the reference
+    class."""
 
     def __init__(self, dim, num_heads, window_size=(-1, -1), qk_norm=True, eps=1e-6):
         super().__init__()
@@ -305,17 +314,25 @@ class WanT2VCrossAttention(nn.Module):
         self.norm_k = WanRMSNorm(dim, eps=eps)
 
     def forward(self, x, context, context_lens=None):
-        _require(context_lens is None, "variable text lengths (context_lens) are not supported")
         b = x.shape[0]
+        if context_lens is not None:
+            lens = torch.as_tensor(context_lens, device=x.device).to(torch.int32)
+            _require(tuple(lens.shape) == (b,), "context_lens must hold one length a batch row")
         none = [(0, 0, 0)] * b
         no_rope = _identity_freqs(self.head_dim, x.device)
         q = wan_qk_prologue(self.q(x), None, self.norm_q.weight, None, none, none, 0, no_rope,
                             self.num_heads, eps=self.eps, want_sums=False)[0]
-        k = wan_qk_prologue(self.k(context), None, self.norm_k.weight, None, none, none, 0,
+        cm = _linear_input(context, self.k, self.v)
+        k = wan_qk_prologue(self.k(cm), None, self.norm_k.weight, None, none, none, 0,
                             no_rope, self.num_heads, eps=self.eps, want_sums=False)[0]
-        v = self.v(context).view(b, -1, self.num_heads, self.head_dim).to(torch.bfloat16)
-        from .hip_host import flash_attn_func
-        y = flash_attn_func(q, k, v)
+        v = self.v(cm).view(b, -1, self.num_heads, self.head_dim).to(torch.bfloat16)
+        if context_lens is None:
+            y = flash_attn_func(q, k, v)
+        else:                                       # one document a batch row: its text's real tokens
+            zero = torch.zeros_like(lens)
+            with torch.no_grad():
+                y = masked_attn_func(q, k, v, q_starts=torch.stack([zero, torch.full_like(lens, q.shape[1])], 1),
+                                     k_starts=torch.stack([zero, lens], 1))
         return self.o(y.flatten(2).to(x.dtype))
 
 
@@ -385,10 +402,27 @@ class WanAttentionBlock(nn.Module):
         """self.ffn(h) (Linear, GELU(tanh), Linear; model.py:243-245) with the bias and the
         GELU applied in the first GEMM's epilogue, on its fp32 accumulator: no separate
         elementwise pass over the [tokens, ffn_dim] hidden.  The reference rounds the first
-        Linear's output to bf16 before its GELU; the epilogue rounds once, after it."""
+        Linear's output to bf16 before its GELU; the epilogue rounds once, after it.  In 4 bits the
+        hidden row goes from that accumulator to its codes, which the second product reads."""
         lin0, lin2 = self.ffn[0], self.ffn[2]
+        if isinstance(lin0, MXLinear):
+            return lin2(lin0(h, activation='gelu_tanh', out_dtype='mxfp4'))
         f = torch._addmm_activation(lin0.bias, h.reshape(-1, h.shape[-1]), lin0.weight.t(), use_gelu=True)
         return torch.nn.functional.linear(f, lin2.weight, lin2.bias).view(*h.shape[:-1], lin2.out_features)
+
+
+def quantize_linears(block: WanAttentionBlock) -> WanAttentionBlock:
+    """Replaces a block's q / k / v / o projections (self and cross attention) and both FFN layers by
+    :class:`MXLinear` of their weights, on the GPU: their weights take 17/64 of
+    the bf16 memory, and the products run on the block-scaled matrix instructions.  alpha_1 (one output) stays."""
+    for att in (block.self_attn, block.cross_attn):
+        for name in ("q", "k", "v", "o"):
+            if not isinstance(getattr(att, name), MXLinear):
+                setattr(att, name, MXLinear(getattr(att, name)))
+    for i in (0, 2):
+        if not isinstance(block.ffn[i], MXLinear):
+            block.ffn[i] = MXLinear(block.ffn[i])
+    return block
 
 
 def sinusoidal_embedding_1d(dim, position):
@@ -486,6 +520,13 @@ class WanModel(nn.Module):
                 nn.init.normal_(m.weight, std=0.02)
         nn.init.zeros_(self.head.head.weight)
 
+    def quantize_linears(self):
+        """The blocks' projections and FFN layers in 4 bits from here on (inference; see
+        :func:`quantize_linears`).  Returns the model."""
+        for block in self.blocks:
+            quantize_linears(block)
+        return self
+
     def _patchify(self, conv, u):
         """Conv3d with kernel = stride as a GEMM: [C, F, H, W] -> [F*(H/ph)*(W/pw), dim]."""
         pf, ph, pw = self.patch_size
@@ -537,4 +578,4 @@ class WanModel(nn.Module):
 
 __all__ = ["rope_params", "wan_freqs", "rope_tables", "wan_qk_prologue", "wan_self_attention_core",
            "ln_modulate", "WanSelfAttention", "WanT2VCrossAttention", "WanAttentionBlock",
-           "WanRMSNorm", "WanLayerNorm", "Head", "WanModel", "sinusoidal_embedding_1d"]
+           "WanRMSNorm", "WanLayerNorm", "Head", "WanModel", "quantize_linears", "sinusoidal_embedding_1d"]
