@@ -13,12 +13,25 @@
 
 namespace {
 
-// 8 values of a row from k on, zeros from K on.  kVec: the row starts on 16 bytes; a 16-byte
-// piece that K cuts is read value by value, so that nothing past the row is touched.
-template <typename T, bool kVec>
+// Rows may start at any element: vectors of the element's alignment (global memory takes them)
+typedef bf16x8 bf16x8_a2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+typedef floatx4 floatx4_a4 __attribute__((aligned(4)));
+
+// 8 values of a row from k on, zeros from K on; where K cuts them, value by value, so that nothing past the
+// row is touched.
+template <typename T>
 __device__ __forceinline__ void load8_row(const T* row, int k, int K, float v[8]) {
-  if (kVec && k + 8 <= K) {
-    load8_f32<T>(row + k, v);
+  if (k + 8 <= K) {
+    if constexpr (sizeof(T) == 2) {
+      const bf16x8 x = *reinterpret_cast<const bf16x8_a2*>(row + k);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+    } else {
+      const floatx4 a = *reinterpret_cast<const floatx4_a4*>(row + k), b = *reinterpret_cast<const floatx4_a4*>(row + k + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+    }
     return;
   }
 #pragma unroll
@@ -27,7 +40,7 @@ __device__ __forceinline__ void load8_row(const T* row, int k, int K, float v[8]
 
 }  // namespace
 
-template <typename T, bool kVec>
+template <typename T>
 __global__ void __launch_bounds__(MXQ_THREADS) icsa_mx_quantize_kernel(MxQuantParams p) {
   const int lane = threadIdx.x & 63;
   const int Kp = mx_padded(p.K), per_row = (Kp + MXQ_WAVE_K - 1) / MXQ_WAVE_K;
@@ -42,7 +55,7 @@ __global__ void __launch_bounds__(MXQ_THREADS) icsa_mx_quantize_kernel(MxQuantPa
     const int64_t u = first + i;
     row[i] = u / per_row;
     k[i] = (int)(u % per_row) * MXQ_WAVE_K + 8 * lane;
-    if (u < pieces) load8_row<T, kVec>(reinterpret_cast<const T*>(p.x) + row[i] * p.x_ss, k[i], p.K, v[i]);
+    if (u < pieces) load8_row<T>(reinterpret_cast<const T*>(p.x) + row[i] * p.x_ss, k[i], p.K, v[i]);
   }
 #pragma unroll
   for (int i = 0; i < MXQ_AHEAD; ++i) {
@@ -72,23 +85,16 @@ hipError_t launch_mx_quantize(const MxQuantParams& p, hipStream_t stream) {
   const int64_t per_wg = (MXQ_THREADS / 64) * MXQ_AHEAD;
   const int64_t grid = (pieces + per_wg - 1) / per_wg;
   if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-  const int es = p.x_dtype == ICSA_DT_F32 ? 4 : 2;
-  const bool vec = (reinterpret_cast<uintptr_t>(p.x) % 16 == 0) && (p.x_ss * es) % 16 == 0;
   const dim3 g((unsigned)grid), b(MXQ_THREADS);
-  if (es == 4) {
-    if (vec) hipLaunchKernelGGL((icsa_mx_quantize_kernel<float, true>), g, b, 0, stream, p);
-    else hipLaunchKernelGGL((icsa_mx_quantize_kernel<float, false>), g, b, 0, stream, p);
-  } else {
-    if (vec) hipLaunchKernelGGL((icsa_mx_quantize_kernel<bf16, true>), g, b, 0, stream, p);
-    else hipLaunchKernelGGL((icsa_mx_quantize_kernel<bf16, false>), g, b, 0, stream, p);
-  }
+  if (p.x_dtype == ICSA_DT_F32) hipLaunchKernelGGL(icsa_mx_quantize_kernel<float>, g, b, 0, stream, p);
+  else hipLaunchKernelGGL(icsa_mx_quantize_kernel<bf16>, g, b, 0, stream, p);
   return hipGetLastError();
 }
 
 // Values of 8 codes a lane.  A code's value times a power of two has at most two significant
 // bits, so bf16 holds every value (2^-128, the least, is a bf16 subnormal); the product with a
 // subnormal scale is exact in f32, and its upper half is the bf16.
-template <typename T, bool kVec>
+template <typename T>
 __global__ void __launch_bounds__(MXQ_THREADS) icsa_mx_dequantize_kernel(MxDequantParams p) {
   const int lane = threadIdx.x & 63;
   const int Kp = mx_padded(p.K), per_row = (p.K + MXQ_WAVE_K - 1) / MXQ_WAVE_K;
@@ -126,17 +132,17 @@ __global__ void __launch_bounds__(MXQ_THREADS) icsa_mx_dequantize_kernel(MxDequa
       unsigned short h[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[e] = (unsigned short)(__float_as_uint(v[e]) >> 16);
-      if (kVec && k[i] + 8 <= p.K) {
-        *reinterpret_cast<u32x4*>(dst) = u32x4{h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16,
+      if (k[i] + 8 <= p.K) {
+        *reinterpret_cast<u32x4_a2*>(dst) = u32x4{h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16,
                                                h[4] | (unsigned)h[5] << 16, h[6] | (unsigned)h[7] << 16};
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (k[i] + e < p.K) reinterpret_cast<unsigned short*>(dst)[e] = h[e];
       }
-    } else if (kVec && k[i] + 8 <= p.K) {
-      *reinterpret_cast<floatx4*>(dst) = floatx4{v[0], v[1], v[2], v[3]};
-      *reinterpret_cast<floatx4*>(dst + 4) = floatx4{v[4], v[5], v[6], v[7]};
+    } else if (k[i] + 8 <= p.K) {
+      *reinterpret_cast<floatx4_a4*>(dst) = floatx4{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<floatx4_a4*>(dst + 4) = floatx4{v[4], v[5], v[6], v[7]};
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -151,15 +157,8 @@ hipError_t launch_mx_dequantize(const MxDequantParams& p, hipStream_t stream) {
   const int64_t per_wg = (MXQ_THREADS / 64) * MXQ_AHEAD;
   const int64_t grid = (pieces + per_wg - 1) / per_wg;
   if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-  const int es = p.out_dtype == ICSA_DT_F32 ? 4 : 2;
-  const bool vec = (reinterpret_cast<uintptr_t>(p.out) % 16 == 0) && (p.o_ss * es) % 16 == 0;
   const dim3 g((unsigned)grid), b(MXQ_THREADS);
-  if (es == 4) {
-    if (vec) hipLaunchKernelGGL((icsa_mx_dequantize_kernel<float, true>), g, b, 0, stream, p);
-    else hipLaunchKernelGGL((icsa_mx_dequantize_kernel<float, false>), g, b, 0, stream, p);
-  } else {
-    if (vec) hipLaunchKernelGGL((icsa_mx_dequantize_kernel<bf16, true>), g, b, 0, stream, p);
-    else hipLaunchKernelGGL((icsa_mx_dequantize_kernel<bf16, false>), g, b, 0, stream, p);
-  }
+  if (p.out_dtype == ICSA_DT_F32) hipLaunchKernelGGL(icsa_mx_dequantize_kernel<float>, g, b, 0, stream, p);
+  else hipLaunchKernelGGL(icsa_mx_dequantize_kernel<bf16>, g, b, 0, stream, p);
   return hipGetLastError();
 }
