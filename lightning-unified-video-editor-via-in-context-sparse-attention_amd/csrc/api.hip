@@ -668,7 +668,7 @@ int icsa_mx_dequantize(const void* codes, const void* scales, int64_t M, int K, 
 
 int64_t icsa_mx_linear_workspace_size(int64_t M, int N, int K, int x_dtype) {
   if (M < 0 || N <= 0 || K <= 0) return -1;
-  if (x_dtype == ICSA_MXFP4) return 0;
+  if (x_dtype == ICSA_MXFP4 || mx_rows_takes_raw(M, K)) return 0;
   return align256(icsa_mx_codes_size(M, K)) + align256(icsa_mx_scales_size(M, K));
 }
 
@@ -704,6 +704,12 @@ int icsa_mx_linear(const void* x, const void* x_scales, int x_dtype, int64_t x_s
   p.out = out; p.out_scales = reinterpret_cast<unsigned char*>(out_scales);
   p.out_kind = out_dtype == ICSA_MXFP4 ? MX_OUT_MXFP4 : out_dtype == ICSA_F32 ? MX_OUT_F32 : MX_OUT_BF16;
   p.o_ss = out_dtype == ICSA_MXFP4 ? mx_padded(N) / 2 : o_ss;
+  p.x_raw = x; p.x_dtype = x_dtype; p.x_ss = x_ss; p.K = K;
+  if (x_dtype != ICSA_MXFP4 && mx_rows_takes_raw(M, K)) {
+    ICSA_HIP_TRY(launch_mx_rows(p, reinterpret_cast<hipStream_t>(stream_)), "mx product of few rows");
+    return ICSA_OK;
+  }
+  p.x_raw = nullptr;
   if (x_dtype != ICSA_MXFP4) {
     unsigned char* codes = reinterpret_cast<unsigned char*>(workspace);
     unsigned char* scales = codes + align256(icsa_mx_codes_size(M, K));

@@ -247,8 +247,14 @@ struct MxGemmParams {
   int gelu;
   void* out; int out_kind; int64_t o_ss;                   // MxOut; o_ss: element row stride (codes: Np / 2)
   unsigned char* out_scales;                               // [Np / 256, M, 8]
+  const void* x_raw; int x_dtype; int64_t x_ss; int K;     // x not quantised yet: see mx_rows_takes_raw
+  int m_first, m_last;                                     // token rows of a launch
 };
-hipError_t launch_mx_gemm(const MxGemmParams& p, hipStream_t stream);
+hipError_t launch_mx_gemm(MxGemmParams p, hipStream_t stream);
+// few token rows (mx_rows.hip)
+bool mx_rows_takes(int M, int N);
+bool mx_rows_takes_raw(int64_t M, int K);
+hipError_t launch_mx_rows(const MxGemmParams& p, hipStream_t stream);
 
 // ---------------------------------------------------------------- attention under masks (masked_attn.hip)
 #define MA_ROWS 128                  // rows (query, head of the group) of a workgroup

@@ -42,3 +42,48 @@ __device__ __forceinline__ unsigned mx_pack8(const float v[8]) {
   r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], 1.f, 3);
   return r;
 }
+
+// Rows may start at any element: vectors of the element's alignment (global memory takes them)
+typedef bf16x8 bf16x8_a2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+typedef bf16x4 bf16x4_a2 __attribute__((aligned(2)));
+typedef floatx4 floatx4_a4 __attribute__((aligned(4)));
+
+// 8 values of a row from k on, zeros from K on; where K cuts them, value by value, so that nothing past the
+// row is touched.
+template <typename T>
+__device__ __forceinline__ void load8_row(const T* row, int k, int K, float v[8]) {
+  if (k + 8 <= K) {
+    if constexpr (sizeof(T) == 2) {
+      const bf16x8 x = *reinterpret_cast<const bf16x8_a2*>(row + k);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+    } else {
+      const floatx4 a = *reinterpret_cast<const floatx4_a4*>(row + k), b = *reinterpret_cast<const floatx4_a4*>(row + k + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = k + i < K ? (float)row[k + i] : 0.f;
+}
+
+// Scale byte of a block whose 32 values four neighbouring lanes hold, 8 each; the magnitudes are
+// compared as f32 bit patterns without their sign, where NaN and infinity come out on top.
+__device__ __forceinline__ unsigned mx_quantize8(const float v[8]) {
+  unsigned amax = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(v[e]) & 0x7fffffffu);
+  amax = max(amax, (unsigned)__shfl_xor((int)amax, 1, 64));
+  amax = max(amax, (unsigned)__shfl_xor((int)amax, 2, 64));
+  return mx_scale_byte(amax);
+}
+// Their codes under that scale
+__device__ __forceinline__ unsigned mx_codes8(const float v[8], unsigned s) {
+  const float f = mx_inv_scale(s);
+  float t[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) t[e] = v[e] * f;
+  return s == 255 ? 0u : mx_pack8(t);
+}

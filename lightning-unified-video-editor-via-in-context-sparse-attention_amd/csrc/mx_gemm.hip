@@ -1,49 +1,29 @@
 // Product of microscaled 4-bit operands: y[m][n] = act(sum_k x[m][k] w[n][k] + bias[n]).
 //
-// v_mfma_scale_f32_32x32x64_f8f6f4 takes one block of 32 codes (16 bytes) and its scale byte from
-// each lane: lane l holds row l % 32, and k block l / 32 of the two that a step covers.  Which two blocks
-// of a row's group of eight go together is free as long as both operands agree: step s takes
-// blocks s (lanes 0-31) and 4 + s (lanes 32-63), so that a lane's four scale bytes of a group are
-// one aligned dword of the scale layout, picked by the instruction's own byte select.
+// A workgroup computes tiles of TN x TM outputs (n x m) over groups of 256 k, a full 128-byte line of every row, which arrive by
+// direct global->LDS loads.  16-byte chunk c of tile row r sits at chunk c ^ (r / 2 % 8): 16 consecutive rows' reads of one chunk
+// touch every bank once.  A group is 4 steps of 64 k.  The operands of a step are read from LDS while the one before
+// multiplies; the wait for the next group and the barrier come before the last step's products, whose operands are in
+// registers by then, so the matrix pipe runs through them, and the freed buffer takes the group kBufs further on, its loads spread
+// over that step and the next.  The stream of groups runs across a workgroup's tiles: the next tile's first groups arrive
+// while this one's outputs are written.
 //
-// The weights are the A operand: a lane then holds one token (accumulator column) and, of every 32
-// outputs, 4 groups of 4 consecutive ones.
-//
-// A workgroup of 4 waves computes TN x TM outputs (n x m) over tiles of 128 k (64 bytes of every row), which arrive by
-// direct global->LDS loads, three buffers.  16-byte chunk c of tile row r sits at chunk c ^ (r / 4 % 4): 16
-// consecutive rows' reads of one chunk touch every bank once.  A tile is 2 steps.  The operands of a step are read
-// while the one before multiplies; the wait for the next tile and the barrier come before the
-// second step's products, whose operands are in registers by then, so the matrix pipe runs through them, and the
-// freed buffer takes the tile three further on.  Two workgroups share a CU: one's waits, barriers and
-// epilogue run beside the other's products.
+// What bounds it: the loads into LDS.  Timing copies of an earlier form (128 x 256 tiles of 128 k, two workgroups a CU, 14,040 x 5,120
+// x 13,824): 553 us; without loads in the loop 379; with half of them 438; the same bytes in full 128-byte lines instead of
+// halves 460.  So: full lines, and the largest tile (256 x 256, 8 waves of 64 x 128, two a SIMD): a third fewer bytes an
+// operation, 478 us, 4.2 PFLOP/s; loads spread over two steps instead of one 454.  65,520 x 13,824 x 5,120 with GELU: 2.41 ms,
+// 3.84 PFLOP/s, 2.7 times the bf16 library product's rate at this size (6.46 ms); about 7 of a tile's 45 us are the GELU (two
+// transcendentals an output, nothing to overlap them with).  Without loads in the loop it takes 2.16 ms.
+#include <algorithm>
 #include <type_traits>
 
-#include "attn_tile.h"
-#include "icsa_kernels.h"
-#include "mx_common.h"
+#include "mx_tile.h"
 
-#define MXG_THREADS 256
-#define MXG_ROW 64                                     // bytes of codes of a tile row (128 k)
-#define MXG_BUFS 3
+#define MXG_STAGE 2048                                 // bytes of output staging of a wave
+#define MXG_CUS 256
+#define MXG_BAND 4                                     // token tiles that go together in the order; 2.56 ms against 2.69 with 8
 
 namespace {
-
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-// byte `kSel` of each scale register, both operands e2m1 (format 4)
-template <int kSel>
-__device__ __forceinline__ floatx16 mx_mfma(i32x4 a, i32x4 b, floatx16 c, int sa, int sb) {
-  const i32x8 a8 = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, b8 = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a8, b8, c, 4, 4, kSel, sa, kSel, sb);
-}
-
-// gelu(t) = t / (1 + exp(-2 sqrt(2 / pi) (t + 0.044715 t^3))): no difference of near values on
-// either side of zero.  exp2 of a large argument is infinity and the factor 0.
-__device__ __forceinline__ float gelu_tanh(float t) {
-  const float u = t * fmaf(0.044715f * t, t, 1.f);
-  return t * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * (-2.f * 0.7978845608028654f * 1.4426950408889634f)));
-}
 
 // LDS DMA with a uniform byte offset
 __device__ __forceinline__ void lds_dma16s(unsigned lds_addr, int voff, u32x4 rs, int soff) {
@@ -51,309 +31,251 @@ __device__ __forceinline__ void lds_dma16s(unsigned lds_addr, int voff, u32x4 rs
                :: "s"(lds_addr), "v"(voff), "s"(rs), "s"(soff) : "memory", "m0");
 }
 
-// Outputs of a row that are written: in 4 bits its padding too
-__host__ __device__ __forceinline__ int out_columns(const MxGemmParams& p) {
-  return p.out_kind == MX_OUT_MXFP4 ? mx_padded(p.N) : p.N;
-}
-
-__device__ __forceinline__ float bias_at(const MxGemmParams& p, int n) {
-  if (p.bias == nullptr || n >= p.N) return 0.f;
-  return p.bias_dtype == ICSA_DT_F32 ? reinterpret_cast<const float*>(p.bias)[n]
-                                     : (float)reinterpret_cast<const bf16*>(p.bias)[n];
-}
-
-// Rows may start at any element: vectors of the element's alignment (global memory takes them)
-typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
-typedef floatx4 floatx4_a4 __attribute__((aligned(4)));
-
-// bias and activation of one 32 (n) x 32 (m) accumulator tile
-__device__ __forceinline__ void tile_values(const MxGemmParams& p, const floatx16& acc, const float* bias, float v[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = acc[i] + bias[i];
-  if (p.gelu) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = gelu_tanh(v[i]);
-  }
-}
-
-// The tile's outputs n0 .. n0 + 31 of token m (this lane's) in 4 bits
-__device__ __forceinline__ void store_mx(const MxGemmParams& p, float v[16], int n0, int m) {
-  const int hl = (threadIdx.x & 63) >> 5, Np = mx_padded(p.N);
-  unsigned amax = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if (n0 + 8 * (i >> 2) + 4 * hl + (i & 3) >= p.N) v[i] = 0.f;         // the padding: zeros
-    amax = max(amax, __float_as_uint(v[i]) & 0x7fffffffu);
-  }
-  const auto w = __builtin_amdgcn_permlane32_swap(amax, amax, false, false);
-  const unsigned s = mx_scale_byte(max(w[0], w[1]));
-  const float f = mx_inv_scale(s);
-  unsigned q[2];                                       // 4 groups of 4 codes: 16 bits each
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float t[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = v[8 * h + e] * f;
-    q[h] = s == 255 ? 0u : mx_pack8(t);
-  }
-  // lanes l and l ^ 32 hold alternating groups of 4 codes (hl = 0 first): lower lanes gather the
-  // block's first 16 codes, upper lanes the last 16
-  const auto x = __builtin_amdgcn_permlane32_swap(q[0], q[1], false, false);
-  const unsigned lo = x[0], hi = x[1];                 // this half's codes of groups 2 hl, 2 hl + 1: from hl = 0, 1
-  const u32x2 c = {(lo & 0xffffu) | hi << 16, lo >> 16 | (hi & 0xffff0000u)};
-  if (m < p.M && n0 < Np) {
-    *reinterpret_cast<u32x2*>(reinterpret_cast<unsigned char*>(p.out) + (int64_t)m * p.o_ss + n0 / 2 + 8 * hl) = c;
-    if (hl == 0)
-      p.out_scales[((int64_t)(n0 / MX_GROUP) * p.M + m) * MX_GROUP_BLOCKS + n0 / MX_BLOCK % MX_GROUP_BLOCKS] = (unsigned char)s;
-  }
-}
-
-__device__ __forceinline__ void store_f32(const MxGemmParams& p, const float v[16], int n0, int m) {
-  const int hl = (threadIdx.x & 63) >> 5;
-  if (m >= p.M) return;
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    const int n = n0 + 8 * g + 4 * hl;
-    float* dst = reinterpret_cast<float*>(p.out) + (int64_t)m * p.o_ss + n;
-    if (n + 4 <= p.N) *reinterpret_cast<floatx4_a4*>(dst) = floatx4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
-    else
-#pragma unroll
-      for (int e = 0; e < 4; ++e) if (n + e < p.N) dst[e] = v[4 * g + e];
-  }
-}
-
-// bf16 rows pass through 4 KB of the wave's LDS, 64 outputs of 32 tokens at a time, so that a store
-// instruction writes 8 full lines of 128 bytes.  16-byte chunk c of row r at c ^ (r / 2 % 8).
-__device__ __forceinline__ void stage_bf16(unsigned char* stage, const float v[16], int i) {
-  const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5;
-#pragma unroll
-  for (int pr = 0; pr < 2; ++pr) {                     // lane halves swap: outputs 8 (2 pr + hl) .. + 7
-    bf16x4 lo, hi;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) { lo[e] = (bf16)v[8 * pr + e]; hi[e] = (bf16)v[8 * pr + 4 + e]; }
-    const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-    const auto w0 = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
-    const auto w1 = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
-    *reinterpret_cast<u32x4*>(stage + li * 128 + (((4 * i + 2 * pr + hl) ^ ((li >> 1) & 7)) << 4)) = u32x4{w0[0], w1[0], w0[1], w1[1]};
-  }
-}
-__device__ __forceinline__ void store_staged(const MxGemmParams& p, const unsigned char* stage, int n0, int m0) {
-  const int lane = threadIdx.x & 63, n = n0 + 8 * (lane & 7);
-#pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int r = 8 * x + (lane >> 3), m = m0 + r;
-    const u32x4 c = *reinterpret_cast<const u32x4*>(stage + r * 128 + (((lane & 7) ^ ((r >> 1) & 7)) << 4));
-    bf16* dst = reinterpret_cast<bf16*>(p.out) + (int64_t)m * p.o_ss + n;
-    if (m < p.M && n + 8 <= p.N) *reinterpret_cast<u32x4_a2*>(dst) = c;
-    else if (m < p.M) {
-      const bf16x8 b = __builtin_bit_cast(bf16x8, c);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) if (n + e < p.N) dst[e] = b[e];
-    }
-  }
-}
-
 }  // namespace
 
-// WN x WM accumulator tiles of 32 x 32 a wave, waves 2 x 2: TN = 64 WN outputs, TM = 64 WM tokens
-template <int WN, int WM, int kOut>
-__global__ void __launch_bounds__(MXG_THREADS, 2) icsa_mx_gemm_kernel(MxGemmParams p) {
-  constexpr int TN = 64 * WN, TM = 64 * WM, kBuf = (TN + TM) * MXG_ROW, kScales = (TN + TM) * MX_GROUP_BLOCKS;
-  constexpr int kLoads = (TN + TM) / 64;                               // code loads of a wave and tile: 16 rows each
-  constexpr int kScaleLoads = (TN + TM) / 128;                         // scale loads of a wave and group: 32 rows each
+// WN x WM accumulator tiles of 32 x 32 a wave, NN x NM waves: TN = 32 WN NN outputs, TM = 32 WM NM tokens
+template <int WN, int WM, int NN, int NM, int kBufs, int kOut>
+__global__ void __launch_bounds__(64 * NN * NM, 2) icsa_mx_gemm_kernel(MxGemmParams p) {
+  constexpr int TN = 32 * WN * NN, TM = 32 * WM * NM, kWaves = NN * NM, kRows = TN + TM;
+  constexpr int kCodes = kRows * MXG_LINE, kBuf = kCodes + kRows * MX_GROUP_BLOCKS;
+  constexpr int kCodeLoads = kRows / 8 / kWaves;                       // of a wave and group: 8 rows each
+  constexpr int kScaleLoads = kRows / 32 / kWaves;                     // 32 rows each
+  constexpr int kLoads = kCodeLoads + kScaleLoads, kLoadsW = TN / 8 / kWaves;
+  constexpr int kProd = WN * WM, kOps = WN + WM;
+  constexpr int kFirst = (kLoads + 2) / 4;                             // loads issued in the step behind the barrier
+  static_assert(kCodeLoads * 8 * kWaves == kRows && kScaleLoads * 32 * kWaves == kRows && kLoadsW * 8 * kWaves == TN, "whole loads");
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wn = wave >> 1, wm = wave & 1;
+  const int wn = wave / NM, wm = wave % NM;
 
-  // tile order: 8 token tiles at a time, output tiles outermost among them: the workgroups that an
-  // XCD runs together share few token and weight tiles
-  const int tiles_n = (out_columns(p) + TN - 1) / TN, tiles_m = (p.M + TM - 1) / TM;
-  const int w = xcd_remap(blockIdx.x, tiles_n * tiles_m);
-  if (w < 0) return;
-  const int band = w / (8 * tiles_n), in_band = w - band * 8 * tiles_n;
-  const int rows = min(8, tiles_m - band * 8);
-  const int m0 = (band * 8 + in_band % rows) * TM, n0 = in_band / rows * TN;
+  // ---- this workgroup's tiles ----  each XCD has one run of the tile order, its workgroups take turns.  In the order,
+  // MXG_BAND token tiles go together, output tiles outermost among them: what an XCD runs at a time
+  // shares few token and weight tiles
+  const int tiles_n = (out_columns(p) + TN - 1) / TN, tiles_m = (p.m_last - p.m_first + TM - 1) / TM, n_work = tiles_n * tiles_m;
+  const int per_xcd = (n_work + 7) / 8, slots = gridDim.x / 8;
+  const int w_end = min(n_work, ((int)blockIdx.x % 8 + 1) * per_xcd);
+  int w = (int)blockIdx.x % 8 * per_xcd + (int)blockIdx.x / 8;
+  if (w >= w_end) return;
 
   // ---- loads ----  rows are checked by the resources' ranges (in the lane's offset alone: k, which is
   // always inside a row, is the scalar offset)
-  const int64_t line = (int64_t)p.groups * (MX_GROUP / 2);             // bytes of a row of codes
-  const u32x4 rs_w = dma_rsrc(p.w + n0 * line, min(TN, p.N - n0) * line);
-  const u32x4 rs_x = dma_rsrc(p.x + m0 * line, min(TM, p.M - m0) * line);
-  const unsigned lds0 = lds_u32(smem), lds_scales = lds0 + MXG_BUFS * kBuf;
-  const int lr = lane >> 2, lchunk = ((lane & 3) ^ ((lr >> 2) & 3)) << 4;
-  int ofs[kLoads];
+  const int64_t line = (int64_t)p.groups * MXG_LINE;                   // bytes of a row of codes
+  int ofs[kCodeLoads];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i)
-    ofs[i] = (int)(((i < WN ? wave * 16 * WN + 16 * i : wave * 16 * WM + 16 * (i - WN)) + lr) * line) + lchunk;
-  const int n_tiles = 2 * p.groups;
-  // past the last tile: an empty range, into a buffer that nobody reads any more
-  auto load_codes = [&](int t, unsigned buf, int i) __attribute__((always_inline)) {
-    const bool is_w = i < WN;
-    u32x4 rs = is_w ? rs_w : rs_x;
-    rs[2] = t < n_tiles ? rs[2] : 0;
-    const int row = is_w ? wave * 16 * WN + 16 * i : TN + wave * 16 * WM + 16 * (i - WN);
-    lds_dma16s(buf + row * MXG_ROW, ofs[i], rs, t * MXG_ROW);
-  };
-  // a group's scales, with its first tile: 32 rows a load (4 bytes a lane: the range ends at a row, 8 bytes)
-  unsigned long long s_ptr[kScaleLoads];
-  unsigned s_len[kScaleLoads], s_step[kScaleLoads];
-#pragma unroll
-  for (int i = 0; i < kScaleLoads; ++i) {
-    const int at = 32 * (wave * kScaleLoads + i);
-    const bool tok = at >= TN;
-    const int R = tok ? p.M : p.N, r0 = tok ? m0 + at - TN : n0 + at;
-    const u32x4 rs = dma_rsrc((tok ? p.x_scales : p.w_scales) + (int64_t)r0 * MX_GROUP_BLOCKS, (int64_t)min(32, R - r0) * MX_GROUP_BLOCKS);
-    s_ptr[i] = (unsigned long long)rs[1] << 32 | rs[0];
-    s_len[i] = rs[2];
-    s_step[i] = (unsigned)R * MX_GROUP_BLOCKS;
+  for (int i = 0; i < kCodeLoads; ++i) {
+    const int r = (i < kLoadsW ? wave * kLoadsW + i : wave * (kCodeLoads - kLoadsW) + i - kLoadsW) * 8 + (lane >> 3);
+    ofs[i] = (int)(r * line) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
   }
-  auto load_scales = [&](int g, int i) __attribute__((always_inline)) {      // called for g = 0, 1, 2, ...
-    const u32x4 rs = {(unsigned)s_ptr[i], (unsigned)(s_ptr[i] >> 32), g < p.groups ? s_len[i] : 0, 0x00020000u};
-    lds_dma4(lds_scales + (g & 1) * kScales + 256 * (wave * kScaleLoads + i), 4 * lane, rs);
-    s_ptr[i] += s_step[i];
+  // what a tile is loaded from: [0] weights' codes, [1] tokens' codes, [2 ..] this wave's scale loads (32 rows; 4 bytes a
+  // lane, as a range ends at a row's 8 bytes)
+  struct Source {
+    unsigned long long ptr[2 + kScaleLoads];
+    unsigned len[2 + kScaleLoads];
+    int m0, n0;
+  };
+  auto source = [&](int t) __attribute__((always_inline)) {            // of tile t (behind the last: empty ranges)
+    const int band = t / (MXG_BAND * tiles_n), in_band = t - band * MXG_BAND * tiles_n;
+    const int rows = max(1, min(MXG_BAND, tiles_m - band * MXG_BAND));
+    Source s;
+    s.m0 = __builtin_amdgcn_readfirstlane(p.m_first + (band * MXG_BAND + in_band % rows) * TM);      // (quotients and clamps are vector instructions)
+    s.n0 = __builtin_amdgcn_readfirstlane(in_band / rows * TN);
+    auto range = [&](int x, const unsigned char* base, int64_t row_bytes, int r0, int n) {
+      s.ptr[x] = (unsigned long long)base + (t < w_end ? r0 * row_bytes : 0);
+      s.len[x] = (unsigned)__builtin_amdgcn_readfirstlane(t < w_end ? max(n, 0) * (int)row_bytes : 0);
+    };
+    range(0, p.w, line, s.n0, min(TN, p.N - s.n0));
+    range(1, p.x, line, s.m0, min(TM, p.m_last - s.m0));
+#pragma unroll
+    for (int i = 0; i < kScaleLoads; ++i) {
+      const int at = 32 * (wave * kScaleLoads + i);
+      const bool tok = at >= TN;
+      const int r0 = tok ? s.m0 + at - TN : s.n0 + at;
+      range(2 + i, tok ? p.x_scales : p.w_scales, MX_GROUP_BLOCKS, r0, min(32, (tok ? p.m_last : p.N) - r0));
+    }
+    return s;
+  };
+  const unsigned lds0 = lds_u32(smem);
+  Source src = source(w), nsrc = source(w + slots);                    // of the load cursor's tile, and of the one after it
+  int lg = 0;                                                          // its group
+  auto load = [&](unsigned buf, int i) __attribute__((always_inline)) {
+    const int x = i < kLoadsW ? 0 : i < kCodeLoads ? 1 : 2 + i - kCodeLoads;
+    const u32x4 rs = {(unsigned)src.ptr[x], (unsigned)(src.ptr[x] >> 32) & 0xffffu, src.len[x], 0x00020000u};
+    if (i < kCodeLoads) {
+      const int row = i < kLoadsW ? (wave * kLoadsW + i) * 8 : TN + (wave * (kCodeLoads - kLoadsW) + i - kLoadsW) * 8;
+      lds_dma16s(buf + row * MXG_LINE, ofs[i], rs, lg * MXG_LINE);
+    } else {
+      lds_dma4(buf + kCodes + 256 * (wave * kScaleLoads + i - kCodeLoads), 4 * lane, rs);
+    }
+  };
+  auto advance = [&]() __attribute__((always_inline)) {                // by selects: the loop's body stays one block
+    ++lg;
+    const bool wrap = lg == p.groups;
+    lg = wrap ? 0 : lg;
+#pragma unroll
+    for (int x = 0; x < 2 + kScaleLoads; ++x) {
+      if (x >= 2) {
+        const int at = 32 * (wave * kScaleLoads + x - 2);
+        src.ptr[x] += (unsigned)(at >= TN ? p.M : p.N) * (unsigned long long)MX_GROUP_BLOCKS;
+      }
+      src.ptr[x] = wrap ? nsrc.ptr[x] : src.ptr[x];
+      src.len[x] = wrap ? nsrc.len[x] : src.len[x];
+    }
   };
 
-  floatx16 acc[WN][WM] = {};
+  floatx16 acc[WN][WM];
   i32x4 a[2][WN], b[2][WM];
-  u32x2 ga[WN], gb[WM];                                                // a group's scales
-  int sa[WN], sb[WM];                                                  // a tile's: bytes 0, 1 for steps 0, 1
-  int rd[2];                                                           // operand read offsets of steps 0, 1; + 32 rows a sub-tile
+  int sa[WN], sb[WM], na[WN], nb[WM];                                  // scales: byte s for step s; of this group, the next
+  int rd[4];                                                           // operand read offsets of the steps; + 32 rows a sub-tile
 #pragma unroll
-  for (int s = 0; s < 2; ++s) rd[s] = li * MXG_ROW + (((2 * hl + s) ^ ((li >> 2) & 3)) << 4);
-  const unsigned char* base = smem;                                    // of the tile that is read
-  auto read_a = [&](int s, int i) { a[s][i] = *reinterpret_cast<const i32x4*>(base + rd[s] + (wn * WN + i) * 32 * MXG_ROW); };
-  auto read_b = [&](int s, int j) { b[s][j] = *reinterpret_cast<const i32x4*>(base + rd[s] + (TN + (wm * WM + j) * 32) * MXG_ROW); };
-  auto read_scales = [&](int g) __attribute__((always_inline)) {
-    const unsigned char* t = smem + MXG_BUFS * kBuf + (g & 1) * kScales + li * MX_GROUP_BLOCKS;
-#pragma unroll
-    for (int i = 0; i < WN; ++i) ga[i] = *reinterpret_cast<const u32x2*>(t + (wn * WN + i) * 32 * MX_GROUP_BLOCKS);
-#pragma unroll
-    for (int j = 0; j < WM; ++j) gb[j] = *reinterpret_cast<const u32x2*>(t + (TN + (wm * WM + j) * 32) * MX_GROUP_BLOCKS);
+  for (int s = 0; s < 4; ++s) rd[s] = li * MXG_LINE + (((4 * hl + s) ^ ((li >> 1) & 7)) << 4);
+  auto read_op = [&](unsigned buf, int s, int to, int x) __attribute__((always_inline)) {
+    const unsigned char* t = smem + buf + rd[s];
+    if (x < WN) a[to][x] = *reinterpret_cast<const i32x4*>(t + (wn * WN + x) * 32 * MXG_LINE);
+    else if (x < kOps) b[to][x - WN] = *reinterpret_cast<const i32x4*>(t + (TN + (wm * WM + x - WN) * 32) * MXG_LINE);
   };
-  auto tile_scales = [&](int half) __attribute__((always_inline)) {
+  auto read_scales = [&](unsigned buf) __attribute__((always_inline)) {
+    const unsigned char* t = smem + buf + kCodes + li * MX_GROUP_BLOCKS + 4 * hl;
 #pragma unroll
-    for (int i = 0; i < WN; ++i) sa[i] = (int)(ga[i][half] >> (16 * hl));
+    for (int i = 0; i < WN; ++i) na[i] = *reinterpret_cast<const int*>(t + (wn * WN + i) * 32 * MX_GROUP_BLOCKS);
 #pragma unroll
-    for (int j = 0; j < WM; ++j) sb[j] = (int)(gb[j][half] >> (16 * hl));
+    for (int j = 0; j < WM; ++j) nb[j] = *reinterpret_cast<const int*>(t + (TN + (wm * WM + j) * 32) * MX_GROUP_BLOCKS);
   };
+  // the products of step kS; the operands of the step after it (of buffer `buf`) are read between them, and loads
+  // l0 .. l1 - 1 of the cursor's group go out to buffer `to`
+  auto step = [&](auto s_c, unsigned buf, int l0, int l1, unsigned to) __attribute__((always_inline)) {
+    constexpr int kS = decltype(s_c)::value, kFrom = kS & 1, kNext = (kS + 1) & 3;
+#pragma unroll
+    for (int x = 0; x < kProd; ++x) {
+      read_op(buf, kNext, kFrom ^ 1, x);
+      if (x == kProd - 1) {                                            // fewer products than operands
+#pragma unroll
+        for (int y = kProd; y < kOps; ++y) read_op(buf, kNext, kFrom ^ 1, y);
+      }
+#pragma unroll
+      for (int y = l0; y < l1; ++y)
+        if ((y - l0) * kProd / (l1 - l0) == x) load(lds0 + to, y);
+      __builtin_amdgcn_sched_barrier(0);
+      acc[x / WM][x % WM] = mx_mfma<kS>(a[kFrom][x / WM], b[kFrom][x % WM], acc[x / WM][x % WM], sa[x / WM], sb[x % WM]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  unsigned char* const stage = smem + kBufs * kBuf + wave * MXG_STAGE;
 
-  unsigned cur = 0, nxt = kBuf, nn = 2 * kBuf;                         // buffers of tiles t, t + 1, t + 2
+  unsigned cur = 0, last = (kBufs - 1) * kBuf;                         // buffer of group g; of the cursor's group (g + kBufs - 1)
 #pragma unroll
-  for (int t = 0; t < 3; ++t) {
+  for (int g = 0; g < kBufs; ++g) {
+    if (g > 0) advance();
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) load_codes(t, lds0 + t * kBuf, i);
-    if ((t & 1) == 0)
-#pragma unroll
-      for (int i = 0; i < kScaleLoads; ++i) load_scales(t >> 1, i);
+    for (int i = 0; i < (g == kBufs - 1 ? kFirst : kLoads); ++i) load(lds0 + g * kBuf, i);
   }
-  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(2 * kLoads + kScaleLoads) : "memory");   // tile 0
+  asm volatile("s_waitcnt vmcnt(%0)" :: "n"((kBufs - 2) * kLoads + kFirst) : "memory");    // group 0
   ATT_BARRIER();
   read_scales(0);
 #pragma unroll
-  for (int i = 0; i < WN; ++i) read_a(0, i);
+  for (int x = 0; x < kOps; ++x) read_op(0, 0, 0, x);
+
+  int m0 = src.m0, n0 = src.n0;
+  for (;;) {
 #pragma unroll
-  for (int j = 0; j < WM; ++j) read_b(0, j);
-  // one tile: kHalf 0 or 1 of its group
-  auto tile_pass = [&](auto half_c, int t) __attribute__((always_inline)) {
-    constexpr int kHalf = decltype(half_c)::value;
-    tile_scales(kHalf);
-    // step 0; the operands of step 1 are read meanwhile
+    for (int i = 0; i < WN; ++i)
 #pragma unroll
-    for (int x = 0; x < WN * WM; ++x) {
-      if (x < WN) read_a(1, x);
-      else if (x < WN + WM) read_b(1, x - WN);
-      if (WN * WM < WN + WM && x == WN * WM - 1) {                     // fewer products than operands
+      for (int e = 0; e < 16; ++e) {
+        const float x = bias_at(p, n0 + (wn * WN + i) * 32 + 8 * (e >> 2) + 4 * hl + (e & 3));
 #pragma unroll
-        for (int y = WN * WM; y < WN + WM; ++y) read_b(1, y - WN);
+        for (int j = 0; j < WM; ++j) acc[i][j][e] = x;
       }
-      __builtin_amdgcn_sched_barrier(0);
-      acc[x / WM][x % WM] = mx_mfma<0>(a[0][x / WM], b[0][x % WM], acc[x / WM][x % WM], sa[x / WM], sb[x % WM]);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int g = 0; g < p.groups; ++g) {
+#pragma unroll
+      for (int i = 0; i < WN; ++i) sa[i] = na[i];
+#pragma unroll
+      for (int j = 0; j < WM; ++j) sb[j] = nb[j];
+      step(std::integral_constant<int, 0>{}, cur, kFirst, kLoads, last);
+      step(std::integral_constant<int, 1>{}, cur, 0, 0, 0);
+      step(std::integral_constant<int, 2>{}, cur, 0, 0, 0);
+      asm volatile("s_waitcnt vmcnt(%0)" :: "n"((kBufs - 2) * kLoads) : "memory");         // group g + 1
+      ATT_BARRIER();                                                   // everybody's; and everybody has read group g
+      last = cur;
+      cur = cur == (kBufs - 1) * kBuf ? 0 : cur + kBuf;
+      read_scales(cur);
+      advance();
+      step(std::integral_constant<int, 3>{}, cur, 0, kFirst, last);
     }
-    // tile t + 1 is there when the loads of t + 2 alone are left (with its group's scales if t is even)
-    if (kHalf == 0) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kLoads + kScaleLoads) : "memory");
-    else asm volatile("s_waitcnt vmcnt(%0)" :: "n"(kLoads) : "memory");
-    ATT_BARRIER();                                                     // everybody's; and everybody has read tile t
-    base = smem + nxt;
-    if (kHalf == 1) read_scales((t + 1) >> 1);
-    // step 1; the operands of the next tile's step 0 are read and tile t + 3 is requested meanwhile
+    // ---- this tile's outputs, while the next one's first groups arrive ----
 #pragma unroll
-    for (int x = 0; x < WN * WM; ++x) {
-      if (x < WN) read_a(0, x);
-      else if (x < WN + WM) read_b(0, x - WN);
-      if (WN * WM < WN + WM && x == WN * WM - 1) {
+    for (int j = 0; j < WM; ++j)
 #pragma unroll
-        for (int y = WN * WM; y < WN + WM; ++y) read_b(0, y - WN);
+      for (int i = 0; i < WN; ++i) {
+        const int n = n0 + (wn * WN + i) * 32, mt = m0 + (wm * WM + j) * 32;
+        float v[16];
+        tile_values(p, acc[i][j], v);
+        if constexpr (kOut == MX_OUT_MXFP4) store_mx(p, v, n, mt + li);
+        else if constexpr (kOut == MX_OUT_F32) store_f32(p, v, n, mt + li);
+        else store_bf16(p, stage, v, n, mt);
+        __builtin_amdgcn_sched_barrier(0);                             // one sub-tile's temporaries at a time
       }
-      if (kHalf == 1 && x < kScaleLoads) load_scales((t + 3) >> 1, x);
-      if (x < kLoads) load_codes(t + 3, lds0 + cur, x);
-      if (x == WN * WM - 1) {
-#pragma unroll
-        for (int y = WN * WM; y < kLoads; ++y) load_codes(t + 3, lds0 + cur, y);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      acc[x / WM][x % WM] = mx_mfma<1>(a[1][x / WM], b[1][x % WM], acc[x / WM][x % WM], sa[x / WM], sb[x % WM]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    const unsigned done = cur;
-    cur = nxt; nxt = nn; nn = done;
-  };
-  for (int t = 0; t < n_tiles; t += 2) {
-    tile_pass(std::integral_constant<int, 0>{}, t);
-    tile_pass(std::integral_constant<int, 1>{}, t + 1);
+    w += slots;
+    if (w >= w_end) break;
+    m0 = nsrc.m0; n0 = nsrc.n0;
+    nsrc = source(w + slots);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                     // the empty loads
-  ATT_BARRIER();                                                       // everybody's: the buffers are free
-  float bias[WN][16];
-#pragma unroll
-  for (int i = 0; i < WN; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) bias[i][e] = bias_at(p, n0 + (wn * WN + i) * 32 + 8 * (e >> 2) + 4 * hl + (e & 3));
-  unsigned char* const stage = smem + wave * 4096;
-  static_assert(WN == 2, "64 outputs of a token are staged together");
-#pragma unroll
-  for (int j = 0; j < WM; ++j) {
-    const int mt = m0 + (wm * WM + j) * 32;
-#pragma unroll
-    for (int i = 0; i < WN; ++i) {
-      const int n = n0 + (wn * WN + i) * 32;
-      float v[16];
-      tile_values(p, acc[i][j], bias[i], v);
-      if constexpr (kOut == MX_OUT_MXFP4) store_mx(p, v, n, mt + li);
-      else if constexpr (kOut == MX_OUT_F32) store_f32(p, v, n, mt + li);
-      else stage_bf16(stage, v, i);
-    }
-    if constexpr (kOut == MX_OUT_BF16) store_staged(p, stage, n0 + wn * 64, mt);
-  }
 }
 
 namespace {
 
-template <int WN, int WM, int kOut>
+template <int WN, int WM, int NN, int NM, int kBufs, int kOut>
 hipError_t run_mx_gemm(const MxGemmParams& p, hipStream_t stream) {
-  constexpr int TN = 64 * WN, TM = 64 * WM, kLds = (TN + TM) * (MXG_BUFS * MXG_ROW + 2 * MX_GROUP_BLOCKS);
+  constexpr int TN = 32 * WN * NN, TM = 32 * WM * NM;
+  constexpr int kLds = kBufs * (TN + TM) * (MXG_LINE + MX_GROUP_BLOCKS) + NN * NM * MXG_STAGE;
+  static_assert(kLds <= 160 * 1024, "LDS of a CU");
   static std::atomic<unsigned> lds_set{0u};
-  const hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(icsa_mx_gemm_kernel<WN, WM, kOut>), kLds, &lds_set);
+  const hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(icsa_mx_gemm_kernel<WN, WM, NN, NM, kBufs, kOut>), kLds, &lds_set);
   if (e != hipSuccess) return e;
-  const int64_t tiles = (int64_t)((out_columns(p) + TN - 1) / TN) * ((p.M + TM - 1) / TM);
-  if (tiles > 0x7ffffff0LL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((icsa_mx_gemm_kernel<WN, WM, kOut>), dim3(xcd_grid((int)tiles)), dim3(MXG_THREADS), kLds, stream, p);
+  const int64_t tiles = (int64_t)((out_columns(p) + TN - 1) / TN) * ((p.m_last - p.m_first + TM - 1) / TM);
+  if (tiles > 0x3ffffff0LL) return hipErrorInvalidValue;
+  // several tiles a workgroup where its loads run at most one tile ahead, and where a CU holds one workgroup
+  const int64_t most = p.groups >= kBufs && 2 * kLds > 160 * 1024 ? MXG_CUS : tiles;
+  hipLaunchKernelGGL((icsa_mx_gemm_kernel<WN, WM, NN, NM, kBufs, kOut>), dim3(xcd_grid((int)(tiles < most ? tiles : most))),
+                     dim3(64 * NN * NM), kLds, stream, p);
   return hipGetLastError();
 }
 
+// A launch takes rounds of one tile a CU.  Measured (us, one round): a 256 x 256 tile 1.6 a group and 1 to 4 besides, GELU 7; a
+// 128 x 128 tile 0.56 a group and 2.5, GELU 1.7; a launch 4.5.  In units of 0.56 us.
+double rounds_of(int64_t tiles) { return (double)((tiles + MXG_CUS - 1) / MXG_CUS); }
+double big_time(int64_t tiles, const MxGemmParams& p) { return rounds_of(tiles) * (2.9 * p.groups + 4 + 12 * p.gelu); }
+double small_time(int64_t tiles, const MxGemmParams& p) { return rounds_of(tiles) * (p.groups + 4.5 + 3 * p.gelu); }
+
+// 256 x 256 tiles, 128 x 128 tiles, or the first rows in whole rounds of the former and the others in the latter.  All three
+// measured (us, M x N x K): 512 x 5,120 x 4,096 24.3, 12.7, -; 1,560 x 5,120 x 5,120 32.0, 41.3, -; 3,120 x 5,120 x 5,120 67.1, 57.2,
+// 54.7; 9,360 x 2,000 x 5,120 71.0, 72.4, 61.7; 14,040 x 5,120 x 13,824 454.9, 597.0, 450.3; 65,520 x 5,120 x 5,120 817, 1,154, 822.
 template <int kOut>
-hipError_t pick_mx_gemm(const MxGemmParams& p, hipStream_t stream) {
-  const int64_t big = (int64_t)((p.N + 127) / 128) * ((p.M + 255) / 256);
-  if (big >= 512) return run_mx_gemm<2, 4, kOut>(p, stream);
-  return run_mx_gemm<2, 2, kOut>(p, stream);
+hipError_t pick_mx_gemm(MxGemmParams p, hipStream_t stream) {
+  const int64_t cols = out_columns(p), n_big = (cols + 255) / 256, n_small = (cols + 127) / 128;
+  const int64_t m_big = (p.M + 255) / 256, whole = n_big * m_big / MXG_CUS;
+  auto small = [&](int64_t rows) { return small_time(n_small * ((rows + 127) / 128), p); };
+  const int64_t split = std::min<int64_t>(whole * MXG_CUS / n_big, m_big - 1) * 256;      // rows that whole rounds take
+  const double t_big = big_time(n_big * m_big, p), t_small = small(p.M);
+  const double t_split = split > 0 ? big_time(n_big * (split / 256), p) + small(p.M - split) + 8 : t_big + 1;
+  if (t_small <= t_big && t_small <= t_split) return run_mx_gemm<2, 2, 2, 2, 4, kOut>(p, stream);
+  if (t_big <= t_split) return run_mx_gemm<2, 4, 4, 2, 2, kOut>(p, stream);
+  p.m_last = (int)split;
+  const hipError_t e = run_mx_gemm<2, 4, 4, 2, 2, kOut>(p, stream);
+  if (e != hipSuccess) return e;
+  p.m_first = (int)split;
+  p.m_last = p.M;
+  return run_mx_gemm<2, 2, 2, 2, 4, kOut>(p, stream);
 }
 
 }  // namespace
 
-hipError_t launch_mx_gemm(const MxGemmParams& p, hipStream_t stream) {
+hipError_t launch_mx_gemm(MxGemmParams p, hipStream_t stream) {
   // a tile's rows must be addressable with 32-bit offsets
   if ((int64_t)p.groups * (MX_GROUP / 2) * 256 > 0x7fffffffLL) return hipErrorInvalidValue;
+  p.m_first = 0;
+  p.m_last = p.M;
+  if (mx_rows_takes(p.M, p.N)) return launch_mx_rows(p, stream);
   switch (p.out_kind) {
     case MX_OUT_BF16: return pick_mx_gemm<MX_OUT_BF16>(p, stream);
     case MX_OUT_F32: return pick_mx_gemm<MX_OUT_F32>(p, stream);

@@ -11,35 +11,6 @@
 #define MXQ_WAVE_K 512                     // values of one row that a wave takes at a time
 #define MXQ_AHEAD 4                        // such pieces requested together
 
-namespace {
-
-// Rows may start at any element: vectors of the element's alignment (global memory takes them)
-typedef bf16x8 bf16x8_a2 __attribute__((aligned(2)));
-typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
-typedef floatx4 floatx4_a4 __attribute__((aligned(4)));
-
-// 8 values of a row from k on, zeros from K on; where K cuts them, value by value, so that nothing past the
-// row is touched.
-template <typename T>
-__device__ __forceinline__ void load8_row(const T* row, int k, int K, float v[8]) {
-  if (k + 8 <= K) {
-    if constexpr (sizeof(T) == 2) {
-      const bf16x8 x = *reinterpret_cast<const bf16x8_a2*>(row + k);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
-    } else {
-      const floatx4 a = *reinterpret_cast<const floatx4_a4*>(row + k), b = *reinterpret_cast<const floatx4_a4*>(row + k + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = k + i < K ? (float)row[k + i] : 0.f;
-}
-
-}  // namespace
-
 template <typename T>
 __global__ void __launch_bounds__(MXQ_THREADS) icsa_mx_quantize_kernel(MxQuantParams p) {
   const int lane = threadIdx.x & 63;
@@ -60,16 +31,7 @@ __global__ void __launch_bounds__(MXQ_THREADS) icsa_mx_quantize_kernel(MxQuantPa
 #pragma unroll
   for (int i = 0; i < MXQ_AHEAD; ++i) {
     if (first + i >= pieces) return;                     // uniform for the wave
-    unsigned amax = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(v[i][e]) & 0x7fffffffu);
-    amax = max(amax, (unsigned)__shfl_xor((int)amax, 1, 64));
-    amax = max(amax, (unsigned)__shfl_xor((int)amax, 2, 64));
-    const unsigned s = mx_scale_byte(amax);
-    const float f = mx_inv_scale(s);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[i][e] *= f;
-    const unsigned codes = s == 255 ? 0u : mx_pack8(v[i]);
+    const unsigned s = mx_quantize8(v[i]), codes = mx_codes8(v[i], s);
     if (k[i] < Kp) {
       *reinterpret_cast<unsigned*>(p.codes + row[i] * (Kp / 2) + k[i] / 2) = codes;
       if ((lane & 3) == 0)

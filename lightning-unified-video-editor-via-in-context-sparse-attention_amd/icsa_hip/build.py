@@ -19,7 +19,7 @@ BUILD_DIR = os.path.join(CSRC_DIR, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libicsa.so")
 
 SOURCES = ["pool.hip", "compressed.hip", "newkv.hip", "gather.hip", "flash_attn.hip", "sparse_attn.hip", "sparse_bwd.hip",
-           "wan_qk.hip", "wan_block.hip", "mx_quant.hip", "mx_gemm.hip", "masked_attn.hip",
+           "wan_qk.hip", "wan_block.hip", "mx_quant.hip", "mx_gemm.hip", "mx_rows.hip", "masked_attn.hip",
            "api.hip"]
 
 HIP_FLAGS = [
