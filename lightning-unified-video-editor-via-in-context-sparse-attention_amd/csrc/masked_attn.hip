@@ -30,7 +30,9 @@
 #define MA_M_NONE (-3.4028234663852886e38f)           // finite: a tile without visible keys leaves O = l = 0
 #define MA_LOG2E 1.4426950408889634f
 #define MA_TARGET_WG 512                              // two workgroups a CU
+#define MA_MAX_SPLIT 256
 #define MA_MIN_SPLIT_TILES 4                          // key tiles a split part is worth
+#define MA_BIAS_MARGIN ATT_BN
 #define MA_LDS_MAX (160 * 1024)
 
 namespace {
@@ -49,31 +51,52 @@ __host__ __device__ __forceinline__ int ma_fixed_lds(int D) { return 4 * ATT_BN 
 // What a row sees: keys [lo, hi); at: the key position its own query is aligned with.
 struct RowRange { int lo, hi, at; };
 
-__device__ __forceinline__ RowRange row_range(const MaskedAttnParams& p, int b, int i) {
+__device__ __forceinline__ RowRange doc_range(const MaskedAttnParams& p, int i, int q1, int k0, int k1, int prefix) {
   RowRange r = {0, 0, 0};
-  int q1 = p.Sq, k0 = 0, k1 = p.Sk, n = 0;
-  if (p.q_starts != nullptr) {
-    const int* qs = p.q_starts + (int64_t)b * (p.docs + 1);
-    int lo = 0, hi = p.docs + 1;                      // the count of starts <= i
+  k0 = min(max(k0, 0), p.Sk);
+  k1 = min(max(k1, 0), p.Sk);
+  const int64_t at = (int64_t)i + k1 - q1;
+  r.at = (int)max((int64_t)-0x40000000, min((int64_t)0x40000000, at));
+  int64_t end = k1;
+  if (p.causal) end = min(end, max(at + 1, (int64_t)k0 + prefix));
+  if (end > k0) { r.lo = k0; r.hi = (int)end; }
+  return r;
+}
+
+// Of query i (this lane's).  Up to 63 documents: the lanes hold their borders, requested together, and a
+// document is found by counting; more: a search in memory.  Called by whole waves.
+__device__ __forceinline__ RowRange row_range(const MaskedAttnParams& p, int b, int i) {
+  const int lane = threadIdx.x & 63, docs = p.docs;
+  const int* pre = p.prefix != nullptr ? p.prefix + (int64_t)b * docs : nullptr;
+  if (p.q_starts == nullptr) return doc_range(p, i, p.Sq, 0, p.Sk, pre ? pre[0] : 0);
+  const int* qs = p.q_starts + (int64_t)b * (docs + 1);
+  const int* ks = p.k_starts + (int64_t)b * (docs + 1);
+  int n, q1, k0, k1, px = 0;
+  if (docs < 64) {
+    const int own_q = lane <= docs ? qs[lane] : 0x7fffffff, own_k = lane <= docs ? ks[lane] : 0;
+    const int own_p = pre != nullptr && lane < docs ? pre[lane] : 0;
+    n = -1;                                           // the count of starts <= i, less one
+    for (int x = 0; x <= docs; ++x) n += __builtin_amdgcn_readlane(own_q, x) <= i;
+    const int c = min(max(n, 0), docs - 1);
+    q1 = __shfl(own_q, c + 1, 64);
+    k0 = __shfl(own_k, c, 64);
+    k1 = __shfl(own_k, c + 1, 64);
+    px = __shfl(own_p, c, 64);
+  } else {
+    int lo = 0, hi = docs + 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (qs[mid] <= i) lo = mid + 1; else hi = mid;
     }
     n = lo - 1;
-    if (n < 0 || n >= p.docs) return r;               // in front of the first document, or behind the last
-    q1 = qs[n + 1];
-    const int* ks = p.k_starts + (int64_t)b * (p.docs + 1);
-    k0 = min(max(ks[n], 0), p.Sk);
-    k1 = min(max(ks[n + 1], 0), p.Sk);
+    const int c = min(max(n, 0), docs - 1);
+    q1 = qs[c + 1];
+    k0 = ks[c];
+    k1 = ks[c + 1];
+    if (pre != nullptr) px = pre[c];
   }
-  const int64_t at = (int64_t)i + k1 - q1;
-  r.at = (int)max((int64_t)-0x40000000, min((int64_t)0x40000000, at));
-  int64_t end = k1;
-  if (p.causal) {
-    end = min(end, max(at + 1, p.prefix ? (int64_t)k0 + p.prefix[(int64_t)b * p.docs + n] : (int64_t)k0));
-  }
-  if (end > k0) { r.lo = k0; r.hi = (int)end; }
-  return r;
+  if (n < 0 || n >= docs) return RowRange{0, 0, 0};   // in front of the first document, or behind the last
+  return doc_range(p, i, q1, k0, k1, px);
 }
 
 __device__ __forceinline__ int wave_min(int x) {
@@ -164,9 +187,16 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   const int r0 = blk * MA_ROWS + 32 * wave;
   const int rows_valid = min(32, n_rows - r0);
 
+  bf16x8 qf[kSteps];
+  {
+    const bf16* src = p.q + row_at(p.q_sb, p.q_ss, p.q_sh, b, hk, G, min(r0 + li, n_rows - 1)) + 8 * hl;
+#pragma unroll
+    for (int kk = 0; kk < kSteps; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(src + 16 * kk);
+  }
+
   // ---- what the rows see ----
-  RowRange rr = {0, 0, 0};
-  if (li < rows_valid) rr = row_range(p, b, (r0 + li) / G);
+  RowRange rr = row_range(p, b, (r0 + li) / G);
+  if (li >= rows_valid) rr = RowRange{0, 0, 0};
   {
     const bool any = rr.hi > rr.lo;
     const int lo = wave_min(any ? rr.lo : 0x7fffffff), hi = wave_max(any ? rr.hi : 0);
@@ -175,11 +205,13 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
     if (threadIdx.x < 2) ctl[16 + threadIdx.x] = 0;
   }
   const float c = p.scale * MA_LOG2E;
+  const int bias_row = 2 * p.radius + 1 + 2 * MA_BIAS_MARGIN;            // a head's table, its ends repeated over a tile's width
   if constexpr (kBias) {
     const int width = 2 * p.radius + 1;
     const float* src = p.bias + (int64_t)hk * G * width;                 // the group's heads
-    for (int x = threadIdx.x; x < G * width; x += MA_THREADS) {
-      const float f = src[x];            // a type's lowest value stays finite in units of log2, an infinity does not
+    for (int x = threadIdx.x; x < G * bias_row; x += MA_THREADS) {
+      const int h = x / bias_row, at = x - h * bias_row;
+      const float f = src[h * width + min(max(at - MA_BIAS_MARGIN, 0), width - 1)];   // a type's lowest value stays finite in units of log2, an infinity does not
       bias_lds[x] = __builtin_isinf(f) ? f : fminf(fmaxf(f * MA_LOG2E, -3.4028234663852886e38f), 3.4028234663852886e38f);
     }
   }
@@ -220,12 +252,6 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   };
   if (t0 < t1) load_tile(t0);
 
-  bf16x8 qf[kSteps];
-  {
-    const bf16* src = p.q + row_at(p.q_sb, p.q_ss, p.q_sh, b, hk, G, min(r0 + li, n_rows - 1)) + 8 * hl;
-#pragma unroll
-    for (int kk = 0; kk < kSteps; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(src + 16 * kk);
-  }
   int kro[kSteps], vro[kSub];                        // operand read offsets (bytes); + 32 rows a sub-tile
 #pragma unroll
   for (int kk = 0; kk < kSteps; ++kk) kro[kk] = li * T::kRow + (((2 * kk + hl) ^ T::kswz(li)) << 4);
@@ -235,7 +261,7 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
     vro[ds] = row * T::kRow + (((col >> 3) ^ T::vswz(row)) << 4) + (col & 7) * 2;
   }
   unsigned char* const scratch = scratch_all + wave * MA_SCRATCH_WAVE;
-  const float* const my_bias = kBias ? bias_lds + ((r0 + li) % G) * (2 * p.radius + 1) + p.radius : nullptr;
+  const float* const my_bias = kBias ? bias_lds + ((r0 + li) % G) * bias_row + MA_BIAS_MARGIN + p.radius : nullptr;
 
   floatx16 o[kSub] = {};
   float m_ref = MA_M_NONE, l_run = 0.f;
@@ -281,37 +307,35 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
       for (int sub = 0; sub < 2; ++sub)
         s[sub] = mfma32x32x16(*reinterpret_cast<const bf16x8*>(ks + kro[kk] + sub * 32 * T::kRow), qf[kk], s[sub]);
     }
-    // scores in units of log2
+    // Scores in units of log2, as base + mul * s.  Capped: cap tanh(x) = cap - 2 cap r with r = 1 / (1 + exp(2 x)), so
+    // s becomes r; with a bias s becomes the score itself.
+    const float in = kCap ? 2.f * MA_LOG2E * p.scale / p.softcap : 0.f, top = kCap ? p.softcap * MA_LOG2E : 0.f;
     if constexpr (kCap) {
-      const float in = 2.f * MA_LOG2E * p.scale / p.softcap, top = p.softcap * MA_LOG2E;
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {               // cap tanh(x) = cap - 2 cap / (1 + exp(2 x))
-          const float e = __builtin_amdgcn_exp2f(s[sub][i] * in);
-          s[sub][i] = fmaf(-2.f * top, __builtin_amdgcn_rcpf(1.f + e), top);
-        }
+        for (int i = 0; i < 16; ++i)
+          s[sub][i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[sub][i] * in));
     }
     if constexpr (kBias) {
       const int d0 = j0 - rr.at + 4 * hl, R = p.radius;
+      const float f = kCap ? -2.f * top : c;
       if (__ballot(!(d0 >= R || d0 + ATT_BN <= -R)) == 0ull) {           // the whole tile past the table's ends
-        const float x = my_bias[d0 > 0 ? R : -R];
+        const float x = my_bias[d0 > 0 ? R : -R] + top;
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[sub][i] = kCap ? s[sub][i] + x : fmaf(s[sub][i], c, x);
+          for (int i = 0; i < 16; ++i) s[sub][i] = fmaf(s[sub][i], f, x);
       } else {
+        // a row's 64 distances lie inside the table and its margins, or are past one end alike
+        const float* t = my_bias + min(max(d0, -R - MA_BIAS_MARGIN + 4 * hl), R + 4 * hl);
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float x = my_bias[min(max(d0 + 32 * sub + 8 * (i >> 2) + (i & 3), -R), R)];
-            s[sub][i] = kCap ? s[sub][i] + x : fmaf(s[sub][i], c, x);
-          }
+          for (int i = 0; i < 16; ++i) s[sub][i] = fmaf(s[sub][i], f, t[32 * sub + 8 * (i >> 2) + (i & 3)] + top);
       }
     }
-    constexpr bool kScaled = kCap || kBias;            // s already in log2 units
-    const float cs = kScaled ? 1.f : c;
+    const float base = kBias ? 0.f : top, mul = kBias ? 1.f : kCap ? -2.f * top : c;
     if (partial) {
       // keys outside [lo, hi) as one 64-bit word: element i of sub-tile sub is key 32 sub + 8 (i / 4) + 4 hl + i % 4
       const int a = min(max(rr.lo - j0, 0), 64), z = min(max(rr.hi - j0, 0), 64);
@@ -324,19 +348,21 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
         for (int i = 0; i < 16; ++i) {
           const int kbit = 8 * (i >> 2) + (i & 3);
           const unsigned all = (unsigned)((int)(wd << (31 - kbit)) >> 31);
-          s[sub][i] = __uint_as_float((all & 0xff800000u) | (__float_as_uint(s[sub][i]) & ~all));
+          // score -inf: s is -inf, or +inf where the factor is negative
+          s[sub][i] = __uint_as_float((all & (kCap && !kBias ? 0x7f800000u : 0xff800000u)) | (__float_as_uint(s[sub][i]) & ~all));
         }
       }
     }
     bf16x8 pf[4];
     float rs = 0.f;
     if (!first) {
+      const float off = base - m_ref;
       float rsv[4] = {};
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[sub][i], cs, -m_ref));
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[sub][i], mul, off));
           rsv[i & 3] += e;
           pf[2 * sub + (i >> 3)][i & 7] = (bf16)e;
         }
@@ -347,8 +373,8 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[sub][i]);
-      mx = xhalf_max(mx) * cs;
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, kCap && !kBias ? -s[sub][i] : s[sub][i]);
+      mx = fmaf(xhalf_max(mx), fabsf(mul), base);
       const float mn = mx > m_ref ? mx : m_ref;
       const float al = __builtin_amdgcn_exp2f(m_ref - mn);
 #pragma unroll
@@ -357,12 +383,13 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
         for (int i = 0; i < 16; ++i) o[ds][i] *= al;
       l_run *= al;
       m_ref = mn;
+      const float off = base - m_ref;
       rs = 0.f;
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[sub][i], cs, -m_ref));
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[sub][i], mul, off));
           rs += e;
           pf[2 * sub + (i >> 3)][i & 7] = (bf16)e;
         }
@@ -411,16 +438,23 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
 
   if (rows_valid <= 0) return;
   if (p.n_split > 1) {
-    // raw O, reference max and the two halves' sums: [item][wave][ds][g][lane][4], [2][64]
-    float* dst = p.part + ((int64_t)((bh * (int64_t)n_blk + blk) * p.n_split + split) * MA_WAVES + wave) * (D * 32 + 128);
+    // a row's raw O, reference max and sum: [item][split][row][D], then [item][split][2][row]
+    const int64_t part = ((int64_t)bh * n_blk + blk) * p.n_split + split;
+    const float l = xhalf_sum(l_run);
+    if (li < rows_valid) {
+      float* dst = p.part + (part * MA_ROWS + 32 * wave + li) * D + 4 * hl;
 #pragma unroll
-    for (int ds = 0; ds < kSub; ++ds)
+      for (int ds = 0; ds < kSub; ++ds)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<floatx4*>(dst + ((ds * 4 + g) * 64 + lane) * 4) =
-            some ? floatx4{o[ds][4 * g], o[ds][4 * g + 1], o[ds][4 * g + 2], o[ds][4 * g + 3]} : floatx4{};
-    dst[D * 32 + lane] = some ? m_ref : MA_M_NONE;
-    dst[D * 32 + 64 + lane] = some ? l_run : 0.f;
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<floatx4*>(dst + 32 * ds + 8 * g) =
+              some ? floatx4{o[ds][4 * g], o[ds][4 * g + 1], o[ds][4 * g + 2], o[ds][4 * g + 3]} : floatx4{};
+      if (hl == 0) {
+        float* ml = p.part + (int64_t)p.B * p.Hk * n_blk * p.n_split * MA_ROWS * D + part * 2 * MA_ROWS + 32 * wave + li;
+        ml[0] = some ? m_ref : MA_M_NONE;
+        ml[MA_ROWS] = some ? l : 0.f;
+      }
+    }
     return;
   }
   if (!some) {                                         // whatever it holds of tiles that others see whole
@@ -431,36 +465,46 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   store_wave<D>(p, scratch, o, !some || l == 0.f ? 0.f : 1.f / l, b, hk, r0, rows_valid);
 }
 
-// Joins the parts of every item in order (bitwise reproducible): one wave for 32 rows.
+// Joins the parts of every row in order (bitwise reproducible).  256 threads take 1024 / D rows of one item, 4 dims each;
+// a row's threads first work out every part's weight 2^(m_s - max) / sum between them.
 template <int D>
-__global__ void __launch_bounds__(64) icsa_masked_combine_kernel(MaskedAttnParams p) {
-  __shared__ __attribute__((aligned(16))) unsigned char stage[MA_SCRATCH_WAVE];
-  constexpr int kSub = D / 32, kPart = D * 32 + 128;
-  const int lane = threadIdx.x & 63;
-  const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS;
-  const int item = blockIdx.x / MA_WAVES, w = blockIdx.x % MA_WAVES, blk = item % n_blk, bh = item / n_blk;
-  const int r0 = blk * MA_ROWS + 32 * w, rows_valid = min(32, n_rows - r0);
-  if (rows_valid <= 0) return;
-  floatx16 o[kSub] = {};
-  float m = MA_M_NONE, l = 0.f;
-  const float* src = p.part + ((int64_t)item * p.n_split * MA_WAVES + w) * kPart;
-  for (int s = 0; s < p.n_split; ++s, src += (int64_t)MA_WAVES * kPart) {
-    const float ms = src[D * 32 + lane], ls = src[D * 32 + 64 + lane];
-    const float mn = ms > m ? ms : m;
-    const float fo = __builtin_amdgcn_exp2f(m - mn), fn = __builtin_amdgcn_exp2f(ms - mn);
+__global__ void __launch_bounds__(256) icsa_masked_combine_kernel(MaskedAttnParams p) {
+  constexpr int kPer = D / 4, kRows = 256 / kPer;
+  __shared__ float wt[MA_MAX_SPLIT][kRows];
+  const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS, n = p.n_split;
+  const int item = blockIdx.x / (MA_ROWS / kRows), row = blockIdx.x % (MA_ROWS / kRows) * kRows + threadIdx.x / kPer;
+  const int blk = item % n_blk, bh = item / n_blk, r = blk * MA_ROWS + row, t = threadIdx.x % kPer, x = threadIdx.x / kPer;
+  if (blk * MA_ROWS + (int)(blockIdx.x % (MA_ROWS / kRows)) * kRows >= n_rows) return;     // uniform
+  const int64_t part0 = (int64_t)item * n;
+  const float* ml = p.part + (int64_t)p.B * p.Hk * n_blk * n * MA_ROWS * D + part0 * 2 * MA_ROWS + row;
+  const bool on = r < n_rows;
+  float m = MA_M_NONE;
+  for (int s = t; s < n; s += kPer) m = fmaxf(m, on ? ml[(int64_t)s * 2 * MA_ROWS] : MA_M_NONE);
 #pragma unroll
-    for (int ds = 0; ds < kSub; ++ds)
+  for (int o = kPer / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kPer));
+  for (int s = t; s < n; s += kPer) wt[s][x] = on ? __builtin_amdgcn_exp2f(ml[(int64_t)s * 2 * MA_ROWS] - m) : 0.f;
+  __syncthreads();
+  if (!on) return;
+  float l = 0.f;
+  for (int s = 0; s < n; ++s) l = fmaf(ml[(int64_t)s * 2 * MA_ROWS + MA_ROWS], wt[s][x], l);
+  floatx4 o = {};
+  const float* src = p.part + (part0 * MA_ROWS + row) * D + 4 * t;
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const floatx4 v = *reinterpret_cast<const floatx4*>(src + (int64_t)s * MA_ROWS * D);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const floatx4 x = *reinterpret_cast<const floatx4*>(src + ((ds * 4 + g) * 64 + lane) * 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[ds][4 * g + e] = fmaf(x[e], fn, o[ds][4 * g + e] * fo);
-      }
-    l = fmaf(ls, fn, l * fo);
-    m = mn;
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], wt[s][x], o[e]);
   }
-  l = xhalf_sum(l);
-  store_wave<D>(p, stage, o, l == 0.f ? 0.f : 1.f / l, bh / p.Hk, bh % p.Hk, r0, rows_valid);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t off = row_at(p.out.sb, p.out.ss, p.out.sh, bh / p.Hk, bh % p.Hk, G, r) + 4 * t;
+  if (p.out.dtype == ICSA_DT_BF16) {
+    bf16x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (bf16)(o[e] * inv);
+    *reinterpret_cast<bf16x4*>(reinterpret_cast<bf16*>(p.out.p) + off) = y;
+  } else {
+    *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(p.out.p) + off) = floatx4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+  }
 }
 
 // Parts that an item's keys are cut into: enough workgroups for two a CU, each with a few tiles.
@@ -470,17 +514,17 @@ int masked_attn_splits(int B, int Sq, int Sk, int H, int Hk) {
   if (items <= 0 || items * 2 > MA_TARGET_WG) return 1;
   int64_t n = (MA_TARGET_WG + items - 1) / items;
   n = n < tiles / MA_MIN_SPLIT_TILES ? n : tiles / MA_MIN_SPLIT_TILES;
-  return n < 1 ? 1 : (int)n;
+  return n < 1 ? 1 : n > MA_MAX_SPLIT ? MA_MAX_SPLIT : (int)n;
 }
 
 int64_t masked_attn_part_floats(int B, int Sq, int H, int Hk, int D, int n_split) {
   if (n_split <= 1) return 0;
   const int64_t rows = (int64_t)Sq * (H / Hk);
-  return (int64_t)B * Hk * ((rows + MA_ROWS - 1) / MA_ROWS) * n_split * MA_WAVES * (D * 32 + 128);
+  return (int64_t)B * Hk * ((rows + MA_ROWS - 1) / MA_ROWS) * n_split * MA_ROWS * (D + 2);
 }
 
 bool masked_attn_bias_fits(int H, int Hk, int D, int radius) {
-  return (int64_t)(H / Hk) * (2 * (int64_t)radius + 1) * 4 <= MA_LDS_MAX - ma_fixed_lds(D);
+  return (int64_t)(H / Hk) * (2 * (int64_t)radius + 1 + 2 * MA_BIAS_MARGIN) * 4 <= MA_LDS_MAX - ma_fixed_lds(D);
 }
 
 namespace {
@@ -489,7 +533,7 @@ template <int D, bool kCap, bool kBias>
 hipError_t run_masked(const MaskedAttnParams& p, hipStream_t stream) {
   static std::atomic<unsigned> lds_set{0u};
   const int G = p.H / p.Hk;
-  const int lds = ma_fixed_lds(D) + (kBias ? G * (2 * p.radius + 1) * 4 : 0);
+  const int lds = ma_fixed_lds(D) + (kBias ? G * (2 * p.radius + 1 + 2 * MA_BIAS_MARGIN) * 4 : 0);
   const hipError_t a = ensure_lds_limit(reinterpret_cast<const void*>(icsa_masked_attn_kernel<D, kCap, kBias>), MA_LDS_MAX, &lds_set);
   if (a != hipSuccess) return a;
   const int64_t blocks = (int64_t)p.B * p.Hk * (((int64_t)p.Sq * G + MA_ROWS - 1) / MA_ROWS);
@@ -498,7 +542,7 @@ hipError_t run_masked(const MaskedAttnParams& p, hipStream_t stream) {
                      stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.n_split == 1) return e;
-  hipLaunchKernelGGL(icsa_masked_combine_kernel<D>, dim3((unsigned)(blocks * MA_WAVES)), dim3(64), 0, stream, p);
+  hipLaunchKernelGGL(icsa_masked_combine_kernel<D>, dim3((unsigned)(blocks * (MA_ROWS * D / 1024))), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 

@@ -399,58 +399,69 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
     A query that sees nothing gets zeros; NaN and infinities in keys and values reach only the
     queries that see them.  An inference operator: under an enabled grad mode an input that requires a
     gradient is refused."""
-    _require(all(isinstance(t, torch.Tensor) and t.dtype == torch.bfloat16 for t in (q, k, v)), "q, k, v must be bfloat16")
-    _require(q.is_cuda and k.device == q.device and v.device == q.device, "q, k, v must be on the same GPU")
-    _require(q.ndim == 4 and k.ndim == 4 and k.shape == v.shape and q.shape[0] == k.shape[0] and
-             q.shape[3] == k.shape[3], "q [B, Sq, H, D], k/v [B, Sk, Hk, D] expected")
+    bf16 = torch.bfloat16
+    if q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16:
+        raise IcsaArgumentError("q, k, v must be bfloat16")
+    dev = q.device
+    if not q.is_cuda or k.device != dev or v.device != dev:
+        raise IcsaArgumentError("q, k, v must be on the same GPU")
+    if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise IcsaArgumentError("q [B, Sq, H, D], k/v [B, Sk, Hk, D] expected")
     B, Sq, H, D = q.shape
     Sk, Hk = k.shape[1:3]
-    _require(D in (64, 128), "D must be 64 or 128")
-    _require(B > 0 and Hk > 0 and H > 0 and H % Hk == 0, "H must be a multiple of Hk")
-    _require(not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (q, k, v, bias)),
-             "masked_attn_func has no backward: call it under torch.no_grad()")
-    _require((q_starts is None) == (k_starts is None), "q_starts and k_starts must be given together")
-    docs = 1
-    if q_starts is not None:
-        _require(q_starts.ndim == 2 and q_starts.shape[0] == B and q_starts.shape[1] >= 2 and
-                 q_starts.shape == k_starts.shape, "q_starts and k_starts must be [B, N + 1]")
+    if D not in (64, 128):
+        raise IcsaArgumentError("D must be 64 or 128")
+    if B < 1 or Hk < 1 or H < 1 or H % Hk:
+        raise IcsaArgumentError("H must be a multiple of Hk")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
+        raise IcsaArgumentError("masked_attn_func has no backward: call it under torch.no_grad()")
+    docs, radius = 1, 0
+    if q_starts is not None or k_starts is not None:
+        if q_starts is None or k_starts is None or q_starts.ndim != 2 or q_starts.shape[0] != B or \
+                q_starts.shape[1] < 2 or q_starts.shape != k_starts.shape:
+            raise IcsaArgumentError("q_starts and k_starts must be given together, [B, N + 1]")
         docs = q_starts.shape[1] - 1
-    _require(prefix is None or causal, "prefix needs causal=True")
     if prefix is not None:
-        _require(tuple(prefix.shape) == (B, docs) or (docs == 1 and tuple(prefix.shape) == (B,)),
-                 f"prefix must be [{B}, {docs}]")
-    ints = []
-    for name, t in (("q_starts", q_starts), ("k_starts", k_starts), ("prefix", prefix)):
-        if t is not None:
-            _require(t.dtype == torch.int32 and t.device == q.device, f"{name} must be int32 on the GPU of q")
-            t = t.contiguous()
-        ints.append(t)
-    _require(softcap >= 0, "softcap must not be negative")
-    radius = 0
+        if not causal:
+            raise IcsaArgumentError("prefix needs causal=True")
+        if prefix.shape != (B, docs) and (docs != 1 or prefix.shape != (B,)):
+            raise IcsaArgumentError(f"prefix must be [{B}, {docs}]")
+
+    def int32(t):
+        if t is None:
+            return None
+        if t.dtype != torch.int32 or t.device != dev:
+            raise IcsaArgumentError("q_starts, k_starts and prefix must be int32 on the GPU of q")
+        return t.contiguous()
+
+    q_starts, k_starts, prefix = int32(q_starts), int32(k_starts), int32(prefix)
+    if not softcap >= 0:
+        raise IcsaArgumentError("softcap must not be negative")
     if bias is not None:
-        _require(bias.dtype == torch.float32 and bias.device == q.device and bias.ndim == 2 and bias.shape[0] == H and
-                 bias.shape[1] % 2 == 1, f"bias must be float32 [{H}, 2 R + 1] on the GPU of q")
+        if bias.dtype != torch.float32 or bias.device != dev or bias.ndim != 2 or bias.shape[0] != H or bias.shape[1] % 2 != 1:
+            raise IcsaArgumentError(f"bias must be float32 [{H}, 2 R + 1] on the GPU of q")
         radius = bias.shape[1] // 2
         bias = bias.contiguous()
-    out_dtype = out_dtype or torch.bfloat16
-    _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be bfloat16 or float32")
+    out_dtype = out_dtype or bf16
+    if out_dtype not in (bf16, torch.float32):
+        raise IcsaArgumentError("out_dtype must be bfloat16 or float32")
     q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in map(inner_contiguous, (q, k, v)))
     out = torch.empty(B, Sq, H, D, dtype=out_dtype, device=q.device)
     L = _lib.lib()
     ws_bytes = L.icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D)
     if ws_bytes < 0:
         raise _lib.IcsaError("icsa_masked_attn_workspace_size", int(ws_bytes))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    with on_device(q.device):
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    with on_device(dev):
         rc = L.icsa_masked_attn(
-            ptr(q), *q.stride()[:3],
-            ptr(k), *k.stride()[:3],
-            ptr(v), *v.stride()[:3],
+            q.data_ptr(), *q.stride()[:3],
+            k.data_ptr(), *k.stride()[:3],
+            v.data_ptr(), *v.stride()[:3],
             B, Sq, Sk, H, Hk, D,
-            ptr(ints[0]), ptr(ints[1]), docs, int(causal), ptr(ints[2]),
+            ptr(q_starts), ptr(k_starts), docs, int(causal), ptr(prefix),
             float(D ** -0.5 if softmax_scale is None else softmax_scale), float(softcap), ptr(bias), radius,
-            ptr(out), dtype_code(out), *out.stride()[:3],
-            ptr(ws), ws_bytes, stream_ptr(q.device))
+            out.data_ptr(), _lib.BF16 if out_dtype == bf16 else _lib.F32, *out.stride()[:3],
+            ptr(ws), ws_bytes, stream_ptr(dev))
     _lib.check("icsa_masked_attn", rc)
     return out
 

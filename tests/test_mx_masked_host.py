@@ -24,7 +24,8 @@ def test_sizes():
         Kp = -(-K // 256) * 256
         assert L.icsa_mx_codes_size(M, K) == M * Kp // 2 and L.icsa_mx_scales_size(M, K) == M * Kp // 32
         assert L.icsa_mx_linear_workspace_size(M, 8, K, _lib.MXFP4) == 0
-        assert L.icsa_mx_linear_workspace_size(M, 8, K, _lib.BF16) >= M * Kp * 17 // 32
+        # one or two rows are quantised inside the product
+        assert L.icsa_mx_linear_workspace_size(M, 8, K, _lib.BF16) >= (M * Kp * 17 // 32 if M > 2 else 0)
     assert L.icsa_mx_codes_size(-1, 4) == -1 and L.icsa_mx_scales_size(4, 0) == -1
     assert L.icsa_mx_linear_workspace_size(4, 0, 4, _lib.BF16) == -1
     assert L.icsa_masked_attn_workspace_size(1, 9373, 9373, 12, 12, 128) == 0
