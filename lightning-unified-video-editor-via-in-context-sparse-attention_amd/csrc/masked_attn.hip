@@ -33,6 +33,12 @@
 #define MA_MAX_SPLIT 256
 #define MA_MIN_SPLIT_TILES 4                          // key tiles a split part is worth
 #define MA_BIAS_MARGIN ATT_BN
+#ifndef MA_AHEAD
+#define MA_AHEAD 4
+#endif
+#ifndef MA_PRIO
+#define MA_PRIO(x) __builtin_amdgcn_s_setprio(x)
+#endif
 #define MA_LDS_MAX (160 * 1024)
 
 namespace {
@@ -300,12 +306,22 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
     if (rows_valid <= 0) continue;                                     // a wave without rows moves tiles only
     const bool partial = wg_partial && __ballot(j0 < see_lo || j0 + ATT_BN > see_hi) != 0ull;   // for some row of the wave
 
+    // operands are read MA_AHEAD products ahead of their use
     floatx16 s[2] = {};
+    {
+      bf16x8 ka[2 * kSteps];
+      auto k_op = [&](int x) __attribute__((always_inline)) { ka[x] = *reinterpret_cast<const bf16x8*>(ks + kro[x >> 1] + (x & 1) * 32 * T::kRow); };
 #pragma unroll
-    for (int kk = 0; kk < kSteps; ++kk) {
+      for (int x = 0; x < MA_AHEAD; ++x) k_op(x);
+      __builtin_amdgcn_sched_barrier(0);
+      MA_PRIO(1);
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
-        s[sub] = mfma32x32x16(*reinterpret_cast<const bf16x8*>(ks + kro[kk] + sub * 32 * T::kRow), qf[kk], s[sub]);
+      for (int x = 0; x < 2 * kSteps; ++x) {
+        if (x + MA_AHEAD < 2 * kSteps) k_op(x + MA_AHEAD);
+        s[x & 1] = mfma32x32x16(ka[x], qf[x >> 1], s[x & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      MA_PRIO(0);
     }
     // Scores in units of log2, as base + mul * s.  Capped: cap tanh(x) = cap - 2 cap r with r = 1 / (1 + exp(2 x)), so
     // s becomes r; with a bias s becomes the score itself.
@@ -398,15 +414,25 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
     l_run += rs;
 
     if (!(partial && uni(ctl[16 + (t & 1)]) == t + 1)) {
+      bf16x8 va[4 * kSub];
+      auto v_op = [&](int x) __attribute__((always_inline)) {
+        const unsigned char* at = vs + vro[x % kSub] + x / kSub * 16 * T::kRow;
+        const rt_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rt_lds_v4s)at);
+        const rt_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rt_lds_v4s)(at + 8 * T::kRow));
+        const short __attribute__((ext_vector_type(8))) a8 = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        va[x] = __builtin_bit_cast(bf16x8, a8);
+      };
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+      for (int x = 0; x < MA_AHEAD; ++x) v_op(x);
+      __builtin_amdgcn_sched_barrier(0);
+      MA_PRIO(1);
 #pragma unroll
-        for (int ds = 0; ds < kSub; ++ds) {
-          const rt_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rt_lds_v4s)(vs + vro[ds] + m * 16 * T::kRow));
-          const rt_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((rt_lds_v4s)(vs + vro[ds] + (m * 16 + 8) * T::kRow));
-          const short __attribute__((ext_vector_type(8))) a8 = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          o[ds] = mfma32x32x16(__builtin_bit_cast(bf16x8, a8), pf[m], o[ds]);
-        }
+      for (int x = 0; x < 4 * kSub; ++x) {
+        if (x + MA_AHEAD < 4 * kSub) v_op(x + MA_AHEAD);
+        o[x % kSub] = mfma32x32x16(va[x], pf[x / kSub], o[x % kSub]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      MA_PRIO(0);
     } else {
       // key by key, to the rows that see it: P through the wave's scratch, 32 keys at a time
 #pragma unroll
