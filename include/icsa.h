@@ -363,8 +363,8 @@ int icsa_wan_ln_modulate(const void* x, int x_dtype, int64_t x_sb, int64_t x_ss,
                          const float* shift, const float* scale, int64_t mod_sb, float eps,
                          int B, int S, int dim, void* out, int64_t o_sb, int64_t o_ss, void* stream);
 
-/* Workspace bytes of icsa_masked_attn (partials of keys split over workgroups; 0 for most sizes). */
-int64_t icsa_masked_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D);
+/* Workspace bytes of icsa_masked_attn (sums of keys split over workgroups; 0 for most sizes). */
+int64_t icsa_masked_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs, int causal);
 
 /* Attention under masks: out_i = sum_j softmax_j(s_ij) v_j over the keys that query i sees,
  *   s_ij = cap tanh(scale q_i.k_j / cap) + bias[h][clamp(j - p_i, -radius, radius) + radius]

@@ -268,9 +268,11 @@ struct MaskedAttnParams {
   float scale, softcap;                           // softcap 0: none
   const float* bias; int radius;                  // [H, 2 radius + 1] or null
   OutView out;
-  int n_split; float* part;                       // key ranges an item is split into; their partials
+  int n_whole, n_split; float* part;              // MaskedPlan; the parts' sums
 };
-int masked_attn_splits(int B, int Sq, int Sk, int H, int Hk);
-int64_t masked_attn_part_floats(int B, int Sq, int H, int Hk, int D, int n_split);
+// items 0 .. n_whole - 1 are taken whole, the keys of the others in n_split parts
+struct MaskedPlan { int n_whole, n_split; };
+MaskedPlan masked_attn_plan(int B, int Sq, int Sk, int H, int Hk, bool alike);
+int64_t masked_attn_part_floats(int B, int Sq, int H, int Hk, int D, MaskedPlan f);
 bool masked_attn_bias_fits(int H, int Hk, int D, int radius);
 hipError_t launch_masked_attn(const MaskedAttnParams& p, hipStream_t stream);

@@ -31,6 +31,8 @@
 #define MA_LOG2E 1.4426950408889634f
 #define MA_TARGET_WG 512                              // two workgroups a CU
 #define MA_MAX_SPLIT 256
+#define MA_TAIL_ROUNDS 8                              // up to so many rounds a last, incomplete one is cut in parts
+#define MA_TAIL_TILES 32                              // from so many key tiles on
 #define MA_MIN_SPLIT_TILES 4                          // key tiles a split part is worth
 #define MA_BIAS_MARGIN ATT_BN
 #ifndef MA_AHEAD
@@ -184,11 +186,14 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS;
-  const int64_t items = (int64_t)p.B * p.Hk * n_blk * p.n_split;
-  const int w = xcd_remap(blockIdx.x, (int)items);
+  // whole items, then parts of items, each list dealt to the XCDs in runs; last row blocks first: under a
+  // causal mask they are the longest
+  const int n_parts = (p.B * p.Hk * n_blk - p.n_whole) * p.n_split, whole_wg = xcd_grid(p.n_whole);
+  const bool cut = (int)blockIdx.x >= whole_wg;
+  const int w = cut ? xcd_remap(blockIdx.x - whole_wg, n_parts) : xcd_remap(blockIdx.x, p.n_whole);
   if (w < 0) return;
-  // last row blocks first: under a causal mask they are the longest
-  const int split = w % p.n_split, blk = n_blk - 1 - w / p.n_split % n_blk, bh = w / p.n_split / n_blk;
+  const int item = cut ? p.n_whole + w / p.n_split : w, split = cut ? w % p.n_split : 0, n_split = cut ? p.n_split : 1;
+  const int blk = n_blk - 1 - item % n_blk, bh = item / n_blk;
   const int b = bh / p.Hk, hk = bh % p.Hk;
   const int r0 = blk * MA_ROWS + 32 * wave;
   const int rows_valid = min(32, n_rows - r0);
@@ -229,8 +234,8 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   int t0 = 0, t1 = 0;
   if (u_hi > u_lo) {
     const int first = u_lo / ATT_BN, n = (u_hi + ATT_BN - 1) / ATT_BN - first;
-    t0 = first + (int)((int64_t)n * split / p.n_split);
-    t1 = first + (int)((int64_t)n * (split + 1) / p.n_split);
+    t0 = first + (int)((int64_t)n * split / n_split);
+    t1 = first + (int)((int64_t)n * (split + 1) / n_split);
   }
 
   // ---- loads ----
@@ -463,32 +468,27 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   }
 
   if (rows_valid <= 0) return;
-  if (p.n_split > 1) {
-    // a row's raw O, reference max and sum: [item][split][row][D], then [item][split][2][row]
-    const int64_t part = ((int64_t)bh * n_blk + blk) * p.n_split + split;
-    const float l = xhalf_sum(l_run);
-    if (li < rows_valid) {
-      float* dst = p.part + (part * MA_ROWS + 32 * wave + li) * D + 4 * hl;
-#pragma unroll
-      for (int ds = 0; ds < kSub; ++ds)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<floatx4*>(dst + 32 * ds + 8 * g) =
-              some ? floatx4{o[ds][4 * g], o[ds][4 * g + 1], o[ds][4 * g + 2], o[ds][4 * g + 3]} : floatx4{};
-      if (hl == 0) {
-        float* ml = p.part + (int64_t)p.B * p.Hk * n_blk * p.n_split * MA_ROWS * D + part * 2 * MA_ROWS + 32 * wave + li;
-        ml[0] = some ? m_ref : MA_M_NONE;
-        ml[MA_ROWS] = some ? l : 0.f;
-      }
-    }
-    return;
-  }
+  const float l = xhalf_sum(l_run);
   if (!some) {                                         // whatever it holds of tiles that others see whole
 #pragma unroll
     for (int ds = 0; ds < kSub; ++ds) o[ds] = floatx16{};
   }
-  const float l = xhalf_sum(l_run);
-  store_wave<D>(p, scratch, o, !some || l == 0.f ? 0.f : 1.f / l, b, hk, r0, rows_valid);
+  if (!cut) {
+    store_wave<D>(p, scratch, o, !some || l == 0.f ? 0.f : 1.f / l, b, hk, r0, rows_valid);
+  } else if (li < rows_valid) {
+    // a row's raw O, reference max and sum: [part][row][D], then [part][2][row]
+    float* dst = p.part + ((int64_t)w * MA_ROWS + 32 * wave + li) * D + 4 * hl;
+#pragma unroll
+    for (int ds = 0; ds < kSub; ++ds)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<floatx4*>(dst + 32 * ds + 8 * g) = floatx4{o[ds][4 * g], o[ds][4 * g + 1], o[ds][4 * g + 2], o[ds][4 * g + 3]};
+    if (hl == 0) {
+      float* ml = p.part + (int64_t)n_parts * MA_ROWS * D + (int64_t)w * 2 * MA_ROWS + 32 * wave + li;
+      ml[0] = some ? m_ref : MA_M_NONE;
+      ml[MA_ROWS] = some ? l : 0.f;
+    }
+  }
 }
 
 // Joins the parts of every row in order (bitwise reproducible).  256 threads take 1024 / D rows of one item, 4 dims each;
@@ -498,11 +498,11 @@ __global__ void __launch_bounds__(256) icsa_masked_combine_kernel(MaskedAttnPara
   constexpr int kPer = D / 4, kRows = 256 / kPer;
   __shared__ float wt[MA_MAX_SPLIT][kRows];
   const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS, n = p.n_split;
-  const int item = blockIdx.x / (MA_ROWS / kRows), row = blockIdx.x % (MA_ROWS / kRows) * kRows + threadIdx.x / kPer;
-  const int blk = item % n_blk, bh = item / n_blk, r = blk * MA_ROWS + row, t = threadIdx.x % kPer, x = threadIdx.x / kPer;
+  const int n_items = p.B * p.Hk * n_blk, x_item = blockIdx.x / (MA_ROWS / kRows), item = p.n_whole + x_item, row = blockIdx.x % (MA_ROWS / kRows) * kRows + threadIdx.x / kPer;
+  const int blk = n_blk - 1 - item % n_blk, bh = item / n_blk, r = blk * MA_ROWS + row, t = threadIdx.x % kPer, x = threadIdx.x / kPer;
   if (blk * MA_ROWS + (int)(blockIdx.x % (MA_ROWS / kRows)) * kRows >= n_rows) return;     // uniform
-  const int64_t part0 = (int64_t)item * n;
-  const float* ml = p.part + (int64_t)p.B * p.Hk * n_blk * n * MA_ROWS * D + part0 * 2 * MA_ROWS + row;
+  const int64_t part0 = (int64_t)x_item * n;
+  const float* ml = p.part + (int64_t)(n_items - p.n_whole) * n * MA_ROWS * D + part0 * 2 * MA_ROWS + row;
   const bool on = r < n_rows;
   float m = MA_M_NONE;
   for (int s = t; s < n; s += kPer) m = fmaxf(m, on ? ml[(int64_t)s * 2 * MA_ROWS] : MA_M_NONE);
@@ -533,20 +533,36 @@ __global__ void __launch_bounds__(256) icsa_masked_combine_kernel(MaskedAttnPara
   }
 }
 
-// Parts that an item's keys are cut into: enough workgroups for two a CU, each with a few tiles.
-int masked_attn_splits(int B, int Sq, int Sk, int H, int Hk) {
+// Which items are whole, and how many parts the others' keys are cut into.  Few items: all in parts, enough for MA_TARGET_WG
+// workgroups of a few tiles each.  Some rounds of alike items (no causal mask, no documents; else the hardware fills the gaps as
+// items end): the last, incomplete round's items in parts, as many as make the rounds come out shortest, where a part is long
+// against its sums' way through memory.
+MaskedPlan masked_attn_plan(int B, int Sq, int Sk, int H, int Hk, bool alike) {
+  MaskedPlan f = {0, 1};
   const int64_t rows = (int64_t)Sq * (H / Hk), items = (int64_t)B * Hk * ((rows + MA_ROWS - 1) / MA_ROWS);
   const int tiles = (Sk + ATT_BN - 1) / ATT_BN;
-  if (items <= 0 || items * 2 > MA_TARGET_WG) return 1;
-  int64_t n = (MA_TARGET_WG + items - 1) / items;
-  n = n < tiles / MA_MIN_SPLIT_TILES ? n : tiles / MA_MIN_SPLIT_TILES;
-  return n < 1 ? 1 : n > MA_MAX_SPLIT ? MA_MAX_SPLIT : (int)n;
+  f.n_whole = (int)items;
+  if (items <= 0) return f;
+  if (items * 2 <= MA_TARGET_WG) {
+    int64_t n = (MA_TARGET_WG + items - 1) / items;
+    n = n < tiles / MA_MIN_SPLIT_TILES ? n : tiles / MA_MIN_SPLIT_TILES;
+    if (n > 1) { f.n_whole = 0; f.n_split = n > MA_MAX_SPLIT ? MA_MAX_SPLIT : (int)n; }
+    return f;
+  }
+  const int64_t tail = items % MA_TARGET_WG;
+  if (!alike || tail == 0 || items > MA_TAIL_ROUNDS * MA_TARGET_WG || tiles < MA_TAIL_TILES) return f;
+  double best = 1.0;
+  for (int n = 2; n <= 8 && tiles / n >= MA_TAIL_TILES / 4; ++n) {
+    const double rounds = (double)((tail * n + MA_TARGET_WG - 1) / MA_TARGET_WG) / n + 0.03 * n;
+    if (rounds < best) { best = rounds; f.n_split = n; }
+  }
+  if (f.n_split > 1) f.n_whole = (int)(items - tail);
+  return f;
 }
 
-int64_t masked_attn_part_floats(int B, int Sq, int H, int Hk, int D, int n_split) {
-  if (n_split <= 1) return 0;
-  const int64_t rows = (int64_t)Sq * (H / Hk);
-  return (int64_t)B * Hk * ((rows + MA_ROWS - 1) / MA_ROWS) * n_split * MA_ROWS * (D + 2);
+int64_t masked_attn_part_floats(int B, int Sq, int H, int Hk, int D, MaskedPlan f) {
+  const int64_t rows = (int64_t)Sq * (H / Hk), items = (int64_t)B * Hk * ((rows + MA_ROWS - 1) / MA_ROWS);
+  return (items - f.n_whole) * f.n_split * MA_ROWS * (D + 2);
 }
 
 bool masked_attn_bias_fits(int H, int Hk, int D, int radius) {
@@ -562,13 +578,13 @@ hipError_t run_masked(const MaskedAttnParams& p, hipStream_t stream) {
   const int lds = ma_fixed_lds(D) + (kBias ? G * (2 * p.radius + 1 + 2 * MA_BIAS_MARGIN) * 4 : 0);
   const hipError_t a = ensure_lds_limit(reinterpret_cast<const void*>(icsa_masked_attn_kernel<D, kCap, kBias>), MA_LDS_MAX, &lds_set);
   if (a != hipSuccess) return a;
-  const int64_t blocks = (int64_t)p.B * p.Hk * (((int64_t)p.Sq * G + MA_ROWS - 1) / MA_ROWS);
-  if (blocks * p.n_split > 0x3fffffffLL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((icsa_masked_attn_kernel<D, kCap, kBias>), dim3(xcd_grid((int)(blocks * p.n_split))), dim3(MA_THREADS), lds,
-                     stream, p);
+  const int64_t items = (int64_t)p.B * p.Hk * (((int64_t)p.Sq * G + MA_ROWS - 1) / MA_ROWS), cut = items - p.n_whole;
+  if (items > 0x3fffffffLL || cut * p.n_split > 0x3fffffffLL) return hipErrorInvalidValue;
+  const int grid = xcd_grid(p.n_whole) + xcd_grid((int)(cut * p.n_split));
+  hipLaunchKernelGGL((icsa_masked_attn_kernel<D, kCap, kBias>), dim3(grid), dim3(MA_THREADS), lds, stream, p);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.n_split == 1) return e;
-  hipLaunchKernelGGL(icsa_masked_combine_kernel<D>, dim3((unsigned)(blocks * (MA_ROWS * D / 1024))), dim3(256), 0, stream, p);
+  if (e != hipSuccess || cut == 0) return e;
+  hipLaunchKernelGGL(icsa_masked_combine_kernel<D>, dim3((unsigned)(cut * (MA_ROWS * D / 1024))), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 

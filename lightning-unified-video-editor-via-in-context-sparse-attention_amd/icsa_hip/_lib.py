@@ -183,7 +183,7 @@ _SIGNATURES = {
         _p, _p, _i, _l, _p, _p,
         _p, _i, _i, _l, _i, _i, _p, _p,
         _i, _l, _p, _l, _p]),
-    "icsa_masked_attn_workspace_size": (_l, [_i, _i, _i, _i, _i, _i]),
+    "icsa_masked_attn_workspace_size": (_l, [_i, _i, _i, _i, _i, _i, _i, _i]),
     "icsa_masked_attn": (_i, [
         _p, _l, _l, _l,
         _p, _l, _l, _l,

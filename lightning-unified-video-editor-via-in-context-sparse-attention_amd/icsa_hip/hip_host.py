@@ -448,7 +448,7 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
     q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in map(inner_contiguous, (q, k, v)))
     out = torch.empty(B, Sq, H, D, dtype=out_dtype, device=q.device)
     L = _lib.lib()
-    ws_bytes = L.icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D)
+    ws_bytes = L.icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D, docs, int(causal))
     if ws_bytes < 0:
         raise _lib.IcsaError("icsa_masked_attn_workspace_size", int(ws_bytes))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None

@@ -28,10 +28,10 @@ def test_sizes():
         assert L.icsa_mx_linear_workspace_size(M, 8, K, _lib.BF16) >= (M * Kp * 17 // 32 if M > 2 else 0)
     assert L.icsa_mx_codes_size(-1, 4) == -1 and L.icsa_mx_scales_size(4, 0) == -1
     assert L.icsa_mx_linear_workspace_size(4, 0, 4, _lib.BF16) == -1
-    assert L.icsa_masked_attn_workspace_size(1, 9373, 9373, 12, 12, 128) == 0
-    assert L.icsa_masked_attn_workspace_size(1, 1, 65536, 40, 8, 128) > 0
-    assert L.icsa_masked_attn_workspace_size(1, 1, 65536, 40, 7, 128) == -1
-    assert L.icsa_masked_attn_workspace_size(1, 1, 65536, 40, 8, 96) == -1
+    assert L.icsa_masked_attn_workspace_size(1, 9373, 9373, 12, 12, 128, 1, 1) == 0
+    assert L.icsa_masked_attn_workspace_size(1, 1, 65536, 40, 8, 128, 1, 0) > 0
+    assert L.icsa_masked_attn_workspace_size(1, 1, 65536, 40, 7, 128, 1, 0) == -1
+    assert L.icsa_masked_attn_workspace_size(1, 1, 65536, 40, 8, 96, 1, 0) == -1
 
 
 def _mx_linear_args(**kw):
