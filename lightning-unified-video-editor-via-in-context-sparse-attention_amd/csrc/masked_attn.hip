@@ -186,14 +186,16 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS;
-  // whole items, then parts of items, each list dealt to the XCDs in runs; last row blocks first: under a
-  // causal mask they are the longest
-  const int n_parts = (p.B * p.Hk * n_blk - p.n_whole) * p.n_split, whole_wg = xcd_grid(p.n_whole);
+  // Whole items, then parts of items.  Alike ones: each list dealt to the XCDs in runs, a head's items side by side.  Under a causal
+  // mask: the longest rows of every head first, so that the last items to start are short ones; workgroups go round the
+  // XCDs, so an XCD has the same few heads all the way.
+  const int BH = p.B * p.Hk, n_parts = (BH * n_blk - p.n_whole) * p.n_split, whole_wg = xcd_grid(p.n_whole);
   const bool cut = (int)blockIdx.x >= whole_wg;
-  const int w = cut ? xcd_remap(blockIdx.x - whole_wg, n_parts) : xcd_remap(blockIdx.x, p.n_whole);
-  if (w < 0) return;
+  int w = cut ? blockIdx.x - whole_wg : blockIdx.x;
+  if (!p.causal) w = xcd_remap(w, cut ? n_parts : p.n_whole);
+  if (w < 0 || w >= (cut ? n_parts : p.n_whole)) return;
   const int item = cut ? p.n_whole + w / p.n_split : w, split = cut ? w % p.n_split : 0, n_split = cut ? p.n_split : 1;
-  const int blk = n_blk - 1 - item % n_blk, bh = item / n_blk;
+  const int blk = n_blk - 1 - (p.causal ? item / BH : item % n_blk), bh = p.causal ? item % BH : item / n_blk;
   const int b = bh / p.Hk, hk = bh % p.Hk;
   const int r0 = blk * MA_ROWS + 32 * wave;
   const int rows_valid = min(32, n_rows - r0);
@@ -498,11 +500,11 @@ __global__ void __launch_bounds__(256) icsa_masked_combine_kernel(MaskedAttnPara
   constexpr int kPer = D / 4, kRows = 256 / kPer;
   __shared__ float wt[MA_MAX_SPLIT][kRows];
   const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS, n = p.n_split;
-  const int n_items = p.B * p.Hk * n_blk, x_item = blockIdx.x / (MA_ROWS / kRows), item = p.n_whole + x_item, row = blockIdx.x % (MA_ROWS / kRows) * kRows + threadIdx.x / kPer;
-  const int blk = n_blk - 1 - item % n_blk, bh = item / n_blk, r = blk * MA_ROWS + row, t = threadIdx.x % kPer, x = threadIdx.x / kPer;
+  const int x_item = blockIdx.x / (MA_ROWS / kRows), item = p.n_whole + x_item, row = blockIdx.x % (MA_ROWS / kRows) * kRows + threadIdx.x / kPer;
+  const int BH = p.B * p.Hk, blk = n_blk - 1 - (p.causal ? item / BH : item % n_blk), bh = p.causal ? item % BH : item / n_blk, r = blk * MA_ROWS + row, t = threadIdx.x % kPer, x = threadIdx.x / kPer;
   if (blk * MA_ROWS + (int)(blockIdx.x % (MA_ROWS / kRows)) * kRows >= n_rows) return;     // uniform
   const int64_t part0 = (int64_t)x_item * n;
-  const float* ml = p.part + (int64_t)(n_items - p.n_whole) * n * MA_ROWS * D + part0 * 2 * MA_ROWS + row;
+  const float* ml = p.part + (int64_t)(BH * n_blk - p.n_whole) * n * MA_ROWS * D + part0 * 2 * MA_ROWS + row;
   const bool on = r < n_rows;
   float m = MA_M_NONE;
   for (int s = t; s < n; s += kPer) m = fmaxf(m, on ? ml[(int64_t)s * 2 * MA_ROWS] : MA_M_NONE);
