@@ -706,6 +706,7 @@ int icsa_mx_linear(const void* x, const void* x_scales, int x_dtype, int64_t x_s
   p.out_kind = out_dtype == ICSA_MXFP4 ? MX_OUT_MXFP4 : out_dtype == ICSA_F32 ? MX_OUT_F32 : MX_OUT_BF16;
   p.o_ss = out_dtype == ICSA_MXFP4 ? mx_padded(N) / 2 : o_ss;
   p.x_raw = x; p.x_dtype = x_dtype; p.x_ss = x_ss; p.K = K;
+  p.m_first = 0; p.m_last = (int)M;
   if (x_dtype != ICSA_MXFP4 && mx_rows_takes_raw(M, K)) {
     ICSA_HIP_TRY(launch_mx_rows(p, reinterpret_cast<hipStream_t>(stream_)), "mx product of few rows");
     return ICSA_OK;

@@ -265,7 +265,7 @@ hipError_t pick_mx_gemm(MxGemmParams p, hipStream_t stream) {
   if (e != hipSuccess) return e;
   p.m_first = (int)split;
   p.m_last = p.M;
-  return run_mx_gemm<2, 2, 2, 2, 4, kOut>(p, stream);
+  return mx_rows_takes(p.M - p.m_first, p.N) ? launch_mx_rows(p, stream) : run_mx_gemm<2, 2, 2, 2, 4, kOut>(p, stream);
 }
 
 }  // namespace

@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(1024) icsa_mx_rows_kernel(MxGemmParams p) {
     __syncthreads();
   }
   auto token_frag = [&](int t, int gg) -> MxFrag {
-    const int m = min(32 * t + li, p.M - 1);
+    const int m = min(p.m_first + 32 * t + li, p.m_last - 1);
     if constexpr (kSrc == 0) return load_frag(p.x, p.x_scales, line, p.M, m, gg, hl);
     else return load_frag(smem, xs, lds_line, p.M, m, gg, hl);
   };
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(1024) icsa_mx_rows_kernel(MxGemmParams p) {
       *reinterpret_cast<floatx4*>(red + ((wave * 4 + q) * 64 + lane) * 4) =
           floatx4{acc[t][4 * q], acc[t][4 * q + 1], acc[t][4 * q + 2], acc[t][4 * q + 3]};
     __syncthreads();
-    const int m = 32 * t + li;
+    const int m = p.m_first + 32 * t + li;
     auto total = [&](int q) -> floatx4 {
       floatx4 s = *reinterpret_cast<const floatx4*>(red + (q * 64 + lane) * 4);
       for (int v = 1; v < nw; ++v) {
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(1024) icsa_mx_rows_kernel(MxGemmParams p) {
     } else if (wave < 4) {
       const floatx4 s = total(wave);
       const int n = n0 + 8 * wave + 4 * hl;
-      if (m < p.M) {
+      if (m < p.m_last) {
         if constexpr (kOut == MX_OUT_F32) {
           float* dst = reinterpret_cast<float*>(p.out) + (int64_t)m * p.o_ss + n;
           if (n + 4 <= p.N) *reinterpret_cast<floatx4_a4*>(dst) = s;
@@ -168,7 +168,7 @@ hipError_t pick_mx_rows(const MxGemmParams& p, hipStream_t stream) {
   if (p.x_raw != nullptr) {
     return p.x_dtype == ICSA_DT_F32 ? run_mx_rows<1, 2, kOut>(p, stream) : run_mx_rows<1, 1, kOut>(p, stream);
   }
-  if (p.M <= 32) return run_mx_rows<1, 0, kOut>(p, stream);
+  if (p.m_last - p.m_first <= 32) return run_mx_rows<1, 0, kOut>(p, stream);
   return run_mx_rows<2, 0, kOut>(p, stream);
 }
 

@@ -79,7 +79,7 @@ __device__ __forceinline__ void store_mx(const MxGemmParams& p, float v[16], int
   const auto x = __builtin_amdgcn_permlane32_swap(q[0], q[1], false, false);
   const unsigned lo = x[0], hi = x[1];                 // this half's codes of groups 2 hl, 2 hl + 1: from hl = 0, 1
   const u32x2 c = {(lo & 0xffffu) | hi << 16, lo >> 16 | (hi & 0xffff0000u)};
-  if (m < p.M && n0 < Np) {
+  if (m < p.m_last && n0 < Np) {
     *reinterpret_cast<u32x2*>(reinterpret_cast<unsigned char*>(p.out) + (int64_t)m * p.o_ss + n0 / 2 + 8 * hl) = c;
     if (hl == 0)
       p.out_scales[((int64_t)(n0 / MX_GROUP) * p.M + m) * MX_GROUP_BLOCKS + n0 / MX_BLOCK % MX_GROUP_BLOCKS] = (unsigned char)s;
@@ -88,7 +88,7 @@ __device__ __forceinline__ void store_mx(const MxGemmParams& p, float v[16], int
 
 __device__ __forceinline__ void store_f32(const MxGemmParams& p, const float v[16], int n0, int m) {
   const int hl = (threadIdx.x & 63) >> 5;
-  if (m >= p.M) return;
+  if (m >= p.m_last) return;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const int n = n0 + 8 * g + 4 * hl;
@@ -120,8 +120,8 @@ __device__ __forceinline__ void store_bf16(const MxGemmParams& p, unsigned char*
     const int r = 16 * x + (lane >> 2), m = m0 + r;
     const u32x4 c = *reinterpret_cast<const u32x4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 2) & 3)) << 4));
     bf16* dst = reinterpret_cast<bf16*>(p.out) + (int64_t)m * p.o_ss + n;
-    if (m < p.M && n + 8 <= p.N) *reinterpret_cast<u32x4_a2*>(dst) = c;
-    else if (m < p.M) {
+    if (m < p.m_last && n + 8 <= p.N) *reinterpret_cast<u32x4_a2*>(dst) = c;
+    else if (m < p.m_last) {
       const bf16x8 b = __builtin_bit_cast(bf16x8, c);
 #pragma unroll
       for (int e = 0; e < 8; ++e) if (n + e < p.N) dst[e] = b[e];

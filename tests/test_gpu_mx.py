@@ -125,8 +125,9 @@ def test_linear(gpu, M, N, K, out_dtype, act, bias):
 
 
 def test_linear_large_tiles(gpu):
-    """Sizes that take the large tile (whole tiles for every compute unit), whole and ragged."""
-    for M, N, K in ((4096, 4096, 512), (4099, 4110, 300)):
+    """Sizes that take the large tile, whole and ragged, with several tiles a workgroup; sizes whose last rows go to
+    smaller tiles or to the kernel of few rows; one group of k."""
+    for M, N, K in ((4096, 4096, 512), (4099, 4110, 300), (3120, 5120, 1300), (9360, 2000, 1000), (4660, 4000, 900), (5000, 4500, 200)):
         print(f"[mx] large {M}x{N}x{K}", flush=True)
         _linear_case(gpu, M, N, K, BF, BF, None, torch.float32, M)
 
