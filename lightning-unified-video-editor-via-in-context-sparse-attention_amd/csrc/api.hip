@@ -594,8 +594,8 @@ int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
   if (!q_starts != !k_starts) return fail(ICSA_EINVAL, "q_starts and k_starts must be both given or both NULL");
   if (docs < 1 || (!q_starts && docs != 1)) return fail(ICSA_EINVAL, "docs=%d without document starts", docs);
   if (prefix && !causal) return fail(ICSA_EINVAL, "a prefix needs the causal mask");
-  if (!std::isfinite(scale) || !std::isfinite(softcap) || softcap < 0.f)
-    return fail(ICSA_EINVAL, "scale and softcap must be finite, softcap not negative");
+  if (!std::isfinite(scale) || !std::isfinite(softcap) || scale <= 0.f || softcap < 0.f)
+    return fail(ICSA_EINVAL, "scale must be positive and finite, softcap finite and not negative");
   if (bias && (radius < 0 || !masked_attn_bias_fits(H, Hk, D, radius)))
     return fail(ICSA_EUNSUPPORTED, "bias of radius %d for %d heads a key head does not fit the LDS", radius, H / Hk);
   if (Sq == 0) return ICSA_OK;

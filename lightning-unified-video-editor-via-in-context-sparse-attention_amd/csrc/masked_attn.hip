@@ -6,19 +6,28 @@
 // a tile of keys serves them all (one query token of a group is one tile of rows).
 //
 // A workgroup of 4 waves takes 128 rows of one (batch, key head) over the 64-key tiles of the union of
-// their ranges, or over one of n_split equal parts of it where rows are few (icsa_masked_combine_kernel joins
-// the parts).  Only tiles that some row sees in part are masked.  Scores are computed transposed, S^T = K Q^T: a lane
-// holds one row and 32 of a tile's 64 keys, the other 32 are in lane ^ 32 (attn_tile.h).  P goes to
-// the second product from its registers; V is read transposed from its row-major tile.
+// their ranges, or over one of n_split equal parts of it (icsa_masked_combine_kernel joins the parts): where rows are few, and
+// for the items of a last, incomplete round.  Only tiles that some row sees in part are masked.  Scores are
+// computed transposed, S^T = K Q^T: a lane holds one row and 32 of a tile's 64 keys, the other 32 are in lane ^ 32
+// (attn_tile.h).  P goes to the second product from its registers; V is read transposed from its row-major tile.
 //
-// K and V tiles arrive by direct global->LDS loads, two buffers, one barrier a tile: the tile after next is
-// requested when everybody has passed the barrier behind the last use of its buffer.  Two
-// workgroups share a CU: one's exponentials run beside the other's products.
+// K and V tiles arrive by direct global->LDS loads, two buffers, one barrier a tile: behind it the next tile is
+// requested into the buffer that everybody has left.  Two workgroups share a CU: one's exponentials run beside the
+// other's products.  Products read their operands from LDS three ahead of their use, with raised priority.
 //
 // Values in masked places: scores are replaced, not added to, so a NaN of a masked key does not
 // matter; V rows that no row of the workgroup sees are cleared in LDS; and where a partly visible tile holds
 // a V that is not finite, 0 * V would reach rows that do not see it, so that tile is added key by
-// key to the rows that do (add_tile_by_key).
+// key to the rows that do.
+//
+// What bounds it (two waves a SIMD): the vector instructions and the products of a tile side by side, 830 and 1,024 cycles a
+// wave with heads of 128; capped scores add two transcendentals an element (1,340).  9,373 tokens, 12 heads of 128: dense 610 us
+// (0.89 PFLOP/s in two rounds of workgroups, the second 73 % full), causal 317 (0.85), a prefix and capped scores 480 (0.64);
+// 32,760 tokens, 5 heads 2.87 ms (0.96); 9,373 tokens, 12 heads of 64 340 us (0.79).  One query of 40 heads over 8 key heads of
+// 65,536 keys: 43 us for 268 MB and 11.6 for joining 64 parts.  Short documents (packed prompts of 350 keys, 40 heads, 32,760
+// queries: 415 us) add the way of Q and the output through memory, 140 us at the copy rate, which two
+// workgroups a CU do not hide.  Several items a workgroup, with the next one's start before the last one's stores, was
+// slower there (495 us: 20 spilled registers, and items of different lengths dealt out beforehand).
 #include "attn_tile.h"
 #include "icsa_kernels.h"
 
@@ -35,12 +44,7 @@
 #define MA_TAIL_TILES 32                              // from so many key tiles on
 #define MA_MIN_SPLIT_TILES 4                          // key tiles a split part is worth
 #define MA_BIAS_MARGIN ATT_BN
-#ifndef MA_AHEAD
-#define MA_AHEAD 4
-#endif
-#ifndef MA_PRIO
-#define MA_PRIO(x) __builtin_amdgcn_s_setprio(x)
-#endif
+#define MA_AHEAD 3                                    // operands read ahead; 4 and 6 measured alike or 3 % slower
 #define MA_LDS_MAX (160 * 1024)
 
 namespace {
@@ -63,7 +67,7 @@ __device__ __forceinline__ RowRange doc_range(const MaskedAttnParams& p, int i, 
   RowRange r = {0, 0, 0};
   k0 = min(max(k0, 0), p.Sk);
   k1 = min(max(k1, 0), p.Sk);
-  const int64_t at = (int64_t)i + k1 - q1;
+  const int64_t at = (int64_t)i + k1 - min(q1, p.Sq);
   r.at = (int)max((int64_t)-0x40000000, min((int64_t)0x40000000, at));
   int64_t end = k1;
   if (p.causal) end = min(end, max(at + 1, (int64_t)k0 + prefix));
@@ -116,6 +120,20 @@ __device__ __forceinline__ int wave_max(int x) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) x = max(x, __shfl_xor(x, o, 64));
   return x;
+}
+
+// Sum of a lane's 32 probabilities as they go into the second product, rounded to bf16: where few keys carry a row, what their
+// rounding adds to the product it adds to the sum, and the quotient does not see it.  Two values an instruction.
+__device__ __forceinline__ float sum_p(const bf16x8 pf[4]) {
+  const bf16x2 one = {(bf16)1.f, (bf16)1.f};
+  float r[4];
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    r[m] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) r[m] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{pf[m][e], pf[m][e + 1]}, one, r[m], false);
+  }
+  return (r[0] + r[1]) + (r[2] + r[3]);
 }
 
 // One wave's 32 rows of 32 dims to the output: through 2 KB of the wave's LDS, so that bf16
@@ -224,8 +242,9 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
     const float* src = p.bias + (int64_t)hk * G * width;                 // the group's heads
     for (int x = threadIdx.x; x < G * bias_row; x += MA_THREADS) {
       const int h = x / bias_row, at = x - h * bias_row;
-      const float f = src[h * width + min(max(at - MA_BIAS_MARGIN, 0), width - 1)];   // a type's lowest value stays finite in units of log2, an infinity does not
-      bias_lds[x] = __builtin_isinf(f) ? f : fminf(fmaxf(f * MA_LOG2E, -3.4028234663852886e38f), 3.4028234663852886e38f);
+      const float f = src[h * width + min(max(at - MA_BIAS_MARGIN, 0), width - 1)];
+      // a type's lowest value stays finite in units of log2; infinities and NaN are kept
+      bias_lds[x] = !__builtin_isfinite(f) ? f : fminf(fmaxf(f * MA_LOG2E, -3.4028234663852886e38f), 3.4028234663852886e38f);
     }
   }
   __syncthreads();
@@ -321,14 +340,14 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
 #pragma unroll
       for (int x = 0; x < MA_AHEAD; ++x) k_op(x);
       __builtin_amdgcn_sched_barrier(0);
-      MA_PRIO(1);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int x = 0; x < 2 * kSteps; ++x) {
         if (x + MA_AHEAD < 2 * kSteps) k_op(x + MA_AHEAD);
         s[x & 1] = mfma32x32x16(ka[x], qf[x >> 1], s[x & 1]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      MA_PRIO(0);
+      __builtin_amdgcn_s_setprio(0);
     }
     // Scores in units of log2, as base + mul * s.  Capped: cap tanh(x) = cap - 2 cap r with r = 1 / (1 + exp(2 x)), so
     // s becomes r; with a bias s becomes the score itself.
@@ -380,16 +399,11 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
     float rs = 0.f;
     if (!first) {
       const float off = base - m_ref;
-      float rsv[4] = {};
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[sub][i], mul, off));
-          rsv[i & 3] += e;
-          pf[2 * sub + (i >> 3)][i & 7] = (bf16)e;
-        }
-      rs = (rsv[0] + rsv[1]) + (rsv[2] + rsv[3]);
+        for (int i = 0; i < 16; ++i) pf[2 * sub + (i >> 3)][i & 7] = (bf16)__builtin_amdgcn_exp2f(fmaf(s[sub][i], mul, off));
+      rs = sum_p(pf);
     }
     if (first || __ballot(!(rs <= MA_PSUM_MAX)) != 0ull) {
       float mx = -INFINITY;
@@ -407,15 +421,11 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
       l_run *= al;
       m_ref = mn;
       const float off = base - m_ref;
-      rs = 0.f;
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[sub][i], mul, off));
-          rs += e;
-          pf[2 * sub + (i >> 3)][i & 7] = (bf16)e;
-        }
+        for (int i = 0; i < 16; ++i) pf[2 * sub + (i >> 3)][i & 7] = (bf16)__builtin_amdgcn_exp2f(fmaf(s[sub][i], mul, off));
+      rs = sum_p(pf);
       first = false;
     }
     l_run += rs;
@@ -432,14 +442,14 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
 #pragma unroll
       for (int x = 0; x < MA_AHEAD; ++x) v_op(x);
       __builtin_amdgcn_sched_barrier(0);
-      MA_PRIO(1);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int x = 0; x < 4 * kSub; ++x) {
         if (x + MA_AHEAD < 4 * kSub) v_op(x + MA_AHEAD);
         o[x % kSub] = mfma32x32x16(va[x], pf[x / kSub], o[x % kSub]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      MA_PRIO(0);
+      __builtin_amdgcn_s_setprio(0);
     } else {
       // key by key, to the rows that see it: P through the wave's scratch, 32 keys at a time
 #pragma unroll

@@ -394,7 +394,7 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
             keys that all of its queries see.
         softcap: scores become ``softcap * tanh(score / softcap)``; 0 leaves them.
         bias: float32 [H, 2 R + 1], added to the (capped) scores: ``bias[h, clamp(j - p_i, -R, R) + R]``.
-        softmax_scale: default ``D ** -0.5``.
+        softmax_scale: positive, default ``D ** -0.5``.
 
     A query that sees nothing gets zeros; NaN and infinities in keys and values reach only the
     queries that see them.  An inference operator: under an enabled grad mode an input that requires a
@@ -435,8 +435,9 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
         return t.contiguous()
 
     q_starts, k_starts, prefix = int32(q_starts), int32(k_starts), int32(prefix)
-    if not softcap >= 0:
-        raise IcsaArgumentError("softcap must not be negative")
+    scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
+    if not (scale > 0 and softcap >= 0):
+        raise IcsaArgumentError("softmax_scale must be positive and softcap not negative")
     if bias is not None:
         if bias.dtype != torch.float32 or bias.device != dev or bias.ndim != 2 or bias.shape[0] != H or bias.shape[1] % 2 != 1:
             raise IcsaArgumentError(f"bias must be float32 [{H}, 2 R + 1] on the GPU of q")
@@ -459,7 +460,7 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
             v.data_ptr(), *v.stride()[:3],
             B, Sq, Sk, H, Hk, D,
             ptr(q_starts), ptr(k_starts), docs, int(causal), ptr(prefix),
-            float(D ** -0.5 if softmax_scale is None else softmax_scale), float(softcap), ptr(bias), radius,
+            scale, float(softcap), ptr(bias), radius,
             out.data_ptr(), _lib.BF16 if out_dtype == bf16 else _lib.F32, *out.stride()[:3],
             ptr(ws), ws_bytes, stream_ptr(dev))
     _lib.check("icsa_masked_attn", rc)

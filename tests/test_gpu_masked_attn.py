@@ -80,13 +80,66 @@ def test_documents(gpu, case, mask, D):
     if mask == "prefix":
         kw["prefix"] = _i32([[11 * n + 5 for n in range(qs.shape[1] - 1)]] * B)
     if case == 6:
-        # the oracle takes the clamped keys: the last document ends at the last key
-        ref, bound = O.attention(*_inputs(B, 200, 210, 2, 1, D, case), **{**kw, "k_starts": ks.clamp(max=210)})
+        # the oracle takes the clamped borders: the last document ends at the last query and key
+        ref, bound = O.attention(*_inputs(B, 200, 210, 2, 1, D, case),
+                                 **{**kw, "q_starts": qs.clamp(max=200), "k_starts": ks.clamp(max=210)})
         out = masked_attn_func(*(t.to(gpu) for t in _inputs(B, 200, 210, 2, 1, D, case)),
                                **{n: x.to(gpu) if isinstance(x, torch.Tensor) else x for n, x in kw.items()})
         assert ((out.double().cpu() - ref).abs() <= bound + 2.0 ** -8 * ref.abs()).all()
         return
     _check(gpu, *_inputs(B, 200, 210, 2, 1, D, case), **kw)
+
+
+@pytest.mark.parametrize("n", [62, 63, 64, 65, 150])
+def test_many_documents(gpu, n):
+    """Around the number of documents whose borders fit a wave's lanes, one query to several each, some empty."""
+    print(f"[masked] {n} documents", flush=True)
+    g = torch.Generator().manual_seed(n)
+    qs = torch.sort(torch.randint(0, 201, (2, n + 1), generator=g), 1).values.to(torch.int32)
+    ks = torch.sort(torch.randint(0, 301, (2, n + 1), generator=g), 1).values.to(torch.int32)
+    kw = dict(q_starts=qs, k_starts=ks)
+    _check(gpu, *_inputs(2, 200, 300, 2, 1, 64, n), **kw)
+    _check(gpu, *_inputs(2, 200, 300, 2, 1, 64, n), causal=True, prefix=torch.full((2, n), 2, dtype=torch.int32), **kw)
+
+
+def test_starts_that_decrease_stay_inside(gpu):
+    """Borders in no order: no promise on the values, but nothing outside the tensors is read and what is written is finite."""
+    q, k, v = _inputs(1, 300, 300, 2, 2, 64, 1)
+    g = torch.Generator().manual_seed(2)
+    for n in (5, 80):
+        st = torch.randint(-1000, 1000, (2, 1, n + 1), generator=g, dtype=torch.int32)
+        out = masked_attn_func(q.to(gpu), k.to(gpu), v.to(gpu), q_starts=st[0].to(gpu), k_starts=st[1].to(gpu), causal=True)
+        assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("softcap", [0.0, 4.0])
+def test_softmax_scale(gpu, softcap):
+    q, k, v = _inputs(1, 90, 130, 2, 2, 128, 12)
+    for scale in (1e-4, 0.3):
+        _check(gpu, q, k, v, softmax_scale=scale, softcap=softcap)
+    with pytest.raises(ValueError):
+        masked_attn_func(q.to(gpu), k.to(gpu), v.to(gpu), softmax_scale=-1.0)
+
+
+def test_bias_not_a_number(gpu):
+    """A NaN of the table reaches the rows that see a key at its distance."""
+    q, k, v = _inputs(1, 40, 40, 2, 2, 64, 13)
+    bias = torch.zeros(2, 9)
+    bias[1, 6] = math.nan                                    # two keys ahead, head 1
+    out = masked_attn_func(q.to(gpu), k.to(gpu), v.to(gpu), bias=bias.to(gpu)).cpu()
+    assert torch.isfinite(out[:, :, 0]).all()
+    assert torch.isnan(out[0, :38, 1]).all() and torch.isfinite(out[0, 38:, 1]).all()
+
+
+def test_last_round_in_parts(gpu):
+    """Alike items that leave the last round of workgroups short: its items' keys in parts.  Against the dense kernel, both
+    within (2^-8 of P + 2^-8 of the output + the scores' few 2^-20) max |v|."""
+    for H, S, D in ((9, 8300, 128), (12, 6200, 128)):
+        q, k, v = (torch.randn(1, S, H, D, device=gpu).to(BF) for _ in range(3))
+        out, ref = masked_attn_func(q, k, v), flash_attn_func(q, k, v)
+        top = v.abs().max().item()
+        assert (out.float() - ref.float()).abs().max().item() <= 2.0 ** -6 * 1.05 * top
+        assert torch.equal(out, masked_attn_func(q, k, v))
 
 
 @pytest.mark.parametrize("D,R,cap,H,Hk", [(64, 0, 0.0, 3, 3), (64, 16, 0.0, 4, 2), (128, 128, 0.0, 2, 2), (128, 5, 30.0, 2, 1),

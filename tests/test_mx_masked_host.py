@@ -83,7 +83,8 @@ def _masked_args(**kw):
     (dict(B=0), _lib.EINVAL), (dict(Sq=-1), _lib.EINVAL), (dict(H=3, Hk=2), _lib.EINVAL), (dict(Hk=0), _lib.EINVAL),
     (dict(D=96), _lib.EUNSUPPORTED), (dict(Sq=1 << 30, H=2), _lib.EUNSUPPORTED), (dict(od=2), _lib.EINVAL),
     (dict(qst=PTR), _lib.EINVAL), (dict(docs=2), _lib.EINVAL), (dict(docs=0, qst=PTR, kst=PTR), _lib.EINVAL),
-    (dict(prefix=PTR), _lib.EINVAL), (dict(scale=math.inf), _lib.EINVAL), (dict(cap=-1.0), _lib.EINVAL),
+    (dict(prefix=PTR), _lib.EINVAL), (dict(scale=math.inf), _lib.EINVAL), (dict(scale=0.0), _lib.EINVAL),
+    (dict(scale=-0.1), _lib.EINVAL), (dict(cap=-1.0), _lib.EINVAL),
     (dict(cap=math.nan), _lib.EINVAL), (dict(bias=PTR, radius=-1), _lib.EUNSUPPORTED),
     (dict(bias=PTR, radius=1 << 20), _lib.EUNSUPPORTED), (dict(q=0), _lib.EINVAL), (dict(k=0), _lib.EINVAL),
     (dict(out=0), _lib.EINVAL), (dict(q=PTR + 2), _lib.EINVAL), (dict(k_ss=130), _lib.EINVAL), (dict(k_ss=-128), _lib.EINVAL),
