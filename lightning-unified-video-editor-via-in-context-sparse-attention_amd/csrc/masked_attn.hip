@@ -24,7 +24,7 @@
 // wave with heads of 128; capped scores add two transcendentals an element (1,340).  9,373 tokens, 12 heads of 128: dense 610 us
 // (0.89 PFLOP/s in two rounds of workgroups, the second 73 % full), causal 317 (0.85), a prefix and capped scores 480 (0.64);
 // 32,760 tokens, 5 heads 2.87 ms (0.96); 9,373 tokens, 12 heads of 64 340 us (0.79).  One query of 40 heads over 8 key heads of
-// 65,536 keys: 43 us for 268 MB and 11.6 for joining 64 parts.  Short documents (packed prompts of 350 keys, 40 heads, 32,760
+// 65,536 keys: 43 us for 268 MB and 5 for joining 64 parts.  Short documents (packed prompts of 350 keys, 40 heads, 32,760
 // queries: 415 us) add the way of Q and the output through memory, 140 us at the copy rate, which two
 // workgroups a CU do not hide.  Several items a workgroup, with the next one's start before the last one's stores, was
 // slower there (495 us: 20 spilled registers, and items of different lengths dealt out beforehand).
@@ -40,6 +40,7 @@
 #define MA_LOG2E 1.4426950408889634f
 #define MA_TARGET_WG 512                              // two workgroups a CU
 #define MA_MAX_SPLIT 256
+#define MA_FEW_PARTS 16                               // from so many parts on a row's are shared by thread groups
 #define MA_TAIL_ROUNDS 8                              // up to so many rounds a last, incomplete one is cut in parts
 #define MA_TAIL_TILES 32                              // from so many key tiles on
 #define MA_MIN_SPLIT_TILES 4                          // key tiles a split part is worth
@@ -503,36 +504,56 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   }
 }
 
-// Joins the parts of every row in order (bitwise reproducible).  256 threads take 1024 / D rows of one item, 4 dims each;
-// a row's threads first work out every part's weight 2^(m_s - max) / sum between them.
-template <int D>
+// Joins the parts of every row, in a fixed order (bitwise reproducible).  256 threads, D / 4 for each of their rows (4 dims a
+// thread); kFew, where parts are many and rows few: one row, whose parts the 1024 / D thread groups share.
+template <int D, bool kFew>
 __global__ void __launch_bounds__(256) icsa_masked_combine_kernel(MaskedAttnParams p) {
-  constexpr int kPer = D / 4, kRows = 256 / kPer;
+  constexpr int kPer = D / 4, kGroups = 256 / kPer, kRows = kFew ? 1 : kGroups;
   __shared__ float wt[MA_MAX_SPLIT][kRows];
+  __shared__ __attribute__((aligned(16))) float acc[kFew ? kGroups : 1][D];
   const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS, n = p.n_split;
-  const int x_item = blockIdx.x / (MA_ROWS / kRows), item = p.n_whole + x_item, row = blockIdx.x % (MA_ROWS / kRows) * kRows + threadIdx.x / kPer;
-  const int BH = p.B * p.Hk, blk = n_blk - 1 - (p.causal ? item / BH : item % n_blk), bh = p.causal ? item % BH : item / n_blk, r = blk * MA_ROWS + row, t = threadIdx.x % kPer, x = threadIdx.x / kPer;
-  if (blk * MA_ROWS + (int)(blockIdx.x % (MA_ROWS / kRows)) * kRows >= n_rows) return;     // uniform
+  const int t = threadIdx.x % kPer, grp = threadIdx.x / kPer, x = kFew ? 0 : grp;
+  const int x_item = blockIdx.x / (MA_ROWS / kRows), row = blockIdx.x % (MA_ROWS / kRows) * kRows + x, item = p.n_whole + x_item;
+  const int BH = p.B * p.Hk, blk = n_blk - 1 - (p.causal ? item / BH : item % n_blk), bh = p.causal ? item % BH : item / n_blk;
+  const int r = blk * MA_ROWS + row;
+  if (r - x >= n_rows) return;                        // uniform: the block's first row
+  const bool on = r < n_rows;
   const int64_t part0 = (int64_t)x_item * n;
   const float* ml = p.part + (int64_t)(BH * n_blk - p.n_whole) * n * MA_ROWS * D + part0 * 2 * MA_ROWS + row;
-  const bool on = r < n_rows;
-  float m = MA_M_NONE;
+  // every part's weight 2^(m_s - max), and the sum of the row, by the row's first threads
+  float m = MA_M_NONE, l = 0.f;
   for (int s = t; s < n; s += kPer) m = fmaxf(m, on ? ml[(int64_t)s * 2 * MA_ROWS] : MA_M_NONE);
 #pragma unroll
   for (int o = kPer / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kPer));
-  for (int s = t; s < n; s += kPer) wt[s][x] = on ? __builtin_amdgcn_exp2f(ml[(int64_t)s * 2 * MA_ROWS] - m) : 0.f;
-  __syncthreads();
-  if (!on) return;
-  float l = 0.f;
-  for (int s = 0; s < n; ++s) l = fmaf(ml[(int64_t)s * 2 * MA_ROWS + MA_ROWS], wt[s][x], l);
-  floatx4 o = {};
-  const float* src = p.part + (part0 * MA_ROWS + row) * D + 4 * t;
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const floatx4 v = *reinterpret_cast<const floatx4*>(src + (int64_t)s * MA_ROWS * D);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], wt[s][x], o[e]);
+  for (int s = t; s < n; s += kPer) {
+    const float w = on ? __builtin_amdgcn_exp2f(ml[(int64_t)s * 2 * MA_ROWS] - m) : 0.f;
+    if (on) l = fmaf(ml[(int64_t)s * 2 * MA_ROWS + MA_ROWS], w, l);
+    if (!kFew || grp == 0) wt[s][x] = w;
   }
+#pragma unroll
+  for (int o = kPer / 2; o >= 1; o >>= 1) l += __shfl_xor(l, o, kPer);
+  __syncthreads();
+  floatx4 o = {};
+  if (on) {
+    const float* src = p.part + (part0 * MA_ROWS + row) * D + 4 * t;
+    const int s1 = kFew ? n * (grp + 1) / kGroups : n;
+#pragma unroll 8
+    for (int s = kFew ? n * grp / kGroups : 0; s < s1; ++s) {
+      const floatx4 v = *reinterpret_cast<const floatx4*>(src + (int64_t)s * MA_ROWS * D);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(v[e], wt[s][x], o[e]);
+    }
+  }
+  if constexpr (kFew) {
+    *reinterpret_cast<floatx4*>(&acc[grp][4 * t]) = o;
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll
+    for (int y = 1; y < kGroups; ++y)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += acc[y][4 * t + e];
+  }
+  if (!on) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t off = row_at(p.out.sb, p.out.ss, p.out.sh, bh / p.Hk, bh % p.Hk, G, r) + 4 * t;
   if (p.out.dtype == ICSA_DT_BF16) {
@@ -596,7 +617,10 @@ hipError_t run_masked(const MaskedAttnParams& p, hipStream_t stream) {
   hipLaunchKernelGGL((icsa_masked_attn_kernel<D, kCap, kBias>), dim3(grid), dim3(MA_THREADS), lds, stream, p);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || cut == 0) return e;
-  hipLaunchKernelGGL(icsa_masked_combine_kernel<D>, dim3((unsigned)(cut * (MA_ROWS * D / 1024))), dim3(256), 0, stream, p);
+  if (p.n_split >= MA_FEW_PARTS)
+    hipLaunchKernelGGL((icsa_masked_combine_kernel<D, true>), dim3((unsigned)(cut * MA_ROWS)), dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((icsa_masked_combine_kernel<D, false>), dim3((unsigned)(cut * (MA_ROWS * D / 1024))), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
