@@ -258,6 +258,26 @@ hipError_t launch_mx_rows(const MxGemmParams& p, hipStream_t stream);
 
 // ---------------------------------------------------------------- attention under masks (masked_attn.hip)
 #define MA_ROWS 128                  // rows (query, head of the group) of a workgroup
+// n / d for 0 <= n < 2^31 by a multiplication (Granlund and Montgomery): a kernel's integer division takes 25
+// vector instructions, also of uniform values
+struct FastDiv {
+  unsigned d, m, s1, s2;
+  __host__ __device__ __forceinline__ unsigned div(unsigned n) const {
+#ifdef __HIP_DEVICE_COMPILE__
+    const unsigned t = __umulhi(m, n);
+#else
+    const unsigned t = (unsigned)(((unsigned long long)m * n) >> 32);
+#endif
+    return (t + ((n - t) >> s1)) >> s2;
+  }
+  __host__ __device__ __forceinline__ unsigned mod(unsigned n) const { return n - div(n) * d; }
+};
+inline FastDiv fast_div(unsigned d) {
+  unsigned l = 0;
+  while ((1ull << l) < d) ++l;
+  const unsigned m = (unsigned)(((1ull << 32) * ((1ull << l) - d)) / d + 1);
+  return FastDiv{d, m, l < 1 ? l : 1u, l < 1 ? 0u : l - 1};
+}
 struct MaskedAttnParams {
   const bf16* q; int64_t q_sb, q_ss, q_sh;        // [B, Sq, H, D]
   const bf16* k; int64_t k_sb, k_ss, k_sh;        // [B, Sk, Hk, D]
@@ -269,10 +289,11 @@ struct MaskedAttnParams {
   const float* bias; int radius;                  // [H, 2 radius + 1] or null
   OutView out;
   int n_whole, n_split; float* part;              // MaskedPlan; the parts' sums
+  FastDiv by_g, by_blk, by_hk, by_bh, by_split;   // heads of a group, row blocks, key heads, B Hk, parts (set by the launch)
 };
 // items 0 .. n_whole - 1 are taken whole, the keys of the others in n_split parts
 struct MaskedPlan { int n_whole, n_split; };
 MaskedPlan masked_attn_plan(int B, int Sq, int Sk, int H, int Hk, bool alike);
 int64_t masked_attn_part_floats(int B, int Sq, int H, int Hk, int D, MaskedPlan f);
 bool masked_attn_bias_fits(int H, int Hk, int D, int radius);
-hipError_t launch_masked_attn(const MaskedAttnParams& p, hipStream_t stream);
+hipError_t launch_masked_attn(MaskedAttnParams p, hipStream_t stream);

@@ -13,7 +13,7 @@
 //
 // K and V tiles arrive by direct global->LDS loads, two buffers, one barrier a tile: behind it the next tile is
 // requested into the buffer that everybody has left.  Two workgroups share a CU: one's exponentials run beside the
-// other's products.  Products read their operands from LDS three ahead of their use, with raised priority.
+// other's products.  Products read their operands from LDS four ahead of their use, with raised priority.
 //
 // Values in masked places: scores are replaced, not added to, so a NaN of a masked key does not
 // matter; V rows that no row of the workgroup sees are cleared in LDS; and where a partly visible tile holds
@@ -45,7 +45,7 @@
 #define MA_TAIL_TILES 32                              // from so many key tiles on
 #define MA_MIN_SPLIT_TILES 4                          // key tiles a split part is worth
 #define MA_BIAS_MARGIN ATT_BN
-#define MA_AHEAD 3                                    // operands read ahead; 4 and 6 measured alike or 3 % slower
+#define MA_AHEAD 4                                    // operands read ahead; 2, 3 and 5 measured alike or up to 3 % slower
 #define MA_LDS_MAX (160 * 1024)
 
 namespace {
@@ -123,6 +123,14 @@ __device__ __forceinline__ int wave_max(int x) {
   return x;
 }
 
+// a where the mask's bits are set, b elsewhere (the compiler makes a comparison and a select of the C form, three
+// instructions with the mask's instead of two)
+__device__ __forceinline__ unsigned bit_select(unsigned mask, unsigned a, unsigned b) {
+  unsigned r;
+  asm("v_bfi_b32 %0, %1, %2, %3" : "=v"(r) : "v"(mask), "v"(a), "v"(b));
+  return r;
+}
+
 // Sum of a lane's 32 probabilities as they go into the second product, rounded to bf16: where few keys carry a row, what their
 // rounding adds to the product it adds to the sum, and the quotient does not see it.  Two values an instruction.
 __device__ __forceinline__ float sum_p(const bf16x8 pf[4]) {
@@ -170,18 +178,19 @@ __device__ __forceinline__ void store_dims32(unsigned char* stage, const float v
 }
 
 // element offset of row r (query r / G, head hk G + r % G) in a [B, S, H, D] tensor
-__device__ __forceinline__ int64_t row_at(int64_t sb, int64_t ss, int64_t sh, int b, int hk, int G, int r) {
-  return (int64_t)b * sb + (int64_t)(r / G) * ss + (int64_t)(hk * G + r % G) * sh;
+__device__ __forceinline__ int64_t row_at(int64_t sb, int64_t ss, int64_t sh, int b, int hk, const FastDiv& g, int r) {
+  const unsigned i = g.d == 1 ? r : g.div(r);
+  return (int64_t)b * sb + (int64_t)i * ss + (int64_t)(hk * g.d + r - i * g.d) * sh;
 }
 
 template <int D>
 __device__ __forceinline__ void store_wave(const MaskedAttnParams& p, unsigned char* stage, const floatx16 o[D / 32],
                                            float inv_l, int b, int hk, int r0, int rows_valid) {
-  const int lane = threadIdx.x & 63, li = lane & 31, G = p.H / p.Hk;
+  const int lane = threadIdx.x & 63, li = lane & 31;
   int64_t off[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) off[i] = row_at(p.out.sb, p.out.ss, p.out.sh, b, hk, G, r0 + 16 * i + (lane >> 2));
-  const int64_t own = row_at(p.out.sb, p.out.ss, p.out.sh, b, hk, G, r0 + li);
+  for (int i = 0; i < 2; ++i) off[i] = row_at(p.out.sb, p.out.ss, p.out.sh, b, hk, p.by_g, r0 + 16 * i + (lane >> 2));
+  const int64_t own = row_at(p.out.sb, p.out.ss, p.out.sh, b, hk, p.by_g, r0 + li);
 #pragma unroll
   for (int ds = 0; ds < D / 32; ++ds) {
     float v[16];
@@ -204,7 +213,7 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   float* const bias_lds = reinterpret_cast<float*>(scratch_all + MA_WAVES * MA_SCRATCH_WAVE + MA_CTL_BYTES);
   const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS;
+  const int G = p.by_g.d, n_rows = p.Sq * G, n_blk = p.by_blk.d;
   // Whole items, then parts of items.  Alike ones: each list dealt to the XCDs in runs, a head's items side by side.  Under a causal
   // mask: the longest rows of every head first, so that the last items to start are short ones; workgroups go round the
   // XCDs, so an XCD has the same few heads all the way.
@@ -213,26 +222,31 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   int w = cut ? blockIdx.x - whole_wg : blockIdx.x;
   if (!p.causal) w = xcd_remap(w, cut ? n_parts : p.n_whole);
   if (w < 0 || w >= (cut ? n_parts : p.n_whole)) return;
-  const int item = cut ? p.n_whole + w / p.n_split : w, split = cut ? w % p.n_split : 0, n_split = cut ? p.n_split : 1;
-  const int blk = n_blk - 1 - (p.causal ? item / BH : item % n_blk), bh = p.causal ? item % BH : item / n_blk;
-  const int b = bh / p.Hk, hk = bh % p.Hk;
+  const int item = cut ? p.n_whole + (int)p.by_split.div(w) : w, split = cut ? (int)p.by_split.mod(w) : 0;
+  const int blk = n_blk - 1 - (int)(p.causal ? p.by_bh.div(item) : p.by_blk.mod(item)), bh = p.causal ? p.by_bh.mod(item) : p.by_blk.div(item);
+  const int b = p.by_hk.div(bh), hk = p.by_hk.mod(bh);
   const int r0 = blk * MA_ROWS + 32 * wave;
   const int rows_valid = min(32, n_rows - r0);
 
   bf16x8 qf[kSteps];
   {
-    const bf16* src = p.q + row_at(p.q_sb, p.q_ss, p.q_sh, b, hk, G, min(r0 + li, n_rows - 1)) + 8 * hl;
+    const bf16* src = p.q + row_at(p.q_sb, p.q_ss, p.q_sh, b, hk, p.by_g, min(r0 + li, n_rows - 1)) + 8 * hl;
 #pragma unroll
     for (int kk = 0; kk < kSteps; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(src + 16 * kk);
   }
 
   // ---- what the rows see ----
-  RowRange rr = row_range(p, b, (r0 + li) / G);
+  RowRange rr = row_range(p, b, G == 1 ? r0 + li : p.by_g.div(r0 + li));
   if (li >= rows_valid) rr = RowRange{0, 0, 0};
   {
     const bool any = rr.hi > rr.lo;
-    const int lo = wave_min(any ? rr.lo : 0x7fffffff), hi = wave_max(any ? rr.hi : 0);
-    const int in_lo = wave_max(any ? rr.lo : 0), in_hi = wave_min(any ? rr.hi : 0x7fffffff);
+    int lo = any ? rr.lo : 0x7fffffff, hi = any ? rr.hi : 0, in_lo = any ? rr.lo : 0, in_hi = any ? rr.hi : 0x7fffffff;
+    if (__ballot(rr.lo != __builtin_amdgcn_readfirstlane(rr.lo) || rr.hi != __builtin_amdgcn_readfirstlane(rr.hi)) != 0ull) {
+      lo = wave_min(lo);                               // unless all rows see the same
+      hi = wave_max(hi);
+      in_lo = wave_max(in_lo);
+      in_hi = wave_min(in_hi);
+    }
     if (lane == 0) { ctl[wave] = lo; ctl[4 + wave] = hi; ctl[8 + wave] = in_lo; ctl[12 + wave] = in_hi; }
     if (threadIdx.x < 2) ctl[16 + threadIdx.x] = 0;
   }
@@ -256,8 +270,13 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   int t0 = 0, t1 = 0;
   if (u_hi > u_lo) {
     const int first = u_lo / ATT_BN, n = (u_hi + ATT_BN - 1) / ATT_BN - first;
-    t0 = first + (int)((int64_t)n * split / n_split);
-    t1 = first + (int)((int64_t)n * (split + 1) / n_split);
+    t0 = first;
+    t1 = first + n;
+    if (cut) {                                         // equal parts, the first ones a tile longer
+      const int q = p.by_split.div(n), more = n - q * p.n_split;
+      t0 = first + q * split + min(split, more);
+      t1 = t0 + q + (split < more);
+    }
   }
 
   // ---- loads ----
@@ -294,7 +313,7 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
     vro[ds] = row * T::kRow + (((col >> 3) ^ T::vswz(row)) << 4) + (col & 7) * 2;
   }
   unsigned char* const scratch = scratch_all + wave * MA_SCRATCH_WAVE;
-  const float* const my_bias = kBias ? bias_lds + ((r0 + li) % G) * bias_row + MA_BIAS_MARGIN + p.radius : nullptr;
+  const float* const my_bias = kBias ? bias_lds + (G == 1 ? 0 : p.by_g.mod(r0 + li)) * bias_row + MA_BIAS_MARGIN + p.radius : nullptr;
 
   floatx16 o[kSub] = {};
   float m_ref = MA_M_NONE, l_run = 0.f;
@@ -314,7 +333,7 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
       // this wave's 16 V rows: those that no row sees cleared, the others looked at
       const int row = 16 * wave + (lane >> 2), key = j0 + row;
       u32x4* own = reinterpret_cast<u32x4*>(vs + row * T::kRow + (lane & 3) * (T::kRow / 4));
-      bool bad = false;
+      unsigned bad = 0;
       if (key < u_lo || key >= u_hi) {
 #pragma unroll
         for (int e = 0; e < T::kRow / 64; ++e) own[e] = u32x4{0u, 0u, 0u, 0u};
@@ -323,10 +342,10 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
         for (int e = 0; e < T::kRow / 64; ++e) {
           const u32x4 x = own[e];
 #pragma unroll
-          for (int f = 0; f < 4; ++f) bad |= (x[f] & 0x7f80u) == 0x7f80u || (x[f] & 0x7f800000u) == 0x7f800000u;
+          for (int f = 0; f < 4; ++f) bad |= (x[f] & 0x7f807f80u) + 0x00800080u;     // a full exponent carries into the sign's bit
         }
       }
-      if (__ballot(bad) != 0ull && lane == 0) ctl[16 + (t & 1)] = t + 1;
+      if (__ballot((bad & 0x80008000u) != 0u) != 0ull && lane == 0) ctl[16 + (t & 1)] = t + 1;
     }
     ATT_BARRIER();
     if (t + 1 < t1) load_tile(t + 1);
@@ -390,9 +409,9 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int kbit = 8 * (i >> 2) + (i & 3);
-          const unsigned all = (unsigned)((int)(wd << (31 - kbit)) >> 31);
+          const unsigned all = (unsigned)__builtin_amdgcn_sbfe((int)wd, kbit, 1);    // the bit, over the whole word
           // score -inf: s is -inf, or +inf where the factor is negative
-          s[sub][i] = __uint_as_float((all & (kCap && !kBias ? 0x7f800000u : 0xff800000u)) | (__float_as_uint(s[sub][i]) & ~all));
+          s[sub][i] = __uint_as_float(bit_select(all, kCap && !kBias ? 0x7f800000u : 0xff800000u, __float_as_uint(s[sub][i])));
         }
       }
     }
@@ -487,7 +506,7 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
     for (int ds = 0; ds < kSub; ++ds) o[ds] = floatx16{};
   }
   if (!cut) {
-    store_wave<D>(p, scratch, o, !some || l == 0.f ? 0.f : 1.f / l, b, hk, r0, rows_valid);
+    store_wave<D>(p, scratch, o, !some || l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l), b, hk, r0, rows_valid);
   } else if (li < rows_valid) {
     // a row's raw O, reference max and sum: [part][row][D], then [part][2][row]
     float* dst = p.part + ((int64_t)w * MA_ROWS + 32 * wave + li) * D + 4 * hl;
@@ -511,10 +530,11 @@ __global__ void __launch_bounds__(256) icsa_masked_combine_kernel(MaskedAttnPara
   constexpr int kPer = D / 4, kGroups = 256 / kPer, kRows = kFew ? 1 : kGroups;
   __shared__ float wt[MA_MAX_SPLIT][kRows];
   __shared__ __attribute__((aligned(16))) float acc[kFew ? kGroups : 1][D];
-  const int G = p.H / p.Hk, n_rows = p.Sq * G, n_blk = (n_rows + MA_ROWS - 1) / MA_ROWS, n = p.n_split;
+  const int G = p.by_g.d, n_rows = p.Sq * G, n_blk = p.by_blk.d, n = p.n_split;
   const int t = threadIdx.x % kPer, grp = threadIdx.x / kPer, x = kFew ? 0 : grp;
   const int x_item = blockIdx.x / (MA_ROWS / kRows), row = blockIdx.x % (MA_ROWS / kRows) * kRows + x, item = p.n_whole + x_item;
-  const int BH = p.B * p.Hk, blk = n_blk - 1 - (p.causal ? item / BH : item % n_blk), bh = p.causal ? item % BH : item / n_blk;
+  const int BH = p.B * p.Hk, blk = n_blk - 1 - (int)(p.causal ? p.by_bh.div(item) : p.by_blk.mod(item)),
+            bh = p.causal ? p.by_bh.mod(item) : p.by_blk.div(item);
   const int r = blk * MA_ROWS + row;
   if (r - x >= n_rows) return;                        // uniform: the block's first row
   const bool on = r < n_rows;
@@ -555,7 +575,7 @@ __global__ void __launch_bounds__(256) icsa_masked_combine_kernel(MaskedAttnPara
   }
   if (!on) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t off = row_at(p.out.sb, p.out.ss, p.out.sh, bh / p.Hk, bh % p.Hk, G, r) + 4 * t;
+  const int64_t off = row_at(p.out.sb, p.out.ss, p.out.sh, p.by_hk.div(bh), p.by_hk.mod(bh), p.by_g, r) + 4 * t;
   if (p.out.dtype == ICSA_DT_BF16) {
     bf16x4 y;
 #pragma unroll
@@ -633,7 +653,13 @@ hipError_t pick_masked(const MaskedAttnParams& p, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_masked_attn(const MaskedAttnParams& p, hipStream_t stream) {
+hipError_t launch_masked_attn(MaskedAttnParams p, hipStream_t stream) {
+  const int G = p.H / p.Hk;
+  p.by_g = fast_div(G);
+  p.by_blk = fast_div((unsigned)(((int64_t)p.Sq * G + MA_ROWS - 1) / MA_ROWS));
+  p.by_hk = fast_div(p.Hk);
+  p.by_bh = fast_div(p.B * p.Hk);
+  p.by_split = fast_div(p.n_split);
   // a tile's rows must be addressable with 32-bit offsets
   if (p.k_ss * 2 * ATT_BN > 0x7fffffffLL || p.v_ss * 2 * ATT_BN > 0x7fffffffLL) return hipErrorInvalidValue;
   return p.D == 128 ? pick_masked<128>(p, stream) : pick_masked<64>(p, stream);
