@@ -374,6 +374,20 @@ def flash_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dropout_p
     return out
 
 
+def _rows16(t: torch.Tensor):
+    """t [B, S, H, D] bf16 with a unit stride in each row and rows on 16 bytes (itself where they are), and its
+    address and outer strides."""
+    s0, s1, s2, s3 = t.stride()
+    p = t.data_ptr()
+    if s3 != 1 or (p | ((s0 | s1 | s2) << 1)) & 15:
+        t = t.contiguous()
+        if t.data_ptr() & 15:
+            t = t.clone()
+        s0, s1, s2, _ = t.stride()
+        p = t.data_ptr()
+    return t, (p, s0, s1, s2)
+
+
 def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_starts: torch.Tensor = None,
                      k_starts: torch.Tensor = None, causal: bool = False, prefix: torch.Tensor = None,
                      softcap: float = 0.0, bias: torch.Tensor = None, softmax_scale: float = None,
@@ -427,14 +441,11 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
         if prefix.shape != (B, docs) and (docs != 1 or prefix.shape != (B,)):
             raise IcsaArgumentError(f"prefix must be [{B}, {docs}]")
 
-    def int32(t):
-        if t is None:
-            return None
-        if t.dtype != torch.int32 or t.device != dev:
-            raise IcsaArgumentError("q_starts, k_starts and prefix must be int32 on the GPU of q")
-        return t.contiguous()
-
-    q_starts, k_starts, prefix = int32(q_starts), int32(k_starts), int32(prefix)
+    if q_starts is not None or prefix is not None:
+        for t in (q_starts, k_starts, prefix):
+            if t is not None and (t.dtype != torch.int32 or t.device != dev):
+                raise IcsaArgumentError("q_starts, k_starts and prefix must be int32 on the GPU of q")
+        q_starts, k_starts, prefix = (None if t is None else t.contiguous() for t in (q_starts, k_starts, prefix))
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
     if not (scale > 0 and softcap >= 0):
         raise IcsaArgumentError("softmax_scale must be positive and softcap not negative")
@@ -446,23 +457,23 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
     out_dtype = out_dtype or bf16
     if out_dtype not in (bf16, torch.float32):
         raise IcsaArgumentError("out_dtype must be bfloat16 or float32")
-    q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in map(inner_contiguous, (q, k, v)))
-    out = torch.empty(B, Sq, H, D, dtype=out_dtype, device=q.device)
+    q, qa = _rows16(q)
+    k, ka = _rows16(k)
+    v, va = _rows16(v)
+    out = torch.empty(B, Sq, H, D, dtype=out_dtype, device=dev)
     L = _lib.lib()
-    ws_bytes = L.icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D, docs, int(causal))
-    if ws_bytes < 0:
-        raise _lib.IcsaError("icsa_masked_attn_workspace_size", int(ws_bytes))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    wsp, ws_bytes = 0, L.icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D, docs, int(causal))
+    if ws_bytes:
+        if ws_bytes < 0:
+            raise _lib.IcsaError("icsa_masked_attn_workspace_size", int(ws_bytes))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        wsp = ws.data_ptr()
     with on_device(dev):
         rc = L.icsa_masked_attn(
-            q.data_ptr(), *q.stride()[:3],
-            k.data_ptr(), *k.stride()[:3],
-            v.data_ptr(), *v.stride()[:3],
-            B, Sq, Sk, H, Hk, D,
-            ptr(q_starts), ptr(k_starts), docs, int(causal), ptr(prefix),
-            scale, float(softcap), ptr(bias), radius,
-            out.data_ptr(), _lib.BF16 if out_dtype == bf16 else _lib.F32, *out.stride()[:3],
-            ptr(ws), ws_bytes, stream_ptr(dev))
+            *qa, *ka, *va, B, Sq, Sk, H, Hk, D,
+            ptr(q_starts), ptr(k_starts), docs, int(causal), ptr(prefix), scale, softcap, ptr(bias), radius,
+            out.data_ptr(), _lib.BF16 if out_dtype is bf16 else _lib.F32, Sq * H * D, H * D, D,
+            wsp, ws_bytes, stream_ptr(dev))
     _lib.check("icsa_masked_attn", rc)
     return out
 

@@ -97,7 +97,7 @@ class MXFP4Tensor:
             raise IcsaArgumentError("codes must be on the GPU")
         if dtype not in _OUT_CODES:
             raise IcsaArgumentError("dtype must be bfloat16 or float32")
-        out = torch.empty(self.shape, dtype=dtype, device=dev)
+        out = torch.empty(*self.shape, dtype=dtype, device=dev)
         with on_device(dev):
             rc = _lib.lib().icsa_mx_dequantize(*self._ptrs, self.rows, K, out.data_ptr(), _OUT_CODES[dtype], K, stream_ptr(dev))
         _lib.check("icsa_mx_dequantize", rc)
@@ -170,7 +170,7 @@ def mx_linear(x, weight: MXFP4Tensor, bias: torch.Tensor = None, activation: str
         out = MXFP4Tensor._empty(shape, dev)
         (op, osc), o_code = out._ptrs, _lib.MXFP4
     else:
-        out = torch.empty(shape, dtype=out_dtype, device=dev)
+        out = torch.empty(*shape, dtype=out_dtype, device=dev)
         op, osc, o_code = out.data_ptr(), 0, _OUT_CODES[out_dtype]
     with on_device(dev):
         rc = L.icsa_mx_linear(xp, xs, x_code, x_ss, *weight._ptrs, bp, b_code, _ACTIVATIONS[activation],
