@@ -596,6 +596,11 @@ int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
   if (prefix && !causal) return fail(ICSA_EINVAL, "a prefix needs the causal mask");
   if (!std::isfinite(scale) || !std::isfinite(softcap) || scale <= 0.f || softcap < 0.f)
     return fail(ICSA_EINVAL, "scale must be positive and finite, softcap finite and not negative");
+  // Capped scores are a difference of numbers of the cap's size: over 4,096 its f32 rounding would pass that of the
+  // probabilities to bf16.  The factors to units of log2 must be finite numbers.
+  if (softcap > 0.f && (softcap > 4096.f || softcap < 1e-30f || !std::isfinite(4.f * scale / softcap)))
+    return fail(ICSA_EUNSUPPORTED, "softcap %g: 0 (none), or up to 4096 and not vanishing beside the scale", (double)softcap);
+  if (!std::isfinite(2.f * scale)) return fail(ICSA_EUNSUPPORTED, "scale %g is too large", (double)scale);
   if (bias && (radius < 0 || !masked_attn_bias_fits(H, Hk, D, radius)))
     return fail(ICSA_EUNSUPPORTED, "bias of radius %d for %d heads a key head does not fit the LDS", radius, H / Hk);
   if (Sq == 0) return ICSA_OK;
@@ -604,11 +609,13 @@ int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
       (Sk > 0 && (!row_ok(k, ICSA_BF16, k_sb, k_ss, k_sh) || !row_ok(v, ICSA_BF16, v_sb, v_ss, v_sh))))
     return fail(ICSA_EINVAL, "rows must be 16-byte aligned (pointers and strides)");
   if (k_ss < 0 || v_ss < 0) return fail(ICSA_EINVAL, "negative key stride");
+  if (Sk > 1 && (k_ss > 0x7fffffffLL / 128 || v_ss > 0x7fffffffLL / 128))
+    return fail(ICSA_EUNSUPPORTED, "64 rows of k and v must lie within 2 GiB");
   MaskedAttnParams p;
   std::memset(&p, 0, sizeof(p));
   p.q = reinterpret_cast<const bf16*>(q); p.q_sb = q_sb; p.q_ss = q_ss; p.q_sh = q_sh;
-  p.k = reinterpret_cast<const bf16*>(k); p.k_sb = k_sb; p.k_ss = k_ss; p.k_sh = k_sh;
-  p.v = reinterpret_cast<const bf16*>(v); p.v_sb = v_sb; p.v_ss = v_ss; p.v_sh = v_sh;
+  p.k = reinterpret_cast<const bf16*>(k); p.k_sb = k_sb; p.k_ss = Sk > 1 ? k_ss : 0; p.k_sh = k_sh;
+  p.v = reinterpret_cast<const bf16*>(v); p.v_sb = v_sb; p.v_ss = Sk > 1 ? v_ss : 0; p.v_sh = v_sh;
   p.B = B; p.Sq = Sq; p.Sk = Sk; p.H = H; p.Hk = Hk; p.D = D;
   p.q_starts = q_starts; p.k_starts = k_starts; p.docs = docs; p.causal = causal != 0; p.prefix = prefix;
   p.scale = scale; p.softcap = softcap; p.bias = bias; p.radius = radius;
@@ -624,8 +631,10 @@ int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
 }
 
 // ---- 4-bit floating point ----
-int64_t icsa_mx_codes_size(int64_t M, int K) { return M < 0 || K <= 0 ? -1 : M * (mx_padded(K) / 2); }
-int64_t icsa_mx_scales_size(int64_t M, int K) { return M < 0 || K <= 0 ? -1 : M * (mx_padded(K) / MX_BLOCK); }
+static_assert((int64_t)ICSA_MX_MAX_K / 2 * 256 <= 0x7fffffffLL, "256 rows of codes lie within 32-bit offsets");
+static bool mx_sizes_ok(int64_t M, int K) { return M >= 0 && M <= ICSA_MX_MAX_ROWS && K > 0 && K <= ICSA_MX_MAX_K; }
+int64_t icsa_mx_codes_size(int64_t M, int K) { return mx_sizes_ok(M, K) ? M * (mx_padded(K) / 2) : -1; }
+int64_t icsa_mx_scales_size(int64_t M, int K) { return mx_sizes_ok(M, K) ? M * (mx_padded(K) / MX_BLOCK) : -1; }
 
 static int check_mx_operand(const void* codes, const void* scales, const char* name) {
   if (!codes || !scales) return fail(ICSA_EINVAL, "%s: codes or scales are NULL", name);
@@ -668,7 +677,7 @@ int icsa_mx_dequantize(const void* codes, const void* scales, int64_t M, int K, 
 }
 
 int64_t icsa_mx_linear_workspace_size(int64_t M, int N, int K, int x_dtype) {
-  if (M < 0 || N <= 0 || K <= 0) return -1;
+  if (!mx_sizes_ok(M, K) || !mx_sizes_ok(N, K) || N == 0) return -1;
   if (x_dtype == ICSA_MXFP4 || mx_rows_takes_raw(M, K)) return 0;
   return align256(icsa_mx_codes_size(M, K)) + align256(icsa_mx_scales_size(M, K));
 }

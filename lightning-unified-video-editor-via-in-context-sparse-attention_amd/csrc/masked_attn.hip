@@ -660,7 +660,5 @@ hipError_t launch_masked_attn(MaskedAttnParams p, hipStream_t stream) {
   p.by_hk = fast_div(p.Hk);
   p.by_bh = fast_div(p.B * p.Hk);
   p.by_split = fast_div(p.n_split);
-  // a tile's rows must be addressable with 32-bit offsets
-  if (p.k_ss * 2 * ATT_BN > 0x7fffffffLL || p.v_ss * 2 * ATT_BN > 0x7fffffffLL) return hipErrorInvalidValue;
   return p.D == 128 ? pick_masked<128>(p, stream) : pick_masked<64>(p, stream);
 }

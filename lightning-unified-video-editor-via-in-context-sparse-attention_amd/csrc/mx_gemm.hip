@@ -271,8 +271,6 @@ hipError_t pick_mx_gemm(MxGemmParams p, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_mx_gemm(MxGemmParams p, hipStream_t stream) {
-  // a tile's rows must be addressable with 32-bit offsets
-  if ((int64_t)p.groups * (MX_GROUP / 2) * 256 > 0x7fffffffLL) return hipErrorInvalidValue;
   p.m_first = 0;
   p.m_last = p.M;
   if (mx_rows_takes(p.M, p.N)) return launch_mx_rows(p, stream);

@@ -406,7 +406,7 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
             sees the keys up to it.
         prefix: int32 [B, N] ([B] without documents), with ``causal``: a document's first
             keys that all of its queries see.
-        softcap: scores become ``softcap * tanh(score / softcap)``; 0 leaves them.
+        softcap: scores become ``softcap * tanh(score / softcap)`` (up to 4096); 0 leaves them.
         bias: float32 [H, 2 R + 1], added to the (capped) scores: ``bias[h, clamp(j - p_i, -R, R) + R]``.
         softmax_scale: positive, default ``D ** -0.5``.
 
@@ -440,7 +440,6 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
             raise IcsaArgumentError("prefix needs causal=True")
         if prefix.shape != (B, docs) and (docs != 1 or prefix.shape != (B,)):
             raise IcsaArgumentError(f"prefix must be [{B}, {docs}]")
-
     if q_starts is not None or prefix is not None:
         for t in (q_starts, k_starts, prefix):
             if t is not None and (t.dtype != torch.int32 or t.device != dev):

@@ -44,7 +44,7 @@ class MXFP4Tensor:
     256; a block's values are its codes' times ``2^(scale - 127)``, 255 stands for NaN.  Both
     16-byte aligned."""
 
-    __slots__ = ("_codes", "_scales", "_buf", "_ptrs", "shape", "rows", "device")
+    __slots__ = ("_codes", "_scales", "_buf", "shape", "rows", "device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape):
         shape = torch.Size(shape)
@@ -57,7 +57,7 @@ class MXFP4Tensor:
             raise IcsaArgumentError(f"codes must be [{rows}, {Kp // 2}] and scales [{Kp // MX_GROUP}, {rows}, 8]")
         if codes.device != scales.device or not codes.is_contiguous() or not scales.is_contiguous():
             raise IcsaArgumentError("codes and scales must be contiguous, on one device")
-        self._codes, self._scales, self._buf, self._ptrs = codes, scales, None, (codes.data_ptr(), scales.data_ptr())
+        self._codes, self._scales, self._buf = codes, scales, None
         self.shape, self.rows, self.device = shape, rows, codes.device
 
     @classmethod
@@ -67,11 +67,16 @@ class MXFP4Tensor:
         rows, Kp = math.prod(shape[:-1]), _padded(shape[-1])
         n = rows * (Kp // 2)                                      # a multiple of 128
         t._buf = torch.empty(n + rows * (Kp // 32), dtype=torch.uint8, device=device)
-        p = t._buf.data_ptr()
         t._codes = t._scales = None
-        t._ptrs = (p, p + n)
         t.shape, t.rows, t.device = torch.Size(shape), rows, t._buf.device
         return t
+
+    def _ptrs(self):
+        """Addresses of the codes and the scales."""
+        if self._buf is None:
+            return self._codes.data_ptr(), self._scales.data_ptr()
+        p = self._buf.data_ptr()
+        return p, p + self.rows * (_padded(self.shape[-1]) // 2)
 
     @property
     def codes(self) -> torch.Tensor:
@@ -99,7 +104,7 @@ class MXFP4Tensor:
             raise IcsaArgumentError("dtype must be bfloat16 or float32")
         out = torch.empty(*self.shape, dtype=dtype, device=dev)
         with on_device(dev):
-            rc = _lib.lib().icsa_mx_dequantize(*self._ptrs, self.rows, K, out.data_ptr(), _OUT_CODES[dtype], K, stream_ptr(dev))
+            rc = _lib.lib().icsa_mx_dequantize(*self._ptrs(), self.rows, K, out.data_ptr(), _OUT_CODES[dtype], K, stream_ptr(dev))
         _lib.check("icsa_mx_dequantize", rc)
         return out
 
@@ -123,7 +128,7 @@ def mx_quantize(x: torch.Tensor) -> MXFP4Tensor:
     t = MXFP4Tensor._empty(x.shape, dev)
     r = _rows(x)
     with on_device(dev):
-        rc = _lib.lib().icsa_mx_quantize(r.data_ptr(), code, r.stride(0), t.rows, t.shape[-1], *t._ptrs, stream_ptr(dev))
+        rc = _lib.lib().icsa_mx_quantize(r.data_ptr(), code, r.stride(0), t.rows, t.shape[-1], *t._ptrs(), stream_ptr(dev))
     _lib.check("icsa_mx_quantize", rc)
     return t
 
@@ -156,24 +161,24 @@ def mx_linear(x, weight: MXFP4Tensor, bias: torch.Tensor = None, activation: str
         bp = bias.data_ptr()
     L = _lib.lib()
     if mx_in:
-        M, (xp, xs), x_code, x_ss, wsp, ws_bytes = x.rows, x._ptrs, _lib.MXFP4, 0, 0, 0
+        M, (xp, xs), x_code, x_ss, wsp, ws_bytes = x.rows, x._ptrs(), _lib.MXFP4, 0, 0, 0
     else:
         r = _rows(x)
         M, xp, xs, x_code, x_ss = r.shape[0], r.data_ptr(), 0, dtype_code(r), r.stride(0)
         ws_bytes = L.icsa_mx_linear_workspace_size(M, N, K, x_code)
         wsp = 0
-        if ws_bytes:
+        if ws_bytes > 0:
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
             wsp = ws.data_ptr()
     shape = (*x.shape[:-1], N)
     if out_dtype == "mxfp4":
         out = MXFP4Tensor._empty(shape, dev)
-        (op, osc), o_code = out._ptrs, _lib.MXFP4
+        (op, osc), o_code = out._ptrs(), _lib.MXFP4
     else:
         out = torch.empty(*shape, dtype=out_dtype, device=dev)
         op, osc, o_code = out.data_ptr(), 0, _OUT_CODES[out_dtype]
     with on_device(dev):
-        rc = L.icsa_mx_linear(xp, xs, x_code, x_ss, *weight._ptrs, bp, b_code, _ACTIVATIONS[activation],
+        rc = L.icsa_mx_linear(xp, xs, x_code, x_ss, *weight._ptrs(), bp, b_code, _ACTIVATIONS[activation],
                               M, N, K, op, osc, o_code, N, wsp, ws_bytes, stream_ptr(dev))
     _lib.check("icsa_mx_linear", rc)
     return out

@@ -241,3 +241,25 @@ def test_same_as_dense_attention(gpu):
     for fn in (flash_attn_func, masked_attn_func):
         out = fn(q.to(gpu), k.to(gpu), v.to(gpu)).double().cpu()
         assert ((out - ref).abs() <= bound + 2.0 ** -8 * ref.abs()).all()
+
+
+@pytest.mark.parametrize("cap", [1e-3, 4096.0])
+def test_smallest_and_largest_caps(gpu, cap):
+    """The bound counts a few roundings of numbers of the cap's size."""
+    q, k, v = _inputs(1, 70, 200, 2, 1, 64, 21, 3.0)
+    _check(gpu, q, k, v, causal=True, softcap=cap)
+    _check(gpu, q, k, v, softcap=cap, bias=torch.randn(2, 9))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_far_apart(gpu, D):
+    """Rows 512 KB apart, 4.7 GB a tensor: what lies behind 32-bit offsets equals the same rows side by side."""
+    big = torch.zeros(1, 9001, 1 << 18, dtype=BF, device=gpu)
+    views = [big[:, :, 1000 * i:1000 * i + 2 * D].unflatten(2, (2, D)) for i in range(3)]
+    for x in views:
+        x.normal_()
+    q, k, v = views
+    near = [x.contiguous() for x in views]
+    for kw in (dict(causal=True), dict(softcap=20.0)):
+        assert torch.equal(masked_attn_func(q, k, v, **kw), masked_attn_func(*near, **kw))
+    assert torch.equal(masked_attn_func(q[:, -1:], k, v), masked_attn_func(near[0][:, -1:], *near[1:]))

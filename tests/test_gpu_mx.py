@@ -174,3 +174,23 @@ def test_not_finite_rows_stay_apart(gpu):
         bad = torch.zeros(M, 300, dtype=torch.bool)
         bad[1], bad[3], bad[:, 17] = True, True, True
         assert torch.equal(torch.isnan(y), bad)
+
+
+def test_rows_far_apart(gpu):
+    """Rows behind 32-bit offsets, of the values, the codes and the results, equal the same rows on their own.  A row's
+    sums do not depend on the tile it is in (steps of k in order in every tile)."""
+    big = torch.zeros(9001, 1 << 18, dtype=BF, device=gpu)
+    x = big[:, 1000:1600]
+    x.normal_()
+    a, b = mx_quantize(x), mx_quantize(x.contiguous())
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    a, b = mx_quantize(big), mx_quantize(big[-70:])
+    assert torch.equal(a.codes[-70:], b.codes) and torch.equal(a.scales[:, -70:], b.scales)
+    del big, x, a, b
+    x = torch.randn(70001, 256, device=gpu).to(BF)
+    w = mx_quantize(torch.randn(32776, 256, device=gpu) / 16)
+    bias = torch.randn(32776, device=gpu)
+    assert torch.equal(mx_linear(x, w, bias)[-300:], mx_linear(x[-300:], w, bias))
+    y, z = (mx_linear(t, w, bias, "gelu_tanh", "mxfp4") for t in (x, x[-300:]))
+    assert torch.equal(y.codes[-300:], z.codes) and torch.equal(y.scales[:, -300:], z.scales)
+    assert torch.equal(y.dequantize(torch.float32)[-300:], z.dequantize(torch.float32))

@@ -28,6 +28,9 @@ def test_sizes():
         assert L.icsa_mx_linear_workspace_size(M, 8, K, _lib.BF16) >= (M * Kp * 17 // 32 if M > 2 else 0)
     assert L.icsa_mx_codes_size(-1, 4) == -1 and L.icsa_mx_scales_size(4, 0) == -1
     assert L.icsa_mx_linear_workspace_size(4, 0, 4, _lib.BF16) == -1
+    over = (1 << 31) - 1                         # past the limits, where rounding up would overflow
+    assert L.icsa_mx_codes_size(4, over) == L.icsa_mx_scales_size(4, over) == L.icsa_mx_codes_size(1 << 62, 4) == -1
+    assert L.icsa_mx_linear_workspace_size(4, 8, over, _lib.BF16) == L.icsa_mx_linear_workspace_size(4, over, 8, _lib.F32) == -1
     assert L.icsa_masked_attn_workspace_size(1, 9373, 9373, 12, 12, 128, 1, 1) == 0
     assert L.icsa_masked_attn_workspace_size(1, 1, 65536, 40, 8, 128, 1, 0) > 0
     assert L.icsa_masked_attn_workspace_size(1, 1, 65536, 40, 7, 128, 1, 0) == -1
@@ -88,7 +91,9 @@ def _masked_args(**kw):
     (dict(cap=math.nan), _lib.EINVAL), (dict(bias=PTR, radius=-1), _lib.EUNSUPPORTED),
     (dict(bias=PTR, radius=1 << 20), _lib.EUNSUPPORTED), (dict(q=0), _lib.EINVAL), (dict(k=0), _lib.EINVAL),
     (dict(out=0), _lib.EINVAL), (dict(q=PTR + 2), _lib.EINVAL), (dict(k_ss=130), _lib.EINVAL), (dict(k_ss=-128), _lib.EINVAL),
-    (dict(Sk=65536), _lib.EWORKSPACE),
+    (dict(Sk=65536), _lib.EWORKSPACE), (dict(cap=4097.0), _lib.EUNSUPPORTED), (dict(cap=1e-31), _lib.EUNSUPPORTED),
+    (dict(cap=1e-20, scale=1e20), _lib.EUNSUPPORTED), (dict(scale=2e38), _lib.EUNSUPPORTED),
+    (dict(k_ss=1 << 24), _lib.EUNSUPPORTED), (dict(v_ss=1 << 24), _lib.EUNSUPPORTED),
 ])
 def test_masked_attn_refuses(kw, code):
     L = _lib.lib()
