@@ -406,9 +406,9 @@ class WanAttentionBlock(nn.Module):
         hidden row goes from that accumulator to its codes, which the second product reads."""
         lin0, lin2 = self.ffn[0], self.ffn[2]
         if isinstance(lin0, MXLinear):
-            return lin2(lin0(h, activation='gelu_tanh', out_dtype='mxfp4'))
+            return lin2(lin0(h, activation='gelu_tanh', out_dtype='mxfp4' if isinstance(lin2, MXLinear) else None))
         f = torch._addmm_activation(lin0.bias, h.reshape(-1, h.shape[-1]), lin0.weight.t(), use_gelu=True)
-        return torch.nn.functional.linear(f, lin2.weight, lin2.bias).view(*h.shape[:-1], lin2.out_features)
+        return lin2(f).view(*h.shape[:-1], lin2.out_features)
 
 
 def quantize_linears(block: WanAttentionBlock) -> WanAttentionBlock:

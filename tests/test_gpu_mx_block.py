@@ -56,6 +56,21 @@ def test_block_with_quantized_layers(gpu, lens):
     assert not torch.equal(out, before)
 
 
+@torch.no_grad()
+def test_one_quantized_ffn_layer(gpu):
+    """Either FFN layer alone in 4 bits: the other takes its bf16 results, or gives it bf16."""
+    h = torch.randn(1, 130, 256, device=gpu).to(BF)
+    for i in (0, 2):
+        blk = _block(gpu, 256, 512, 2)
+        blk.ffn[i] = MXLinear(blk.ffn[i])
+        l0, l2 = blk.ffn[0], blk.ffn[2]
+        if i == 0:
+            ref = nn.functional.linear(l0(h, activation="gelu_tanh"), l2.weight, l2.bias)
+        else:
+            ref = l2(torch._addmm_activation(l0.bias, h[0], l0.weight.t(), use_gelu=True))[None]
+        assert torch.equal(blk._ffn(h), ref)
+
+
 def test_model_quantizes_every_block(gpu):
     m = wan.WanModel(in_dim=4, dim=256, ffn_dim=512, freq_dim=32, text_dim=64, out_dim=4, num_heads=2, num_layers=2, text_len=16)
     m.init_weights()
