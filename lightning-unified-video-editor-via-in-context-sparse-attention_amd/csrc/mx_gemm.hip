@@ -11,9 +11,10 @@
 // What bounds it: the loads into LDS.  Timing copies of an earlier form (128 x 256 tiles of 128 k, two workgroups a CU, 14,040 x 5,120
 // x 13,824): 553 us; without loads in the loop 379; with half of them 438; the same bytes in full 128-byte lines instead of
 // halves 460.  So: full lines, and the largest tile (256 x 256, 8 waves of 64 x 128, two a SIMD): a third fewer bytes an
-// operation, 478 us, 4.2 PFLOP/s; loads spread over two steps instead of one 454.  65,520 x 13,824 x 5,120 with GELU: 2.41 ms,
-// 3.84 PFLOP/s, 2.7 times the bf16 library product's rate at this size (6.46 ms); about 7 of a tile's 45 us are the GELU (two
-// transcendentals an output, nothing to overlap them with).  Without loads in the loop it takes 2.16 ms.
+// operation, 478 us, 4.2 PFLOP/s; loads spread over two steps instead of one 454.  65,520 x 13,824 x 5,120 with GELU: 2.35 ms,
+// 3.95 PFLOP/s, 2.7 times the bf16 library product's rate at this size (6.46 ms); 1.6 of a tile's 43 us are the GELU (two
+// transcendentals an output, nothing to overlap them with); an earlier form without loads in the loop 2.16 ms.  4 waves of 128 x 128,
+// a third fewer bytes out of LDS but one wave a SIMD, were slower: 14,040 x 5,120 x 13,824 538 us against 462.
 #include <algorithm>
 #include <type_traits>
 
@@ -162,6 +163,18 @@ __global__ void __launch_bounds__(64 * NN * NM, 2) icsa_mx_gemm_kernel(MxGemmPar
   };
   unsigned char* const stage = smem + kBufs * kBuf + wave * MXG_STAGE;
 
+  // The accumulators start with the bias: lane l holds the wave's output l's.  The next tile's is loaded before the products and
+  // taken where the wait for a group's loads stands: at the tile's end that wait would include the outputs' stores (2.31 ms against
+  // 2.26 of 65,520 x 13,824 x 5,120; 512 x 5,120 x 4,096 14.1 against 12.9 us)
+  static_assert(WN == 2, "a bias value a lane");
+  const bool bias32 = p.bias_dtype == ICSA_DT_F32;
+  auto wave_bias = [&](int n) {                                        // its bits as they are: a conversion would wait for them
+    const int at = n + wn * 64 + lane;
+    if (p.bias == nullptr || (unsigned)at >= (unsigned)p.N) return 0;   // (past the last tile n may be anything)
+    return bias32 ? reinterpret_cast<const int*>(p.bias)[at] : (int)reinterpret_cast<const unsigned short*>(p.bias)[at];
+  };
+  int bias = wave_bias(src.n0);
+
   unsigned cur = 0, last = (kBufs - 1) * kBuf;                         // buffer of group g; of the cursor's group (g + kBufs - 1)
 #pragma unroll
   for (int g = 0; g < kBufs; ++g) {
@@ -176,16 +189,25 @@ __global__ void __launch_bounds__(64 * NN * NM, 2) icsa_mx_gemm_kernel(MxGemmPar
   for (int x = 0; x < kOps; ++x) read_op(0, 0, 0, x);
 
   int m0 = src.m0, n0 = src.n0;
+  asm volatile("" : "+v"(bias));
   for (;;) {
+    bias <<= bias32 ? 0 : 16;
 #pragma unroll
-    for (int i = 0; i < WN; ++i)
+    for (int i = 0; i < WN; ++i) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float x = bias_at(p, n0 + (wn * WN + i) * 32 + 8 * (e >> 2) + 4 * hl + (e & 3));
+        const int at = 32 * i + 8 * (e >> 2) + (e & 3);
+        const float x = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (at + 4 * hl), bias));
 #pragma unroll
         for (int j = 0; j < WM; ++j) acc[i][j][e] = x;
       }
-    for (int g = 0; g < p.groups; ++g) {
+#pragma unroll
+      for (int j = 0; j < WM; ++j) asm volatile("" : "+v"(acc[i][j]));   // registers of their own: one value for all is copied too late
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    bias = wave_bias(nsrc.n0);                         // (past the last tile: not used)
+    int g = 0;
+    do {
 #pragma unroll
       for (int i = 0; i < WN; ++i) sa[i] = na[i];
 #pragma unroll
@@ -194,13 +216,14 @@ __global__ void __launch_bounds__(64 * NN * NM, 2) icsa_mx_gemm_kernel(MxGemmPar
       step(std::integral_constant<int, 1>{}, cur, 0, 0, 0);
       step(std::integral_constant<int, 2>{}, cur, 0, 0, 0);
       asm volatile("s_waitcnt vmcnt(%0)" :: "n"((kBufs - 2) * kLoads) : "memory");         // group g + 1
+      if constexpr (kBufs == 2) asm volatile("" : "+v"(bias));
       ATT_BARRIER();                                                   // everybody's; and everybody has read group g
       last = cur;
       cur = cur == (kBufs - 1) * kBuf ? 0 : cur + kBuf;
       read_scales(cur);
       advance();
       step(std::integral_constant<int, 3>{}, cur, 0, kFirst, last);
-    }
+    } while (++g < p.groups);
     // ---- this tile's outputs, while the next one's first groups arrive ----
 #pragma unroll
     for (int j = 0; j < WM; ++j)
@@ -241,11 +264,11 @@ hipError_t run_mx_gemm(const MxGemmParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// A launch takes rounds of one tile a CU.  Measured (us, one round): a 256 x 256 tile 1.6 a group and 1 to 4 besides, GELU 7; a
-// 128 x 128 tile 0.56 a group and 2.5, GELU 1.7; a launch 4.5.  In units of 0.56 us.
+// A launch takes rounds of one tile a CU.  Measured (us, one round): a 256 x 256 tile 1.6 a group and 1 to 4 besides, GELU 3.4; a
+// 128 x 128 tile 0.56 a group and 2.5, GELU 0.5; a launch 4.5.  In units of 0.56 us.
 double rounds_of(int64_t tiles) { return (double)((tiles + MXG_CUS - 1) / MXG_CUS); }
-double big_time(int64_t tiles, const MxGemmParams& p) { return rounds_of(tiles) * (2.9 * p.groups + 4 + 12 * p.gelu); }
-double small_time(int64_t tiles, const MxGemmParams& p) { return rounds_of(tiles) * (p.groups + 4.5 + 3 * p.gelu); }
+double big_time(int64_t tiles, const MxGemmParams& p) { return rounds_of(tiles) * (2.9 * p.groups + 4 + 6 * p.gelu); }
+double small_time(int64_t tiles, const MxGemmParams& p) { return rounds_of(tiles) * (p.groups + 4.5 + 1 * p.gelu); }
 
 // 256 x 256 tiles, 128 x 128 tiles, or the first rows in whole rounds of the former and the others in the latter.  All three
 // measured (us, M x N x K): 512 x 5,120 x 4,096 24.3, 12.7, -; 1,560 x 5,120 x 5,120 32.0, 41.3, -; 3,120 x 5,120 x 5,120 67.1, 57.2,
