@@ -17,8 +17,8 @@
 //
 // Values in masked places: scores are replaced, not added to, so a NaN of a masked key does not
 // matter; V rows that no row of the workgroup sees are cleared in LDS; and where a partly visible tile holds
-// a V that is not finite, 0 * V would reach rows that do not see it, so that tile is added key by
-// key to the rows that do.
+// a V that is not finite, 0 * V would reach rows that do not see it: such values are cleared too, and added at
+// the end to the rows that see them.
 //
 // What bounds it (two waves a SIMD): the vector instructions and the products of a tile side by side, 830 and 1,024 cycles a
 // wave with heads of 128; capped scores add two transcendentals an element (1,340).  9,373 tokens, 12 heads of 128: dense 610 us
@@ -145,6 +145,9 @@ __device__ __forceinline__ float sum_p(const bf16x8 pf[4]) {
   return (r[0] + r[1]) + (r[2] + r[3]);
 }
 
+// The sign bits of those of two bf16 that are infinite or NaN: a full exponent carries into them
+__device__ __forceinline__ unsigned not_finite2(unsigned x) { return ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+
 // One wave's 32 rows of 32 dims to the output: through 2 KB of the wave's LDS, so that bf16
 // stores are 64-byte segments.  v: this lane's 16 values (dims 8 (e / 4) + 4 hl + e % 4 of row li).
 template <int kB16>
@@ -209,7 +212,7 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   constexpr int kSteps = D / 16, kSub = D / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   unsigned char* const scratch_all = smem + 4 * T::kBytes;
-  int* const ctl = reinterpret_cast<int*>(scratch_all + MA_WAVES * MA_SCRATCH_WAVE);   // ranges of the 4 waves, 2 flags
+  int* const ctl = reinterpret_cast<int*>(scratch_all + MA_WAVES * MA_SCRATCH_WAVE);   // ranges of the 4 waves, a flag
   float* const bias_lds = reinterpret_cast<float*>(scratch_all + MA_WAVES * MA_SCRATCH_WAVE + MA_CTL_BYTES);
   const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
       in_hi = wave_min(in_hi);
     }
     if (lane == 0) { ctl[wave] = lo; ctl[4 + wave] = hi; ctl[8 + wave] = in_lo; ctl[12 + wave] = in_hi; }
-    if (threadIdx.x < 2) ctl[16 + threadIdx.x] = 0;
+    if (threadIdx.x == 0) ctl[16] = 0;
   }
   const float c = p.scale * MA_LOG2E;
   const int bias_row = 2 * p.radius + 1 + 2 * MA_BIAS_MARGIN;            // a head's table, its ends repeated over a tile's width
@@ -292,15 +295,22 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   const unsigned lds0 = lds_u32(smem);
   auto kbuf = [&](int t) { return smem + (t & 1) * T::kBytes; };
   auto vbuf = [&](int t) { return smem + (2 + (t & 1)) * T::kBytes; };
+  // the next tile's: addresses and lengths move on by a tile (64-bit products would take 60 scalar instructions)
+  const int k_row = (int)p.k_ss * 2, v_row = (int)p.v_ss * 2;
+  unsigned long long k_at = (unsigned long long)(kb + (int64_t)t0 * ATT_BN * p.k_ss), v_at = (unsigned long long)(vb + (int64_t)t0 * ATT_BN * p.v_ss);
+  int left = p.Sk - t0 * ATT_BN;
   auto load_tile = [&](int t) __attribute__((always_inline)) {
-    const int rows = min(ATT_BN, p.Sk - t * ATT_BN);
-    const u32x4 krs = dma_rsrc(kb + (int64_t)t * ATT_BN * p.k_ss, ((rows - 1) * p.k_ss + D) * 2);
-    const u32x4 vrs = dma_rsrc(vb + (int64_t)t * ATT_BN * p.v_ss, ((rows - 1) * p.v_ss + D) * 2);
+    const int rows = min(ATT_BN, left) - 1;
+    const u32x4 krs = {(unsigned)k_at, (unsigned)(k_at >> 32) & 0xffffu, (unsigned)(rows * k_row + 2 * D), 0x00020000u};
+    const u32x4 vrs = {(unsigned)v_at, (unsigned)(v_at >> 32) & 0xffffu, (unsigned)(rows * v_row + 2 * D), 0x00020000u};
     const unsigned at = lds0 + (t & 1) * T::kBytes + wave * 16 * T::kRow;
 #pragma unroll
     for (int i = 0; i < T::kLoads; ++i) lds_dma16(at + 1024 * i, kofs[i], krs);
 #pragma unroll
     for (int i = 0; i < T::kLoads; ++i) lds_dma16(at + 2 * T::kBytes + 1024 * i, vofs[i], vrs);
+    k_at += (unsigned)(ATT_BN * k_row);
+    v_at += (unsigned)(ATT_BN * v_row);
+    left -= ATT_BN;
   };
   if (t0 < t1) load_tile(t0);
 
@@ -339,13 +349,20 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
         for (int e = 0; e < T::kRow / 64; ++e) own[e] = u32x4{0u, 0u, 0u, 0u};
       } else {
 #pragma unroll
-        for (int e = 0; e < T::kRow / 64; ++e) {
-          const u32x4 x = own[e];
-#pragma unroll
-          for (int f = 0; f < 4; ++f) bad |= (x[f] & 0x7f807f80u) + 0x00800080u;     // a full exponent carries into the sign's bit
+        for (int e = 0; e < T::kRow / 64; ++e) bad |= not_finite2(own[e][0]) | not_finite2(own[e][1]) | not_finite2(own[e][2]) | not_finite2(own[e][3]);
+      }
+      if (__ballot(bad != 0u) != 0ull) {
+        if (lane == 0) ctl[16] = 1;
+        if (bad != 0u) {
+#pragma unroll 1
+          for (int e = 0; e < T::kRow / 4; e += 4) {
+            unsigned short* const x = reinterpret_cast<unsigned short*>(own) + e / 2;
+            const unsigned y = *reinterpret_cast<const unsigned*>(x), m = not_finite2(y);
+            if (m & 0x8000u) x[0] = 0;
+            if (m & 0x80000000u) x[1] = 0;
+          }
         }
       }
-      if (__ballot((bad & 0x80008000u) != 0u) != 0ull && lane == 0) ctl[16 + (t & 1)] = t + 1;
     }
     ATT_BARRIER();
     if (t + 1 < t1) load_tile(t + 1);
@@ -450,7 +467,7 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
     }
     l_run += rs;
 
-    if (!(partial && uni(ctl[16 + (t & 1)]) == t + 1)) {
+    {
       bf16x8 va[4 * kSub];
       auto v_op = [&](int x) __attribute__((always_inline)) {
         const unsigned char* at = vs + vro[x % kSub] + x / kSub * 16 * T::kRow;
@@ -470,36 +487,30 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
         __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_s_setprio(0);
-    } else {
-      // key by key, to the rows that see it: P through the wave's scratch, 32 keys at a time
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        bf16* const ps = reinterpret_cast<bf16*>(scratch);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ps[(8 * (i >> 2) + 4 * hl + (i & 3)) * 32 + li] = pf[2 * sub + (i >> 3)][i & 7];
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll 1
-        for (int x = 0; x < 32; ++x) {
-          const int row = 32 * sub + x, key = j0 + row;
-          const float pv = (float)ps[x * 32 + li];
-          const bool vis = key >= rr.lo && key < rr.hi;
-#pragma unroll
-          for (int ds = 0; ds < kSub; ++ds)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int col = 32 * ds + 8 * g + 4 * hl;
-              const bf16x4 v4 = *reinterpret_cast<const bf16x4*>(vs + row * T::kRow + (((col >> 3) ^ T::vswz(row)) << 4) + (col & 7) * 2);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                o[ds][4 * g + e] = vis ? fmaf(pv, (float)v4[e], o[ds][4 * g + e]) : o[ds][4 * g + e];
-            }
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
     }
   }
 
   if (rows_valid <= 0) return;
+  if (uni(ctl[16]) != 0) {                             // what was cleared, from memory, to the rows that see it
+    for (int t = t0; t < t1; ++t) {
+      if (t * ATT_BN >= a_lo && (t + 1) * ATT_BN <= a_hi) continue;
+#pragma unroll 1
+      for (int key = max(t * ATT_BN, u_lo); key < min((t + 1) * ATT_BN, u_hi); ++key) {
+        const bool vis = key >= rr.lo && key < rr.hi;
+#pragma unroll
+        for (int ds = 0; ds < kSub; ++ds)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const bf16x4 v4 = *reinterpret_cast<const bf16x4*>(vb + (int64_t)key * p.v_ss + 32 * ds + 8 * g + 4 * hl);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = (float)v4[e];
+              o[ds][4 * g + e] += vis && !__builtin_isfinite(v) ? v : 0.f;
+            }
+          }
+      }
+    }
+  }
   const float l = xhalf_sum(l_run);
   if (!some) {                                         // whatever it holds of tiles that others see whole
 #pragma unroll
