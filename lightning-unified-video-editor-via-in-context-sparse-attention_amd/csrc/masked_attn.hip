@@ -270,17 +270,16 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
   const int u_lo = uni(min(min(ctl[0], ctl[1]), min(ctl[2], ctl[3]))), u_hi = uni(max(max(ctl[4], ctl[5]), max(ctl[6], ctl[7])));
   const int a_lo = uni(max(max(ctl[8], ctl[9]), max(ctl[10], ctl[11]))), a_hi = uni(min(min(ctl[12], ctl[13]), min(ctl[14], ctl[15])));
-  int t0 = 0, t1 = 0;
+  int t0 = 0, t1 = 0;                                  // tiles from key u_lo on
   if (u_hi > u_lo) {
-    const int first = u_lo / ATT_BN, n = (u_hi + ATT_BN - 1) / ATT_BN - first;
-    t0 = first;
-    t1 = first + n;
+    t1 = (u_hi - u_lo + ATT_BN - 1) / ATT_BN;
     if (cut) {                                         // equal parts, the first ones a tile longer
-      const int q = p.by_split.div(n), more = n - q * p.n_split;
-      t0 = first + q * split + min(split, more);
+      const int q = p.by_split.div(t1), more = t1 - q * p.n_split;
+      t0 = q * split + min(split, more);
       t1 = t0 + q + (split < more);
     }
   }
+  const int key0 = u_lo + t0 * ATT_BN;
 
   // ---- loads ----
   const bf16* kb = p.k + (int64_t)b * p.k_sb + (int64_t)hk * p.k_sh;
@@ -297,8 +296,8 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   auto vbuf = [&](int t) { return smem + (2 + (t & 1)) * T::kBytes; };
   // the next tile's: addresses and lengths move on by a tile (64-bit products would take 60 scalar instructions)
   const int k_row = (int)p.k_ss * 2, v_row = (int)p.v_ss * 2;
-  unsigned long long k_at = (unsigned long long)(kb + (int64_t)t0 * ATT_BN * p.k_ss), v_at = (unsigned long long)(vb + (int64_t)t0 * ATT_BN * p.v_ss);
-  int left = p.Sk - t0 * ATT_BN;
+  unsigned long long k_at = (unsigned long long)(kb + (int64_t)key0 * p.k_ss), v_at = (unsigned long long)(vb + (int64_t)key0 * p.v_ss);
+  int left = p.Sk - key0;
   auto load_tile = [&](int t) __attribute__((always_inline)) {
     const int rows = min(ATT_BN, left) - 1;
     const u32x4 krs = {(unsigned)k_at, (unsigned)(k_at >> 32) & 0xffffu, (unsigned)(rows * k_row + 2 * D), 0x00020000u};
@@ -334,7 +333,7 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   const int see_lo = some ? rr.lo : 0, see_hi = some ? rr.hi : 0x7fffffff;
 
   for (int t = t0; t < t1; ++t) {
-    const int j0 = t * ATT_BN;
+    const int j0 = u_lo + t * ATT_BN;
     unsigned char* const ks = kbuf(t);
     unsigned char* const vs = vbuf(t);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -344,7 +343,7 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
       const int row = 16 * wave + (lane >> 2), key = j0 + row;
       u32x4* own = reinterpret_cast<u32x4*>(vs + row * T::kRow + (lane & 3) * (T::kRow / 4));
       unsigned bad = 0;
-      if (key < u_lo || key >= u_hi) {
+      if (key >= u_hi) {
 #pragma unroll
         for (int e = 0; e < T::kRow / 64; ++e) own[e] = u32x4{0u, 0u, 0u, 0u};
       } else {
@@ -493,9 +492,10 @@ __global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedA
   if (rows_valid <= 0) return;
   if (uni(ctl[16]) != 0) {                             // what was cleared, from memory, to the rows that see it
     for (int t = t0; t < t1; ++t) {
-      if (t * ATT_BN >= a_lo && (t + 1) * ATT_BN <= a_hi) continue;
+      const int j0 = u_lo + t * ATT_BN;
+      if (j0 >= a_lo && j0 + ATT_BN <= a_hi) continue;
 #pragma unroll 1
-      for (int key = max(t * ATT_BN, u_lo); key < min((t + 1) * ATT_BN, u_hi); ++key) {
+      for (int key = j0; key < min(j0 + ATT_BN, u_hi); ++key) {
         const bool vis = key >= rr.lo && key < rr.hi;
 #pragma unroll
         for (int ds = 0; ds < kSub; ++ds)
