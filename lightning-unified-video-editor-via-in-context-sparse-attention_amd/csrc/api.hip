@@ -578,7 +578,7 @@ static int check_masked_sizes(int B, int Sq, int Sk, int H, int Hk, int D) {
 
 int64_t icsa_masked_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs, int causal) {
   if (check_masked_sizes(B, Sq, Sk, H, Hk, D)) return -1;
-  return align256(masked_attn_part_floats(B, Sq, H, Hk, D, masked_attn_plan(B, Sq, Sk, H, Hk, docs <= 1 && !causal)) * 4);
+  return align256(masked_attn_part_floats(B, Sq, H, Hk, D, masked_attn_plan(B, Sq, Sk, H, Hk, D, docs <= 1 && !causal)) * 4);
 }
 
 int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
@@ -620,7 +620,7 @@ int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
   p.q_starts = q_starts; p.k_starts = k_starts; p.docs = docs; p.causal = causal != 0; p.prefix = prefix;
   p.scale = scale; p.softcap = softcap; p.bias = bias; p.radius = radius;
   p.out = OutView{out, o_sb, o_ss, o_sh, out_dtype};
-  const MaskedPlan plan = masked_attn_plan(B, Sq, Sk, H, Hk, docs <= 1 && !causal);
+  const MaskedPlan plan = masked_attn_plan(B, Sq, Sk, H, Hk, D, docs <= 1 && !causal);
   p.n_whole = plan.n_whole; p.n_split = plan.n_split;
   const int64_t need = icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D, docs, causal);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))

@@ -293,7 +293,7 @@ struct MaskedAttnParams {
 };
 // items 0 .. n_whole - 1 are taken whole, the keys of the others in n_split parts
 struct MaskedPlan { int n_whole, n_split; };
-MaskedPlan masked_attn_plan(int B, int Sq, int Sk, int H, int Hk, bool alike);
+MaskedPlan masked_attn_plan(int B, int Sq, int Sk, int H, int Hk, int D, bool alike);
 int64_t masked_attn_part_floats(int B, int Sq, int H, int Hk, int D, MaskedPlan f);
 bool masked_attn_bias_fits(int H, int Hk, int D, int radius);
 hipError_t launch_masked_attn(MaskedAttnParams p, hipStream_t stream);

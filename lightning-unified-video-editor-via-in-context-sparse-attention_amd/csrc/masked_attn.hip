@@ -38,7 +38,7 @@
 #define MA_PSUM_MAX 18446744073709551616.0f           // as in the dense kernel: the reference max is raised past it
 #define MA_M_NONE (-3.4028234663852886e38f)           // finite: a tile without visible keys leaves O = l = 0
 #define MA_LOG2E 1.4426950408889634f
-#define MA_TARGET_WG 512                              // two workgroups a CU
+#define MA_CUS 256
 #define MA_MAX_SPLIT 256
 #define MA_FEW_PARTS 16                               // from so many parts on a row's are shared by thread groups
 #define MA_TAIL_ROUNDS 8                              // up to so many rounds a last, incomplete one is cut in parts
@@ -58,6 +58,10 @@ template <int D> struct Tile {
   static __device__ __forceinline__ int kswz(int r) { return D == 128 ? (r & 15) : ((r >> 1) & 7); }
   static __device__ __forceinline__ int vswz(int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; }
 };
+
+// Workgroups a CU holds: registers for three with heads of 64 (4 x 512 tokens of 64 heads with bias and documents 42.5 us with
+// two, 40.0 with three)
+__host__ __device__ constexpr int ma_wg_per_cu(int D) { return D == 64 ? 3 : 2; }
 
 __host__ __device__ __forceinline__ int ma_fixed_lds(int D) { return 4 * ATT_BN * D * 2 + MA_WAVES * MA_SCRATCH_WAVE + MA_CTL_BYTES; }
 
@@ -207,7 +211,7 @@ __device__ __forceinline__ void store_wave(const MaskedAttnParams& p, unsigned c
 }  // namespace
 
 template <int D, bool kCap, bool kBias>
-__global__ void __launch_bounds__(MA_THREADS, 2) icsa_masked_attn_kernel(MaskedAttnParams p) {
+__global__ void __launch_bounds__(MA_THREADS, ma_wg_per_cu(D)) icsa_masked_attn_kernel(MaskedAttnParams p) {
   typedef Tile<D> T;
   constexpr int kSteps = D / 16, kSub = D / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -597,30 +601,36 @@ __global__ void __launch_bounds__(256) icsa_masked_combine_kernel(MaskedAttnPara
   }
 }
 
-// Which items are whole, and how many parts the others' keys are cut into.  Few items: all in parts, enough for MA_TARGET_WG
-// workgroups of a few tiles each.  Some rounds of alike items (no causal mask, no documents; else the hardware fills the gaps as
-// items end): the last, incomplete round's items in parts, as many as make the rounds come out shortest, where a part is long
-// against its sums' way through memory.
-MaskedPlan masked_attn_plan(int B, int Sq, int Sk, int H, int Hk, bool alike) {
-  MaskedPlan f = {0, 1};
+// Which items are whole, and how many parts the others' keys are cut into.  Few items: all in parts, enough to fill the chip
+// with workgroups of a few tiles each (rows of a block at most read keys from memory: two workgroups a CU, which leave fewer sums to
+// join; one token, 65,536 keys of 8 heads of 64: 32.4 us, with three 36.4).  Some rounds of alike items (no causal mask, no
+// documents; else the hardware fills the gaps as items end): the last, incomplete round's items in parts, as many as make the
+// rounds come out shortest, where a part is long against its sums' way through memory; rounds of two or three workgroups a CU, which share its
+// rate (heads of 64: 16 x 9,373 tokens 381 us by two, 402 by three; 24 x 4,000 over 8,000 keys 228 and 216).
+MaskedPlan masked_attn_plan(int B, int Sq, int Sk, int H, int Hk, int D, bool alike) {
   const int64_t rows = (int64_t)Sq * (H / Hk), items = (int64_t)B * Hk * ((rows + MA_ROWS - 1) / MA_ROWS);
   const int tiles = (Sk + ATT_BN - 1) / ATT_BN;
-  f.n_whole = (int)items;
+  MaskedPlan f = {(int)items, 1};
   if (items <= 0) return f;
-  if (items * 2 <= MA_TARGET_WG) {
-    int64_t n = (MA_TARGET_WG + items - 1) / items;
+  const int most = MA_CUS * ma_wg_per_cu(D), fill = rows <= MA_ROWS ? 2 * MA_CUS : most;
+  if (items * 2 <= fill) {
+    int64_t n = (fill + items - 1) / items;
     n = n < tiles / MA_MIN_SPLIT_TILES ? n : tiles / MA_MIN_SPLIT_TILES;
     if (n > 1) { f.n_whole = 0; f.n_split = n > MA_MAX_SPLIT ? MA_MAX_SPLIT : (int)n; }
     return f;
   }
-  const int64_t tail = items % MA_TARGET_WG;
-  if (!alike || tail == 0 || items > MA_TAIL_ROUNDS * MA_TARGET_WG || tiles < MA_TAIL_TILES) return f;
-  double best = 1.0;
-  for (int n = 2; n <= 8 && tiles / n >= MA_TAIL_TILES / 4; ++n) {
-    const double rounds = (double)((tail * n + MA_TARGET_WG - 1) / MA_TARGET_WG) / n + 0.03 * n;
-    if (rounds < best) { best = rounds; f.n_split = n; }
+  if (!alike || items > MA_TAIL_ROUNDS * 2 * MA_CUS || tiles < MA_TAIL_TILES) return f;
+  double best = 0.;
+  for (int slots = 2 * MA_CUS; slots <= most; slots += MA_CUS) {
+    const int64_t tail = items % slots;
+    for (int n = 1; n <= 8 && (n == 1 || tiles / n >= MA_TAIL_TILES / 4); ++n) {
+      const double last = (double)((tail * n + slots - 1) / slots) / n + (n > 1 ? 0.03 * n : 0.), time = slots * (items / slots + last);
+      if (best != 0. && time >= best) continue;
+      best = time;
+      f.n_split = n;
+      f.n_whole = (int)(n > 1 ? items - tail : items);
+    }
   }
-  if (f.n_split > 1) f.n_whole = (int)(items - tail);
   return f;
 }
 
