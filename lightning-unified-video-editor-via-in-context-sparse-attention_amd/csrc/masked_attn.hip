@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(MA_THREADS, ma_wg_per_cu(D)) icsa_masked_attn_
       const int d0 = j0 - rr.at + 4 * hl, R = p.radius;
       const float f = kCap ? -2.f * top : c;
       if (__ballot(!(d0 >= R || d0 + ATT_BN <= -R)) == 0ull) {           // the whole tile past the table's ends
-        const float x = my_bias[d0 > 0 ? R : -R] + top;
+        const float end = my_bias[d0 > 0 ? R : -R], x = kCap ? end + top : end;
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
@@ -414,10 +414,13 @@ __global__ void __launch_bounds__(MA_THREADS, ma_wg_per_cu(D)) icsa_masked_attn_
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[sub][i] = fmaf(s[sub][i], f, t[32 * sub + 8 * (i >> 2) + (i & 3)] + top);
+          for (int i = 0; i < 16; ++i) {
+            const float x = t[32 * sub + 8 * (i >> 2) + (i & 3)];
+            s[sub][i] = fmaf(s[sub][i], f, kCap ? x + top : x);
+          }
       }
     }
-    const float base = kBias ? 0.f : top, mul = kBias ? 1.f : kCap ? -2.f * top : c;
+    const float base = kBias || !kCap ? 0.f : top, mul = kBias ? 1.f : kCap ? -2.f * top : c;
     if (partial) {
       // keys outside [lo, hi) as one 64-bit word: element i of sub-tile sub is key 32 sub + 8 (i / 4) + 4 hl + i % 4
       const int a = min(max(rr.lo - j0, 0), 64), z = min(max(rr.hi - j0, 0), 64);
