@@ -61,14 +61,13 @@ class MXFP4Tensor:
         self.shape, self.rows, self.device = shape, rows, codes.device
 
     @classmethod
-    def _empty(cls, shape, device) -> "MXFP4Tensor":
+    def _empty(cls, shape: torch.Size, rows: int, device) -> "MXFP4Tensor":
         """Codes and scales side by side in one new buffer; the views of it are made when asked for."""
         t = cls.__new__(cls)
-        rows, Kp = math.prod(shape[:-1]), _padded(shape[-1])
-        n = rows * (Kp // 2)                                      # a multiple of 128
-        t._buf = torch.empty(n + rows * (Kp // 32), dtype=torch.uint8, device=device)
+        n = rows * (_padded(shape[-1]) // 2)                      # bytes of codes, a multiple of 128; a 16th of them is scales
+        t._buf = torch.empty(n + n // 16, dtype=torch.uint8, device=device)
         t._codes = t._scales = None
-        t.shape, t.rows, t.device = torch.Size(shape), rows, t._buf.device
+        t.shape, t.rows, t.device = shape, rows, device
         return t
 
     def _ptrs(self):
@@ -76,7 +75,7 @@ class MXFP4Tensor:
         if self._buf is None:
             return self._codes.data_ptr(), self._scales.data_ptr()
         p = self._buf.data_ptr()
-        return p, p + self.rows * (_padded(self.shape[-1]) // 2)
+        return p, p + self._buf.shape[0] // 17 * 16
 
     @property
     def codes(self) -> torch.Tensor:
@@ -121,14 +120,15 @@ def mx_quantize(x: torch.Tensor) -> MXFP4Tensor:
     ``2^(floor(log2 max|x|) - 2)``, codes are rounded to the nearest (ties to even), what is over 6
     scales becomes 6, and a block with a NaN or an infinity reads as NaN."""
     _no_grad_inputs(x)
-    if not x.is_cuda or x.dim() < 1 or x.shape[-1] < 1:
+    shape, dev = x.shape, x.device
+    if not x.is_cuda or len(shape) < 1 or shape[-1] < 1:
         raise IcsaArgumentError("x must be [..., K] with K > 0, on the GPU")
-    code = dtype_code(x)
-    dev = x.device
-    t = MXFP4Tensor._empty(x.shape, dev)
+    code, K = dtype_code(x), shape[-1]
+    rows = x.numel() // K
+    t = MXFP4Tensor._empty(shape, rows, dev)
     r = _rows(x)
     with on_device(dev):
-        rc = _lib.lib().icsa_mx_quantize(r.data_ptr(), code, r.stride(0), t.rows, t.shape[-1], *t._ptrs(), stream_ptr(dev))
+        rc = _lib.lib().icsa_mx_quantize(r.data_ptr(), code, r.stride(0), rows, K, *t._ptrs(), stream_ptr(dev))
     _lib.check("icsa_mx_quantize", rc)
     return t
 
@@ -172,7 +172,7 @@ def mx_linear(x, weight: MXFP4Tensor, bias: torch.Tensor = None, activation: str
             wsp = ws.data_ptr()
     shape = (*x.shape[:-1], N)
     if out_dtype == "mxfp4":
-        out = MXFP4Tensor._empty(shape, dev)
+        out = MXFP4Tensor._empty(torch.Size(shape), M, dev)
         (op, osc), o_code = out._ptrs(), _lib.MXFP4
     else:
         out = torch.empty(*shape, dtype=out_dtype, device=dev)
