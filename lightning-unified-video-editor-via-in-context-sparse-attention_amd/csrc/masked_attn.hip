@@ -20,21 +20,23 @@
 // a V that is not finite, 0 * V would reach rows that do not see it: such values are cleared too, and added at
 // the end to the rows that see them.
 //
-// What bounds it (two waves a SIMD): the vector instructions and the products of a tile side by side, 830 and 1,024 cycles a
-// wave with heads of 128; capped scores add two transcendentals an element (1,340).  9,373 tokens, 12 heads of 128: dense 610 us
-// (0.89 PFLOP/s in two rounds of workgroups, the second 73 % full), causal 317 (0.85), a prefix and capped scores 480 (0.64);
-// 32,760 tokens, 5 heads 2.87 ms (0.96); 9,373 tokens, 12 heads of 64 340 us (0.79).  One query of 40 heads over 8 key heads of
-// 65,536 keys: 43 us for 268 MB and 5 for joining 64 parts.  Short documents (packed prompts of 350 keys, 40 heads, 32,760
-// queries: 415 us) add the way of Q and the output through memory, 140 us at the copy rate, which two
-// workgroups a CU do not hide.  Several items a workgroup, with the next one's start before the last one's stores, was
-// slower there (495 us: 20 spilled registers, and items of different lengths dealt out beforehand).
+// What bounds it (two waves a SIMD): the vector instructions and the products of a tile side by side, 550 to 800 and 1,024 cycles
+// a wave with heads of 128, and the clock, 1.7 to 2.1 GHz under them; capped scores add two transcendentals an element.  9,373
+// tokens, 12 heads of 128: dense 525 us (1.03 PFLOP/s in two rounds of workgroups, the second 73 % full), causal 282 (0.96), a prefix
+// and capped scores 375 to 415 (matrix pipe busy 36 %, vector pipe 54 %); 32,760 tokens, 5 heads 2.41 ms (1.14); 9,373 tokens, 12 heads
+// of 64 301 us (0.90).  One query of 40 heads over 8 key heads of 65,536 keys: 43 us for 268 MB and 6 for joining 64 parts.  Short
+// documents (packed prompts of 350 keys, 40 heads, 32,760 queries: 314 to 346 us) add the way of Q and the output
+// through memory, 140 us at the copy rate, and each workgroup's start, which two workgroups a CU do not hide.
+// Tried and slower: the next tile's scores between the exponentials of the one at hand (dense 541 -> 564 us; heads of 64 310 -> 357);
+// several items a workgroup; tanh as a polynomial where x is small (prefix 415 -> 429).  A second way through the loop for
+// values that are not finite made the compiler copy O every tile: dense 605 us.
 #include "attn_tile.h"
 #include "icsa_kernels.h"
 
 #define MA_THREADS 256
 #define MA_WAVES 4
-#define MA_SCRATCH_WAVE 2048                          // per wave: staged output rows, or half a tile's P
-#define MA_CTL_BYTES 256                              // per-wave ranges, flags
+#define MA_SCRATCH_WAVE 2048                          // per wave: staged output rows
+#define MA_CTL_BYTES 256                              // per-wave ranges, a flag
 #define MA_PSUM_MAX 18446744073709551616.0f           // as in the dense kernel: the reference max is raised past it
 #define MA_M_NONE (-3.4028234663852886e38f)           // finite: a tile without visible keys leaves O = l = 0
 #define MA_LOG2E 1.4426950408889634f
