@@ -263,3 +263,31 @@ def test_rows_far_apart(gpu, D):
     for kw in (dict(causal=True), dict(softcap=20.0)):
         assert torch.equal(masked_attn_func(q, k, v, **kw), masked_attn_func(*near, **kw))
     assert torch.equal(masked_attn_func(q[:, -1:], k, v), masked_attn_func(near[0][:, -1:], *near[1:]))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq,Sk,kw", [(300, 300, {}), (40, 5000, {}), (200, 330, dict(softcap=5.0)),
+                                      (150, 400, dict(q_starts=[[0, 70, 150]], k_starts=[[0, 33, 400]]))])
+def test_infinities_of_values_keep_their_sign(gpu, Sq, Sk, kw, D):
+    """Infinite and NaN values near the causal border (in tiles that some rows see in part, several of them a
+    tile, whole items and parts): the queries that see one get it, of its sign, NaN for both signs; all others
+    what they get without."""
+    print(f"[masked] inf {Sq}x{Sk} {kw} D={D}", flush=True)
+    q, k, v = _inputs(1, Sq, Sk, 2, 1, D, 31)
+    bad = {Sk - 100: (3, math.inf), Sk - 61: (D - 1, -math.inf), Sk - 60: (3, -math.inf), Sk - 2: (17, math.nan), Sk - 40: (40, math.inf)}
+    vb = v.clone()
+    for key, (d, x) in bad.items():
+        vb[0, key, 0, d] = x
+    kw = {n: _i32(x) if isinstance(x, list) else x for n, x in kw.items()}
+    dev = {n: x.to(gpu) if isinstance(x, torch.Tensor) else x for n, x in kw.items()}
+    got = masked_attn_func(q.to(gpu), k.to(gpu), vb.to(gpu), causal=True, **dev).double().cpu()
+    clean = v.clone()
+    for key, (d, _) in bad.items():
+        clean[0, key, 0, d] = 0
+    plain = masked_attn_func(q.to(gpu), k.to(gpu), clean.to(gpu), causal=True, **dev).double().cpu()
+    see, _ = O.visible(1, Sq, Sk, kw.get("q_starts"), kw.get("k_starts"), True)
+    want = plain.clone()
+    for key, (d, x) in bad.items():
+        want[0, see[0, :, key], :, d] += x
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got, nan=0.0, posinf=1e30, neginf=-1e30), torch.nan_to_num(want, nan=0.0, posinf=1e30, neginf=-1e30))

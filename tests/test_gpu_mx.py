@@ -194,3 +194,17 @@ def test_rows_far_apart(gpu):
     y, z = (mx_linear(t, w, bias, "gelu_tanh", "mxfp4") for t in (x, x[-300:]))
     assert torch.equal(y.codes[-300:], z.codes) and torch.equal(y.scales[:, -300:], z.scales)
     assert torch.equal(y.dequantize(torch.float32)[-300:], z.dequantize(torch.float32))
+
+
+@pytest.mark.parametrize("M,N,K", [(300, 700, 600), (4099, 4110, 300), (9360, 2001, 520)])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_bias_of_either_type_and_any_start(gpu, M, N, K, dtype):
+    """Over several tiles a workgroup, ragged ends, a bias that starts behind another tensor's first element: the result is
+    that without a bias, of the same f32 sums, and the bias (an f32 addition at another place: K + 2 steps of 2^-24 at most)."""
+    print(f"[mx] bias {M}x{N}x{K} {dtype}", flush=True)
+    x, w = mx_quantize(_x(M, K, BF, 1, 0.7).to(gpu)), mx_quantize((_x(N, K, torch.float32, 2, 0.3) / math.sqrt(K)).to(gpu))
+    b = torch.randn(N + 1, generator=torch.Generator().manual_seed(3)).to(dtype).to(gpu)[1:]
+    plain = mx_linear(x, w, None, out_dtype=torch.float32).double()
+    y = mx_linear(x, w, b, out_dtype=torch.float32).double()
+    mass = mx_linear(mx_quantize(x.dequantize().abs()), mx_quantize(w.dequantize().abs()), None, out_dtype=torch.float32).double()
+    assert ((y - plain - b.double()).abs() <= 2.0 ** -24 * (K + 2) * (1.01 * mass + b.double().abs())).all()
