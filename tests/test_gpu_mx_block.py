@@ -109,6 +109,36 @@ def test_cross_attention_text_lengths(gpu):
         ca(x, ctx, [1, 2])
 
 
+@torch.no_grad()
+@pytest.mark.parametrize("quantized", [False, True])
+def test_text_lengths_change_under_a_captured_graph(gpu, quantized):
+    B, S, L, dim, H = 3, 70, 40, 256, 2
+    ca = wan.WanT2VCrossAttention(dim, H).to(gpu).to(BF)
+    if quantized:
+        for n in ("q", "k", "v", "o"):
+            setattr(ca, n, MXLinear(getattr(ca, n)))
+    x, ctx = torch.randn(B, S, dim, device=gpu).to(BF), torch.randn(B, L, dim, device=gpu).to(BF)
+    lens = torch.tensor([40, 17, 0], device=gpu)
+    all_lens = [lens.clone(), torch.tensor([1, 40, 39], device=gpu), torch.tensor([0, 0, 8], device=gpu)]
+    refs = [ca(x, ctx, n) for n in all_lens]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ca(x, ctx, lens)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = ca(x, ctx, lens)
+    for _ in range(2):
+        for n, r in zip(all_lens, refs):
+            lens.copy_(n)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, r)
+            assert torch.equal(ca(x, ctx, n), r)
+
+
 def _together(x, w1, b1, w2, k, v, starts):
     """A layer into 4 bits, a layer out of them, attention of its result under documents."""
     h = mx_linear(x, w1, b1, activation="gelu_tanh", out_dtype="mxfp4")
