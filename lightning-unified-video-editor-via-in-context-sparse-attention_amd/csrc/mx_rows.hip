@@ -77,68 +77,66 @@ __global__ void __launch_bounds__(1024) icsa_mx_rows_kernel(MxGemmParams p) {
       acc[t] = mx_mfma<3>(wf.c[3], xf[t].c[3], acc[t], wf.s, xf[t].s);
     }
   }
-  // ---- the waves' sums, one token tile at a time: [wave][quarter][lane][4] ----
+  // ---- the waves' sums: [wave][token tile][quarter][lane][4] ----  a wave adds up one quarter of one tile
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    if (t > 0) __syncthreads();
+  for (int t = 0; t < MT; ++t)
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<floatx4*>(red + ((wave * 4 + q) * 64 + lane) * 4) =
+      *reinterpret_cast<floatx4*>(red + (((wave * MT + t) * 4 + q) * 64 + lane) * 4) =
           floatx4{acc[t][4 * q], acc[t][4 * q + 1], acc[t][4 * q + 2], acc[t][4 * q + 3]};
-    __syncthreads();
-    const int m = p.m_first + 32 * t + li;
-    auto total = [&](int q) -> floatx4 {
-      floatx4 s = *reinterpret_cast<const floatx4*>(red + (q * 64 + lane) * 4);
-      for (int v = 1; v < nw; ++v) {
-        const floatx4 x = *reinterpret_cast<const floatx4*>(red + ((v * 4 + q) * 64 + lane) * 4);
+  __syncthreads();
+  auto total = [&](int t, int q) -> floatx4 {
+    const float* src = red + ((t * 4 + q) * 64 + lane) * 4;
+    floatx4 s = *reinterpret_cast<const floatx4*>(src);
+    for (int v = 1; v < nw; ++v) {
+      const floatx4 x = *reinterpret_cast<const floatx4*>(src + v * MT * 1024);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[e] += x[e];
-      }
+      for (int e = 0; e < 4; ++e) s[e] += x[e];
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[e] += bias_at(p, n0 + 8 * q + 4 * hl + e);
-        if (p.gelu) s[e] = gelu_tanh(s[e]);
-      }
-      return s;
-    };
-    if constexpr (kOut == MX_OUT_MXFP4) {
-      if (wave == 0) {                                 // a block's scale takes all of its 32 outputs
-        float v[16];
+    for (int e = 0; e < 4; ++e) {
+      s[e] += bias_at(p, n0 + 8 * q + 4 * hl + e);
+      if (p.gelu) s[e] = gelu_tanh(s[e]);
+    }
+    return s;
+  };
+  if constexpr (kOut == MX_OUT_MXFP4) {
+    if (wave >= MT) return;                            // a block's scale takes all of its 32 outputs
+    float v[16];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const floatx4 s = total(q);
+    for (int q = 0; q < 4; ++q) {
+      const floatx4 s = total(wave, q);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[4 * q + e] = s[e];
-        }
-        store_mx(p, v, n0, m);
-      }
-    } else if (wave < 4) {
-      const floatx4 s = total(wave);
-      const int n = n0 + 8 * wave + 4 * hl;
-      if (m < p.m_last) {
-        if constexpr (kOut == MX_OUT_F32) {
-          float* dst = reinterpret_cast<float*>(p.out) + (int64_t)m * p.o_ss + n;
-          if (n + 4 <= p.N) *reinterpret_cast<floatx4_a4*>(dst) = s;
-          else
+      for (int e = 0; e < 4; ++e) v[4 * q + e] = s[e];
+    }
+    store_mx(p, v, n0, p.m_first + 32 * wave + li);
+  } else {
+    for (int u = wave; u < 4 * MT; u += nw) {
+      const floatx4 s = total(u >> 2, u & 3);
+      const int n = n0 + 8 * (u & 3) + 4 * hl, m = p.m_first + 32 * (u >> 2) + li;
+      if (m >= p.m_last) continue;
+      if constexpr (kOut == MX_OUT_F32) {
+        float* dst = reinterpret_cast<float*>(p.out) + (int64_t)m * p.o_ss + n;
+        if (n + 4 <= p.N) *reinterpret_cast<floatx4_a4*>(dst) = s;
+        else
 #pragma unroll
-            for (int e = 0; e < 4; ++e) if (n + e < p.N) dst[e] = s[e];
-        } else {
-          bf16* dst = reinterpret_cast<bf16*>(p.out) + (int64_t)m * p.o_ss + n;
-          bf16x4 b;
+          for (int e = 0; e < 4; ++e) if (n + e < p.N) dst[e] = s[e];
+      } else {
+        bf16* dst = reinterpret_cast<bf16*>(p.out) + (int64_t)m * p.o_ss + n;
+        bf16x4 b;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] = (bf16)s[e];
-          if (n + 4 <= p.N) *reinterpret_cast<bf16x4_a2*>(dst) = b;
-          else
+        for (int e = 0; e < 4; ++e) b[e] = (bf16)s[e];
+        if (n + 4 <= p.N) *reinterpret_cast<bf16x4_a2*>(dst) = b;
+        else
 #pragma unroll
-            for (int e = 0; e < 4; ++e) if (n + e < p.N) dst[e] = b[e];
-        }
+          for (int e = 0; e < 4; ++e) if (n + e < p.N) dst[e] = b[e];
       }
     }
   }
 }
 
 // Against the tile kernel (128 x 128 tiles, one workgroup for 128 outputs whatever the rows; us, codes in, N x K): 5,120 x
-// 5,120 at 1 / 32 / 64 rows 9.1 / 8.9 / 11.5 to 12.9 / 13.5 / 13.6; 5,120 x 13,824 11.1 / 15.7 / 24.8 to 27.0 / 27.1 /
+// 5,120 at 1 / 32 / 64 rows 9.1 / 8.5 / 10.8 to 12.9 / 13.5 / 13.6; 5,120 x 13,824 11.1 / 15.7 / 24.2 to 27.0 / 27.1 /
 // 27.4; 13,824 x 5,120 10.0 / 13.6 / 22.8 to 13.1 / 13.5 / 14.5; 30,720 x 5,120 at 1 / 4 / 16 rows 19.5 / 20.3 / 23.4 to
 // 19.7 / 18.2 / 18.4: many outputs fill the chip with tiles, whose lines are read whole.
 bool mx_rows_takes(int M, int N) { return M <= 2 || (M <= 32 && N <= 16384) || (M <= 64 && N <= 8192); }
@@ -153,9 +151,11 @@ namespace {
 template <int MT, int kSrc, int kOut>
 hipError_t run_mx_rows(const MxGemmParams& p, hipStream_t stream) {
   const int blocks = (out_columns(p) + 31) / 32;
-  int nw = 4;                                          // waves: 16 a CU and more, not more than groups
-  while (nw < 16 && blocks * nw < 4096 && nw < p.groups) nw *= 2;
-  const int lds = nw * 4096 + (kSrc != 0 ? p.M * (p.groups * (MXG_LINE + MX_GROUP_BLOCKS) + MXR_PAD) + 16 : 0);
+  // waves: 16 a CU and more, not more than groups; 16 in a workgroup where each CU has one (32 x 13,824 x 5,120, 432 workgroups: 14.1 us
+  // with 8, 14.7 with 16; 2 x 5,120 x 13,824, 160 workgroups: 13.2 and 12.1)
+  int nw = 4;
+  while (nw < 16 && blocks * nw < (nw < 8 ? 4096 : 2048) && nw < p.groups) nw *= 2;
+  const int lds = nw * MT * 4096 + (kSrc != 0 ? p.M * (p.groups * (MXG_LINE + MX_GROUP_BLOCKS) + MXR_PAD) + 16 : 0);
   static std::atomic<unsigned> lds_set{0u};
   const hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(icsa_mx_rows_kernel<MT, kSrc, kOut>), 160 * 1024, &lds_set);
   if (e != hipSuccess) return e;
