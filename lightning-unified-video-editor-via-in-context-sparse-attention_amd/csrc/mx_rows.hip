@@ -2,8 +2,9 @@
 // matrix instruction's registers.
 //
 // A workgroup has 32 outputs and up to 32 MT tokens; its waves share the groups of k between them and add their
-// sums through LDS in wave order (bitwise reproducible).  A lane reads 64 contiguous bytes of its weight row a group, the next
-// group's while it multiplies.  For up to MXR_RAW_ROWS rows of bf16 or f32 the workgroup quantises x itself into LDS:
+// sums through LDS in wave order (bitwise reproducible).  A lane reads 64 contiguous bytes of its weight row and of its token rows a
+// group, the next group's while it multiplies (the token rows' without that: 1 x 30,720 x 5,120 21.6 us against 19.6, 64 x 5,120 x
+// 13,824 24.2 against 22.8).  For up to MXR_RAW_ROWS rows of bf16 or f32 the workgroup quantises x itself into LDS:
 // one launch instead of two.
 #include "mx_tile.h"
 
@@ -28,9 +29,12 @@ __device__ __forceinline__ MxFrag load_frag(const unsigned char* codes, const un
 
 }  // namespace
 
+// most waves of a workgroup: two token tiles' operands, read a group ahead, need 154 registers
+constexpr int mx_rows_waves(int mt) { return mt == 1 ? 16 : 8; }
+
 // kSrc: x in 4 bits (0), bf16 (1) or f32 (2)
 template <int MT, int kSrc, int kOut>
-__global__ void __launch_bounds__(1024) icsa_mx_rows_kernel(MxGemmParams p) {
+__global__ void __launch_bounds__(64 * mx_rows_waves(MT)) icsa_mx_rows_kernel(MxGemmParams p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5, nw = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -63,12 +67,21 @@ __global__ void __launch_bounds__(1024) icsa_mx_rows_kernel(MxGemmParams p) {
     else return load_frag(smem, xs, lds_line, p.M, m, gg, hl);
   };
   floatx16 acc[MT] = {};
+  MxFrag xnext[MT];
+  if (wave < p.groups) {
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xnext[t] = token_frag(t, wave);
+  }
   for (int g = wave; g < p.groups; g += nw) {
     const MxFrag wf = wnext;
-    if (g + nw < p.groups) wnext = weight_frag(g + nw);
     MxFrag xf[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xf[t] = token_frag(t, g);
+    for (int t = 0; t < MT; ++t) xf[t] = xnext[t];
+    if (g + nw < p.groups) {
+      wnext = weight_frag(g + nw);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) xnext[t] = token_frag(t, g + nw);
+    }
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       acc[t] = mx_mfma<0>(wf.c[0], xf[t].c[0], acc[t], wf.s, xf[t].s);
@@ -136,12 +149,12 @@ __global__ void __launch_bounds__(1024) icsa_mx_rows_kernel(MxGemmParams p) {
 }
 
 // Against the tile kernel (128 x 128 tiles, one workgroup for 128 outputs whatever the rows; us, codes in, N x K): 5,120 x
-// 5,120 at 1 / 32 / 64 rows 9.1 / 8.5 / 10.8 to 12.9 / 13.5 / 13.6; 5,120 x 13,824 11.1 / 15.7 / 24.2 to 27.0 / 27.1 /
-// 27.4; 13,824 x 5,120 10.0 / 13.6 / 22.8 to 13.1 / 13.5 / 14.5; 30,720 x 5,120 at 1 / 4 / 16 rows 19.5 / 20.3 / 23.4 to
-// 19.7 / 18.2 / 18.4: many outputs fill the chip with tiles, whose lines are read whole.
-bool mx_rows_takes(int M, int N) { return M <= 2 || (M <= 32 && N <= 16384) || (M <= 64 && N <= 8192); }
+// 5,120 at 1 / 32 / 64 rows 8.9 / 8.5 / 10.6 to 12.9 / 13.5 / 13.6; 5,120 x 13,824 11.1 / 15.7 / 22.8 to 27.0 / 27.1 /
+// 27.4; 13,824 x 5,120 10.0 / 12.9 / 22.8 to 13.1 / 13.5 / 14.5; 30,720 x 5,120 at 1 / 4 / 16 rows 19.7 / 20.7 / 25.1 to
+// 18.9 / 18.9 / 19.2, 20,480 x 5,120 15.7 / 16.4 / 19.0 to 13.5 / 13.5 / 13.7: many outputs fill the chip with tiles, whose lines are read whole.
+bool mx_rows_takes(int M, int N) { return (M <= 32 && N <= 16384) || (M <= 64 && N <= 8192); }
 
-// 30,720 x 5,120 with the quantisation in the call: 19.9 us at one row, 22.3 in two launches; 25.1 at four rows, 21.5 in two
+// 30,720 x 5,120 with the quantisation in the call: 18.3 us at one row, 21.5 in two launches; 25.1 at four rows, 21.5 in two
 bool mx_rows_takes_raw(int64_t M, int K) {
   return M <= MXR_RAW_ROWS && M * (mx_padded(K) / 2 + MXR_PAD + mx_padded(K) / MX_BLOCK) <= 64 * 1024;
 }
@@ -152,9 +165,9 @@ template <int MT, int kSrc, int kOut>
 hipError_t run_mx_rows(const MxGemmParams& p, hipStream_t stream) {
   const int blocks = (out_columns(p) + 31) / 32;
   // waves: 16 a CU and more, not more than groups; 16 in a workgroup where each CU has one (32 x 13,824 x 5,120, 432 workgroups: 14.1 us
-  // with 8, 14.7 with 16; 2 x 5,120 x 13,824, 160 workgroups: 13.2 and 12.1)
+  // with 8, 14.7 with 16; 2 x 5,120 x 13,824, 160 workgroups: 13.2 and 12.1, before token rows were read ahead)
   int nw = 4;
-  while (nw < 16 && blocks * nw < (nw < 8 ? 4096 : 2048) && nw < p.groups) nw *= 2;
+  while (nw < mx_rows_waves(MT) && blocks * nw < (nw < 8 ? 4096 : 2048) && nw < p.groups) nw *= 2;
   const int lds = nw * MT * 4096 + (kSrc != 0 ? p.M * (p.groups * (MXG_LINE + MX_GROUP_BLOCKS) + MXR_PAD) + 16 : 0);
   static std::atomic<unsigned> lds_set{0u};
   const hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(icsa_mx_rows_kernel<MT, kSrc, kOut>), 160 * 1024, &lds_set);
