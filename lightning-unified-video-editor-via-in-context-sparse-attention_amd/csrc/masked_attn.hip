@@ -244,6 +244,19 @@ __global__ void __launch_bounds__(MA_THREADS, ma_wg_per_cu(D)) icsa_masked_attn_
     for (int kk = 0; kk < kSteps; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(src + 16 * kk);
   }
 
+  // the heads' bias tables, their ends repeated over a tile's width: the first values requested here, with the rows' borders
+  const int bias_width = 2 * p.radius + 1, bias_row = bias_width + 2 * MA_BIAS_MARGIN;
+  auto bias_value = [&](int x) {
+    const int h = G == 1 ? 0 : x / bias_row, at = x - h * bias_row;
+    return p.bias[(int64_t)(hk * G + h) * bias_width + min(max(at - MA_BIAS_MARGIN, 0), bias_width - 1)];
+  };
+  float bias_first[2] = {0.f, 0.f};
+  if constexpr (kBias) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (threadIdx.x + MA_THREADS * i < (unsigned)(G * bias_row)) bias_first[i] = bias_value(threadIdx.x + MA_THREADS * i);
+  }
+
   // ---- what the rows see ----
   RowRange rr = row_range(p, b, G == 1 ? r0 + li : p.by_g.div(r0 + li));
   if (li >= rows_valid) rr = RowRange{0, 0, 0};
@@ -260,13 +273,10 @@ __global__ void __launch_bounds__(MA_THREADS, ma_wg_per_cu(D)) icsa_masked_attn_
     if (threadIdx.x == 0) ctl[16] = 0;
   }
   const float c = p.scale * MA_LOG2E;
-  const int bias_row = 2 * p.radius + 1 + 2 * MA_BIAS_MARGIN;            // a head's table, its ends repeated over a tile's width
   if constexpr (kBias) {
-    const int width = 2 * p.radius + 1;
-    const float* src = p.bias + (int64_t)hk * G * width;                 // the group's heads
-    for (int x = threadIdx.x; x < G * bias_row; x += MA_THREADS) {
-      const int h = x / bias_row, at = x - h * bias_row;
-      const float f = src[h * width + min(max(at - MA_BIAS_MARGIN, 0), width - 1)];
+    int i = 0;
+    for (int x = threadIdx.x; x < G * bias_row; x += MA_THREADS, ++i) {
+      const float f = i == 0 ? bias_first[0] : i == 1 ? bias_first[1] : bias_value(x);
       // a type's lowest value stays finite in units of log2; infinities and NaN are kept
       bias_lds[x] = !__builtin_isfinite(f) ? f : fminf(fmaxf(f * MA_LOG2E, -3.4028234663852886e38f), 3.4028234663852886e38f);
     }
