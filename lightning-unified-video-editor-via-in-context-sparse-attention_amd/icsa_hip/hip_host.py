@@ -427,7 +427,8 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
         raise IcsaArgumentError("D must be 64 or 128")
     if B < 1 or Hk < 1 or H < 1 or H % Hk:
         raise IcsaArgumentError("H must be a multiple of Hk")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
         raise IcsaArgumentError("masked_attn_func has no backward: call it under torch.no_grad()")
     docs, radius = 1, 0
     if q_starts is not None or k_starts is not None:
