@@ -251,8 +251,7 @@ struct MxGemmParams {
   int m_first, m_last;                                     // token rows of a launch
 };
 hipError_t launch_mx_gemm(MxGemmParams p, hipStream_t stream);
-// few token rows (mx_rows.hip)
-bool mx_rows_takes(int M, int N);
+// few token rows (mx_rows.hip; mx_plan.h: which)
 bool mx_rows_takes_raw(int64_t M, int K);
 hipError_t launch_mx_rows(const MxGemmParams& p, hipStream_t stream);
 

@@ -15,13 +15,12 @@
 // 3.95 PFLOP/s, 2.7 times the bf16 library product's rate at this size (6.46 ms); 1.6 of a tile's 43 us are the GELU (two
 // transcendentals an output, nothing to overlap them with); an earlier form without loads in the loop 2.16 ms.  4 waves of 128 x 128,
 // a third fewer bytes out of LDS but one wave a SIMD, were slower: 14,040 x 5,120 x 13,824 538 us against 462.
-#include <algorithm>
 #include <type_traits>
 
+#include "mx_plan.h"
 #include "mx_tile.h"
 
 #define MXG_STAGE 2048                                 // bytes of output staging of a wave
-#define MXG_CUS 256
 #define MXG_BAND 4                                     // token tiles that go together in the order; 2.56 ms against 2.69 with 8
 
 namespace {
@@ -264,31 +263,18 @@ hipError_t run_mx_gemm(const MxGemmParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// A launch takes rounds of one tile a CU.  Measured (us, one round): a 256 x 256 tile 1.6 a group and 1 to 4 besides, GELU 3.4; a
-// 128 x 128 tile 0.56 a group and 2.5, GELU 0.5; a launch 4.5.  In units of 0.56 us.
-double rounds_of(int64_t tiles) { return (double)((tiles + MXG_CUS - 1) / MXG_CUS); }
-double big_time(int64_t tiles, const MxGemmParams& p) { return rounds_of(tiles) * (2.9 * p.groups + 4 + 6 * p.gelu); }
-double small_time(int64_t tiles, const MxGemmParams& p) { return rounds_of(tiles) * (p.groups + 4.5 + 1 * p.gelu); }
-
-// 256 x 256 tiles, 128 x 128 tiles, or the first rows in whole rounds of the former and the others in the latter.  All three
-// measured (us, M x N x K): 512 x 5,120 x 4,096 24.3, 12.7, -; 1,560 x 5,120 x 5,120 32.0, 41.3, -; 3,120 x 5,120 x 5,120 67.1, 57.2,
-// 54.7; 9,360 x 2,000 x 5,120 71.0, 72.4, 61.7; 14,040 x 5,120 x 13,824 454.9, 597.0, 450.3; 65,520 x 5,120 x 5,120 817, 1,154, 822.
 template <int kOut>
 hipError_t pick_mx_gemm(MxGemmParams p, hipStream_t stream) {
-  const int64_t cols = out_columns(p), n_big = (cols + 255) / 256, n_small = (cols + 127) / 128;
-  const int64_t m_big = (p.M + 255) / 256, whole = n_big * m_big / MXG_CUS;
-  auto small = [&](int64_t rows) { return small_time(n_small * ((rows + 127) / 128), p); };
-  const int64_t split = std::min<int64_t>(whole * MXG_CUS / n_big, m_big - 1) * 256;      // rows that whole rounds take
-  const double t_big = big_time(n_big * m_big, p), t_small = small(p.M);
-  const double t_split = split > 0 ? big_time(n_big * (split / 256), p) + small(p.M - split) + 8 : t_big + 1;
-  if (t_small <= t_big && t_small <= t_split) return run_mx_gemm<2, 2, 2, 2, 4, kOut>(p, stream);
-  if (t_big <= t_split) return run_mx_gemm<2, 4, 4, 2, 2, kOut>(p, stream);
-  p.m_last = (int)split;
-  const hipError_t e = run_mx_gemm<2, 4, 4, 2, 2, kOut>(p, stream);
-  if (e != hipSuccess) return e;
-  p.m_first = (int)split;
-  p.m_last = p.M;
-  return mx_rows_takes(p.M - p.m_first, p.N) ? launch_mx_rows(p, stream) : run_mx_gemm<2, 2, 2, 2, 4, kOut>(p, stream);
+  const int large = (int)mx_large_rows(p.M, out_columns(p), p.groups, p.gelu != 0);
+  if (large > 0) {
+    p.m_last = large;
+    const hipError_t e = run_mx_gemm<2, 4, 4, 2, 2, kOut>(p, stream);
+    if (e != hipSuccess || large == p.M) return e;
+    p.m_first = large;
+    p.m_last = p.M;
+    if (mx_rows_takes(p.M - large, p.N)) return launch_mx_rows(p, stream);
+  }
+  return run_mx_gemm<2, 2, 2, 2, 4, kOut>(p, stream);
 }
 
 }  // namespace

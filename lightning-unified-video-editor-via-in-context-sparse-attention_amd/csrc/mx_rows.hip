@@ -148,12 +148,6 @@ __global__ void __launch_bounds__(64 * mx_rows_waves(MT)) icsa_mx_rows_kernel(Mx
   }
 }
 
-// Against the tile kernel (128 x 128 tiles, one workgroup for 128 outputs whatever the rows; us, codes in, N x K): 5,120 x
-// 5,120 at 1 / 32 / 64 rows 8.9 / 8.5 / 10.6 to 12.9 / 13.5 / 13.6; 5,120 x 13,824 11.1 / 15.7 / 22.8 to 27.0 / 27.1 /
-// 27.4; 13,824 x 5,120 10.0 / 12.9 / 22.8 to 13.1 / 13.5 / 14.5; 30,720 x 5,120 at 1 / 4 / 16 rows 19.7 / 20.7 / 25.1 to
-// 18.9 / 18.9 / 19.2, 20,480 x 5,120 15.7 / 16.4 / 19.0 to 13.5 / 13.5 / 13.7: many outputs fill the chip with tiles, whose lines are read whole.
-bool mx_rows_takes(int M, int N) { return (M <= 32 && N <= 16384) || (M <= 64 && N <= 8192); }
-
 // 30,720 x 5,120 with the quantisation in the call: 18.3 us at one row, 21.5 in two launches; 25.1 at four rows, 21.5 in two
 bool mx_rows_takes_raw(int64_t M, int K) {
   return M <= MXR_RAW_ROWS && M * (mx_padded(K) / 2 + MXR_PAD + mx_padded(K) / MX_BLOCK) <= 64 * 1024;
