@@ -71,3 +71,29 @@ def attention(q, k, v, *, q_starts=None, k_starts=None, causal=False, prefix=Non
             e = 2.0 ** -23 * (D * torch.where(see[b], mass, 0.0).amax(-1) + 8 * torch.where(see[b], size, 0.0).amax(-1) + 8)
             bound[b, :, h] = (2.0 ** -8 + 2.5 * e)[:, None] * (p @ torch.where(fine, vv.abs(), 0.0)) + 1e-30
     return out, bound
+
+
+def one_head(q, k, v, lo, hi, at, *, scale, softcap=0.0, bias=None):
+    """(out, bound) float64 of one head, on its inputs' device: q [R, D], k, v [Sk, D], row i sees the keys [lo_i, hi_i) and
+    stands at key at_i (all [R]); bias [2 R + 1].  The bound is :func:`attention`'s.  Values have to be finite."""
+    q, k, v = q.double(), k.double(), v.double()
+    kt = k.t().contiguous()
+    s = scale * (q @ kt)
+    mass = scale * (q.abs() @ kt.abs())
+    size = s.abs()
+    if softcap:
+        s = softcap * torch.tanh(s / softcap)
+        size = size.clamp(max=8 * softcap) + softcap
+    j = torch.arange(k.shape[0], device=q.device)[None]
+    if bias is not None:
+        R = bias.shape[0] // 2
+        x = bias.double()[(j - at[:, None]).clamp(-R, R) + R]
+        s = s + x
+        size = size + x.abs()
+    see = (j >= lo[:, None]) & (j < hi[:, None])
+    none = ~see.any(-1)
+    s = s.masked_fill(~see, -math.inf)
+    p = torch.exp(s - torch.where(none, 0.0, s.amax(-1))[:, None])
+    p = p / torch.where(none, 1.0, p.sum(-1))[:, None]
+    e = 2.0 ** -23 * (q.shape[1] * torch.where(see, mass, 0.0).amax(-1) + 8 * torch.where(see, size, 0.0).amax(-1) + 8)
+    return p @ v, (2.0 ** -8 + 2.5 * e)[:, None] * (p @ v.abs()) + 1e-30
