@@ -265,9 +265,8 @@ class WanSelfAttention(nn.Module):
     capture = None    # a dict here receives the workspace views (decisions) of the next call
 
     def forward(self, x, seq_lens, grid_sizes, source_video_grid_sizes, TAG, freqs):
-        xm = _linear_input(x, self.q, self.k, self.v)
         res = wan_self_attention_core(
-            self.q(xm), self.k(xm), self.v(xm), self.alpha_1(x), self.norm_q.weight,
+            *_project(x, self.q, self.k, self.v), self.alpha_1(x), self.norm_q.weight,
             self.norm_k.weight, grid_sizes, source_video_grid_sizes, TAG, freqs,
             self.num_heads, self.eps, out_dtype=x.dtype, keep_workspace=self.capture is not None)
         if self.capture is not None:
@@ -277,9 +276,13 @@ class WanSelfAttention(nn.Module):
         return self.o(res.flatten(2))
 
 
-def _linear_input(x, *layers):
-    """x, in 4 bits where all of the layers that read it are MXLinear: quantised once for them."""
-    return mx_quantize(x) if all(isinstance(m, MXLinear) for m in layers) else x
+def _project(x, *layers):
+    """The layers' results for x, of x's type.  Where all of them are MXLinear x is quantised once for them; its codes do
+    not know its type, so the layers are told."""
+    if all(isinstance(m, MXLinear) for m in layers):
+        xm = mx_quantize(x)
+        return [m(xm, out_dtype=x.dtype) for m in layers]
+    return [m(x) for m in layers]
 
 
 class WanLayerNorm(nn.LayerNorm):
@@ -322,10 +325,10 @@ class WanT2VCrossAttention(nn.Module):
         no_rope = _identity_freqs(self.head_dim, x.device)
         q = wan_qk_prologue(self.q(x), None, self.norm_q.weight, None, none, none, 0, no_rope,
                             self.num_heads, eps=self.eps, want_sums=False)[0]
-        cm = _linear_input(context, self.k, self.v)
-        k = wan_qk_prologue(self.k(cm), None, self.norm_k.weight, None, none, none, 0,
+        yk, yv = _project(context, self.k, self.v)
+        k = wan_qk_prologue(yk, None, self.norm_k.weight, None, none, none, 0,
                             no_rope, self.num_heads, eps=self.eps, want_sums=False)[0]
-        v = self.v(cm).view(b, -1, self.num_heads, self.head_dim).to(torch.bfloat16)
+        v = yv.view(b, -1, self.num_heads, self.head_dim).to(torch.bfloat16)
         if context_lens is None:
             y = flash_attn_func(q, k, v)
         else:                                       # one document a batch row: its text's real tokens
@@ -406,7 +409,9 @@ class WanAttentionBlock(nn.Module):
         hidden row goes from that accumulator to its codes, which the second product reads."""
         lin0, lin2 = self.ffn[0], self.ffn[2]
         if isinstance(lin0, MXLinear):
-            return lin2(lin0(h, activation='gelu_tanh', out_dtype='mxfp4' if isinstance(lin2, MXLinear) else None))
+            if isinstance(lin2, MXLinear):
+                return lin2(lin0(h, activation='gelu_tanh', out_dtype='mxfp4'), out_dtype=h.dtype)
+            return lin2(lin0(h, activation='gelu_tanh'))
         f = torch._addmm_activation(lin0.bias, h.reshape(-1, h.shape[-1]), lin0.weight.t(), use_gelu=True)
         return lin2(f).view(*h.shape[:-1], lin2.out_features)
 
