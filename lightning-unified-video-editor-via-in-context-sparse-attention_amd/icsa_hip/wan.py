@@ -285,6 +285,21 @@ def _project(x, *layers):
     return [m(x) for m in layers]
 
 
+def _gelu_pair(lin0, lin2, h):
+    """lin2(GELU(tanh)(lin0(h))) of h's type, lin0 an MXLinear: GELU in its epilogue, and where lin2 is one too the hidden row
+    goes from the f32 accumulator to its codes, which the second product reads."""
+    if isinstance(lin2, MXLinear):
+        return lin2(lin0(h, activation='gelu_tanh', out_dtype='mxfp4'), out_dtype=h.dtype)
+    return lin2(lin0(h, activation='gelu_tanh'))
+
+
+def _f32_linear(lin, z):
+    """lin(z) of a float32 z in float32, as in the reference's autocast(float32) regions (an MXLinear's result has z's type)."""
+    if isinstance(lin, MXLinear):
+        return lin(z)
+    return nn.functional.linear(z, lin.weight.float(), lin.bias.float())
+
+
 class WanLayerNorm(nn.LayerNorm):
     """Parameter holder of the reference's WanLayerNorm (model.py:117-122); applied by
     ``ln_modulate``."""
@@ -405,13 +420,10 @@ class WanAttentionBlock(nn.Module):
         """self.ffn(h) (Linear, GELU(tanh), Linear; model.py:243-245) with the bias and the
         GELU applied in the first GEMM's epilogue, on its fp32 accumulator: no separate
         elementwise pass over the [tokens, ffn_dim] hidden.  The reference rounds the first
-        Linear's output to bf16 before its GELU; the epilogue rounds once, after it.  In 4 bits the
-        hidden row goes from that accumulator to its codes, which the second product reads."""
+        Linear's output to bf16 before its GELU; the epilogue rounds once, after it."""
         lin0, lin2 = self.ffn[0], self.ffn[2]
         if isinstance(lin0, MXLinear):
-            if isinstance(lin2, MXLinear):
-                return lin2(lin0(h, activation='gelu_tanh', out_dtype='mxfp4'), out_dtype=h.dtype)
-            return lin2(lin0(h, activation='gelu_tanh'))
+            return _gelu_pair(lin0, lin2, h)
         f = torch._addmm_activation(lin0.bias, h.reshape(-1, h.shape[-1]), lin0.weight.t(), use_gelu=True)
         return lin2(f).view(*h.shape[:-1], lin2.out_features)
 
@@ -419,7 +431,8 @@ class WanAttentionBlock(nn.Module):
 def quantize_linears(block: WanAttentionBlock) -> WanAttentionBlock:
     """Replaces a block's q / k / v / o projections (self and cross attention) and both FFN layers by
     :class:`MXLinear` of their weights, on the GPU: their weights take 17/64 of
-    the bf16 memory, and the products run on the block-scaled matrix instructions.  alpha_1 (one output) stays."""
+    the bf16 memory, and the products run on the block-scaled matrix instructions.  alpha_1 (one output) stays.  The model's
+    text, time and head layers stay too; an MXLinear put in the place of one of them is taken."""
     for att in (block.self_attn, block.cross_attn):
         for name in ("q", "k", "v", "o"):
             if not isinstance(getattr(att, name), MXLinear):
@@ -457,8 +470,7 @@ class Head(nn.Module):
     def forward(self, x, e):
         e = (self.modulation.float() + e.float().unsqueeze(1)).chunk(2, dim=1)
         n = nn.functional.layer_norm(x.float(), (self.dim,), eps=self.eps)
-        return nn.functional.linear(n * (1 + e[1]) + e[0], self.head.weight.float(),
-                                    self.head.bias.float())
+        return _f32_linear(self.head, n * (1 + e[1]) + e[0])
 
 
 class WanModel(nn.Module):
@@ -551,16 +563,16 @@ class WanModel(nn.Module):
         rows = [torch.cat([u, v], dim=0) for u, v in zip(xs, ss)]
         _require(max(r.shape[0] for r in rows) <= seq_len, "seq_len smaller than the token count")
         xb = torch.stack([torch.cat([r, r.new_zeros(seq_len - r.shape[0], self.dim)]) for r in rows])
-        def f32_linear(lin, z):                  # the reference's autocast(float32) region
-            return nn.functional.linear(z, lin.weight.float(), lin.bias.float())
-
         temb = sinusoidal_embedding_1d(self.freq_dim, t).float().to(dev)
-        e = f32_linear(self.time_embedding[2],
-                       nn.functional.silu(f32_linear(self.time_embedding[0], temb)))
-        e0 = f32_linear(self.time_projection[1], nn.functional.silu(e)).unflatten(1, (6, self.dim))
-        ctx = self.text_embedding(torch.stack([
-            torch.cat([u, u.new_zeros(self.text_len - u.size(0), u.size(1))]) for u in context]).to(
-                self.text_embedding[0].weight.dtype))
+        e = _f32_linear(self.time_embedding[2],
+                        nn.functional.silu(_f32_linear(self.time_embedding[0], temb)))
+        e0 = _f32_linear(self.time_projection[1], nn.functional.silu(e)).unflatten(1, (6, self.dim))
+        text = torch.stack([torch.cat([u, u.new_zeros(self.text_len - u.size(0), u.size(1))]) for u in context])
+        text0 = self.text_embedding[0]
+        if isinstance(text0, MXLinear):
+            ctx = _gelu_pair(text0, self.text_embedding[2], text.to(xb.dtype))
+        else:
+            ctx = self.text_embedding(text.to(text0.weight.dtype))
         seq_lens = torch.tensor([r.shape[0] for r in rows], dtype=torch.long)
         h = xb
         for block in self.blocks:

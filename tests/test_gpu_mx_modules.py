@@ -1,4 +1,5 @@
-"""Types of the 4-bit layers in the modules: results in the input's type also where an input is quantised once for several layers."""
+"""Types and places of the 4-bit layers in the modules: results in the input's type also where an input is quantised once for
+several layers, and MXLinear in the model's text and time layers and its head."""
 import pytest
 import torch
 import torch.nn as nn
@@ -71,3 +72,44 @@ def test_ffn_keeps_the_input_type(gpu, dtype):
     y = blk._ffn(h)
     assert y.dtype == dtype
     assert torch.equal(y, mx_linear(l0(h, "gelu_tanh", "mxfp4"), l2.weight, l2.bias, out_dtype=dtype))
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("text", [(0,), (2,), (0, 2)])
+def test_text_and_time_layers_of_the_model(gpu, text):
+    """MXLinear in the place of a Linear of the text embedding, the time embedding, the time projection and the head: each is
+    called once; the time layers and the head in float32, the text layers in the weights' type."""
+    torch.manual_seed(2)
+    m = wan.WanModel(in_dim=4, dim=256, ffn_dim=512, freq_dim=32, text_dim=64, out_dim=4, num_heads=2, num_layers=1, text_len=16)
+    m.init_weights()
+    nn.init.normal_(m.head.head.weight, std=0.02)
+    m = m.to(gpu).to(BF)
+    lat, ctx = torch.randn(4, 2, 32, 32, device=gpu).to(BF), [torch.randn(12, 64, device=gpu).to(BF)]
+    args = ([lat], torch.tensor([637.0], device=gpu), ctx, 1024, [lat])
+    plain = m(*args)[0]
+    calls = {}
+    for name, seq, i in [("time0", m.time_embedding, 0), ("time2", m.time_embedding, 2), ("proj", m.time_projection, 1),
+                         *((f"text{i}", m.text_embedding, i) for i in text)]:
+        seq[i] = MXLinear(seq[i])
+        seq[i].register_forward_hook(lambda mod, x, y, name=name: calls.setdefault(name, []).append(y))
+    m.head.head = MXLinear(m.head.head)
+    m.head.head.register_forward_hook(lambda mod, x, y: calls.setdefault("head", []).append(y))
+    out = m(*args)[0]
+    assert torch.isfinite(out).all() and out.shape == plain.shape and out.dtype == plain.dtype
+    assert torch.equal(out, m(*args)[0])
+    assert sorted(calls) == sorted(["time0", "time2", "proj", "head", *(f"text{i}" for i in text)])
+    for name, ys in calls.items():
+        assert len(ys) == 2
+        if not name.startswith("text"):
+            assert ys[0].dtype == torch.float32
+    # the text embedding: GELU between its layers, whichever of them are in 4 bits
+    t0, t2 = m.text_embedding[0], m.text_embedding[2]
+    padded = torch.zeros(1, 16, 64, dtype=BF, device=gpu)
+    padded[0, :12] = ctx[0]
+    if text == (0, 2):
+        assert torch.equal(calls["text2"][0], mx_linear(mx_linear(padded, t0.weight, t0.bias, "gelu_tanh", "mxfp4"), t2.weight, t2.bias))
+    elif text == (0,):
+        assert torch.equal(calls["text0"][0], mx_linear(padded, t0.weight, t0.bias, "gelu_tanh"))
+    else:
+        hidden = nn.functional.gelu(t0(padded), approximate="tanh")
+        assert torch.equal(calls["text2"][0], mx_linear(hidden, t2.weight, t2.bias))
