@@ -409,7 +409,8 @@ int64_t icsa_mx_scales_size(int64_t M, int K);
 /* x [M, K] bf16 or f32 (row stride x_ss elements, any alignment) to codes and scales. */
 int icsa_mx_quantize(const void* x, int x_dtype, int64_t x_ss, int64_t M, int K, void* codes, void* scales, void* stream);
 
-/* The values of codes and scales, bf16 (which holds each of them) or f32 [M, K]. */
+/* The values of codes and scales, bf16 or f32 [M, K].  Either type holds each value that icsa_mx_quantize writes; values
+ * from 2^128 on (codes of 4 and 6 under scale byte 253, of 2 and more under 254) become infinities. */
 int icsa_mx_dequantize(const void* codes, const void* scales, int64_t M, int K, void* out, int out_dtype, int64_t o_ss,
                        void* stream);
 

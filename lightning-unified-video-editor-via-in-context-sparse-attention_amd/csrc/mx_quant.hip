@@ -60,7 +60,8 @@ hipError_t launch_mx_quantize(const MxQuantParams& p, hipStream_t stream) {
 }
 
 // Values of 8 codes a lane.  A code's value times a power of two has at most two significant
-// bits, so bf16 holds every value (2^-128, the least, is a bf16 subnormal); the product with a
+// bits, so bf16 holds every value below 2^128 (2^-128, the least, is a bf16 subnormal; from 2^128 on, under
+// bytes that the quantisation does not write, both types have infinities); the product with a
 // subnormal scale is exact in f32, and its upper half is the bf16.
 template <typename T, int kAhead>
 __global__ void __launch_bounds__(MXQ_THREADS) icsa_mx_dequantize_kernel(MxDequantParams p) {

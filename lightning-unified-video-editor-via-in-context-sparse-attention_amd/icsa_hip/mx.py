@@ -95,7 +95,8 @@ class MXFP4Tensor:
         return f"MXFP4Tensor(shape={tuple(self.shape)}, device={self.device})"
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The values as bf16 (which holds each of them exactly) or float32, a new tensor."""
+        """The values as bf16 or float32, a new tensor: exactly, but for those from 2^128 on (scale bytes 253 and 254, which
+        :func:`mx_quantize` does not write), which become infinities."""
         dev, K = self.device, self.shape[-1]
         if dev.type != "cuda":
             raise IcsaArgumentError("codes must be on the GPU")

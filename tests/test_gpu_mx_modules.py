@@ -1,10 +1,13 @@
 """Types and places of the 4-bit layers in the modules: results in the input's type also where an input is quantised once for
-several layers, and MXLinear in the model's text and time layers and its head."""
+several layers, MXLinear in the model's text and time layers and its head, and what the layers' containers read as."""
+import math
+
 import pytest
 import torch
 import torch.nn as nn
 
-from icsa_hip import MXLinear, mx_linear, wan
+from icsa_hip import MXFP4Tensor, MXLinear, mx_linear, wan
+from oracle import mxfp4 as O
 from oracle import wan_glue as W
 
 pytestmark = pytest.mark.gpu
@@ -113,3 +116,19 @@ def test_text_and_time_layers_of_the_model(gpu, text):
     else:
         hidden = nn.functional.gelu(t0(padded), approximate="tanh")
         assert torch.equal(calls["text2"][0], mx_linear(hidden, t2.weight, t2.bias))
+
+
+def test_values_past_the_types(gpu):
+    """Scale bytes over 252, which mx_quantize does not write: values from 2^128 on, which neither type holds, read as
+    infinities; all others exactly."""
+    codes = torch.arange(16, dtype=torch.uint8).repeat(16).view(1, 256)
+    codes = codes[:, 0::2] | (codes[:, 1::2] << 4)
+    scales = torch.tensor([252, 253, 254, 255, 0, 1, 127, 200], dtype=torch.uint8).view(1, 1, 8)
+    t = MXFP4Tensor(codes.to(gpu), scales.to(gpu), (1, 256))
+    ref = O.values(codes, scales, 256)
+    ref = torch.where(ref.abs() >= 2.0 ** 128, torch.sign(ref) * math.inf, ref)
+    for dt in (BF, torch.float32):
+        got = t.dequantize(dt).cpu().double()
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        assert torch.equal(torch.nan_to_num(got, nan=0.0, posinf=1e300, neginf=-1e300),
+                           torch.nan_to_num(ref, nan=0.0, posinf=1e300, neginf=-1e300))
