@@ -368,8 +368,8 @@ int64_t icsa_masked_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, in
 
 /* Attention under masks: out_i = sum_j softmax_j(s_ij) v_j over the keys that query i sees,
  *   s_ij = cap tanh(scale q_i.k_j / cap) + bias[h][clamp(j - p_i, -radius, radius) + radius]
- * (scale > 0; softcap up to 4096, 0: no cap; bias NULL: none).  q, out [B, Sq, H, D], k, v [B, Sk, Hk, D] bf16 (out bf16 or
- * f32), D 64 or 128, H a multiple of Hk: heads h H / Hk .. share key head h.
+ * (scale > 0; softcap up to 4096, 0: no cap; bias NULL: none, finite values past +-2.36e38 count as that).
+ * q, out [B, Sq, H, D], k, v [B, Sk, Hk, D] bf16 (out bf16 or f32), D 64 or 128, H a multiple of Hk: heads h H / Hk .. share key head h.
  * q_starts, k_starts: device int32 [B, docs + 1], not decreasing: document n of batch row b has queries
  * q_starts[b][n] .. q_starts[b][n + 1] - 1 and keys likewise, and sees its own keys alone; queries
  * outside every document see nothing.  NULL: one document of everything.  Values past the lengths

@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(MA_THREADS, ma_wg_per_cu(D)) icsa_masked_attn_
     int i = 0;
     for (int x = threadIdx.x; x < G * bias_row; x += MA_THREADS, ++i) {
       const float f = i == 0 ? bias_first[0] : i == 1 ? bias_first[1] : bias_value(x);
-      // a type's lowest value stays finite in units of log2; infinities and NaN are kept
+      // a type's lowest value stays finite in units of log2 (biases past 2^128 / log2(e) = 2.36e38 are one); infinities and
+      // NaN are kept
       bias_lds[x] = !__builtin_isfinite(f) ? f : fminf(fmaxf(f * MA_LOG2E, -3.4028234663852886e38f), 3.4028234663852886e38f);
     }
   }

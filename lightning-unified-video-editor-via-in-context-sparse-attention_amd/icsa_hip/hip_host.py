@@ -408,6 +408,7 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
             keys that all of its queries see.
         softcap: scores become ``softcap * tanh(score / softcap)`` (up to 4096); 0 leaves them.
         bias: float32 [H, 2 R + 1], added to the (capped) scores: ``bias[h, clamp(j - p_i, -R, R) + R]``.
+            Finite values past +-2.36e38 count as that.
         softmax_scale: positive, default ``D ** -0.5``.
 
     A query that sees nothing gets zeros; NaN and infinities in keys and values reach only the
