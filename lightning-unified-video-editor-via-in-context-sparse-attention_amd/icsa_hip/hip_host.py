@@ -380,11 +380,13 @@ def _rows16(t: torch.Tensor):
     s0, s1, s2, s3 = t.stride()
     p = t.data_ptr()
     if s3 != 1 or (p | ((s0 | s1 | s2) << 1)) & 15:
-        t = t.contiguous()
-        if t.data_ptr() & 15:
-            t = t.clone()
-        s0, s1, s2, _ = t.stride()
-        p = t.data_ptr()
+        n0, n1, n2, n3 = t.shape                    # a stride over one element may be anything, also in a contiguous tensor
+        s0, s1, s2 = s0 if n0 > 1 else 0, s1 if n1 > 1 else 0, s2 if n2 > 1 else 0
+        if s3 != 1 or (p | ((s0 | s1 | s2) << 1)) & 15:
+            t = t.contiguous()
+            if t.data_ptr() & 15:
+                t = t.clone(memory_format=torch.contiguous_format)
+            p, s0, s1, s2 = t.data_ptr(), n1 * n2 * n3, n2 * n3, n3
     return t, (p, s0, s1, s2)
 
 
