@@ -334,8 +334,11 @@ class WanT2VCrossAttention(nn.Module):
     def forward(self, x, context, context_lens=None):
         b = x.shape[0]
         if context_lens is not None:
-            lens = torch.as_tensor(context_lens, device=x.device).to(torch.int32)
+            lens = torch.as_tensor(context_lens, device=x.device)
+            _require(not (lens.is_floating_point() or lens.is_complex() or lens.dtype == torch.bool),
+                     "context_lens must be whole numbers")
             _require(tuple(lens.shape) == (b,), "context_lens must hold one length a batch row")
+            lens = lens.to(torch.int32)
         none = [(0, 0, 0)] * b
         no_rope = _identity_freqs(self.head_dim, x.device)
         q = wan_qk_prologue(self.q(x), None, self.norm_q.weight, None, none, none, 0, no_rope,
