@@ -313,7 +313,8 @@ class WanT2VCrossAttention(nn.Module):
     single-tensor, unrotated mode, dense attention over the text tokens through
     ``icsa_flash_attn``, or with ``context_lens`` (int [B]: each batch row's real text tokens; a
     row of length 0 gets zeros) through ``icsa_masked_attn``.  Same parameters as the reference
-    class."""
+    class.  The attention is an inference path with and without lengths: under an enabled grad mode its
+    result carries no gradient to q, k, v and what they come from, and nothing is raised."""
 
     def __init__(self, dim, num_heads, window_size=(-1, -1), qk_norm=True, eps=1e-6):
         super().__init__()
@@ -351,7 +352,7 @@ class WanT2VCrossAttention(nn.Module):
             y = flash_attn_func(q, k, v)
         else:                                       # one document a batch row: its text's real tokens
             zero = torch.zeros_like(lens)
-            with torch.no_grad():
+            with torch.no_grad():                   # as flash_attn_func does by itself
                 y = masked_attn_func(q, k, v, q_starts=torch.stack([zero, torch.full_like(lens, q.shape[1])], 1),
                                      k_starts=torch.stack([zero, lens], 1))
         return self.o(y.flatten(2).to(x.dtype))

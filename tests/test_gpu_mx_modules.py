@@ -132,3 +132,13 @@ def test_values_past_the_types(gpu):
         assert torch.equal(torch.isnan(got), torch.isnan(ref))
         assert torch.equal(torch.nan_to_num(got, nan=0.0, posinf=1e300, neginf=-1e300),
                            torch.nan_to_num(ref, nan=0.0, posinf=1e300, neginf=-1e300))
+
+
+@pytest.mark.parametrize("lens", [None, [24]])
+def test_cross_attention_carries_no_gradient(gpu, lens):
+    """With lengths as without: the output projection alone learns."""
+    ca = wan.WanT2VCrossAttention(256, 2).to(gpu).to(BF)
+    x, ctx = torch.randn(1, 70, 256, device=gpu).to(BF), torch.randn(1, 40, 256, device=gpu).to(BF)
+    ca(x, ctx, lens).float().sum().backward()
+    assert ca.o.weight.grad is not None
+    assert all(m.weight.grad is None for m in (ca.q, ca.k, ca.v, ca.norm_q, ca.norm_k))
