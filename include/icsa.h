@@ -376,7 +376,8 @@ int64_t icsa_masked_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, in
  * are clamped.  causal: query i of a document of Lq queries and Lk keys stands at its key
  * p_i = i + Lk - Lq and sees keys up to it; prefix (device int32 [B, docs], with causal): the document's
  * first keys that all of its queries see.  A query that sees nothing gets zeros.  NaN and infinities in
- * keys and values reach only the queries that see them.
+ * keys and values reach only the queries that see them (an infinite value with its sign where its weight does not round to
+ * 0, which may make it NaN; a bias of -inf gives a key no weight but does not unsee it).
  * (The reference's own attention wrapper for ragged lengths: wanx/attention.py:18-85.) */
 int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                      const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,

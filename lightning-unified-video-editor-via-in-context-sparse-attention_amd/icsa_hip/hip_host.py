@@ -414,7 +414,8 @@ def masked_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_sta
         softmax_scale: positive, default ``D ** -0.5``.
 
     A query that sees nothing gets zeros; NaN and infinities in keys and values reach only the
-    queries that see them.  An inference operator: under an enabled grad mode an input that requires a
+    queries that see them (an infinity of a value with its sign where its weight does not round to 0, which
+    may make it NaN; a bias of -inf gives a key no weight but does not unsee it).  An inference operator: under an enabled grad mode an input that requires a
     gradient is refused."""
     bf16 = torch.bfloat16
     if q.dtype != bf16 or k.dtype != bf16 or v.dtype != bf16:
