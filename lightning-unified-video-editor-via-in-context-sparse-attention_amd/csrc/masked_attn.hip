@@ -12,18 +12,19 @@
 // (attn_tile.h).  P goes to the second product from its registers; V is read transposed from its row-major tile.
 //
 // K and V tiles arrive by direct global->LDS loads, two buffers, one barrier a tile: behind it the next tile is
-// requested into the buffer that everybody has left.  Two workgroups share a CU: one's exponentials run beside the
-// other's products.  Products read their operands from LDS four ahead of their use, with raised priority.
+// requested into the buffer that everybody has left.  Two workgroups share a CU, three with heads of 64: one's exponentials run
+// beside another's products.  Products read their operands from LDS four ahead of their use, with raised priority.
 //
 // Values in masked places: scores are replaced, not added to, so a NaN of a masked key does not
 // matter; V rows that no row of the workgroup sees are cleared in LDS; and where a partly visible tile holds
 // a V that is not finite, 0 * V would reach rows that do not see it: such values are cleared too, and added at
 // the end to the rows that see them.
 //
-// What bounds it (two waves a SIMD): the vector instructions and the products of a tile side by side, 550 to 800 and 1,024 cycles
-// a wave with heads of 128, and the clock, 1.7 to 2.1 GHz under them; capped scores add two transcendentals an element.  9,373
-// tokens, 12 heads of 128: dense 525 us (1.03 PFLOP/s in two rounds of workgroups, the second 73 % full), causal 282 (0.96), a prefix
-// and capped scores 375 to 415 (matrix pipe busy 36 %, vector pipe 54 %); 32,760 tokens, 5 heads 2.41 ms (1.14); 9,373 tokens, 12 heads
+// What bounds it (two waves a SIMD with heads of 128, three with 64): the vector instructions and the products of a tile side by
+// side, 550 to 800 and 1,024 cycles a wave with heads of 128, and the clock, 1.7 to 2.1 GHz under them; capped scores add two
+// transcendentals an element.  9,373 tokens, 12 heads of 128: dense 525 us (1.03 PFLOP/s in two rounds of workgroups, the second 73 %
+// full), causal 282 (0.96), a prefix and capped scores 375 to 415 (matrix pipe busy 36 %, vector pipe 54 %: neither is full, a
+// SIMD's waves do not keep to opposite phases by themselves); 32,760 tokens, 5 heads 2.41 ms (1.14); 9,373 tokens, 12 heads
 // of 64 301 us (0.90).  One query of 40 heads over 8 key heads of 65,536 keys: 43 us for 268 MB and 6 for joining 64 parts.  Short
 // documents (packed prompts of 350 keys, 40 heads, 32,760 queries: 314 to 346 us) add the way of Q and the output
 // through memory, 140 us at the copy rate, and each workgroup's start, which two workgroups a CU do not hide.
@@ -137,8 +138,10 @@ __device__ __forceinline__ unsigned bit_select(unsigned mask, unsigned a, unsign
   return r;
 }
 
-// Sum of a lane's 32 probabilities as they go into the second product, rounded to bf16: where few keys carry a row, what their
-// rounding adds to the product it adds to the sum, and the quotient does not see it.  Two values an instruction.
+// Sum of a lane's 32 probabilities as they go into the second product.  They are rounded to bf16, the matrix instruction's type, as
+// in the framework's other attention kernels (2^-8 of a weight at most; 0.0023 of the outputs in the 2-norm with the outputs' own
+// rounding, 0.0017 without): where few keys carry a row, what their rounding adds to the product it adds to the sum, and the
+// quotient does not see it.  Two values an instruction.
 __device__ __forceinline__ float sum_p(const bf16x8 pf[4]) {
   const bf16x2 one = {(bf16)1.f, (bf16)1.f};
   float r[4];

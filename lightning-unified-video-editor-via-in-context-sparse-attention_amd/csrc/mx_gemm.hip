@@ -11,17 +11,19 @@
 // What bounds it: the loads into LDS.  Timing copies of an earlier form (128 x 256 tiles of 128 k, two workgroups a CU, 14,040 x 5,120
 // x 13,824): 553 us; without loads in the loop 379; with half of them 438; the same bytes in full 128-byte lines instead of
 // halves 460.  So: full lines, and the largest tile (256 x 256, 8 waves of 64 x 128, two a SIMD): a third fewer bytes an
-// operation, 478 us, 4.2 PFLOP/s; loads spread over two steps instead of one 454.  65,520 x 13,824 x 5,120 with GELU: 2.35 ms,
-// 3.95 PFLOP/s, 2.7 times the bf16 library product's rate at this size (6.46 ms); 1.6 of a tile's 43 us are the GELU (two
+// operation, 478 us, 4.2 PFLOP/s; loads spread over two steps instead of one 454.  65,520 x 13,824 x 5,120 with GELU: 2.37 ms,
+// 3.92 PFLOP/s, 2.7 times the bf16 library product's rate at this size (6.46 ms); 1.6 of a tile's 43 us are the GELU (two
 // transcendentals an output, nothing to overlap them with); an earlier form without loads in the loop 2.16 ms.  4 waves of 128 x 128,
-// a third fewer bytes out of LDS but one wave a SIMD, were slower: 14,040 x 5,120 x 13,824 538 us against 462.
+// a third fewer bytes out of LDS but one wave a SIMD, were slower: 14,040 x 5,120 x 13,824 538 us against 462.  (Times of pairs are of
+// the form at hand when it was measured.)  Long k does better, 13,056 x 5,120 x 13,824 4.75 PFLOP/s: of a tile's 43 us with 20
+// groups some 5 are the accumulators' start and the stores, when all waves are out of the loop at once.
 #include <type_traits>
 
 #include "mx_plan.h"
 #include "mx_tile.h"
 
 #define MXG_STAGE 2048                                 // bytes of output staging of a wave
-#define MXG_BAND 4                                     // token tiles that go together in the order; 2.56 ms against 2.69 with 8
+#define MXG_BAND 4                                     // token tiles that go together in the order; 8: 5 % more time at 65,520 x 13,824 x 5,120
 
 namespace {
 
@@ -163,8 +165,8 @@ __global__ void __launch_bounds__(64 * NN * NM, 2) icsa_mx_gemm_kernel(MxGemmPar
   unsigned char* const stage = smem + kBufs * kBuf + wave * MXG_STAGE;
 
   // The accumulators start with the bias: lane l holds the wave's output l's.  The next tile's is loaded before the products and
-  // taken where the wait for a group's loads stands: at the tile's end that wait would include the outputs' stores (2.31 ms against
-  // 2.26 of 65,520 x 13,824 x 5,120; 512 x 5,120 x 4,096 14.1 against 12.9 us)
+  // taken where the wait for a group's loads stands: at the tile's end that wait would include the outputs' stores (2 % more
+  // time at 65,520 x 13,824 x 5,120, 9 % at 512 x 5,120 x 4,096)
   static_assert(WN == 2, "a bias value a lane");
   const bool bias32 = p.bias_dtype == ICSA_DT_F32;
   auto wave_bias = [&](int n) {                                        // its bits as they are: a conversion would wait for them

@@ -6,11 +6,17 @@
 
 #define MXG_CUS 256
 
-// The kernel of few rows against the tile kernel (128 x 128 tiles, one workgroup for 128 outputs whatever the rows; us, codes in,
-// N x K): 5,120 x 5,120 at 1 / 32 / 64 rows 8.9 / 8.5 / 10.6 to 12.9 / 13.5 / 13.6; 5,120 x 13,824 11.1 / 15.7 / 22.8 to
-// 27.0 / 27.1 / 27.4; 13,824 x 5,120 10.0 / 12.9 / 22.8 to 13.1 / 13.5 / 14.5; 30,720 x 5,120 at 1 / 4 / 16 rows 19.7 / 20.7 /
-// 25.1 to 18.9 / 18.9 / 19.2, 20,480 x 5,120 15.7 / 16.4 / 19.0 to 13.5 / 13.5 / 13.7: many outputs fill the chip with tiles,
-// whose lines are read whole.
+// The kernel of few rows against the tile kernel (128 x 128 tiles, one workgroup for 128 outputs whatever the rows); us in a graph,
+// codes in, N x K at 1 / 32 / 64 rows:
+//   5,120 x 512      2.8 / 3.1 / 4.1    to  5.2 / 5.3 / 5.5      13,824 x 2,048    5.7 / 7.1 / 11.2   to  8.2 / 8.4 / 8.8
+//   5,120 x 2,048    4.3 / 5.1 / 6.5    to  7.9 / 8.1 / 8.5      16,384 x 2,048    5.7 / 7.2 / 11.2   to  8.4 / 8.5 / 9.0
+//   5,120 x 5,120    6.1 / 8.0 / 10.7   to 13.0 / 13.4 / 14.0    13,824 x 5,120   11.2 / 16.4 / 22.4  to 15.5 / 16.7 / 18.1
+//   8,192 x 5,120    6.5 / 8.0 / 10.7   to 13.3 / 13.6 / 14.2    16,384 x 5,120   11.7 / 16.5 / 22.9  to 17.3 / 17.8 / 19.3
+//   5,120 x 13,824  14.0 / 18.8 / 25.2  to 29.0 / 30.4 / 32.9    13,824 x 13,824  25.8 / 37.5 / 49.1  to 33.8 / 34.9 / 36.7
+//   8,192 x 13,824  13.9 / 21.4 / 25.9  to 29.8 / 30.9 / 33.6    20,480 x 5,120   14.5 / 22.7 / 32.0  to 17.6 / 19.3 / 20.4
+//   30,720 x 512     4.4 / 5.2 / 8.3    to  6.3 / 6.5 / 6.9      30,720 x 5,120   18.9 / 29.8 / 42.5  to 19.7 / 21.2 / 23.4
+// Many outputs fill the chip with tiles, whose lines are read whole.  (The rule leaves out k: single rows of many outputs and
+// short ones would still gain, 32 rows of 13,824 x 13,824 lose.)
 inline bool mx_rows_takes(int64_t M, int64_t N) { return (M <= 32 && N <= 16384) || (M <= 64 && N <= 8192); }
 
 // A launch takes rounds of one tile a CU.  Measured (us, one round): a 256 x 256 tile 1.6 a group and 1 to 4 besides, GELU 3.4; a

@@ -158,8 +158,10 @@ namespace {
 template <int MT, int kSrc, int kOut>
 hipError_t run_mx_rows(const MxGemmParams& p, hipStream_t stream) {
   const int blocks = (out_columns(p) + 31) / 32;
-  // waves: 16 a CU and more, not more than groups; 16 in a workgroup where each CU has one (32 x 13,824 x 5,120, 432 workgroups: 14.1 us
-  // with 8, 14.7 with 16; 2 x 5,120 x 13,824, 160 workgroups: 13.2 and 12.1, before token rows were read ahead)
+  // waves: 16 a CU and more, not more than groups; 16 in a workgroup where each CU has one at most.  8 against 16 (us, codes in, 1 /
+  // 16 / 32 rows): 13,824 x 5,120 10.7 / 13.2 / 16.2 to 12.0 / 13.7 / 16.1; 16,384 x 2,048 5.7 / 6.4 / 7.1 to 5.8 / 6.5 / 7.1.  Where
+  // 16 are taken: 5,120 x 5,120 6.0 / 7.0 / 7.9 to 6.2 / 7.1 / 8.0 and 5,120 x 13,824 11.8 / 15.1 / 18.8 to 13.1 / 15.3 / 18.8 with
+  // codes, two rows quantised in the call 7.2 to 6.8 and 15.1 to 15.4; 2,000 x 5,120 so 7.0 to 6.5.
   int nw = 4;
   while (nw < mx_rows_waves(MT) && blocks * nw < (nw < 8 ? 4096 : 2048) && nw < p.groups) nw *= 2;
   const int lds = nw * MT * 4096 + (kSrc != 0 ? p.M * (p.groups * (MXG_LINE + MX_GROUP_BLOCKS) + MXR_PAD) + 16 : 0);

@@ -373,7 +373,7 @@ class WanAttentionBlock(nn.Module):
     and ``forward(x, e, seq_lens, grid_sizes, freqs, context, context_lens,
     source_video_grid_sizes, TAG)``.  The residual stream is float32 as in the reference;
     every residual update + LayerNorm + adaLN modulation is one ``ln_modulate`` pass, the
-    projections and the FFN are library GEMMs, the attentions run in libicsa.so.
+    projections and the FFN are library GEMMs (or MXLinear, see quantize_linears), the attentions run in libicsa.so.
     Only the t2v cross attention is part of this build."""
 
     def __init__(self, cross_attn_type, dim, ffn_dim, num_heads, window_size=(-1, -1),
