@@ -574,7 +574,8 @@ class WanModel(nn.Module):
         text = torch.stack([torch.cat([u, u.new_zeros(self.text_len - u.size(0), u.size(1))]) for u in context])
         text0 = self.text_embedding[0]
         if isinstance(text0, MXLinear):
-            ctx = _gelu_pair(text0, self.text_embedding[2], text.to(xb.dtype))
+            kind = xb.dtype if text0.bias is None else text0.bias.dtype      # the layer's own, as its bias kept it
+            ctx = _gelu_pair(text0, self.text_embedding[2], text.to(kind))
         else:
             ctx = self.text_embedding(text.to(text0.weight.dtype))
         seq_lens = torch.tensor([r.shape[0] for r in rows], dtype=torch.long)

@@ -142,3 +142,20 @@ def test_cross_attention_carries_no_gradient(gpu, lens):
     ca(x, ctx, lens).float().sum().backward()
     assert ca.o.weight.grad is not None
     assert all(m.weight.grad is None for m in (ca.q, ca.k, ca.v, ca.norm_q, ca.norm_k))
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("text", [(0,), (2,), (0, 2)])
+def test_text_layers_of_another_type_than_the_model(gpu, text):
+    """A float32 text embedding in a bf16 model works in float32, its layers in 4 bits or not."""
+    m = wan.WanModel(in_dim=4, dim=256, ffn_dim=512, freq_dim=32, text_dim=64, out_dim=4, num_heads=2, num_layers=1, text_len=16)
+    m.init_weights()
+    m = m.to(gpu).to(BF)
+    m.text_embedding.float()
+    for i in text:
+        m.text_embedding[i] = MXLinear(m.text_embedding[i])
+    seen = []
+    m.text_embedding[2].register_forward_hook(lambda mod, x, y: seen.append(y.dtype))
+    lat, ctx = torch.randn(4, 2, 32, 32, device=gpu).to(BF), [torch.randn(12, 64, device=gpu).to(BF)]
+    out = m([lat], torch.tensor([637.0], device=gpu), ctx, 1024, [lat])[0]
+    assert torch.isfinite(out).all() and seen == [torch.float32]
