@@ -30,7 +30,11 @@ def attention(q, k, v, *, q_starts=None, k_starts=None, causal=False, prefix=Non
     bound, for f32 scores, P rounded to bf16 and f32 sums: a score is off by at most
     2^-23 (D scale sum |q k| + 8 (|s| + cap + |bias|) + 8) = e (its additions, the roundings of its
     products, tanh and the exponential, each a few steps), so a probability by a factor exp(+-2 e)
-    (its own and the total's) and by its rounding, 2^-8; the output by those times sum p |v|."""
+    (its own and the total's), which moves the output o by 2.5 e sum p |v| at most.  Rounded weights
+    p (1 + d), |d| <= 2^-8, stand in the product and in the total that divides it:
+    sum p (1 + d) v / sum p (1 + d) - o = sum p d (v - o) / (1 + sum p d), at most
+    2^-8 / (1 - 2^-8) sum p |v - o| <= 1.004 2^-8 (sum p |v| + |o|).  (Two keys, p = 0.9 at v = 0 and 0.1 at
+    v = 1, rounded in opposite directions: 0.18 2^-8, past 2^-8 sum p |v|.)"""
     q, k, v = q.double(), k.double(), v.double()
     B, Sq, H, D = q.shape
     Sk, Hk = k.shape[1:3]
@@ -69,7 +73,9 @@ def attention(q, k, v, *, q_starts=None, k_starts=None, causal=False, prefix=Non
                     o[rows] += torch.where(fine[j], 0.0, p[rows, j, None] * vv[j])
             out[b, :, h] = torch.where(none[:, None], 0.0, o)
             e = 2.0 ** -23 * (D * torch.where(see[b], mass, 0.0).amax(-1) + 8 * torch.where(see[b], size, 0.0).amax(-1) + 8)
-            bound[b, :, h] = (2.0 ** -8 + 2.5 * e)[:, None] * (p @ torch.where(fine, vv.abs(), 0.0)) + 1e-30
+            size = p @ torch.where(fine, vv.abs(), 0.0)
+            own = torch.where(none[:, None], 0.0, p @ torch.where(fine, vv, 0.0)).abs()
+            bound[b, :, h] = 1.004 * 2.0 ** -8 * (size + own) + 2.5 * e[:, None] * size + 1e-30
     return out, bound
 
 
@@ -96,4 +102,5 @@ def one_head(q, k, v, lo, hi, at, *, scale, softcap=0.0, bias=None):
     p = torch.exp(s - torch.where(none, 0.0, s.amax(-1))[:, None])
     p = p / torch.where(none, 1.0, p.sum(-1))[:, None]
     e = 2.0 ** -23 * (q.shape[1] * torch.where(see, mass, 0.0).amax(-1) + 8 * torch.where(see, size, 0.0).amax(-1) + 8)
-    return p @ v, (2.0 ** -8 + 2.5 * e)[:, None] * (p @ v.abs()) + 1e-30
+    out, size = p @ v, p @ v.abs()
+    return out, 1.004 * 2.0 ** -8 * (size + out.abs()) + 2.5 * e[:, None] * size + 1e-30

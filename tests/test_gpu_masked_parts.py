@@ -1,7 +1,7 @@
 """Attention under masks where whole items come first and the last round's items are cut in parts of
 their keys: every row of the first head (whole), of the head in which the parts begin and of the last
-one against float64, under the oracle's bound (a rounding of P, 2^-8 sum p |v|: a lost or wrongly
-weighted part is many times that, test_mx_masked_plan.py).  That each size is dealt out as it says is checked there too."""
+one against float64, under the oracle's bound (roundings of P, 2^-8 (sum p |v| + |o|): a lost or
+wrongly weighted part is past it in every row, test_mx_masked_plan.py).  That each size is dealt out as it says is checked there too."""
 import math
 
 import pytest

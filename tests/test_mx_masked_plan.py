@@ -53,3 +53,17 @@ def test_tolerance_sees_a_wrong_part(D, Sk, n, mistake):
         wrong[:, Sk * part // n:Sk * (part + 1) // n] *= 0.0 if mistake == "lost" else 0.5
         d = (wrong @ v.double() / wrong.sum(1, keepdim=True) - ref).abs()
         assert (d > tol).any(1).all()
+
+
+def test_bound_counts_the_rounding_of_the_total():
+    """Two weights, near 0.9 and 0.1, rounded to bf16 in opposite directions, in the product and in the total: the result is past
+    2^-8 sum p |v| and within the bound."""
+    d = 2.0 ** -8 * 0.99
+    p = torch.tensor([[0.9, 0.1]], dtype=torch.float64)
+    q, k, v = torch.ones(1, 64).double(), torch.log(p).t() / 8 * torch.ones(2, 64), torch.tensor([[0.0], [1.0]]).double().expand(2, 64)
+    one = torch.ones(1, dtype=torch.long)
+    ref, bound = O.one_head(q, k, v, 0 * one, 2 * one, one, scale=64 ** -0.5)
+    assert torch.allclose(ref, torch.full_like(ref, 0.1), atol=1e-12)
+    w = p * torch.tensor([[1 - d, 1 + d]])
+    off = (w @ v / w.sum() - ref).abs()
+    assert (off > 2.0 ** -8 * (p @ v.abs())).all() and (off <= bound).all()
