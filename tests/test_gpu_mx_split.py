@@ -10,9 +10,9 @@ from test_gpu_mx import _linear_case, _x
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
 
-# M, N, K, rows of the large tiles, kernel of the others
-SPLITS = [(9360, 2000, 1300, 8192, "tiles"), (3120, 5120, 4352, 3072, "rows"), (17003, 1001, 1300, 16384, "tiles"),
-          (3081, 5120, 4352, 3072, "rows")]
+# M, N, K, token tiles (of 256 rows) of the first kernel, kernel of the other rows
+SPLITS = [(9360, 2000, 1300, 32, "tiles"), (3120, 5120, 4352, 12, "rows"), (17003, 1001, 1300, 64, "tiles"),
+          (3081, 5120, 4352, 12, "rows")]
 
 
 @pytest.mark.parametrize("M,N,K,first,rest", SPLITS)
