@@ -427,6 +427,75 @@ int icsa_mx_linear(const void* x, const void* x_scales, int x_dtype, int64_t x_s
                    const void* bias, int bias_dtype, int activation, int64_t M, int N, int K, void* out, void* out_scales,
                    int out_dtype, int64_t o_ss, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- Training: cross attention, layer norm, RMS norm and rotary positions, forward and backward ----
+ * (No counterpart in the reference, whose own backward covers the sparse kernel alone; the forwards stand beside
+ * WanT2VCrossAttention, WanLayerNorm, WanRMSNorm and rope_apply: model.py:69-122, 180-188.) */
+
+/* Workspace bytes of icsa_cross_attn_fwd (0 for most sizes). */
+int64_t icsa_cross_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs);
+
+/* Attention of q [B, Sq, H, D] over k, v [B, Sk, Hk, D], all bf16, D 64 or 128: icsa_masked_attn with documents alone, and
+ * for the backward lse f32 [B, Hk, Sq, H / Hk] (NULL: not wanted): log2 of a row's sum of 2^(score log2 e), +inf for a row that
+ * sees nothing. */
+int icsa_cross_attn_fwd(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                        const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                        const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                        int B, int Sq, int Sk, int H, int Hk, int D,
+                        const int32_t* q_starts, const int32_t* k_starts, int docs, float scale,
+                        void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, float* lse,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of icsa_cross_attn_bwd (rows' sums; sums of parts where a side has few rows). */
+int64_t icsa_cross_attn_bwd_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D);
+
+/* Gradients of it from dout (bf16, like q), the forward's out and lse: dq like q, dk, dv like k, bf16 or f32 (grad_dtype); a
+ * NULL one is not computed.  dk and dv are summed over the heads that share them.  No atomics: the same inputs give the
+ * same bits.  Rows and keys outside every document, and those of documents without keys or queries, get zeros; what they hold reaches nothing.
+ * A NaN or an infinity in a document makes gradients of that document NaN, in others nothing. */
+int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t do_sh,
+                        const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                        const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                        const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                        const void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, const float* lse,
+                        int B, int Sq, int Sk, int H, int Hk, int D,
+                        const int32_t* q_starts, const int32_t* k_starts, int docs, float scale, int grad_dtype,
+                        void* dq, int64_t dq_sb, int64_t dq_ss, int64_t dq_sh,
+                        void* dk, int64_t dk_sb, int64_t dk_ss, int64_t dk_sh,
+                        void* dv, int64_t dv_sb, int64_t dv_ss, int64_t dv_sh,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+#define ICSA_NORM_MAX_DIM 8192
+#define ICSA_NORM_MAX_GROUPS 65535
+
+/* y = (x - mean) rstd a + b over rows of dim values, rstd = 1 / sqrt(mean((x - mean)^2) + eps); rms: mean = 0.  x, y
+ * [groups * rows, dim] bf16 or f32, row strides x_ss, y_ss, any alignment; a = gain (1 + gain with plus_one; NULL: 1) and
+ * b = shift (NULL: 0) [groups, dim] of p_dtype, group stride p_sg.  mean, rstd: f32 [groups * rows] for the backward (NULL: not
+ * wanted; rms has no mean).  dim <= ICSA_NORM_MAX_DIM. */
+int icsa_norm_fwd(const void* x, int x_dtype, int64_t x_ss, int64_t rows, int groups, int dim,
+                  const void* gain, const void* shift, int p_dtype, int64_t p_sg, int plus_one, int rms, float eps,
+                  void* y, int y_dtype, int64_t y_ss, float* mean, float* rstd, void* stream);
+
+/* Workspace bytes of icsa_norm_bwd where dgain or dshift is wanted. */
+int64_t icsa_norm_bwd_workspace_size(int64_t rows, int groups, int dim);
+
+/* Gradients of it: dx of x's type (row stride dx_ss), dgain, dshift contiguous [groups, dim] of p_dtype; each may be NULL.  Sums
+ * over rows in a fixed order. */
+int icsa_norm_bwd(const void* dy, int dy_dtype, int64_t dy_ss, const void* x, int x_dtype, int64_t x_ss, int64_t rows, int groups,
+                  int dim, const void* gain, int p_dtype, int64_t p_sg, int plus_one, int rms, const float* mean,
+                  const float* rstd, void* dx, int64_t dx_ss, void* dgain, void* dshift, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
+/* Rotary positions of one or two tensors (q and k) [B, S, H0 or H1, D] bf16 or f32, strides of any alignment, to contiguous y0, y1
+ * (H 0: absent): pair j of a head's first R dims, (x_2j, x_2j+1) interleaved or (x_j, x_{j + R/2}), becomes
+ * (x0 c - x1 s, x0 s + x1 c) with c, s = cos_table, sin_table [table_rows, R / 2] (f32) at the token's position; dims from R on
+ * are copied.  backward: the transposed matrix.  positions: device int32 [B, S, axes], batch stride pos_sb (0: shared);
+ * axes 1 to 4; sections: host int32 [axes], the pairs of each axis (NULL with one axis).  A position outside the table leaves its pairs as they
+ * are. */
+int icsa_rotary(const void* x0, int64_t x0_sb, int64_t x0_ss, int64_t x0_sh, int H0, void* y0,
+                const void* x1, int64_t x1_sb, int64_t x1_ss, int64_t x1_sh, int H1, void* y1, int dtype,
+                int B, int S, int D, int R, int interleaved, int backward, const int32_t* positions, int64_t pos_sb, int axes,
+                const int32_t* sections, const float* cos_table, const float* sin_table, int table_rows, void* stream);
+
 /* Last error message of the calling thread ("" if none). */
 const char* icsa_last_error(void);
 

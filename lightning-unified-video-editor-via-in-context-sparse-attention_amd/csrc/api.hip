@@ -581,14 +581,14 @@ int64_t icsa_masked_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, in
   return align256(masked_attn_part_floats(B, Sq, H, Hk, D, masked_attn_plan(B, Sq, Sk, H, Hk, D, docs <= 1 && !causal)) * 4);
 }
 
-int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+static int masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                      const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
                      const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
                      int B, int Sq, int Sk, int H, int Hk, int D,
                      const int32_t* q_starts, const int32_t* k_starts, int docs, int causal, const int32_t* prefix,
                      float scale, float softcap, const float* bias, int radius,
                      void* out, int out_dtype, int64_t o_sb, int64_t o_ss, int64_t o_sh,
-                     void* workspace, int64_t workspace_bytes, void* stream_) {
+                     float* lse, void* workspace, int64_t workspace_bytes, void* stream_) {
   int rc = check_masked_sizes(B, Sq, Sk, H, Hk, D);
   if (rc || (rc = check_dtype(out_dtype, "out"))) return rc;
   if (!q_starts != !k_starts) return fail(ICSA_EINVAL, "q_starts and k_starts must be both given or both NULL");
@@ -620,6 +620,7 @@ int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
   p.q_starts = q_starts; p.k_starts = k_starts; p.docs = docs; p.causal = causal != 0; p.prefix = prefix;
   p.scale = scale; p.softcap = softcap; p.bias = bias; p.radius = radius;
   p.out = OutView{out, o_sb, o_ss, o_sh, out_dtype};
+  p.lse = lse;
   const MaskedPlan plan = masked_attn_plan(B, Sq, Sk, H, Hk, D, docs <= 1 && !causal);
   p.n_whole = plan.n_whole; p.n_split = plan.n_split;
   const int64_t need = icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D, docs, causal);
@@ -627,6 +628,232 @@ int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
     return fail(ICSA_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   p.part = reinterpret_cast<float*>(workspace);
   ICSA_HIP_TRY(launch_masked_attn(p, reinterpret_cast<hipStream_t>(stream_)), "masked attention");
+  return ICSA_OK;
+}
+
+int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                     const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                     const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                     int B, int Sq, int Sk, int H, int Hk, int D,
+                     const int32_t* q_starts, const int32_t* k_starts, int docs, int causal, const int32_t* prefix,
+                     float scale, float softcap, const float* bias, int radius,
+                     void* out, int out_dtype, int64_t o_sb, int64_t o_ss, int64_t o_sh,
+                     void* workspace, int64_t workspace_bytes, void* stream_) {
+  return masked_attn(q, q_sb, q_ss, q_sh, k, k_sb, k_ss, k_sh, v, v_sb, v_ss, v_sh, B, Sq, Sk, H, Hk, D, q_starts, k_starts, docs,
+                     causal, prefix, scale, softcap, bias, radius, out, out_dtype, o_sb, o_ss, o_sh, nullptr, workspace,
+                     workspace_bytes, stream_);
+}
+
+// ---- cross attention with its backward ----
+int64_t icsa_cross_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs) {
+  return icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D, docs, 0);
+}
+
+int icsa_cross_attn_fwd(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                        const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                        const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                        int B, int Sq, int Sk, int H, int Hk, int D,
+                        const int32_t* q_starts, const int32_t* k_starts, int docs, float scale,
+                        void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, float* lse,
+                        void* workspace, int64_t workspace_bytes, void* stream_) {
+  return masked_attn(q, q_sb, q_ss, q_sh, k, k_sb, k_ss, k_sh, v, v_sb, v_ss, v_sh, B, Sq, Sk, H, Hk, D, q_starts, k_starts, docs,
+                     0, nullptr, scale, 0.f, nullptr, 0, out, ICSA_BF16, o_sb, o_ss, o_sh, lse, workspace, workspace_bytes,
+                     stream_);
+}
+
+namespace {
+struct AttnBwdLayout { int64_t dvec, dq, dk, dv, total; };
+AttnBwdLayout attn_bwd_layout(int B, int Sq, int Sk, int H, int Hk, int D, AttnBwdPlan f) {
+  const int64_t q_rows = (int64_t)B * Sq * H, k_rows = (int64_t)B * Sk * Hk;
+  AttnBwdLayout L;
+  L.dvec = 0;
+  L.dq = align256(q_rows * 4);
+  L.dk = L.dq + (f.q_split > 1 ? align256(f.q_split * q_rows * D * 4) : 0);
+  const int64_t k_part = f.k_split > 1 ? align256(f.k_split * k_rows * D * 4) : 0;
+  L.dv = L.dk + k_part;
+  L.total = L.dv + k_part;
+  return L;
+}
+}  // namespace
+
+int64_t icsa_cross_attn_bwd_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D) {
+  if (check_masked_sizes(B, Sq, Sk, H, Hk, D)) return -1;
+  return attn_bwd_layout(B, Sq, Sk, H, Hk, D, attn_bwd_plan(B, Sq, Sk, H, Hk, D)).total;
+}
+
+int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t do_sh,
+                        const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
+                        const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
+                        const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                        const void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, const float* lse,
+                        int B, int Sq, int Sk, int H, int Hk, int D,
+                        const int32_t* q_starts, const int32_t* k_starts, int docs, float scale, int grad_dtype,
+                        void* dq, int64_t dq_sb, int64_t dq_ss, int64_t dq_sh,
+                        void* dk, int64_t dk_sb, int64_t dk_ss, int64_t dk_sh,
+                        void* dv, int64_t dv_sb, int64_t dv_ss, int64_t dv_sh,
+                        void* workspace, int64_t workspace_bytes, void* stream_) {
+  int rc = check_masked_sizes(B, Sq, Sk, H, Hk, D);
+  if (rc || (rc = check_dtype(grad_dtype, "gradients"))) return rc;
+  if (!q_starts != !k_starts) return fail(ICSA_EINVAL, "q_starts and k_starts must be both given or both NULL");
+  if (docs < 1 || (!q_starts && docs != 1)) return fail(ICSA_EINVAL, "docs=%d without document starts", docs);
+  if (!std::isfinite(scale) || scale <= 0.f || !std::isfinite(2.f * scale))
+    return fail(ICSA_EINVAL, "scale must be positive and finite");
+  if (Sq > 0 && (!dout || !q || !out || !lse)) return fail(ICSA_EINVAL, "null pointer argument");
+  if (Sk > 0 && (!k || !v)) return fail(ICSA_EINVAL, "null pointer argument");
+  auto ok = [](const void* p, int n, int dtype, int64_t s0, int64_t s1, int64_t s2) {
+    return n == 0 || p == nullptr || row_ok(p, dtype, s0, s1, s2);
+  };
+  if (!ok(dout, Sq, ICSA_BF16, do_sb, do_ss, do_sh) || !ok(q, Sq, ICSA_BF16, q_sb, q_ss, q_sh) ||
+      !ok(out, Sq, ICSA_BF16, o_sb, o_ss, o_sh) || !ok(k, Sk, ICSA_BF16, k_sb, k_ss, k_sh) ||
+      !ok(v, Sk, ICSA_BF16, v_sb, v_ss, v_sh) || !ok(dq, Sq, grad_dtype, dq_sb, dq_ss, dq_sh) ||
+      !ok(dk, Sk, grad_dtype, dk_sb, dk_ss, dk_sh) || !ok(dv, Sk, grad_dtype, dv_sb, dv_ss, dv_sh))
+    return fail(ICSA_EINVAL, "rows must be 16-byte aligned (pointers and strides)");
+  if (Sq <= 1) q_ss = do_ss = o_ss = 0;                // strides over one element do not count
+  if (Sk <= 1) k_ss = v_ss = 0;
+  if (H == 1) q_sh = do_sh = 0;
+  if (k_ss < 0 || v_ss < 0 || q_ss < 0 || do_ss < 0 || q_sh < 0 || do_sh < 0)
+    return fail(ICSA_EINVAL, "negative strides");
+  const int64_t most = 0x3fffffffLL, G = H / Hk;       // elements
+  auto far = [&](int64_t ss, int64_t sh) { return ss > most / 65 || (G > 1 && sh > (most - 65 * ss) / G); };
+  if (k_ss > most / 65 || v_ss > most / 65 || far(q_ss, q_sh) || far(do_ss, do_sh))
+    return fail(ICSA_EUNSUPPORTED, "64 rows of q, dout, k and v must lie within 2 GiB");
+  const AttnBwdPlan plan = attn_bwd_plan(B, Sq, Sk, H, Hk, D);
+  const AttnBwdLayout L = attn_bwd_layout(B, Sq, Sk, H, Hk, D, plan);
+  if (L.total > 0 && (!workspace || workspace_bytes < L.total || !aligned16(workspace)))
+    return fail(ICSA_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)L.total);
+  char* ws = reinterpret_cast<char*>(workspace);
+  AttnBwdParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = reinterpret_cast<const bf16*>(q); p.q_sb = q_sb; p.q_ss = q_ss; p.q_sh = q_sh;
+  p.k = reinterpret_cast<const bf16*>(k); p.k_sb = k_sb; p.k_ss = k_ss; p.k_sh = k_sh;
+  p.v = reinterpret_cast<const bf16*>(v); p.v_sb = v_sb; p.v_ss = v_ss; p.v_sh = v_sh;
+  p.o = reinterpret_cast<const bf16*>(out); p.o_sb = o_sb; p.o_ss = o_ss; p.o_sh = o_sh;
+  p.dout = reinterpret_cast<const bf16*>(dout); p.do_sb = do_sb; p.do_ss = do_ss; p.do_sh = do_sh;
+  p.lse = lse;
+  p.B = B; p.Sq = Sq; p.Sk = Sk; p.H = H; p.Hk = Hk; p.D = D;
+  p.q_starts = q_starts; p.k_starts = k_starts; p.docs = docs; p.scale = scale;
+  p.dvec = reinterpret_cast<float*>(ws + L.dvec);
+  p.dq_part = reinterpret_cast<float*>(ws + L.dq);
+  p.dk_part = reinterpret_cast<float*>(ws + L.dk);
+  p.dv_part = reinterpret_cast<float*>(ws + L.dv);
+  p.q_split = plan.q_split; p.k_split = plan.k_split;
+  p.dq = OutView{Sq > 0 ? dq : nullptr, dq_sb, dq_ss, dq_sh, grad_dtype};
+  p.dk = OutView{Sk > 0 ? dk : nullptr, dk_sb, dk_ss, dk_sh, grad_dtype};
+  p.dv = OutView{Sk > 0 ? dv : nullptr, dv_sb, dv_ss, dv_sh, grad_dtype};
+  ICSA_HIP_TRY(launch_attn_bwd(p, reinterpret_cast<hipStream_t>(stream_)), "cross attention backward");
+  return ICSA_OK;
+}
+
+// ---- layer norm and RMS norm ----
+namespace {
+// rows of `es`-byte elements in whole 16-byte chunks of 8 elements
+bool whole_chunks(const void* p, int64_t ss, int64_t rows, int dim, int es) {
+  return dim % 8 == 0 && aligned16(p) && (rows <= 1 || (ss * es) % 16 == 0);
+}
+
+int check_norm(int x_dtype, int y_dtype, int64_t rows, int groups, int dim, const void* gain, const void* shift, int p_dtype) {
+  int rc = check_dtype(x_dtype, "x");
+  if (rc || (rc = check_dtype(y_dtype, "y"))) return rc;
+  if ((gain || shift) && (rc = check_dtype(p_dtype, "parameters"))) return rc;
+  if (rows < 0 || groups <= 0 || dim <= 0) return fail(ICSA_EINVAL, "bad sizes rows=%lld groups=%d dim=%d", (long long)rows, groups, dim);
+  if (dim > ICSA_NORM_MAX_DIM || groups > ICSA_NORM_MAX_GROUPS || rows > (1LL << 40) / groups)
+    return fail(ICSA_EUNSUPPORTED, "dim=%d groups=%d rows=%lld exceed the limits", dim, groups, (long long)rows);
+  return ICSA_OK;
+}
+}  // namespace
+
+int icsa_norm_fwd(const void* x, int x_dtype, int64_t x_ss, int64_t rows, int groups, int dim,
+                  const void* gain, const void* shift, int p_dtype, int64_t p_sg, int plus_one, int rms, float eps,
+                  void* y, int y_dtype, int64_t y_ss, float* mean, float* rstd, void* stream_) {
+  int rc = check_norm(x_dtype, y_dtype, rows, groups, dim, gain, shift, p_dtype);
+  if (rc) return rc;
+  if (!(eps >= 0.f)) return fail(ICSA_EINVAL, "eps must not be negative");
+  if (rows == 0) return ICSA_OK;
+  if (!x || !y) return fail(ICSA_EINVAL, "null pointer argument");
+  if (rstd && !rms && !mean) return fail(ICSA_EINVAL, "rstd without mean");
+  NormParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.x = x; p.x_dtype = x_dtype; p.x_ss = x_ss; p.rows = rows; p.groups = groups; p.dim = dim; p.dim4 = (dim + 3) & ~3;
+  p.gain = gain; p.shift = shift; p.p_dtype = p_dtype; p.p_sg = p_sg; p.plus_one = plus_one != 0; p.rms = rms != 0; p.eps = eps;
+  p.y = y; p.y_dtype = y_dtype; p.y_ss = y_ss; p.mean = mean; p.rstd = rstd;
+  p.vec_x = whole_chunks(x, x_ss, rows * groups, dim, elsize(x_dtype));
+  p.vec_y = whole_chunks(y, y_ss, rows * groups, dim, elsize(y_dtype));
+  ICSA_HIP_TRY(launch_norm_fwd(p, reinterpret_cast<hipStream_t>(stream_)), "norm");
+  return ICSA_OK;
+}
+
+int64_t icsa_norm_bwd_workspace_size(int64_t rows, int groups, int dim) {
+  if (check_norm(ICSA_F32, ICSA_F32, rows, groups, dim, nullptr, nullptr, ICSA_F32)) return -1;
+  if (rows == 0) return 0;
+  return align256((int64_t)groups * norm_bwd_workgroups(rows, dim, groups) * 2 * ((dim + 3) & ~3) * 4);
+}
+
+int icsa_norm_bwd(const void* dy, int dy_dtype, int64_t dy_ss, const void* x, int x_dtype, int64_t x_ss, int64_t rows, int groups,
+                  int dim, const void* gain, int p_dtype, int64_t p_sg, int plus_one, int rms, const float* mean,
+                  const float* rstd, void* dx, int64_t dx_ss, void* dgain, void* dshift, void* workspace,
+                  int64_t workspace_bytes, void* stream_) {
+  const bool sums = dgain || dshift;
+  int rc = check_norm(x_dtype, dy_dtype, rows, groups, dim, sums ? dgain ? dgain : dshift : gain, gain, p_dtype);
+  if (rc) return rc;
+  if (rows == 0) {
+    if (sums) return fail(ICSA_EINVAL, "no rows: the parameters' gradients are the caller's zeros");
+    return ICSA_OK;
+  }
+  if (!dy || !x || !rstd || (!rms && !mean)) return fail(ICSA_EINVAL, "null pointer argument");
+  if (!dx && !sums) return ICSA_OK;
+  const int64_t need = sums ? icsa_norm_bwd_workspace_size(rows, groups, dim) : 0;
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(ICSA_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  NormParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.x = x; p.x_dtype = x_dtype; p.x_ss = x_ss; p.rows = rows; p.groups = groups; p.dim = dim; p.dim4 = (dim + 3) & ~3;
+  p.gain = gain; p.p_dtype = p_dtype; p.p_sg = p_sg; p.plus_one = plus_one != 0; p.rms = rms != 0;
+  p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
+  p.dy = dy; p.y_dtype = dy_dtype; p.dy_ss = dy_ss; p.dx = dx; p.dx_ss = dx_ss; p.dgain = dgain; p.dshift = dshift;
+  p.part = sums ? reinterpret_cast<float*>(workspace) : nullptr;
+  p.vec_x = whole_chunks(x, x_ss, rows * groups, dim, elsize(x_dtype));
+  p.vec_y = whole_chunks(dy, dy_ss, rows * groups, dim, elsize(dy_dtype));
+  p.vec_dx = whole_chunks(dx, dx_ss, rows * groups, dim, elsize(x_dtype));
+  ICSA_HIP_TRY(launch_norm_bwd(p, reinterpret_cast<hipStream_t>(stream_)), "norm backward");
+  return ICSA_OK;
+}
+
+// ---- rotary positions ----
+int icsa_rotary(const void* x0, int64_t x0_sb, int64_t x0_ss, int64_t x0_sh, int H0, void* y0,
+                const void* x1, int64_t x1_sb, int64_t x1_ss, int64_t x1_sh, int H1, void* y1, int dtype,
+                int B, int S, int D, int R, int interleaved, int backward, const int32_t* positions, int64_t pos_sb, int axes,
+                const int32_t* sections, const float* cos_table, const float* sin_table, int table_rows, void* stream_) {
+  int rc = check_dtype(dtype, "x");
+  if (rc) return rc;
+  if (B < 0 || S < 0 || D <= 0 || R <= 0 || R > D || R % 2 != 0 || H0 < 0 || H1 < 0)
+    return fail(ICSA_EINVAL, "bad sizes B=%d S=%d D=%d R=%d H=%d, %d", B, S, D, R, H0, H1);
+  if (axes < 1 || axes > RO_MAX_AXES || table_rows < 1) return fail(ICSA_EINVAL, "axes=%d, table of %d rows", axes, table_rows);
+  if (D > (1 << 20) || H0 > (1 << 20) || H1 > (1 << 20) || (int64_t)std::max(H0, H1) * D > (1 << 30))
+    return fail(ICSA_EUNSUPPORTED, "heads of %d x %d dims", std::max(H0, H1), D);
+  RotaryParams p;
+  std::memset(&p, 0, sizeof(p));
+  int at = 0;
+  for (int a = 0; a < axes; ++a) {
+    const int n = axes == 1 && !sections ? R / 2 : sections ? sections[a] : -1;
+    if (n < 0 || n > R / 2) return fail(ICSA_EINVAL, "sections must be the pairs of each axis");
+    p.ends[a] = at += n;
+  }
+  if (at != R / 2) return fail(ICSA_EINVAL, "sections have %d pairs of %d", at, R / 2);
+  if (B == 0 || S == 0 || (H0 == 0 && H1 == 0)) return ICSA_OK;
+  if (!positions || !cos_table || !sin_table || (H0 && (!x0 || !y0)) || (H1 && (!x1 || !y1)))
+    return fail(ICSA_EINVAL, "null pointer argument");
+  p.x[0] = x0; p.sb[0] = x0_sb; p.ss[0] = x0_ss; p.sh[0] = x0_sh; p.H[0] = H0; p.y[0] = y0;
+  p.x[1] = x1; p.sb[1] = x1_sb; p.ss[1] = x1_ss; p.sh[1] = x1_sh; p.H[1] = H1; p.y[1] = y1;
+  p.tokens = (int64_t)B * S; p.S = S; p.D = D; p.R = R;
+  p.halves = !interleaved; p.back = backward != 0; p.dtype = dtype;
+  p.pos = positions; p.pos_sb = pos_sb; p.axes = axes;
+  p.cos = cos_table; p.sin = sin_table; p.rows = table_rows;
+  auto whole = [&](int i) {                            // rows of whole, aligned 8-element chunks
+    return p.H[i] == 0 || (row_ok(p.x[i], dtype, B > 1 ? p.sb[i] : 0, S > 1 ? p.ss[i] : 0, p.H[i] > 1 ? p.sh[i] : 0) && aligned16(p.y[i]));
+  };
+  const bool vec = D % 8 == 0 && D <= 512 && R % (interleaved ? 8 : 16) == 0 && whole(0) && whole(1) && aligned16(cos_table) &&
+                   aligned16(sin_table);
+  ICSA_HIP_TRY(launch_rotary(p, vec, reinterpret_cast<hipStream_t>(stream_)), "rotary");
   return ICSA_OK;
 }
 

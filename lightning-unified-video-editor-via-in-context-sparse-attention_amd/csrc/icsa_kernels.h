@@ -287,6 +287,7 @@ struct MaskedAttnParams {
   float scale, softcap;                           // softcap 0: none
   const float* bias; int radius;                  // [H, 2 radius + 1] or null
   OutView out;
+  float* lse;                                     // [B, Hk, Sq H / Hk] or null: log2 of every row's sum of 2^score
   int n_whole, n_split; float* part;              // MaskedPlan; the parts' sums
   FastDiv by_g, by_blk, by_hk, by_bh, by_split;   // heads of a group, row blocks, key heads, B Hk, parts (set by the launch)
 };
@@ -296,3 +297,63 @@ MaskedPlan masked_attn_plan(int B, int Sq, int Sk, int H, int Hk, int D, bool al
 int64_t masked_attn_part_floats(int B, int Sq, int H, int Hk, int D, MaskedPlan f);
 bool masked_attn_bias_fits(int H, int Hk, int D, int radius);
 hipError_t launch_masked_attn(MaskedAttnParams p, hipStream_t stream);
+
+// ------------------------------------------------------- backward of attention over documents (attn_bwd.hip)
+struct AttnBwdParams {
+  const bf16* q; int64_t q_sb, q_ss, q_sh;        // [B, Sq, H, D]
+  const bf16* k; int64_t k_sb, k_ss, k_sh;        // [B, Sk, Hk, D]
+  const bf16* v; int64_t v_sb, v_ss, v_sh;
+  const bf16* o; int64_t o_sb, o_ss, o_sh;        // the forward's result
+  const bf16* dout; int64_t do_sb, do_ss, do_sh;
+  const float* lse;                               // [B, Hk, Sq H / Hk], the forward's
+  int B, Sq, Sk, H, Hk, D;
+  const int* q_starts; const int* k_starts; int docs;   // [B, docs + 1] or null (docs = 1)
+  float scale;
+  float* dvec;                                    // [B, Hk, Sq H / Hk]: rowsum(dout o), written by the query-major kernel
+  OutView dq, dk, dv;                             // p null: not wanted
+  int q_split, k_split;                           // AttnBwdPlan
+  float* dq_part; float* dk_part; float* dv_part; // the parts' sums, [part][B Hk][row][D]
+  FastDiv by_g, by_hk, by_qblk, by_kblk;          // set by the launch
+};
+// parts that a query block's keys and a key block's rows are cut into
+struct AttnBwdPlan { int q_split, k_split; };
+AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, int D);
+hipError_t launch_attn_bwd(AttnBwdParams p, hipStream_t stream);
+
+// ---------------------------------------------------------------- layer norm, RMS norm (norm.hip)
+struct NormParams {
+  const void* x; int x_dtype; int64_t x_ss;       // [groups * rows, dim], row stride
+  int64_t rows; int groups, dim, dim4;            // rows of a group; dim4: dim rounded up to 4
+  const void* gain; const void* shift;            // [groups, dim] or null (1 and 0), group stride p_sg
+  int p_dtype; int64_t p_sg;
+  int plus_one, rms;                              // the factor is 1 + gain; no mean
+  float eps;
+  int y_dtype;                                    // of y and dy
+  void* y; int64_t y_ss;
+  float* mean; float* rstd;                       // [groups * rows]; the forward's may be null
+  // backward
+  const void* dy; int64_t dy_ss;
+  void* dx; int64_t dx_ss;                        // x's type, or null
+  void* dgain; void* dshift;                      // [groups, dim] of p_dtype, or null
+  float* part;                                    // [groups, n_wg, 2, dim4], or null
+  int n_wg;                                       // workgroups a group (set by the launch)
+  int vec_x, vec_y, vec_dx;                       // rows of whole, aligned 8-element chunks
+};
+int norm_bwd_workgroups(int64_t rows, int dim, int groups);
+hipError_t launch_norm_fwd(NormParams p, hipStream_t stream);
+hipError_t launch_norm_bwd(NormParams p, hipStream_t stream);
+
+// ---------------------------------------------------------------- rotary positions (rotary.hip)
+#define RO_MAX_AXES 4
+struct RotaryParams {
+  const void* x[2]; void* y[2];                   // [B, S, H[i], D]; y contiguous
+  int64_t sb[2], ss[2], sh[2];
+  int H[2];                                       // 0: absent
+  int64_t tokens; int S, D, R;                    // tokens = B S
+  int halves, back, dtype;
+  const int* pos; int64_t pos_sb;                 // [B, S, axes], batch stride (0: shared)
+  int axes, ends[RO_MAX_AXES];                    // axis a: pairs up to ends[a]
+  const float* cos; const float* sin; int rows;   // [rows, R / 2]
+  int shares;                                     // set by the launch
+};
+hipError_t launch_rotary(RotaryParams p, bool vec, hipStream_t stream);

@@ -28,6 +28,15 @@ from .hip_host import (  # noqa: F401
     sparse_piecewise_attn_tilelang_hosttopk_hip,
 )
 from .mx import MXFP4Tensor, MXLinear, mx_linear, mx_quantize  # noqa: F401
+from .train import (  # noqa: F401
+    cross_attn_bwd_hip,
+    cross_attn_func,
+    cross_attn_fwd_hip,
+    layer_norm_func,
+    rms_norm_func,
+    rotary_func,
+    rotary_table,
+)
 
 __all__ = [
     'Backend',
@@ -45,6 +54,13 @@ __all__ = [
     'MXLinear',
     'mx_quantize',
     'mx_linear',
+    'cross_attn_func',
+    'cross_attn_fwd_hip',
+    'cross_attn_bwd_hip',
+    'layer_norm_func',
+    'rms_norm_func',
+    'rotary_func',
+    'rotary_table',
     'derived_sizes',
     'IcsaArgumentError',
 ]

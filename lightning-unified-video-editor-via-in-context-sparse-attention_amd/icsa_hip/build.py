@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libicsa.so")
 
 SOURCES = ["pool.hip", "compressed.hip", "newkv.hip", "gather.hip", "flash_attn.hip", "sparse_attn.hip", "sparse_bwd.hip",
            "wan_qk.hip", "wan_block.hip", "mx_quant.hip", "mx_gemm.hip", "mx_rows.hip", "masked_attn.hip",
-           "api.hip"]
+           "attn_bwd.hip", "norm.hip", "rotary.hip", "api.hip"]
 
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
