@@ -446,7 +446,7 @@ int icsa_cross_attn_fwd(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Workspace bytes of icsa_cross_attn_bwd (rows' sums; sums of parts where a side has few rows). */
-int64_t icsa_cross_attn_bwd_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D);
+int64_t icsa_cross_attn_bwd_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs);
 
 /* Gradients of it from dout (bf16, like q), the forward's out and lse: dq like q, dk, dv like k, bf16 or f32 (grad_dtype); a
  * NULL one is not computed.  dk and dv are summed over the heads that share them.  No atomics: the same inputs give the

@@ -662,12 +662,12 @@ int icsa_cross_attn_fwd(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
 }
 
 namespace {
-struct AttnBwdLayout { int64_t dvec, dq, dk, dv, total; };
+struct AttnBwdLayout { int64_t rowv, dq, dk, dv, total; };
 AttnBwdLayout attn_bwd_layout(int B, int Sq, int Sk, int H, int Hk, int D, AttnBwdPlan f) {
   const int64_t q_rows = (int64_t)B * Sq * H, k_rows = (int64_t)B * Sk * Hk;
   AttnBwdLayout L;
-  L.dvec = 0;
-  L.dq = align256(q_rows * 4);
+  L.rowv = 0;
+  L.dq = align256(2 * q_rows * 4);
   L.dk = L.dq + (f.q_split > 1 ? align256(f.q_split * q_rows * D * 4) : 0);
   const int64_t k_part = f.k_split > 1 ? align256(f.k_split * k_rows * D * 4) : 0;
   L.dv = L.dk + k_part;
@@ -676,9 +676,9 @@ AttnBwdLayout attn_bwd_layout(int B, int Sq, int Sk, int H, int Hk, int D, AttnB
 }
 }  // namespace
 
-int64_t icsa_cross_attn_bwd_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D) {
+int64_t icsa_cross_attn_bwd_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs) {
   if (check_masked_sizes(B, Sq, Sk, H, Hk, D)) return -1;
-  return attn_bwd_layout(B, Sq, Sk, H, Hk, D, attn_bwd_plan(B, Sq, Sk, H, Hk, D)).total;
+  return attn_bwd_layout(B, Sq, Sk, H, Hk, D, attn_bwd_plan(B, Sq, Sk, H, Hk, docs <= 1)).total;
 }
 
 int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t do_sh,
@@ -717,7 +717,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
   auto far = [&](int64_t ss, int64_t sh) { return ss > most / 65 || (G > 1 && sh > (most - 65 * ss) / G); };
   if (k_ss > most / 65 || v_ss > most / 65 || far(q_ss, q_sh) || far(do_ss, do_sh))
     return fail(ICSA_EUNSUPPORTED, "64 rows of q, dout, k and v must lie within 2 GiB");
-  const AttnBwdPlan plan = attn_bwd_plan(B, Sq, Sk, H, Hk, D);
+  const AttnBwdPlan plan = attn_bwd_plan(B, Sq, Sk, H, Hk, docs <= 1);
   const AttnBwdLayout L = attn_bwd_layout(B, Sq, Sk, H, Hk, D, plan);
   if (L.total > 0 && (!workspace || workspace_bytes < L.total || !aligned16(workspace)))
     return fail(ICSA_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)L.total);
@@ -732,7 +732,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
   p.lse = lse;
   p.B = B; p.Sq = Sq; p.Sk = Sk; p.H = H; p.Hk = Hk; p.D = D;
   p.q_starts = q_starts; p.k_starts = k_starts; p.docs = docs; p.scale = scale;
-  p.dvec = reinterpret_cast<float*>(ws + L.dvec);
+  p.rowv = reinterpret_cast<float*>(ws + L.rowv);
   p.dq_part = reinterpret_cast<float*>(ws + L.dq);
   p.dk_part = reinterpret_cast<float*>(ws + L.dk);
   p.dv_part = reinterpret_cast<float*>(ws + L.dv);

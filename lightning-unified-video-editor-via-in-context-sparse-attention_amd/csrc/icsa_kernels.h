@@ -309,7 +309,7 @@ struct AttnBwdParams {
   int B, Sq, Sk, H, Hk, D;
   const int* q_starts; const int* k_starts; int docs;   // [B, docs + 1] or null (docs = 1)
   float scale;
-  float* dvec;                                    // [B, Hk, Sq H / Hk]: rowsum(dout o), written by the query-major kernel
+  float* rowv;                                    // [2][B, Hk, Sq H / Hk]: -lse / (scale log2 e), -rowsum(dout o), by the query-major kernel
   OutView dq, dk, dv;                             // p null: not wanted
   int q_split, k_split;                           // AttnBwdPlan
   float* dq_part; float* dk_part; float* dv_part; // the parts' sums, [part][B Hk][row][D]
@@ -317,7 +317,7 @@ struct AttnBwdParams {
 };
 // parts that a query block's keys and a key block's rows are cut into
 struct AttnBwdPlan { int q_split, k_split; };
-AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, int D);
+AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, bool alike);   // alike: one document
 hipError_t launch_attn_bwd(AttnBwdParams p, hipStream_t stream);
 
 // ---------------------------------------------------------------- layer norm, RMS norm (norm.hip)

@@ -117,7 +117,7 @@ def cross_attn_bwd_hip(dout, q, k, v, out, lse, q_starts=None, k_starts=None, so
     v, va = _rows16(v)
     out, oa = _rows16(out)
     L = _lib.lib()
-    ws_bytes = L.icsa_cross_attn_bwd_workspace_size(*sizes)
+    ws_bytes = L.icsa_cross_attn_bwd_workspace_size(*sizes, docs)
     if ws_bytes < 0:
         raise _lib.IcsaError("icsa_cross_attn_bwd_workspace_size", int(ws_bytes))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)

@@ -56,8 +56,8 @@ def test_cross_attention_workspaces():
     L = _lib.lib()
     for sizes in ((1, 1, 1, 1, 1, 64), (1, 65520, 512, 40, 40, 128), (2, 9373, 1009, 24, 8, 64), (1, 1, 65536, 40, 8, 128)):
         B, Sq, Sk, H, Hk, D = sizes
-        assert L.icsa_cross_attn_bwd_workspace_size(*sizes) >= 4 * B * Sq * H
-    assert L.icsa_cross_attn_bwd_workspace_size(1, 4, 4, 3, 2, 64) == -1
+        assert L.icsa_cross_attn_bwd_workspace_size(*sizes, 1) >= 4 * B * Sq * H
+    assert L.icsa_cross_attn_bwd_workspace_size(1, 4, 4, 3, 2, 64, 1) == -1
     assert L.icsa_cross_attn_workspace_size(1, 4, 4, 2, 2, 96, 1) == -1
     assert L.icsa_cross_attn_workspace_size(1, 9373, 512, 12, 12, 128, 1) == 0
 
