@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(256) icsa_attn_bwd_join_kernel(AttnBwdParams p
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] += v[e];
   }
-  const int bh = (int)(row / n_st), r = (int)(row - (int64_t)bh * n_st);
+  const int bh = (int)((unsigned)row / (unsigned)n_st), r = (int)row - bh * n_st;         // rows: under 2^28, check_masked_sizes
   const int64_t off = row_at(out.sb, out.ss, out.sh, p.by_hk.div(bh), p.by_hk.mod(bh), KV ? FastDiv{1u, 0u, 1u, 0u} : p.by_g, r) + d;
   if (out.dtype == ICSA_DT_BF16) {
     bf16x4 y;

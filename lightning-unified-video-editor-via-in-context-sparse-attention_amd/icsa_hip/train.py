@@ -20,7 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .hip_host import IcsaArgumentError, _require, _rows16, dtype_code, on_device, ptr, stream_ptr
+from .hip_host import IcsaArgumentError, _require, _rows16, on_device, ptr, stream_ptr
 
 _BF = torch.bfloat16
 _FLOATS = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
@@ -66,6 +66,7 @@ def _check_attn(q, k, v, q_starts, k_starts, softmax_scale):
 
 
 def _attn_fwd(q, k, v, q_starts, k_starts, softmax_scale, want_lse):
+    """(out, lse, and for the backward: q, k, v as the library reads them and the borders; sizes, documents and scale)."""
     sizes, docs, scale, q_starts, k_starts = _check_attn(q, k, v, q_starts, k_starts, softmax_scale)
     B, Sq, _, H, Hk, D = sizes
     dev = q.device
@@ -82,17 +83,44 @@ def _attn_fwd(q, k, v, q_starts, k_starts, softmax_scale, want_lse):
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         wsp = ws.data_ptr()
     with on_device(dev):
-        rc = L.icsa_cross_attn_fwd(*qa, *ka, *va, *sizes, ptr(q_starts), ptr(k_starts), docs, scale,
-                                   out.data_ptr(), Sq * H * D, H * D, D, ptr(lse), wsp, ws_bytes, stream_ptr(dev))
+        rc = L.icsa_cross_attn_fwd(*qa, *ka, *va, *sizes, ptr(q_starts), ptr(k_starts), docs, scale, out.data_ptr(), Sq * H * D, H * D, D,
+                                   ptr(lse), wsp, ws_bytes, stream_ptr(dev))
     _lib.check("icsa_cross_attn_fwd", rc)
-    return out, lse
+    return out, lse, (q, k, v, q_starts, k_starts), (sizes, docs, scale)
+
+
+def _attn_bwd(dout, q, k, v, q_starts, k_starts, out, lse, how, grad_dtype, need):
+    """dq, dk, dv (None where not needed)."""
+    sizes, docs, scale = how
+    B, Sq, Sk, H, Hk, D = sizes
+    dev = dout.device
+    dout, da = _rows16(dout)
+    q, qa = _rows16(q)
+    k, ka = _rows16(k)
+    v, va = _rows16(v)
+    out, oa = _rows16(out)
+    L = _lib.lib()
+    ws_bytes = L.icsa_cross_attn_bwd_workspace_size(*sizes, docs)
+    if ws_bytes < 0:
+        raise _lib.IcsaError("icsa_cross_attn_bwd_workspace_size", int(ws_bytes))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    dq = torch.empty(B, Sq, H, D, dtype=grad_dtype, device=dev) if need[0] else None
+    dk = torch.empty(B, Sk, Hk, D, dtype=grad_dtype, device=dev) if need[1] else None
+    dv = torch.empty(B, Sk, Hk, D, dtype=grad_dtype, device=dev) if need[2] else None
+    qs, ks = (Sq * H * D, H * D, D), (Sk * Hk * D, Hk * D, D)
+    with on_device(dev):
+        rc = L.icsa_cross_attn_bwd(*da, *qa, *ka, *va, *oa, lse.data_ptr(), *sizes, ptr(q_starts), ptr(k_starts), docs, scale,
+                                   _FLOATS[grad_dtype], ptr(dq), *qs, ptr(dk), *ks, ptr(dv), *ks, ws.data_ptr(), ws_bytes,
+                                   stream_ptr(dev))
+    _lib.check("icsa_cross_attn_bwd", rc)
+    return dq, dk, dv
 
 
 @torch.no_grad()
 def cross_attn_fwd_hip(q, k, v, q_starts=None, k_starts=None, softmax_scale=None):
     """``(out, lse)`` of :func:`cross_attn_func`'s forward: out bfloat16 like q, lse float32 [B, Hk, Sq, H / Hk], log2 of each
     row's sum of ``2 ** (score * log2 e)``, +inf for a row that sees nothing."""
-    return _attn_fwd(q, k, v, q_starts, k_starts, softmax_scale, True)
+    return _attn_fwd(q, k, v, q_starts, k_starts, softmax_scale, True)[:2]
 
 
 @torch.no_grad()
@@ -111,41 +139,22 @@ def cross_attn_bwd_hip(dout, q, k, v, out, lse, q_starts=None, k_starts=None, so
         raise IcsaArgumentError("dout, out and lse must be on the GPU of q")
     if grad_dtype not in _FLOATS:
         raise IcsaArgumentError("grad_dtype must be bfloat16 or float32")
-    dout, da = _rows16(dout)
-    q, qa = _rows16(q)
-    k, ka = _rows16(k)
-    v, va = _rows16(v)
-    out, oa = _rows16(out)
-    L = _lib.lib()
-    ws_bytes = L.icsa_cross_attn_bwd_workspace_size(*sizes, docs)
-    if ws_bytes < 0:
-        raise _lib.IcsaError("icsa_cross_attn_bwd_workspace_size", int(ws_bytes))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    grads = [torch.empty(B, n, h, D, dtype=grad_dtype, device=dev) if want else None
-             for want, n, h in zip(need, (Sq, Sk, Sk), (H, Hk, Hk))]
-    qs, ks = (Sq * H * D, H * D, D), (Sk * Hk * D, Hk * D, D)
-    with on_device(dev):
-        rc = L.icsa_cross_attn_bwd(
-            *da, *qa, *ka, *va, *oa, lse.data_ptr(), *sizes, ptr(q_starts), ptr(k_starts), docs, scale, _FLOATS[grad_dtype],
-            ptr(grads[0]), *qs, ptr(grads[1]), *ks, ptr(grads[2]), *ks, ws.data_ptr(), ws_bytes, stream_ptr(dev))
-    _lib.check("icsa_cross_attn_bwd", rc)
-    return tuple(grads)
+    return _attn_bwd(dout, q, k, v, q_starts, k_starts, out, lse, (sizes, docs, scale), grad_dtype, need)
 
 
 class _CrossAttn(torch.autograd.Function):
+    # The backward runs on a thread of autograd's own, where a line of Python costs about three times what it does in the
+    # forward: what was checked there is not checked again.
     @staticmethod
     def forward(ctx, q, k, v, q_starts, k_starts, scale):
-        out, lse = _attn_fwd(q, k, v, q_starts, k_starts, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, q_starts, k_starts)
-        ctx.scale = scale
+        out, lse, read, ctx.how = _attn_fwd(q, k, v, q_starts, k_starts, scale, True)
+        ctx.save_for_backward(*read, out, lse)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, q_starts, k_starts = ctx.saved_tensors
-        grads = cross_attn_bwd_hip(dout, q, k, v, out, lse, q_starts, k_starts, ctx.scale, need=ctx.needs_input_grad[:3])
-        return (*grads, None, None, None)
+        return (*_attn_bwd(dout, *ctx.saved_tensors, ctx.how, _BF, ctx.needs_input_grad), None, None, None)
 
 
 def cross_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_starts: torch.Tensor = None,
@@ -194,7 +203,7 @@ def _param_rows(gain, shift, dim):
 
 
 def _norm_fwd(x, gain, shift, plus_one, rms, eps, out_dtype, keep):
-    """(y, mean, rstd); the statistics where they are to be kept."""
+    """(y, mean, rstd, x's rows); the statistics where the backward is to come."""
     r = _rows(x)
     n, dim = r.shape
     g, s, groups, p_sg = _param_rows(gain, shift, dim)
@@ -206,45 +215,46 @@ def _norm_fwd(x, gain, shift, plus_one, rms, eps, out_dtype, keep):
         mean = None if rms else torch.empty(n, dtype=torch.float32, device=dev)
     with on_device(dev):
         rc = _lib.lib().icsa_norm_fwd(
-            r.data_ptr(), dtype_code(r), _row_stride(r), n // groups, groups, dim, ptr(g), ptr(s),
-            _lib.F32 if g is None else dtype_code(g), p_sg, plus_one, rms, eps, y.data_ptr(), _FLOATS[out_dtype], dim,
+            r.data_ptr(), _FLOATS[r.dtype], _row_stride(r), n // groups, groups, dim, ptr(g), ptr(s),
+            _lib.F32 if g is None else _FLOATS[g.dtype], p_sg, plus_one, rms, eps, y.data_ptr(), _FLOATS[out_dtype], dim,
             ptr(mean), ptr(rstd), stream_ptr(dev))
     _lib.check("icsa_norm_fwd", rc)
-    return y, mean, rstd
+    return y, mean, rstd, r
 
 
 class _Norm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gain, shift, plus_one, rms, eps, out_dtype):
-        y, mean, rstd = _norm_fwd(x, gain, shift, plus_one, rms, eps, out_dtype, True)
-        ctx.save_for_backward(x, gain, mean, rstd)
-        ctx.plus_one, ctx.rms, ctx.shift_shape = plus_one, rms, None if shift is None else shift.shape
+        y, mean, rstd, r = _norm_fwd(x, gain, shift, plus_one, rms, eps, out_dtype, True)
+        ctx.save_for_backward(r, gain, mean, rstd)
+        ctx.how = plus_one, rms, x.shape, None if shift is None else shift.shape
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, gain, mean, rstd = ctx.saved_tensors
-        need_x, need_gain, need_shift = ctx.needs_input_grad[:3]
-        r, d = _rows(x), _rows(dy)
+        r, gain, mean, rstd = ctx.saved_tensors
+        plus_one, rms, x_shape, shift_shape = ctx.how
+        need = ctx.needs_input_grad
+        d = _rows(dy)
         n, dim = r.shape
         g, _, groups, p_sg = _param_rows(gain, None, dim)
-        dev = x.device
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+        dev = r.device
+        dx = torch.empty(x_shape, dtype=r.dtype, device=dev) if need[0] else None
         make = torch.empty if n else torch.zeros
-        dgain = make(gain.shape, dtype=gain.dtype, device=dev) if need_gain else None
-        dshift = make(ctx.shift_shape, dtype=gain.dtype, device=dev) if need_shift else None
+        dgain = make(gain.shape, dtype=gain.dtype, device=dev) if need[1] else None
+        dshift = make(shift_shape, dtype=gain.dtype, device=dev) if need[2] else None
         if n:
             L = _lib.lib()
             wsp = ws_bytes = 0
-            if need_gain or need_shift:
+            if need[1] or need[2]:
                 ws_bytes = L.icsa_norm_bwd_workspace_size(n // groups, groups, dim)
                 ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
                 wsp = ws.data_ptr()
             with on_device(dev):
                 rc = L.icsa_norm_bwd(
-                    d.data_ptr(), dtype_code(d), _row_stride(d), r.data_ptr(), dtype_code(r), _row_stride(r), n // groups,
-                    groups, dim, ptr(g), _lib.F32 if g is None else dtype_code(g), p_sg, ctx.plus_one, ctx.rms, ptr(mean),
+                    d.data_ptr(), _FLOATS[d.dtype], _row_stride(d), r.data_ptr(), _FLOATS[r.dtype], _row_stride(r), n // groups,
+                    groups, dim, ptr(g), _lib.F32 if g is None else _FLOATS[g.dtype], p_sg, plus_one, rms, ptr(mean),
                     ptr(rstd), ptr(dx), dim, ptr(dgain), ptr(dshift), wsp, ws_bytes, stream_ptr(dev))
             _lib.check("icsa_norm_bwd", rc)
         return dx, dgain, dshift, None, None, None, None
@@ -359,7 +369,7 @@ def _rotate(q, k, cos, sin, positions, sections, interleaved, backward):
         sec = ctypes.cast((ctypes.c_int32 * axes)(*sections), ctypes.c_void_p)
     pos_sb = positions.stride(0) if positions.dim() == (2 if sections is None else 3) else 0
     with on_device(dev):
-        rc = _lib.lib().icsa_rotary(*args, dtype_code(q), B, S, D, 2 * cos.shape[1], interleaved, backward,
+        rc = _lib.lib().icsa_rotary(*args, _FLOATS[q.dtype], B, S, D, 2 * cos.shape[1], interleaved, backward,
                                     positions.data_ptr(), pos_sb, axes, sec, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
                                     stream_ptr(dev))
     _lib.check("icsa_rotary", rc)

@@ -25,6 +25,7 @@ from .editing_sparse_attention import Backend, _editing_sparse_attention_hip, de
 from .hip_host import (_require, dtype_code, flash_attn_func, masked_attn_func, on_device, ptr,
                        stream_ptr)
 from .mx import MXLinear, mx_quantize
+from .train import cross_attn_func, rms_norm_func, rotary_func
 
 _rope_cache: dict = {}
 
@@ -142,6 +143,34 @@ def wan_qk_prologue(yq: torch.Tensor, yk, norm_q_weight: torch.Tensor, norm_k_we
             ptr(ws), ws_bytes, stream_ptr(dev))
     _lib.check("icsa_wan_qk_prologue", rc)
     return q, k, qsum, ksum, gate
+
+
+def rope_positions(grid_sizes, source_video_grid_sizes, TAG: int, B: int, S: int, device) -> torch.Tensor:
+    """int32 [B, S, 3]: each token's frame, row and column on the target grid, then (TAG 1) on the source grid from 0 again, and
+    -1 for those that rope_apply leaves unrotated (model.py:69-95)."""
+    pos = torch.full((B, S, 3), -1, dtype=torch.int32)
+    for b in range(B):
+        at = 0
+        for f, h, w in (_grid(grid_sizes[b]), _grid(source_video_grid_sizes[b]))[:2 if TAG == 1 else 1]:
+            i = torch.arange(min(f * h * w, S - at), dtype=torch.int32)
+            pos[b, at:at + len(i)] = torch.stack([i // (h * w), i // w % h, i % w], 1)
+            at += len(i)
+    return pos.to(device)
+
+
+def wan_qk_trainable(yq: torch.Tensor, yk: torch.Tensor, norm_q_weight: torch.Tensor, norm_k_weight: torch.Tensor,
+                     positions: torch.Tensor, freqs: torch.Tensor, num_heads: int, eps: float = 1e-6):
+    """q and k of WanSelfAttention.forward from the projections yq, yk [B, S, dim], bf16 [B, S, H, D] as
+    :func:`wan_qk_prologue` makes them, with gradients to the projections and both norm weights: RMS norm over all heads, then the
+    three-axis rotation at ``positions`` (:func:`rope_positions`).  The normalised row is rounded to bf16 once, after its weight."""
+    B, S, dim = yq.shape
+    _require(yk.shape == yq.shape and dim % num_heads == 0, "yq and yk must be [B, S, dim], dim a multiple of num_heads")
+    D = dim // num_heads
+    cos, sin = rope_tables(freqs, yq.device)
+    third = D // 6
+    q, k = (rms_norm_func(y, w, eps=eps, out_dtype=torch.bfloat16).view(B, S, num_heads, D)
+            for y, w in ((yq, norm_q_weight), (yk, norm_k_weight)))
+    return rotary_func(q, k, cos, sin, positions, sections=(D // 2 - 2 * third, third, third))
 
 
 @torch.no_grad()
@@ -314,10 +343,14 @@ class WanT2VCrossAttention(nn.Module):
     ``icsa_flash_attn``, or with ``context_lens`` (int [B]: each batch row's real text tokens; a
     row of length 0 gets zeros) through ``icsa_masked_attn``.  Same parameters as the reference
     class.  The attention is an inference path with and without lengths: under an enabled grad mode its
-    result carries no gradient to q, k, v and what they come from, and nothing is raised."""
+    result carries no gradient to q, k, v and what they come from, and nothing is raised.
 
-    def __init__(self, dim, num_heads, window_size=(-1, -1), qk_norm=True, eps=1e-6):
+    ``trainable``: the norms and the attention run through ``rms_norm_func`` and ``cross_attn_func`` instead, which have
+    gradients, for x, the text and every parameter (normalised rows are rounded to bf16 once, after their weight)."""
+
+    def __init__(self, dim, num_heads, window_size=(-1, -1), qk_norm=True, eps=1e-6, trainable=False):
         super().__init__()
+        self.trainable = trainable
         self.dim = dim
         self.num_heads = num_heads
         self.head_dim = dim // num_heads
@@ -340,6 +373,8 @@ class WanT2VCrossAttention(nn.Module):
                      "context_lens must be whole numbers")
             _require(tuple(lens.shape) == (b,), "context_lens must hold one length a batch row")
             lens = lens.to(torch.int32)
+        if self.trainable:
+            return self._forward_trainable(x, context, None if context_lens is None else lens)
         none = [(0, 0, 0)] * b
         no_rope = _identity_freqs(self.head_dim, x.device)
         q = wan_qk_prologue(self.q(x), None, self.norm_q.weight, None, none, none, 0, no_rope,
@@ -355,6 +390,18 @@ class WanT2VCrossAttention(nn.Module):
             with torch.no_grad():                   # as flash_attn_func does by itself
                 y = masked_attn_func(q, k, v, q_starts=torch.stack([zero, torch.full_like(lens, q.shape[1])], 1),
                                      k_starts=torch.stack([zero, lens], 1))
+        return self.o(y.flatten(2).to(x.dtype))
+
+    def _forward_trainable(self, x, context, lens):
+        bf16, heads = torch.bfloat16, (self.num_heads, self.head_dim)
+        q = rms_norm_func(self.q(x), self.norm_q.weight, eps=self.eps, out_dtype=bf16).unflatten(2, heads)
+        yk, yv = _project(context, self.k, self.v)
+        k = rms_norm_func(yk, self.norm_k.weight, eps=self.eps, out_dtype=bf16).unflatten(2, heads)
+        starts = {}
+        if lens is not None:
+            zero = torch.zeros_like(lens)
+            starts = dict(q_starts=torch.stack([zero, torch.full_like(lens, q.shape[1])], 1), k_starts=torch.stack([zero, lens], 1))
+        y = cross_attn_func(q, k, yv.unflatten(2, heads).to(bf16), **starts)
         return self.o(y.flatten(2).to(x.dtype))
 
 
@@ -598,6 +645,6 @@ class WanModel(nn.Module):
         return out
 
 
-__all__ = ["rope_params", "wan_freqs", "rope_tables", "wan_qk_prologue", "wan_self_attention_core",
+__all__ = ["rope_params", "wan_freqs", "rope_tables", "rope_positions", "wan_qk_prologue", "wan_qk_trainable", "wan_self_attention_core",
            "ln_modulate", "WanSelfAttention", "WanT2VCrossAttention", "WanAttentionBlock",
            "WanRMSNorm", "WanLayerNorm", "Head", "WanModel", "quantize_linears", "sinusoidal_embedding_1d"]
