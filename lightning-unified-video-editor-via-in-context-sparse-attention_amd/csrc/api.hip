@@ -678,7 +678,8 @@ AttnBwdLayout attn_bwd_layout(int B, int Sq, int Sk, int H, int Hk, int D, AttnB
 
 int64_t icsa_cross_attn_bwd_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs) {
   if (check_masked_sizes(B, Sq, Sk, H, Hk, D)) return -1;
-  return attn_bwd_layout(B, Sq, Sk, H, Hk, D, attn_bwd_plan(B, Sq, Sk, H, Hk, docs <= 1)).total;
+  if (docs < 1) return fail(ICSA_EINVAL, "docs=%d", docs), -1;
+  return attn_bwd_layout(B, Sq, Sk, H, Hk, D, attn_bwd_plan(B, Sq, Sk, H, Hk, docs)).total;
 }
 
 int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t do_sh,
@@ -717,7 +718,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
   auto far = [&](int64_t ss, int64_t sh) { return ss > most / 65 || (G > 1 && sh > (most - 65 * ss) / G); };
   if (k_ss > most / 65 || v_ss > most / 65 || far(q_ss, q_sh) || far(do_ss, do_sh))
     return fail(ICSA_EUNSUPPORTED, "64 rows of q, dout, k and v must lie within 2 GiB");
-  const AttnBwdPlan plan = attn_bwd_plan(B, Sq, Sk, H, Hk, docs <= 1);
+  const AttnBwdPlan plan = attn_bwd_plan(B, Sq, Sk, H, Hk, docs);
   const AttnBwdLayout L = attn_bwd_layout(B, Sq, Sk, H, Hk, D, plan);
   if (L.total > 0 && (!workspace || workspace_bytes < L.total || !aligned16(workspace)))
     return fail(ICSA_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)L.total);
@@ -778,6 +779,7 @@ int icsa_norm_fwd(const void* x, int x_dtype, int64_t x_ss, int64_t rows, int gr
   p.y = y; p.y_dtype = y_dtype; p.y_ss = y_ss; p.mean = mean; p.rstd = rstd;
   p.vec_x = whole_chunks(x, x_ss, rows * groups, dim, elsize(x_dtype));
   p.vec_y = whole_chunks(y, y_ss, rows * groups, dim, elsize(y_dtype));
+  p.vec_p = (!gain || whole_chunks(gain, p_sg, groups, dim, elsize(p_dtype))) && (!shift || whole_chunks(shift, p_sg, groups, dim, elsize(p_dtype)));
   ICSA_HIP_TRY(launch_norm_fwd(p, reinterpret_cast<hipStream_t>(stream_)), "norm");
   return ICSA_OK;
 }
@@ -814,6 +816,7 @@ int icsa_norm_bwd(const void* dy, int dy_dtype, int64_t dy_ss, const void* x, in
   p.vec_x = whole_chunks(x, x_ss, rows * groups, dim, elsize(x_dtype));
   p.vec_y = whole_chunks(dy, dy_ss, rows * groups, dim, elsize(dy_dtype));
   p.vec_dx = whole_chunks(dx, dx_ss, rows * groups, dim, elsize(x_dtype));
+  p.vec_p = !gain || whole_chunks(gain, p_sg, groups, dim, elsize(p_dtype));
   ICSA_HIP_TRY(launch_norm_bwd(p, reinterpret_cast<hipStream_t>(stream_)), "norm backward");
   return ICSA_OK;
 }

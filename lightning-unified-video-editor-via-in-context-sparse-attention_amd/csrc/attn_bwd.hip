@@ -453,19 +453,20 @@ __global__ void __launch_bounds__(256) icsa_attn_bwd_join_kernel(AttnBwdParams p
 
 namespace {
 
-// Parts of an item's walk: as many as make the rounds of workgroups come out shortest, each part's sums costing a few per cent of a
-// round (65,520 queries over 512 keys of 40 heads: 160 items, 3 parts).  Blocks of several documents' rows walk as many times as
-// far as the others: two parts at least where rounds are few (4 clips of 8,190 tokens over 350 keys, 440 items: dk and dv 794 us in one
-// part, 700 in two, 698 in four).
-int parts(int64_t items, int64_t tiles, int slots, bool alike) {
+// Parts of an item's walk (tiles, over all documents): as many as make the rounds of workgroups come out shortest, beside the parts' sums
+// on their way through memory: 256 KB written and read an item and part at some 4.5 TB/s, in the time of an item's tiles at 3.8 us
+// (65,520 queries over 512 keys of 40 heads: 160 items, 3 parts).  Documents differ in length, and blocks with rows of two walk
+// both: four parts at least where rounds are few (4 clips of 1,500 to 17,600 tokens over 320 to 370 keys, 440 items: dk and dv with their sums
+// 1,274 us in one part, 878 in two, 766 in four, 762 in eight; of 8,190 tokens each 794, 700, 698 in one, two, four).
+int parts(int64_t items, int64_t tiles, int docs, int slots) {
   int best = 1;
   double time = 0.;
-  for (int n = 1; n <= AB_MAX_SPLIT && (n == 1 || tiles / n >= AB_MIN_TILES); ++n) {
-    if (n > 1 && items * n > 8 * slots) break;
-    const double t = (double)((items * n + slots - 1) / slots) / n + 0.01 * n;
+  const int64_t walk = tiles / docs > 0 ? tiles / docs : 1;
+  for (int n = 1; n <= AB_MAX_SPLIT && (n == 1 || walk / n >= AB_MIN_TILES); ++n) {
+    const double t = (double)((items * n + slots - 1) / slots) / n + (n > 1 ? items * n / (65. * walk) : 0.);
     if (n == 1 || t < time) { time = t; best = n; }
   }
-  return best == 1 && !alike && items <= 2 * slots && tiles >= 2 * AB_MIN_TILES ? 2 : best;
+  return best < 4 && docs > 1 && items <= 2 * slots && walk >= 4 * AB_MIN_TILES ? 4 : best;
 }
 
 int64_t blocks(int64_t rows) { return (rows + AB_ROWS - 1) / AB_ROWS; }
@@ -499,10 +500,10 @@ hipError_t run_bwd(const AttnBwdParams& p, hipStream_t stream) {
 
 }  // namespace
 
-AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, bool alike) {
+AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, int docs) {
   const int64_t BH = (int64_t)B * Hk, n_q = (int64_t)Sq * (H / Hk);
-  return AttnBwdPlan{parts(BH * blocks(n_q), (Sk + ATT_BN - 1) / ATT_BN, AB_SLOTS, alike),
-                     parts(BH * blocks(Sk), (n_q + ATT_BN - 1) / ATT_BN, AB_SLOTS, alike)};
+  return AttnBwdPlan{parts(BH * blocks(n_q), (Sk + ATT_BN - 1) / ATT_BN, docs, AB_SLOTS),
+                     parts(BH * blocks(Sk), (n_q + ATT_BN - 1) / ATT_BN, docs, AB_SLOTS)};
 }
 
 hipError_t launch_attn_bwd(AttnBwdParams p, hipStream_t stream) {

@@ -317,7 +317,7 @@ struct AttnBwdParams {
 };
 // parts that a query block's keys and a key block's rows are cut into
 struct AttnBwdPlan { int q_split, k_split; };
-AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, bool alike);   // alike: one document
+AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, int docs);
 hipError_t launch_attn_bwd(AttnBwdParams p, hipStream_t stream);
 
 // ---------------------------------------------------------------- layer norm, RMS norm (norm.hip)
@@ -337,7 +337,7 @@ struct NormParams {
   void* dgain; void* dshift;                      // [groups, dim] of p_dtype, or null
   float* part;                                    // [groups, n_wg, 2, dim4], or null
   int n_wg;                                       // workgroups a group (set by the launch)
-  int vec_x, vec_y, vec_dx;                       // rows of whole, aligned 8-element chunks
+  int vec_x, vec_y, vec_dx, vec_p;                // rows of whole, aligned 8-element chunks (p: gain and shift)
 };
 int norm_bwd_workgroups(int64_t rows, int dim, int groups);
 hipError_t launch_norm_fwd(NormParams p, hipStream_t stream);

@@ -4,16 +4,17 @@
 //   u  = dy a;  dx = r (u - mean(u) - xh mean(u xh))            (RMS norm: without mean(u))
 //   da = sum over the group's rows of dy xh;  db = sum of dy
 //
-// A row is held by LPR lanes, 8 NCH elements each: a quarter wave up to 256 elements, a wave up to 1,024, a workgroup of 4 waves
-// up to 8,192.  Workgroups walk their group's rows with a stride and keep a, b and their partial da, db in registers; the next
-// rows are requested before the present ones' sums are taken.  The forward takes the variance of the centred row from the registers (two reductions);
-// the backward's two sums are one.  da and db: every workgroup's partial sums go to memory, and a second kernel adds them
-// in a fixed order (the same inputs give the same bits).
+// A row is held by a quarter wave up to 256 elements, a wave up to 1,024, a workgroup up to 8,192, 8 elements a lane or twice
+// as many.  Workgroups walk their group's rows with a stride and keep a, b and their partial da, db in registers; the next
+// rows are requested before the present ones' sums are taken.  The forward takes the variance of the centred row from the registers
+// (two reductions); the backward's two sums are one.  da and db: every workgroup's partial sums go to memory, and a second
+// kernel adds them in a fixed order (the same inputs give the same bits).
 #include "icsa_kernels.h"
 
 #define NM_THREADS 256
-#define NM_WG_FWD 1024
-#define NM_WG_BWD 512
+#define NM_MAX_THREADS 512                            // 8,192 elements, two chunks of 8 a thread
+#define NM_WAVES 1024                                 // one a SIMD
+#define NM_FEW_ROWS 2                                 // one workgroup a group: 6 rows of 5,120 took it 18 us, six and the second kernel 14
 
 namespace {
 
@@ -80,51 +81,64 @@ template <int LPR> __device__ __forceinline__ float lanes_sum(float x) {
   return x;
 }
 
-// Sums of N values over a row's lanes.  red: one of two buffers in turn, so that one barrier is enough.
+// Sums of N values over a row's lanes (LPR 0: the workgroup's).  red: buffers used in turn, so that one barrier is enough.
 template <int LPR, int N> __device__ __forceinline__ void row_sums(float (&x)[N], float (*red)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = lanes_sum<LPR>(x[i]);
-  if constexpr (LPR == NM_THREADS) {
-    const int wave = threadIdx.x >> 6;
+  for (int i = 0; i < N; ++i) x[i] = lanes_sum<LPR == 16 ? 16 : 64>(x[i]);
+  if constexpr (LPR == 0) {
+    const int waves = blockDim.x >> 6;
     if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) red[wave][i] = x[i];
+      for (int i = 0; i < N; ++i) red[threadIdx.x >> 6][i] = x[i];
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");    // the next row's loads stay in flight
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = (red[0][i] + red[1][i]) + (red[2][i] + red[3][i]);
+    for (int i = 0; i < N; ++i) x[i] = red[0][i];
+    for (int w = 1; w < waves; ++w) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] += red[w][i];
+    }
   }
 }
 
-// a and b of the lane's elements, f32
-template <int NCH, int LPR>
-__device__ __forceinline__ void load_params(const NormParams& p, const void* src, int64_t at, float v[NCH][8], const int n[NCH], float none,
-                                            float plus) {
+// a or b of the lane's elements, f32: `none` where there is none, or plus + the parameter
+template <int NCH>
+__device__ __forceinline__ void load_params(const NormParams& p, const void* src, int64_t at, int t, int lanes, float v[NCH][8],
+                                            const int n[NCH], float none, float plus) {
 #pragma unroll
-  for (int u = 0; u < NCH; ++u)
+  for (int u = 0; u < NCH; ++u) {
+    const int64_t i = at + 8 * (t + u * lanes);
+    if (src == nullptr) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int64_t i = at + 8 * ((int)(threadIdx.x % LPR) + u * LPR) + e;
-      float x = none;
-      if (src != nullptr && e < n[u])
-        x = plus + (p.p_dtype == ICSA_DT_F32 ? reinterpret_cast<const float*>(src)[i] : (float)reinterpret_cast<const bf16*>(src)[i]);
-      v[u][e] = x;
+      for (int e = 0; e < 8; ++e) v[u][e] = none;
+    } else if (p.p_dtype == ICSA_DT_F32) {
+      Raw8<float> x;
+      x.load(reinterpret_cast<const float*>(src) + i, n[u], p.vec_p);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[u][e] = plus + x.at(e);
+    } else {
+      Raw8<bf16> x;
+      x.load(reinterpret_cast<const bf16*>(src) + i, n[u], p.vec_p);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[u][e] = plus + x.at(e);
     }
+  }
 }
 
 }  // namespace
 
 template <typename TX, typename TY, bool RMS, int LPR, int NCH>
-__global__ void __launch_bounds__(NM_THREADS) icsa_norm_fwd_kernel(NormParams p) {
-  constexpr int kRows = NM_THREADS / LPR;
-  __shared__ float red[4][4][1];
-  const int t = threadIdx.x % LPR, sub = threadIdx.x / LPR, g = blockIdx.y;
+__global__ void __launch_bounds__(LPR == 0 ? NM_MAX_THREADS : NM_THREADS) icsa_norm_fwd_kernel(NormParams p) {
+  constexpr int kRows = LPR == 0 ? 1 : NM_THREADS / (LPR == 0 ? 1 : LPR);
+  __shared__ float red[4][NM_MAX_THREADS / 64][1];
+  const int lanes = LPR == 0 ? blockDim.x : LPR, t = LPR == 0 ? threadIdx.x : threadIdx.x % (LPR == 0 ? 1 : LPR),
+            sub = LPR == 0 ? 0 : threadIdx.x / (LPR == 0 ? 1 : LPR), g = blockIdx.y;
   int n[NCH];
 #pragma unroll
-  for (int u = 0; u < NCH; ++u) n[u] = p.dim - 8 * (t + u * LPR);
+  for (int u = 0; u < NCH; ++u) n[u] = p.dim - 8 * (t + u * lanes);
   float a[NCH][8], b[NCH][8];
-  load_params<NCH, LPR>(p, p.gain, g * p.p_sg, a, n, 1.f, p.plus_one ? 1.f : 0.f);
-  load_params<NCH, LPR>(p, p.shift, g * p.p_sg, b, n, 0.f, 0.f);
+  load_params<NCH>(p, p.gain, g * p.p_sg, t, lanes, a, n, 1.f, p.plus_one ? 1.f : 0.f);
+  load_params<NCH>(p, p.shift, g * p.p_sg, t, lanes, b, n, 0.f, 0.f);
   const float inv_n = 1.f / (float)p.dim;
   const TX* x = reinterpret_cast<const TX*>(p.x) + 8 * t;
   TY* y = reinterpret_cast<TY*>(p.y) + 8 * t;
@@ -134,7 +148,7 @@ __global__ void __launch_bounds__(NM_THREADS) icsa_norm_fwd_kernel(NormParams p)
   auto fetch = [&](int64_t r) {
     const TX* src = x + (row0 + min(r, p.rows - 1)) * p.x_ss;
 #pragma unroll
-    for (int u = 0; u < NCH; ++u) next[u].load(src + 8 * u * LPR, n[u], vx);
+    for (int u = 0; u < NCH; ++u) next[u].load(src + 8 * u * lanes, n[u], vx);
   };
   int turn = 0;
   int64_t r = (int64_t)blockIdx.x * kRows + sub;
@@ -173,7 +187,7 @@ __global__ void __launch_bounds__(NM_THREADS) icsa_norm_fwd_kernel(NormParams p)
       float o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = fmaf(v[u][e] * rstd, a[u][e], b[u][e]);
-      store8(dst + 8 * u * LPR, o, n[u], vy);
+      store8(dst + 8 * u * lanes, o, n[u], vy);
     }
     if (t == 0 && p.rstd != nullptr) {
       p.rstd[row0 + r] = rstd;
@@ -183,15 +197,16 @@ __global__ void __launch_bounds__(NM_THREADS) icsa_norm_fwd_kernel(NormParams p)
 }
 
 template <typename TX, typename TY, bool RMS, int LPR, int NCH>
-__global__ void __launch_bounds__(NM_THREADS) icsa_norm_bwd_kernel(NormParams p) {
-  constexpr int kRows = NM_THREADS / LPR;
-  __shared__ float red[2][4][2];
-  const int t = threadIdx.x % LPR, sub = threadIdx.x / LPR, g = blockIdx.y;
+__global__ void __launch_bounds__(LPR == 0 ? NM_MAX_THREADS : NM_THREADS) icsa_norm_bwd_kernel(NormParams p) {
+  constexpr int kRows = LPR == 0 ? 1 : NM_THREADS / (LPR == 0 ? 1 : LPR);
+  __shared__ float red[2][NM_MAX_THREADS / 64][2];
+  const int lanes = LPR == 0 ? blockDim.x : LPR, t = LPR == 0 ? threadIdx.x : threadIdx.x % (LPR == 0 ? 1 : LPR),
+            sub = LPR == 0 ? 0 : threadIdx.x / (LPR == 0 ? 1 : LPR), g = blockIdx.y;
   int n[NCH];
 #pragma unroll
-  for (int u = 0; u < NCH; ++u) n[u] = p.dim - 8 * (t + u * LPR);
+  for (int u = 0; u < NCH; ++u) n[u] = p.dim - 8 * (t + u * lanes);
   float a[NCH][8], da[NCH][8], db[NCH][8];
-  load_params<NCH, LPR>(p, p.gain, g * p.p_sg, a, n, 1.f, p.plus_one ? 1.f : 0.f);
+  load_params<NCH>(p, p.gain, g * p.p_sg, t, lanes, a, n, 1.f, p.plus_one ? 1.f : 0.f);
 #pragma unroll
   for (int u = 0; u < NCH; ++u)
 #pragma unroll
@@ -209,8 +224,8 @@ __global__ void __launch_bounds__(NM_THREADS) icsa_norm_bwd_kernel(NormParams p)
     const int64_t at = row0 + min(r, p.rows - 1);
 #pragma unroll
     for (int u = 0; u < NCH; ++u) {
-      nx[u].load(x + at * p.x_ss + 8 * u * LPR, n[u], vx);
-      ny[u].load(y + at * p.dy_ss + 8 * u * LPR, n[u], vy);
+      nx[u].load(x + at * p.x_ss + 8 * u * lanes, n[u], vx);
+      ny[u].load(y + at * p.dy_ss + 8 * u * lanes, n[u], vy);
     }
     if (!RMS) n_mean = p.mean[at];
     n_rstd = p.rstd[at];
@@ -246,10 +261,25 @@ __global__ void __launch_bounds__(NM_THREADS) icsa_norm_bwd_kernel(NormParams p)
       float o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = rstd * (u8[u][e] - m0 - xh[u][e] * m1);
-      store8(dst + 8 * u * LPR, o, n[u], vd);
+      store8(dst + 8 * u * lanes, o, n[u], vd);
     }
   }
-  if (p.part == nullptr) return;
+  if (p.part == nullptr) {
+    if (kRows > 1 || (p.dgain == nullptr && p.dshift == nullptr)) return;
+    // the group's only workgroup: its sums are the result
+#pragma unroll
+    for (int u = 0; u < NCH; ++u) {
+      const int64_t at = (int64_t)g * p.dim + 8 * (t + u * lanes);
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        void* const out = which ? p.dshift : p.dgain;
+        if (out == nullptr) continue;
+        if (p.p_dtype == ICSA_DT_F32) store8(reinterpret_cast<float*>(out) + at, which ? db[u] : da[u], n[u], false);
+        else store8(reinterpret_cast<bf16*>(out) + at, which ? db[u] : da[u], n[u], false);
+      }
+    }
+    return;
+  }
   // this workgroup's sums: [group][workgroup][da, db][dim padded to 4]
   float* part = p.part + ((int64_t)g * gridDim.x + blockIdx.x) * 2 * p.dim4;
   if constexpr (kRows == 1) {
@@ -258,19 +288,19 @@ __global__ void __launch_bounds__(NM_THREADS) icsa_norm_bwd_kernel(NormParams p)
 #pragma unroll
       for (int e = 0; e < 8; e += 4)
         if (e < n[u]) {                               // whole fours: dim4 is padded
-          const int at = 8 * (t + u * LPR) + e;
+          const int at = 8 * (t + u * lanes) + e;
           *reinterpret_cast<floatx4*>(part + at) = floatx4{da[u][e], da[u][e + 1], da[u][e + 2], da[u][e + 3]};
           *reinterpret_cast<floatx4*>(part + p.dim4 + at) = floatx4{db[u][e], db[u][e + 1], db[u][e + 2], db[u][e + 3]};
         }
   } else {                                            // the workgroup's rows side by side, added in their order
-    __shared__ float all[kRows][8 * NCH * LPR];
+    __shared__ float all[kRows][8 * NCH * (LPR == 0 ? 1 : LPR)];
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < NCH; ++u)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) all[sub][8 * (t + u * LPR) + e] = which ? db[u][e] : da[u][e];
+        for (int e = 0; e < 8; ++e) all[sub][8 * (t + u * lanes) + e] = which ? db[u][e] : da[u][e];
       __syncthreads();
       for (int d = threadIdx.x; d < p.dim; d += NM_THREADS) {
         float s = 0.f;
@@ -312,21 +342,29 @@ __global__ void __launch_bounds__(256) icsa_norm_join_kernel(NormParams p) {
 
 namespace {
 
-int lanes_of(int dim) { return dim <= 256 ? 16 : dim <= 1024 ? 64 : 256; }
+// Threads of a row: a quarter wave, a wave, four waves with one to three chunks a thread, or eight with two.  Other counts of waves
+// leave the SIMDs unequal work: 5,120 elements (28,080 bf16 rows) by 320 threads of two whole chunks 134 us forward and 287 back, by
+// 256 of three, the last half empty, 122 and 185; 8,192 elements (20,000 rows) by 256 of four 180 and 270, by 512 of two 134 and 231.
+int threads_of(int dim) { return dim <= 256 ? 16 : dim <= 1024 ? 64 : dim <= 6144 ? 256 : 512; }
 
-// Workgroups a group of rows is dealt to: `most` over all groups, as few as leave no round incomplete by much
-int workgroups(int64_t rows, int dim, int groups, int most) {
-  const int64_t per = NM_THREADS / lanes_of(dim), n = (rows + per - 1) / per, cap = most / groups > 0 ? most / groups : 1;
-  const int64_t rounds = (n + cap - 1) / cap;
+// Workgroups that a group of rows is dealt to, over all groups, as few as leave no round incomplete by much: three waves a SIMD
+// forward (5,120 f32 elements, 65,520 rows: 394 us, with four 414; 1,000 bf16 elements, 40,000 rows: 40 and 44), four where a row
+// takes eight waves (8,192 elements: 134 us, with three 155); four back, two where their registers leave no more (28,080
+// rows of 5,120: 185, with one and a half 214).  Few rows back: one workgroup, which needs no second kernel for the parameters' gradients.
+int workgroups(int64_t rows, int dim, int groups, bool back) {
+  const int t = threads_of(dim), waves = t <= 64 ? 4 : t / 64;
+  const int64_t per = t <= 64 ? NM_THREADS / t : 1, n = (rows + per - 1) / per;
+  if (back && per == 1 && n <= NM_FEW_ROWS) return 1;
+  const int a_simd = back ? (dim > 4096 ? 2 : 4) : dim > 6144 ? 4 : 3, most = NM_WAVES * a_simd / waves;
+  const int64_t cap = most / groups > 0 ? most / groups : 1, rounds = (n + cap - 1) / cap;
   return (int)((n + rounds - 1) / (rounds > 0 ? rounds : 1));
 }
 
 template <typename TX, typename TY, bool RMS, int LPR, int NCH>
 void go(const NormParams& p, bool back, hipStream_t stream) {
-  if (back)
-    hipLaunchKernelGGL((icsa_norm_bwd_kernel<TX, TY, RMS, LPR, NCH>), dim3(p.n_wg, p.groups), dim3(NM_THREADS), 0, stream, p);
-  else
-    hipLaunchKernelGGL((icsa_norm_fwd_kernel<TX, TY, RMS, LPR, NCH>), dim3(p.n_wg, p.groups), dim3(NM_THREADS), 0, stream, p);
+  const dim3 grid(p.n_wg, p.groups), threads(LPR == 0 ? threads_of(p.dim) : NM_THREADS);
+  if (back) hipLaunchKernelGGL((icsa_norm_bwd_kernel<TX, TY, RMS, LPR, NCH>), grid, threads, 0, stream, p);
+  else hipLaunchKernelGGL((icsa_norm_fwd_kernel<TX, TY, RMS, LPR, NCH>), grid, threads, 0, stream, p);
 }
 
 template <typename TX, typename TY, bool RMS>
@@ -336,10 +374,9 @@ void by_size(const NormParams& p, bool back, hipStream_t stream) {
   else if (n <= 256) go<TX, TY, RMS, 16, 2>(p, back, stream);
   else if (n <= 512) go<TX, TY, RMS, 64, 1>(p, back, stream);
   else if (n <= 1024) go<TX, TY, RMS, 64, 2>(p, back, stream);
-  else if (n <= 2048) go<TX, TY, RMS, 256, 1>(p, back, stream);
-  else if (n <= 4096) go<TX, TY, RMS, 256, 2>(p, back, stream);
-  else if (n <= 6144) go<TX, TY, RMS, 256, 3>(p, back, stream);
-  else go<TX, TY, RMS, 256, 4>(p, back, stream);
+  else if (n <= 2048) go<TX, TY, RMS, 0, 1>(p, back, stream);
+  else if (n <= 4096 || n > 6144) go<TX, TY, RMS, 0, 2>(p, back, stream);
+  else go<TX, TY, RMS, 0, 3>(p, back, stream);
 }
 
 template <bool RMS>
@@ -357,15 +394,16 @@ hipError_t run_norm(const NormParams& p, bool back, hipStream_t stream) {
 
 }  // namespace
 
-int norm_bwd_workgroups(int64_t rows, int dim, int groups) { return workgroups(rows, dim, groups, NM_WG_BWD); }
+int norm_bwd_workgroups(int64_t rows, int dim, int groups) { return workgroups(rows, dim, groups, true); }
 
 hipError_t launch_norm_fwd(NormParams p, hipStream_t stream) {
-  p.n_wg = workgroups(p.rows, p.dim, p.groups, NM_WG_FWD);
+  p.n_wg = workgroups(p.rows, p.dim, p.groups, false);
   return run_norm(p, false, stream);
 }
 
 hipError_t launch_norm_bwd(NormParams p, hipStream_t stream) {
   p.n_wg = norm_bwd_workgroups(p.rows, p.dim, p.groups);
+  if (p.n_wg == 1 && threads_of(p.dim) > 64) p.part = nullptr;      // written by the workgroup itself
   const hipError_t e = run_norm(p, true, stream);
   if (e != hipSuccess || p.part == nullptr) return e;
   hipLaunchKernelGGL(icsa_norm_join_kernel, dim3((p.dim + 63) / 64, 2, p.groups), dim3(256), 0, stream, p);
