@@ -436,19 +436,21 @@ int64_t icsa_cross_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, int
 
 /* Attention of q [B, Sq, H, D] over k, v [B, Sk, Hk, D], all bf16, D 64 or 128: icsa_masked_attn with documents alone, and
  * for the backward lse f32 [B, Hk, Sq, H / Hk] (NULL: not wanted): log2 of a row's sum of 2^(score log2 e), +inf for a row that
- * sees nothing. */
+ * sees nothing, and rest u8 [B, Sq, H, D] (contiguous; NULL: not wanted): what rounding out to bf16 left, in 1/256 of its last
+ * place, + 128. */
 int icsa_cross_attn_fwd(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                         const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
                         const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
                         int B, int Sq, int Sk, int H, int Hk, int D,
                         const int32_t* q_starts, const int32_t* k_starts, int docs, float scale,
-                        void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, float* lse,
+                        void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, float* lse, void* rest,
                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Workspace bytes of icsa_cross_attn_bwd (rows' sums; sums of parts where a side has few rows). */
 int64_t icsa_cross_attn_bwd_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs);
 
-/* Gradients of it from dout (bf16, like q), the forward's out and lse: dq like q, dk, dv like k, bf16 or f32 (grad_dtype); a
+/* Gradients of it from dout (bf16, like q), the forward's out, lse and rest (NULL: rowsum(dout out) is taken from the rounded out, whose
+ * error shows where rows see few keys): dq like q, dk, dv like k, bf16 or f32 (grad_dtype); a
  * NULL one is not computed.  dk and dv are summed over the heads that share them.  No atomics: the same inputs give the
  * same bits.  Rows and keys outside every document, and those of documents without keys or queries, get zeros; what they hold reaches nothing.
  * A NaN or an infinity in a document makes gradients of that document NaN, in others nothing. */
@@ -456,7 +458,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
                         const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                         const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
                         const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
-                        const void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, const float* lse,
+                        const void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, const float* lse, const void* rest,
                         int B, int Sq, int Sk, int H, int Hk, int D,
                         const int32_t* q_starts, const int32_t* k_starts, int docs, float scale, int grad_dtype,
                         void* dq, int64_t dq_sb, int64_t dq_ss, int64_t dq_sh,

@@ -588,7 +588,7 @@ static int masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                      const int32_t* q_starts, const int32_t* k_starts, int docs, int causal, const int32_t* prefix,
                      float scale, float softcap, const float* bias, int radius,
                      void* out, int out_dtype, int64_t o_sb, int64_t o_ss, int64_t o_sh,
-                     float* lse, void* workspace, int64_t workspace_bytes, void* stream_) {
+                     float* lse, unsigned char* rest, void* workspace, int64_t workspace_bytes, void* stream_) {
   int rc = check_masked_sizes(B, Sq, Sk, H, Hk, D);
   if (rc || (rc = check_dtype(out_dtype, "out"))) return rc;
   if (!q_starts != !k_starts) return fail(ICSA_EINVAL, "q_starts and k_starts must be both given or both NULL");
@@ -621,6 +621,7 @@ static int masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
   p.scale = scale; p.softcap = softcap; p.bias = bias; p.radius = radius;
   p.out = OutView{out, o_sb, o_ss, o_sh, out_dtype};
   p.lse = lse;
+  p.rest = rest;
   const MaskedPlan plan = masked_attn_plan(B, Sq, Sk, H, Hk, D, docs <= 1 && !causal);
   p.n_whole = plan.n_whole; p.n_split = plan.n_split;
   const int64_t need = icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D, docs, causal);
@@ -640,7 +641,7 @@ int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                      void* out, int out_dtype, int64_t o_sb, int64_t o_ss, int64_t o_sh,
                      void* workspace, int64_t workspace_bytes, void* stream_) {
   return masked_attn(q, q_sb, q_ss, q_sh, k, k_sb, k_ss, k_sh, v, v_sb, v_ss, v_sh, B, Sq, Sk, H, Hk, D, q_starts, k_starts, docs,
-                     causal, prefix, scale, softcap, bias, radius, out, out_dtype, o_sb, o_ss, o_sh, nullptr, workspace,
+                     causal, prefix, scale, softcap, bias, radius, out, out_dtype, o_sb, o_ss, o_sh, nullptr, nullptr, workspace,
                      workspace_bytes, stream_);
 }
 
@@ -654,11 +655,12 @@ int icsa_cross_attn_fwd(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                         const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
                         int B, int Sq, int Sk, int H, int Hk, int D,
                         const int32_t* q_starts, const int32_t* k_starts, int docs, float scale,
-                        void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, float* lse,
+                        void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, float* lse, void* rest,
                         void* workspace, int64_t workspace_bytes, void* stream_) {
+  if (rest && !aligned16(rest)) return fail(ICSA_EINVAL, "rest must be 16-byte aligned");
   return masked_attn(q, q_sb, q_ss, q_sh, k, k_sb, k_ss, k_sh, v, v_sb, v_ss, v_sh, B, Sq, Sk, H, Hk, D, q_starts, k_starts, docs,
-                     0, nullptr, scale, 0.f, nullptr, 0, out, ICSA_BF16, o_sb, o_ss, o_sh, lse, workspace, workspace_bytes,
-                     stream_);
+                     0, nullptr, scale, 0.f, nullptr, 0, out, ICSA_BF16, o_sb, o_ss, o_sh, lse,
+                     reinterpret_cast<unsigned char*>(rest), workspace, workspace_bytes, stream_);
 }
 
 namespace {
@@ -686,7 +688,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
                         const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                         const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
                         const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
-                        const void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, const float* lse,
+                        const void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, const float* lse, const void* rest,
                         int B, int Sq, int Sk, int H, int Hk, int D,
                         const int32_t* q_starts, const int32_t* k_starts, int docs, float scale, int grad_dtype,
                         void* dq, int64_t dq_sb, int64_t dq_ss, int64_t dq_sh,
@@ -701,6 +703,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
     return fail(ICSA_EINVAL, "scale must be positive and finite");
   if (Sq > 0 && (!dout || !q || !out || !lse)) return fail(ICSA_EINVAL, "null pointer argument");
   if (Sk > 0 && (!k || !v)) return fail(ICSA_EINVAL, "null pointer argument");
+  if (rest && !aligned16(rest)) return fail(ICSA_EINVAL, "rest must be 16-byte aligned");
   auto ok = [](const void* p, int n, int dtype, int64_t s0, int64_t s1, int64_t s2) {
     return n == 0 || p == nullptr || row_ok(p, dtype, s0, s1, s2);
   };
@@ -730,7 +733,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
   p.v = reinterpret_cast<const bf16*>(v); p.v_sb = v_sb; p.v_ss = v_ss; p.v_sh = v_sh;
   p.o = reinterpret_cast<const bf16*>(out); p.o_sb = o_sb; p.o_ss = o_ss; p.o_sh = o_sh;
   p.dout = reinterpret_cast<const bf16*>(dout); p.do_sb = do_sb; p.do_ss = do_ss; p.do_sh = do_sh;
-  p.lse = lse;
+  p.lse = lse; p.rest = reinterpret_cast<const unsigned char*>(rest);
   p.B = B; p.Sq = Sq; p.Sk = Sk; p.H = H; p.Hk = Hk; p.D = D;
   p.q_starts = q_starts; p.k_starts = k_starts; p.docs = docs; p.scale = scale;
   p.rowv = reinterpret_cast<float*>(ws + L.rowv);

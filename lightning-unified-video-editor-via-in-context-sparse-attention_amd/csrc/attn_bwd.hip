@@ -118,11 +118,15 @@ __global__ void __launch_bounds__(AB_THREADS, 2) icsa_attn_bwd_kernel(AttnBwdPar
   if constexpr (!KV) {                                                    // D = rowsum(dO * O), f32
     const bf16* so = p.o + row_at(p.o_sb, p.o_ss, p.o_sh, b, hk, p.by_g, rc) + 8 * hl;
     lse = p.lse[(int64_t)bh * n_q + rc];
+    const unsigned char* sr = p.rest == nullptr ? nullptr
+        : p.rest + row_at((int64_t)p.Sq * p.H * D, (int64_t)p.H * D, D, b, hk, p.by_g, rc) + 8 * hl;
 #pragma unroll
     for (int kk = 0; kk < kSteps; ++kk) {
       const bf16x8 o = *reinterpret_cast<const bf16x8*>(so + 16 * kk);
+      u32x2 w = {0x80808080u, 0x80808080u};                               // nothing
+      if (sr != nullptr) w = *reinterpret_cast<const u32x2*>(sr + 16 * kk);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dd = fmaf((float)b2[kk][e], (float)o[e], dd);
+      for (int e = 0; e < 8; ++e) dd = fmaf((float)b2[kk][e], with_rest(o[e], w[e >> 2], e & 3), dd);
     }
     dd = xhalf_sum(dd);
     if (split == 0 && hl == 0 && r < n_st) {                              // what the key-major kernel's accumulators start with

@@ -117,15 +117,51 @@ __device__ __forceinline__ void store_dims32(unsigned char* stage, const float v
 // What the backward takes of a row: log2 of its sum of 2^score; +inf, with which every weight is 0, where it has none
 __device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? INFINITY : m + __builtin_amdgcn_logf(l); }
 
+// What rounding o to bf16 (b) leaves, in a byte: (o - b) in 1/256 of b's last place, + 128.  The backward's D = rowsum(dO * O) takes O
+// from both: from the rounded O alone D's error, a row's common shift of dP, is as large as dS's own rounding where a row's weight
+// lies on few keys (77 keys: dq 0.0026 from the exact one in the 2-norm, 0.0024 with the byte, 0.0017 is the results' rounding alone; 8 keys:
+// 0.0029 and 0.0025; 3 keys: 0.0036 and 0.0025).
+__device__ __forceinline__ unsigned rest_byte(float o, bf16 b) {
+  const float f = (float)b;
+  const int e = (int)(__float_as_uint(f) >> 23 & 255u);
+  return (unsigned)((int)__builtin_rintf(fminf(fmaxf(__builtin_amdgcn_ldexpf(o - f, 142 - e), -127.f), 127.f)) + 128);
+}
+__device__ __forceinline__ unsigned rest_bytes(const float o[4]) {
+  unsigned w = 0u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w |= rest_byte(o[e], (bf16)o[e]) << (8 * e);
+  return w;
+}
+// and back: byte e of w beside b
+__device__ __forceinline__ float with_rest(bf16 b, unsigned w, int e) {
+  const float f = (float)b;
+  const int x = (int)(__float_as_uint(f) >> 23 & 255u) - 15;              // a 256th of the last place is 2^(x - 127)
+  const float step = x > 0 ? __uint_as_float((unsigned)x << 23) : 0.f;
+  return fmaf((float)((w >> (8 * e)) & 255u) - 128.f, step, f);
+}
+
 // element offset of row r (query r / G, head hk G + r % G) in a [B, S, H, D] tensor
 __device__ __forceinline__ int64_t row_at(int64_t sb, int64_t ss, int64_t sh, int b, int hk, const FastDiv& g, int r) {
   const unsigned i = g.d == 1 ? r : g.div(r);
   return (int64_t)b * sb + (int64_t)i * ss + (int64_t)(hk * g.d + r - i * g.d) * sh;
 }
 
+// The rest bytes of one wave's 32 rows of 32 dims: dims 16 hl .. + 15 of row li in one store (v as in store_dims32)
+__device__ __forceinline__ void store_rest32(const float v[16], int rows_valid, unsigned char* row) {
+  const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5;
+  unsigned w[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) w[g] = rest_bytes(v + 4 * g);
+  const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+  const auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+  if (li < rows_valid) *reinterpret_cast<u32x4*>(row + 16 * hl) = u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// rest: [B, S, H, D] bytes like a contiguous output, or null
 template <int D>
 __device__ __forceinline__ void store_wave(const OutView& out, const FastDiv& by_g, unsigned char* stage, const floatx16 o[D / 32],
-                                           float inv_l, int b, int hk, int r0, int rows_valid) {
+                                           float inv_l, int b, int hk, int r0, int rows_valid,
+                                           unsigned char* rest = nullptr, int Sq = 0, int H = 0) {
   const int lane = threadIdx.x & 63, li = lane & 31;
   int64_t off[2];
 #pragma unroll
@@ -136,6 +172,8 @@ __device__ __forceinline__ void store_wave(const OutView& out, const FastDiv& by
     float v[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = o[ds][e] * inv_l;
+    if (rest != nullptr)
+      store_rest32(v, rows_valid, rest + row_at((int64_t)Sq * H * D, (int64_t)H * D, D, b, hk, by_g, r0 + li) + 32 * ds);
     if (out.dtype == ICSA_DT_BF16) store_dims32<1>(stage, v, rows_valid, off, own, out.p, 32 * ds);
     else store_dims32<0>(stage, v, rows_valid, off, own, out.p, 32 * ds);
   }

@@ -1,0 +1,363 @@
+// Autograd nodes of the training operators (icsa_hip/train.py) over the C ABI of libicsa.so.
+//
+// A Python autograd function runs its backward on a thread of autograd's own, which waits for the interpreter and finds its objects
+// in another core's cache: a layer norm of six rows, forward and backward, took 130 us of host time in Python and XX here, where the
+// backward never enters the interpreter.
+//
+// Arguments have been checked in Python.  The library is the one that the package has loaded, found by its path.  What the
+// backward reads is taken from the saved tensors, not remembered by address: hooks may have moved it.
+#include <torch/extension.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <dlfcn.h>
+
+#include "../../include/icsa.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+typedef c10::optional<Tensor> MaybeTensor;
+
+struct Api {
+  decltype(&icsa_last_error) last_error = nullptr;
+  decltype(&icsa_cross_attn_workspace_size) attn_workspace;
+  decltype(&icsa_cross_attn_fwd) attn_fwd;
+  decltype(&icsa_cross_attn_bwd_workspace_size) attn_bwd_workspace;
+  decltype(&icsa_cross_attn_bwd) attn_bwd;
+  decltype(&icsa_norm_fwd) norm_fwd;
+  decltype(&icsa_norm_bwd_workspace_size) norm_workspace;
+  decltype(&icsa_norm_bwd) norm_bwd;
+  decltype(&icsa_rotary) rotary;
+} api;
+PyObject* g_error = nullptr;                          // icsa_hip._lib.IcsaError
+
+void bind(const std::string& path, py::object error) {
+  void* h = dlopen(path.c_str(), RTLD_NOW | RTLD_LOCAL);
+  TORCH_CHECK(h, "cannot open ", path, ": ", dlerror());
+  auto get = [&](auto& f, const char* name) {
+    f = reinterpret_cast<std::decay_t<decltype(f)>>(dlsym(h, name));
+    TORCH_CHECK(f, path, " lacks ", name);
+  };
+  get(api.attn_workspace, "icsa_cross_attn_workspace_size");
+  get(api.attn_fwd, "icsa_cross_attn_fwd");
+  get(api.attn_bwd_workspace, "icsa_cross_attn_bwd_workspace_size");
+  get(api.attn_bwd, "icsa_cross_attn_bwd");
+  get(api.norm_fwd, "icsa_norm_fwd");
+  get(api.norm_workspace, "icsa_norm_bwd_workspace_size");
+  get(api.norm_bwd, "icsa_norm_bwd");
+  get(api.rotary, "icsa_rotary");
+  get(api.last_error, "icsa_last_error");
+  g_error = error.release().ptr();
+}
+
+struct Failure : public torch::PyTorchError {
+  explicit Failure(const std::string& what) : PyTorchError(what) {}
+  PyObject* python_type() override { return g_error; }
+};
+
+void check(const char* fn, int64_t code) {
+  if (code < 0) throw Failure(std::string(fn) + " failed with status " + std::to_string(code) + ": " + api.last_error());
+}
+
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// An absent tensor is no input of a node, and needs_input_grad does not count it: only the last ones are absent here.
+Tensor get(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
+void* at_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+int code_of(at::ScalarType t) { return t == at::kBFloat16 ? ICSA_BF16 : ICSA_F32; }
+
+Tensor workspace(int64_t bytes, const Tensor& like) {
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+
+// Gradients have none themselves: where a graph of them is asked for they raise when it is used.
+variable_list once(variable_list grads) {
+  if (!c10::GradMode::is_enabled()) return grads;
+  variable_list in;
+  for (const Tensor& g : grads) in.push_back(g.defined() ? g.detach().set_requires_grad(true) : g);
+  torch::autograd::DelayedError error("icsa_hip's training operators have no second derivative", (int64_t)in.size());
+  return error.apply(std::move(in));
+}
+
+// t [B, S, H, D] with a unit stride in each row and rows on 16 bytes (itself where they are), its address and strides
+struct Rows {
+  Tensor t;
+  void* p;
+  int64_t sb, ss, sh;
+};
+Rows rows16(const Tensor& t) {
+  auto of = [](const Tensor& x) {
+    Rows r{x, x.data_ptr(), x.size(0) > 1 ? x.stride(0) : 0, x.size(1) > 1 ? x.stride(1) : 0, x.size(2) > 1 ? x.stride(2) : 0};
+    return r;
+  };
+  auto ok = [](const Rows& r) {
+    return r.t.stride(3) == 1 && ((reinterpret_cast<uintptr_t>(r.p) | (uintptr_t)((r.sb | r.ss | r.sh) * 2)) & 15) == 0;
+  };
+  Rows r = of(t);
+  if (ok(r)) return r;
+  r = of(t.contiguous());
+  return ok(r) ? r : of(t.clone(at::MemoryFormat::Contiguous));
+}
+
+// ------------------------------------------------------------------------------------------ cross attention
+struct AttnSizes {
+  int B, Sq, Sk, H, Hk, D;
+};
+AttnSizes attn_sizes(const Tensor& q, const Tensor& k) {
+  return {(int)q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), (int)k.size(2), (int)q.size(3)};
+}
+
+// out, and with them the state of the backward: lse and rest
+Tensor attn_forward(const Rows& q, const Rows& k, const Rows& v, const Tensor& qs, const Tensor& ks, int64_t docs, double scale,
+                    Tensor* lse, Tensor* rest) {
+  c10::DeviceGuard guard(q.t.device());
+  const AttnSizes z = attn_sizes(q.t, k.t);
+  Tensor out = at::empty({z.B, z.Sq, z.H, z.D}, q.t.options());
+  if (lse != nullptr) {
+    *lse = at::empty({z.B, z.Hk, z.Sq, z.H / z.Hk}, q.t.options().dtype(at::kFloat));
+    *rest = at::empty({z.B, z.Sq, z.H, z.D}, q.t.options().dtype(at::kByte));
+  }
+  const int64_t bytes = api.attn_workspace(z.B, z.Sq, z.Sk, z.H, z.Hk, z.D, (int)docs);
+  check("icsa_cross_attn_workspace_size", bytes);
+  const Tensor ws = workspace(bytes, out);
+  check("icsa_cross_attn_fwd",
+        api.attn_fwd(q.p, q.sb, q.ss, q.sh, k.p, k.sb, k.ss, k.sh, v.p, v.sb, v.ss, v.sh, z.B, z.Sq, z.Sk, z.H, z.Hk, z.D,
+                     (const int32_t*)at_or_null(qs), (const int32_t*)at_or_null(ks), (int)docs, (float)scale, out.data_ptr(),
+                     (int64_t)z.Sq * z.H * z.D, (int64_t)z.H * z.D, z.D, lse ? (float*)lse->data_ptr() : nullptr,
+                     rest ? rest->data_ptr() : nullptr, at_or_null(ws), bytes, stream_of(out)));
+  return out;
+}
+
+struct CrossAttn : public torch::autograd::Function<CrossAttn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const MaybeTensor& qs_,
+                        const MaybeTensor& ks_, int64_t docs, double scale) {
+    const Tensor qs = get(qs_), ks = get(ks_);
+    const Rows q = rows16(q_), k = rows16(k_), v = rows16(v_);
+    Tensor lse, rest, out = attn_forward(q, k, v, qs, ks, docs, scale, &lse, &rest);
+    ctx->save_for_backward({q.t, k.t, v.t, qs, ks, out, lse, rest});
+    ctx->saved_data["docs"] = docs;
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    variable_list res(7);
+    {
+      at::NoGradGuard none;
+      c10::DeviceGuard guard(grads[0].device());
+      const Rows g = rows16(grads[0]), q = rows16(s[0]), k = rows16(s[1]), v = rows16(s[2]), o = rows16(s[5]);
+      const Tensor lse = s[6].contiguous(), rest = s[7].contiguous(), qs = s[3].defined() ? s[3].contiguous() : s[3],
+                   ks = s[4].defined() ? s[4].contiguous() : s[4];
+      const AttnSizes z = attn_sizes(q.t, k.t);
+      const int docs = (int)ctx->saved_data["docs"].toInt();
+      const auto opt = q.t.options();
+      if (ctx->needs_input_grad(0)) res[0] = at::empty({z.B, z.Sq, z.H, z.D}, opt);
+      if (ctx->needs_input_grad(1)) res[1] = at::empty({z.B, z.Sk, z.Hk, z.D}, opt);
+      if (ctx->needs_input_grad(2)) res[2] = at::empty({z.B, z.Sk, z.Hk, z.D}, opt);
+      const int64_t bytes = api.attn_bwd_workspace(z.B, z.Sq, z.Sk, z.H, z.Hk, z.D, docs);
+      check("icsa_cross_attn_bwd_workspace_size", bytes);
+      const Tensor ws = workspace(bytes, q.t);
+      const int64_t qss = (int64_t)z.H * z.D, kss = (int64_t)z.Hk * z.D;
+      check("icsa_cross_attn_bwd",
+            api.attn_bwd(g.p, g.sb, g.ss, g.sh, q.p, q.sb, q.ss, q.sh, k.p, k.sb, k.ss, k.sh, v.p, v.sb, v.ss, v.sh, o.p, o.sb, o.ss, o.sh,
+                         (const float*)lse.data_ptr(), rest.data_ptr(), z.B, z.Sq, z.Sk, z.H, z.Hk, z.D,
+                         (const int32_t*)at_or_null(qs), (const int32_t*)at_or_null(ks), docs,
+                         (float)ctx->saved_data["scale"].toDouble(), ICSA_BF16, at_or_null(res[0]), z.Sq * qss, qss, z.D,
+                         at_or_null(res[1]), z.Sk * kss, kss, z.D, at_or_null(res[2]), z.Sk * kss, kss, z.D, at_or_null(ws), bytes,
+                         stream_of(q.t)));
+    }
+    return once(std::move(res));
+  }
+};
+
+Tensor cross_attn(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& qs, const MaybeTensor& ks, int64_t docs,
+                  double scale) {
+  if (wants_grad({&q, &k, &v})) return CrossAttn::apply(q, k, v, qs, ks, docs, scale);
+  return attn_forward(rows16(q), rows16(k), rows16(v), get(qs), get(ks), docs, scale, nullptr, nullptr);
+}
+
+// ------------------------------------------------------------------------------------------ layer norm, RMS norm
+// t [..., dim] as [rows, dim] with a unit stride in each row
+Tensor rows(const Tensor& t) {
+  const Tensor x = t.size(-1) != 1 && t.stride(-1) != 1 ? t.contiguous() : t;
+  return x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+}
+int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+// gain and shift as [groups, dim] with one group stride
+struct Params {
+  Tensor gain, shift;
+  int groups = 1, code = ICSA_F32;
+  int64_t stride = 0;
+};
+Params params(const Tensor& gain, const Tensor& shift) {
+  Params p;
+  if (!gain.defined()) return p;
+  p.gain = rows(gain);
+  if (shift.defined()) p.shift = rows(shift);
+  if (p.gain.size(0) > 1 && p.shift.defined() && p.gain.stride(0) != p.shift.stride(0)) {
+    p.gain = p.gain.contiguous();
+    p.shift = p.shift.contiguous();
+  }
+  p.groups = (int)p.gain.size(0);
+  p.code = code_of(gain.scalar_type());
+  p.stride = p.gain.stride(0);
+  return p;
+}
+
+Tensor norm_forward(const Tensor& x, const Tensor& r, const Tensor& gain, const Tensor& shift, bool plus_one, bool rms, double eps,
+                    at::ScalarType out, Tensor* mean, Tensor* rstd) {
+  c10::DeviceGuard guard(x.device());
+  const Params p = params(gain, shift);
+  const int64_t n = r.size(0), dim = r.size(1);
+  Tensor y = at::empty(x.sizes(), x.options().dtype(out));
+  if (rstd != nullptr) {
+    *rstd = at::empty({n}, x.options().dtype(at::kFloat));
+    if (!rms) *mean = at::empty({n}, x.options().dtype(at::kFloat));
+  }
+  check("icsa_norm_fwd", api.norm_fwd(r.data_ptr(), code_of(r.scalar_type()), row_stride(r), n / p.groups, p.groups, (int)dim,
+                                      at_or_null(p.gain), at_or_null(p.shift), p.code, p.stride, plus_one, rms, (float)eps, y.data_ptr(),
+                                      code_of(out), dim, mean ? (float*)at_or_null(*mean) : nullptr,
+                                      rstd ? (float*)rstd->data_ptr() : nullptr, stream_of(x)));
+  return y;
+}
+
+struct Norm : public torch::autograd::Function<Norm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const MaybeTensor& gain_, const MaybeTensor& shift_, bool plus_one,
+                        bool rms, double eps, int64_t out) {
+    const Tensor gain = get(gain_), shift = get(shift_);
+    const Tensor r = rows(x);
+    Tensor mean, rstd, y = norm_forward(x, r, gain, shift, plus_one, rms, eps, (at::ScalarType)out, &mean, &rstd);
+    ctx->save_for_backward({r, gain, mean, rstd});
+    ctx->saved_data["how"] = (int64_t)(plus_one | rms << 1);
+    ctx->saved_data["x"] = x.sizes();
+    if (shift.defined()) ctx->saved_data["shift"] = shift.sizes();
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    variable_list res(7);
+    {
+      at::NoGradGuard none;
+      c10::DeviceGuard guard(grads[0].device());
+      const Tensor d = rows(grads[0]), r = rows(s[0]), mean = s[2], rstd = s[3];
+      const Params p = params(s[1], Tensor());
+      const int64_t how = ctx->saved_data["how"].toInt(), n = r.size(0), dim = r.size(1);
+      const bool need_gain = s[1].defined() && ctx->needs_input_grad(1);
+      const bool need_shift = ctx->saved_data.count("shift") != 0 && ctx->needs_input_grad(2), sums = need_gain || need_shift;
+      if (ctx->needs_input_grad(0)) res[0] = at::empty(ctx->saved_data["x"].toIntVector(), r.options());
+      auto make = [&](at::IntArrayRef size) { return n > 0 ? at::empty(size, s[1].options()) : at::zeros(size, s[1].options()); };
+      if (need_gain) res[1] = make(s[1].sizes());
+      if (need_shift) res[2] = make(ctx->saved_data["shift"].toIntVector());
+      if (n > 0) {
+        const int64_t bytes = sums ? api.norm_workspace(n / p.groups, p.groups, (int)dim) : 0;
+        check("icsa_norm_bwd_workspace_size", bytes);
+        const Tensor ws = workspace(bytes, r);
+        check("icsa_norm_bwd", api.norm_bwd(d.data_ptr(), code_of(d.scalar_type()), row_stride(d), r.data_ptr(), code_of(r.scalar_type()),
+                                            row_stride(r), n / p.groups, p.groups, (int)dim, at_or_null(p.gain), p.code, p.stride,
+                                            (int)(how & 1), (int)(how >> 1), (const float*)at_or_null(mean), (const float*)rstd.data_ptr(),
+                                            at_or_null(res[0]), dim, at_or_null(res[1]), at_or_null(res[2]), at_or_null(ws), bytes,
+                                            stream_of(r)));
+      }
+    }
+    return once(std::move(res));
+  }
+};
+
+Tensor norm(const Tensor& x, const MaybeTensor& gain_, const MaybeTensor& shift_, bool plus_one, bool rms, double eps, at::ScalarType out) {
+  const Tensor gain = get(gain_), shift = get(shift_);
+  if (wants_grad({&x, &gain, &shift})) return Norm::apply(x, gain_, shift_, plus_one, rms, eps, (int64_t)out);
+  return norm_forward(x, rows(x), gain, shift, plus_one, rms, eps, out, nullptr, nullptr);
+}
+
+// ------------------------------------------------------------------------------------------ rotary positions
+Tensor unit_last(const Tensor& t) { return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// Both turned (either may be undefined), new and contiguous.  axes 0: one axis without sections.
+std::pair<Tensor, Tensor> rotate(const Tensor& q_, const Tensor& k_, const Tensor& cos, const Tensor& sin, const Tensor& pos,
+                                 const std::vector<int64_t>& sections, bool interleaved, bool back) {
+  const Tensor x[2] = {unit_last(q_), unit_last(k_)};
+  const Tensor& any = x[0].defined() ? x[0] : x[1];
+  c10::DeviceGuard guard(any.device());
+  Tensor y[2];
+  void *xp[2] = {}, *yp[2] = {};
+  int64_t st[2][3] = {};
+  int H[2] = {};
+  for (int i = 0; i < 2; ++i) {
+    if (!x[i].defined()) continue;
+    y[i] = at::empty(x[i].sizes(), x[i].options());
+    xp[i] = x[i].data_ptr();
+    yp[i] = y[i].data_ptr();
+    H[i] = (int)x[i].size(2);
+    for (int d = 0; d < 3; ++d) st[i][d] = x[i].stride(d);
+  }
+  int32_t sec[4] = {};
+  for (size_t i = 0; i < sections.size() && i < 4; ++i) sec[i] = (int32_t)sections[i];
+  const int axes = sections.empty() ? 1 : (int)sections.size();
+  const bool each = pos.dim() == (sections.empty() ? 2 : 3);
+  check("icsa_rotary",
+        api.rotary(xp[0], st[0][0], st[0][1], st[0][2], H[0], yp[0], xp[1], st[1][0], st[1][1], st[1][2], H[1], yp[1],
+                   code_of(any.scalar_type()), (int)any.size(0), (int)any.size(1), (int)any.size(3), 2 * (int)cos.size(1), interleaved,
+                   back, (const int32_t*)pos.data_ptr(), each ? pos.stride(0) : 0, axes, sections.empty() ? nullptr : sec,
+                   (const float*)cos.data_ptr(), (const float*)sin.data_ptr(), (int)cos.size(0), stream_of(any)));
+  return {y[0], y[1]};
+}
+
+struct Rotary : public torch::autograd::Function<Rotary> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const MaybeTensor& k_, const Tensor& cos, const Tensor& sin,
+                               const Tensor& pos, std::vector<int64_t> sections, bool interleaved) {
+    const Tensor k = get(k_);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({cos, sin, pos});
+    auto y = rotate(q, k, cos, sin, pos, sections, interleaved, false);
+    ctx->saved_data["sections"] = std::move(sections);
+    ctx->saved_data["interleaved"] = interleaved;
+    if (!k.defined()) return {y.first};
+    return {y.first, y.second};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    variable_list res(7);
+    {
+      at::NoGradGuard none;
+      const Tensor dq = ctx->needs_input_grad(0) ? grads[0] : Tensor();
+      const Tensor dk = grads.size() > 1 && ctx->needs_input_grad(1) ? grads[1] : Tensor();
+      if (dq.defined() || dk.defined())
+        std::tie(res[0], res[1]) = rotate(dq, dk, s[0].contiguous(), s[1].contiguous(), s[2].contiguous(),
+                                          ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), true);
+    }
+    return once(std::move(res));
+  }
+};
+
+variable_list rotary(const Tensor& q, const MaybeTensor& k_, const Tensor& cos, const Tensor& sin, const Tensor& pos,
+                     std::vector<int64_t> sections, bool interleaved) {
+  const Tensor k = get(k_), c = cos.contiguous(), s = sin.contiguous(), p = pos.contiguous();
+  if (wants_grad({&q, &k})) return Rotary::apply(q, k_, c, s, p, std::move(sections), interleaved);
+  auto y = rotate(q, k, c, s, p, sections, interleaved, false);
+  return k.defined() ? variable_list{y.first, y.second} : variable_list{y.first};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_autograd, m) {
+  m.def("bind", torch::wrap_pybind_function(bind));
+  m.def("cross_attn", torch::wrap_pybind_function(cross_attn));
+  m.def("norm", torch::wrap_pybind_function(norm));
+  m.def("rotary", torch::wrap_pybind_function(rotary));
+}

@@ -288,6 +288,7 @@ struct MaskedAttnParams {
   const float* bias; int radius;                  // [H, 2 radius + 1] or null
   OutView out;
   float* lse;                                     // [B, Hk, Sq H / Hk] or null: log2 of every row's sum of 2^score
+  unsigned char* rest;                            // [B, Sq, H, D] or null: what the output's rounding leaves (rest_byte)
   int n_whole, n_split; float* part;              // MaskedPlan; the parts' sums
   FastDiv by_g, by_blk, by_hk, by_bh, by_split;   // heads of a group, row blocks, key heads, B Hk, parts (set by the launch)
 };
@@ -304,6 +305,7 @@ struct AttnBwdParams {
   const bf16* k; int64_t k_sb, k_ss, k_sh;        // [B, Sk, Hk, D]
   const bf16* v; int64_t v_sb, v_ss, v_sh;
   const bf16* o; int64_t o_sb, o_ss, o_sh;        // the forward's result
+  const unsigned char* rest;                      // and what its rounding left, or null
   const bf16* dout; int64_t do_sb, do_ss, do_sh;
   const float* lse;                               // [B, Hk, Sq H / Hk], the forward's
   int B, Sq, Sk, H, Hk, D;

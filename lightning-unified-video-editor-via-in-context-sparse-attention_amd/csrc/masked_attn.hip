@@ -411,7 +411,8 @@ __global__ void __launch_bounds__(MA_THREADS, ma_wg_per_cu(D)) icsa_masked_attn_
   }
   if (!cut) {
     if (p.lse != nullptr && hl == 0 && li < rows_valid) p.lse[(int64_t)bh * n_rows + r0 + li] = row_lse(m_ref, some ? l : 0.f);
-    store_wave<D>(p.out, p.by_g, scratch, o, !some || l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l), b, hk, r0, rows_valid);
+    store_wave<D>(p.out, p.by_g, scratch, o, !some || l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l), b, hk, r0, rows_valid,
+                  p.rest, p.Sq, p.H);
   } else if (li < rows_valid) {
     // a row's raw O, reference max and sum: [part][row][D], then [part][2][row]
     float* dst = p.part + ((int64_t)w * MA_ROWS + 32 * wave + li) * D + 4 * hl;
@@ -482,6 +483,11 @@ __global__ void __launch_bounds__(256) icsa_masked_combine_kernel(MaskedAttnPara
   if (p.lse != nullptr && t == 0) p.lse[(int64_t)bh * n_rows + r] = row_lse(m, l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t off = row_at(p.out.sb, p.out.ss, p.out.sh, p.by_hk.div(bh), p.by_hk.mod(bh), p.by_g, r) + 4 * t;
+  if (p.rest != nullptr) {
+    const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+    *reinterpret_cast<unsigned*>(p.rest + row_at((int64_t)p.Sq * p.H * D, (int64_t)p.H * D, D, p.by_hk.div(bh), p.by_hk.mod(bh), p.by_g, r) +
+                                 4 * t) = rest_bytes(v);
+  }
   if (p.out.dtype == ICSA_DT_BF16) {
     bf16x4 y;
 #pragma unroll

@@ -202,7 +202,7 @@ _SIGNATURES = {
         _p, _l, _l, _l,
         _i, _i, _i, _i, _i, _i,
         _p, _p, _i, _f,
-        _p, _l, _l, _l, _p,
+        _p, _l, _l, _l, _p, _p,
         _p, _l, _p]),
     "icsa_cross_attn_bwd_workspace_size": (_l, [_i, _i, _i, _i, _i, _i, _i]),
     "icsa_cross_attn_bwd": (_i, [
@@ -210,7 +210,7 @@ _SIGNATURES = {
         _p, _l, _l, _l,
         _p, _l, _l, _l,
         _p, _l, _l, _l,
-        _p, _l, _l, _l, _p,
+        _p, _l, _l, _l, _p, _p,
         _i, _i, _i, _i, _i, _i,
         _p, _p, _i, _f, _i,
         _p, _l, _l, _l,
@@ -256,9 +256,13 @@ def lib():
 
 
 class IcsaError(RuntimeError):
-    """A non-zero status returned by libicsa (message from icsa_last_error)."""
+    """A non-zero status returned by libicsa (message from icsa_last_error; the autograd nodes give the whole text)."""
 
-    def __init__(self, fn: str, code: int):
+    def __init__(self, fn: str, code: int = None):
+        if code is None:
+            super().__init__(fn)
+            self.code = None
+            return
         msg = lib().icsa_last_error().decode("utf-8", "replace")
         super().__init__(f"{fn} failed with status {code}: {msg}")
         self.code = code

@@ -1,10 +1,10 @@
-"""Build ``libicsa.so`` (gfx950) from ``../csrc`` with hipcc.
+"""Build ``libicsa.so`` (gfx950) from ``../csrc`` with hipcc, and ``_autograd.so`` (host code) with g++.
 
 Every HIP source is compiled to an object in ``csrc/_build`` (in parallel), then linked
 into ``icsa_hip/libicsa.so`` next to this file.  The link goes to a
 temporary name first and is renamed into place, so a concurrent loader never sees a
-half-written library.  Run ``python -m icsa_hip.build`` or call
-:func:`build_library`.
+half-written library.  ``_autograd.so`` (the autograd nodes of ``train.py``) is built beside it against the
+installed torch.  Run ``python -m icsa_hip.build`` or call :func:`build_library`.
 """
 from __future__ import annotations
 
@@ -17,6 +17,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC_DIR = os.path.join(os.path.dirname(PKG_DIR), "csrc")
 BUILD_DIR = os.path.join(CSRC_DIR, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "libicsa.so")
+NODES_PATH = os.path.join(PKG_DIR, "_autograd.so")
 
 SOURCES = ["pool.hip", "compressed.hip", "newkv.hip", "gather.hip", "flash_attn.hip", "sparse_attn.hip", "sparse_bwd.hip",
            "wan_qk.hip", "wan_block.hip", "mx_quant.hip", "mx_gemm.hip", "mx_rows.hip", "masked_attn.hip",
@@ -59,6 +60,23 @@ def _run(cmd, verbose):
         print(out, flush=True)
 
 
+def _build_nodes(verbose: bool) -> None:
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = NODES_PATH + f".tmp{os.getpid()}"
+    # torch's headers ask for the platform's name; this file itself holds no device code
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_API_INCLUDE_EXTENSION_H",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          *(x for p in include_paths() for x in ("-isystem", p)), "-isystem", "/opt/rocm/include", "-isystem",
+          sysconfig.get_paths()["include"], os.path.join(CSRC_DIR, "autograd.cpp"), "-o", tmp, f"-L{lib}",
+          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"], verbose)
+    os.replace(tmp, NODES_PATH)
+
+
 def build_library(verbose: bool = False, jobs: int = 8) -> str:
     """Compile every HIP source for gfx950 and link libicsa.so; returns its path."""
     os.makedirs(BUILD_DIR, exist_ok=True)
@@ -71,8 +89,10 @@ def build_library(verbose: bool = False, jobs: int = 8) -> str:
              verbose)
         return obj
 
-    with ThreadPoolExecutor(max_workers=max(1, min(jobs, len(SOURCES)))) as ex:
+    with ThreadPoolExecutor(max_workers=max(1, min(jobs, len(SOURCES) + 1))) as ex:
+        nodes = ex.submit(_build_nodes, verbose)          # the longest one first
         objs = list(ex.map(compile_one, SOURCES))
+        nodes.result()
     tmp = LIB_PATH + f".tmp{os.getpid()}"
     _run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs], verbose)
     os.replace(tmp, LIB_PATH)

@@ -6,18 +6,16 @@
 * :func:`rotary_func`, :func:`rotary_table`: rotary positions, interleaved or in halves, of part of a
   head, over one to four axes, for contexts longer than the trained one.
 
-Each is an autograd function over a pair of library calls; without an enabled grad mode, or inputs that
-require gradients, the forward alone runs and keeps nothing.  Gradients are sums in a fixed order: the same
+Each is an autograd node over a pair of library calls (csrc/autograd.cpp); without an enabled grad mode, or inputs
+that require gradients, the forward alone runs and keeps nothing.  Gradients are sums in a fixed order: the same
 inputs give the same bits.  There is no second derivative.  :func:`cross_attn_fwd_hip` and
 :func:`cross_attn_bwd_hip` are the attention's pair by itself, for callers with their own graph.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .hip_host import IcsaArgumentError, _require, _rows16, on_device, ptr, stream_ptr
@@ -27,8 +25,21 @@ _FLOATS = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 NORM_MAX_DIM = 8192
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+_native = None
+
+
+def _nodes():
+    """The autograd nodes' module, bound to the library that the package has loaded (raises OSError when not built)."""
+    global _native
+    if _native is None:
+        _lib.lib()
+        try:
+            from . import _autograd
+        except ImportError as e:
+            raise OSError("icsa_hip/_autograd.so not found; build it with `python -m icsa_hip.build`") from e
+        _autograd.bind(_lib.lib_path(), _lib.IcsaError)
+        _native = _autograd
+    return _native
 
 
 # ------------------------------------------------------------------------------------------
@@ -65,8 +76,10 @@ def _check_attn(q, k, v, q_starts, k_starts, softmax_scale):
     return (B, Sq, Sk, H, Hk, D), docs, scale, q_starts, k_starts
 
 
-def _attn_fwd(q, k, v, q_starts, k_starts, softmax_scale, want_lse):
-    """(out, lse, and for the backward: q, k, v as the library reads them and the borders; sizes, documents and scale)."""
+@torch.no_grad()
+def cross_attn_fwd_hip(q, k, v, q_starts=None, k_starts=None, softmax_scale=None):
+    """``(out, lse, rest)`` of :func:`cross_attn_func`'s forward: out bfloat16 like q; lse float32 [B, Hk, Sq, H / Hk], log2 of each
+    row's sum of ``2 ** (score * log2 e)``, +inf for a row that sees nothing; rest uint8 like out, what its rounding left."""
     sizes, docs, scale, q_starts, k_starts = _check_attn(q, k, v, q_starts, k_starts, softmax_scale)
     B, Sq, _, H, Hk, D = sizes
     dev = q.device
@@ -74,7 +87,8 @@ def _attn_fwd(q, k, v, q_starts, k_starts, softmax_scale, want_lse):
     k, ka = _rows16(k)
     v, va = _rows16(v)
     out = torch.empty(B, Sq, H, D, dtype=_BF, device=dev)
-    lse = torch.empty(B, Hk, Sq, H // Hk, dtype=torch.float32, device=dev) if want_lse else None
+    rest = torch.empty(B, Sq, H, D, dtype=torch.uint8, device=dev)
+    lse = torch.empty(B, Hk, Sq, H // Hk, dtype=torch.float32, device=dev)
     L = _lib.lib()
     wsp, ws_bytes = 0, L.icsa_cross_attn_workspace_size(*sizes, docs)
     if ws_bytes:
@@ -84,16 +98,30 @@ def _attn_fwd(q, k, v, q_starts, k_starts, softmax_scale, want_lse):
         wsp = ws.data_ptr()
     with on_device(dev):
         rc = L.icsa_cross_attn_fwd(*qa, *ka, *va, *sizes, ptr(q_starts), ptr(k_starts), docs, scale, out.data_ptr(), Sq * H * D, H * D, D,
-                                   ptr(lse), wsp, ws_bytes, stream_ptr(dev))
+                                   lse.data_ptr(), rest.data_ptr(), wsp, ws_bytes, stream_ptr(dev))
     _lib.check("icsa_cross_attn_fwd", rc)
-    return out, lse, (q, k, v, q_starts, k_starts), (sizes, docs, scale)
+    return out, lse, rest
 
 
-def _attn_bwd(dout, q, k, v, q_starts, k_starts, out, lse, how, grad_dtype, need):
-    """dq, dk, dv (None where not needed)."""
-    sizes, docs, scale = how
+@torch.no_grad()
+def cross_attn_bwd_hip(dout, q, k, v, out, lse, rest=None, q_starts=None, k_starts=None, softmax_scale=None, grad_dtype=_BF,
+                       need=(True, True, True)):
+    """Gradients ``(dq, dk, dv)`` (bfloat16 or float32 by ``grad_dtype``; None where ``need`` is false) from the forward's
+    inputs and results.  Without ``rest`` rowsum(dout * out) comes from the rounded out alone, whose error shows in dq and
+    dk where rows see few keys."""
+    sizes, docs, scale, q_starts, k_starts = _check_attn(q, k, v, q_starts, k_starts, softmax_scale)
     B, Sq, Sk, H, Hk, D = sizes
-    dev = dout.device
+    dev = q.device
+    if dout.dtype != _BF or out.dtype != _BF or dout.shape != q.shape or out.shape != q.shape:
+        raise IcsaArgumentError("dout and out must be bfloat16 like q")
+    if lse.dtype != torch.float32 or lse.shape != (B, Hk, Sq, H // Hk) or not lse.is_contiguous():
+        raise IcsaArgumentError(f"lse must be float32 [{B}, {Hk}, {Sq}, {H // Hk}], contiguous")
+    if rest is not None and (rest.dtype != torch.uint8 or rest.shape != q.shape or not rest.is_contiguous()):
+        raise IcsaArgumentError("rest must be uint8 like q, contiguous")
+    if any(t is not None and t.device != dev for t in (dout, out, lse, rest)):
+        raise IcsaArgumentError("dout, out, lse and rest must be on the GPU of q")
+    if grad_dtype not in _FLOATS:
+        raise IcsaArgumentError("grad_dtype must be bfloat16 or float32")
     dout, da = _rows16(dout)
     q, qa = _rows16(q)
     k, ka = _rows16(k)
@@ -109,52 +137,11 @@ def _attn_bwd(dout, q, k, v, q_starts, k_starts, out, lse, how, grad_dtype, need
     dv = torch.empty(B, Sk, Hk, D, dtype=grad_dtype, device=dev) if need[2] else None
     qs, ks = (Sq * H * D, H * D, D), (Sk * Hk * D, Hk * D, D)
     with on_device(dev):
-        rc = L.icsa_cross_attn_bwd(*da, *qa, *ka, *va, *oa, lse.data_ptr(), *sizes, ptr(q_starts), ptr(k_starts), docs, scale,
+        rc = L.icsa_cross_attn_bwd(*da, *qa, *ka, *va, *oa, lse.data_ptr(), ptr(rest), *sizes, ptr(q_starts), ptr(k_starts), docs, scale,
                                    _FLOATS[grad_dtype], ptr(dq), *qs, ptr(dk), *ks, ptr(dv), *ks, ws.data_ptr(), ws_bytes,
                                    stream_ptr(dev))
     _lib.check("icsa_cross_attn_bwd", rc)
     return dq, dk, dv
-
-
-@torch.no_grad()
-def cross_attn_fwd_hip(q, k, v, q_starts=None, k_starts=None, softmax_scale=None):
-    """``(out, lse)`` of :func:`cross_attn_func`'s forward: out bfloat16 like q, lse float32 [B, Hk, Sq, H / Hk], log2 of each
-    row's sum of ``2 ** (score * log2 e)``, +inf for a row that sees nothing."""
-    return _attn_fwd(q, k, v, q_starts, k_starts, softmax_scale, True)[:2]
-
-
-@torch.no_grad()
-def cross_attn_bwd_hip(dout, q, k, v, out, lse, q_starts=None, k_starts=None, softmax_scale=None, grad_dtype=_BF,
-                       need=(True, True, True)):
-    """Gradients ``(dq, dk, dv)`` (bfloat16 or float32 by ``grad_dtype``; None where ``need`` is false) from the forward's
-    inputs, ``out`` and ``lse``."""
-    sizes, docs, scale, q_starts, k_starts = _check_attn(q, k, v, q_starts, k_starts, softmax_scale)
-    B, Sq, Sk, H, Hk, D = sizes
-    dev = q.device
-    if dout.dtype != _BF or out.dtype != _BF or dout.shape != q.shape or out.shape != q.shape:
-        raise IcsaArgumentError("dout and out must be bfloat16 like q")
-    if lse.dtype != torch.float32 or lse.shape != (B, Hk, Sq, H // Hk) or not lse.is_contiguous():
-        raise IcsaArgumentError(f"lse must be float32 [{B}, {Hk}, {Sq}, {H // Hk}], contiguous")
-    if dout.device != dev or out.device != dev or lse.device != dev:
-        raise IcsaArgumentError("dout, out and lse must be on the GPU of q")
-    if grad_dtype not in _FLOATS:
-        raise IcsaArgumentError("grad_dtype must be bfloat16 or float32")
-    return _attn_bwd(dout, q, k, v, q_starts, k_starts, out, lse, (sizes, docs, scale), grad_dtype, need)
-
-
-class _CrossAttn(torch.autograd.Function):
-    # The backward runs on a thread of autograd's own, where a line of Python costs about three times what it does in the
-    # forward: what was checked there is not checked again.
-    @staticmethod
-    def forward(ctx, q, k, v, q_starts, k_starts, scale):
-        out, lse, read, ctx.how = _attn_fwd(q, k, v, q_starts, k_starts, scale, True)
-        ctx.save_for_backward(*read, out, lse)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        return (*_attn_bwd(dout, *ctx.saved_tensors, ctx.how, _BF, ctx.needs_input_grad), None, None, None)
 
 
 def cross_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_starts: torch.Tensor = None,
@@ -170,102 +157,13 @@ def cross_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_star
     A query that sees nothing gets zeros; it, keys outside every document and padding take no part in any gradient and
     get zeros, whatever they and their ``dout`` hold.  A NaN or an infinity inside a document makes gradients of that
     document NaN, and reaches no other."""
-    if _wants_grad(q, k, v):
-        return _CrossAttn.apply(q, k, v, q_starts, k_starts, softmax_scale)
-    return _attn_fwd(q, k, v, q_starts, k_starts, softmax_scale, False)[0]
+    _, docs, scale, q_starts, k_starts = _check_attn(q, k, v, q_starts, k_starts, softmax_scale)
+    return _nodes().cross_attn(q, k, v, q_starts, k_starts, docs, scale)
 
 
 # ------------------------------------------------------------------------------------------
 # layer norm, RMS norm
 # ------------------------------------------------------------------------------------------
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x [..., dim] as [rows, dim] with a unit stride in each row (a view where there is one)."""
-    if x.shape[-1] != 1 and x.stride(-1) != 1:
-        x = x.contiguous()
-    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-
-
-def _row_stride(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
-
-
-def _param_rows(gain, shift, dim):
-    """Both as [G, dim] with a unit stride in each row and one group stride: (gain, shift, G, group stride)."""
-    if gain is None:
-        return None, None, 1, dim
-    g = _rows(gain)
-    if shift is None:
-        return g, None, g.shape[0], g.stride(0)
-    s = _rows(shift)
-    if g.shape[0] > 1 and g.stride(0) != s.stride(0):
-        g, s = g.contiguous(), s.contiguous()
-    return g, s, g.shape[0], g.stride(0)
-
-
-def _norm_fwd(x, gain, shift, plus_one, rms, eps, out_dtype, keep):
-    """(y, mean, rstd, x's rows); the statistics where the backward is to come."""
-    r = _rows(x)
-    n, dim = r.shape
-    g, s, groups, p_sg = _param_rows(gain, shift, dim)
-    dev = x.device
-    y = torch.empty(x.shape, dtype=out_dtype, device=dev)
-    mean = rstd = None
-    if keep:
-        rstd = torch.empty(n, dtype=torch.float32, device=dev)
-        mean = None if rms else torch.empty(n, dtype=torch.float32, device=dev)
-    with on_device(dev):
-        rc = _lib.lib().icsa_norm_fwd(
-            r.data_ptr(), _FLOATS[r.dtype], _row_stride(r), n // groups, groups, dim, ptr(g), ptr(s),
-            _lib.F32 if g is None else _FLOATS[g.dtype], p_sg, plus_one, rms, eps, y.data_ptr(), _FLOATS[out_dtype], dim,
-            ptr(mean), ptr(rstd), stream_ptr(dev))
-    _lib.check("icsa_norm_fwd", rc)
-    return y, mean, rstd, r
-
-
-class _Norm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gain, shift, plus_one, rms, eps, out_dtype):
-        y, mean, rstd, r = _norm_fwd(x, gain, shift, plus_one, rms, eps, out_dtype, True)
-        ctx.save_for_backward(r, gain, mean, rstd)
-        ctx.how = plus_one, rms, x.shape, None if shift is None else shift.shape
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        r, gain, mean, rstd = ctx.saved_tensors
-        plus_one, rms, x_shape, shift_shape = ctx.how
-        need = ctx.needs_input_grad
-        d = _rows(dy)
-        n, dim = r.shape
-        g, _, groups, p_sg = _param_rows(gain, None, dim)
-        dev = r.device
-        dx = torch.empty(x_shape, dtype=r.dtype, device=dev) if need[0] else None
-        make = torch.empty if n else torch.zeros
-        dgain = make(gain.shape, dtype=gain.dtype, device=dev) if need[1] else None
-        dshift = make(shift_shape, dtype=gain.dtype, device=dev) if need[2] else None
-        if n:
-            L = _lib.lib()
-            wsp = ws_bytes = 0
-            if need[1] or need[2]:
-                ws_bytes = L.icsa_norm_bwd_workspace_size(n // groups, groups, dim)
-                ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-                wsp = ws.data_ptr()
-            with on_device(dev):
-                rc = L.icsa_norm_bwd(
-                    d.data_ptr(), _FLOATS[d.dtype], _row_stride(d), r.data_ptr(), _FLOATS[r.dtype], _row_stride(r), n // groups,
-                    groups, dim, ptr(g), _lib.F32 if g is None else _FLOATS[g.dtype], p_sg, plus_one, rms, ptr(mean),
-                    ptr(rstd), ptr(dx), dim, ptr(dgain), ptr(dshift), wsp, ws_bytes, stream_ptr(dev))
-            _lib.check("icsa_norm_bwd", rc)
-        return dx, dgain, dshift, None, None, None, None
-
-
-def _norm(x, gain, shift, plus_one, rms, eps, out_dtype):
-    if _wants_grad(x, gain, shift):
-        return _Norm.apply(x, gain, shift, plus_one, rms, eps, out_dtype)
-    return _norm_fwd(x, gain, shift, plus_one, rms, eps, out_dtype, False)[0]
-
-
 def _check_norm(x, out_dtype, eps, *params):
     if not x.is_cuda or x.dim() < 1 or x.dtype not in _FLOATS:
         raise IcsaArgumentError("x must be bfloat16 or float32 [..., dim] on the GPU")
@@ -298,9 +196,9 @@ def layer_norm_func(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Te
             raise IcsaArgumentError("weight and bias, or scale and shift, not both")
         if weight is None or weight.shape != (dim,) or (bias is not None and bias.shape != (dim,)):
             raise IcsaArgumentError(f"weight and bias must be [{dim}], a bias beside a weight")
-        return _norm(x, weight, bias, 0, 0, eps, out_dtype)
+        return _nodes().norm(x, weight, bias, False, False, eps, out_dtype)
     if scale is None and shift is None:
-        return _norm(x, None, None, 0, 0, eps, out_dtype)
+        return _nodes().norm(x, None, None, False, False, eps, out_dtype)
     if scale is None or shift is None or scale.shape != shift.shape:
         raise IcsaArgumentError("scale and shift come together, alike in shape")
     n = scale.dim()
@@ -309,7 +207,7 @@ def layer_norm_func(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Te
         scale.numel() == x.shape[0] * dim
     if not (one or each):
         raise IcsaArgumentError(f"scale and shift must be [{dim}], [1, .., {dim}], or [B, {dim}] or [B, 1, .., {dim}] for x [B, .., {dim}]")
-    return _norm(x, scale, shift, 1, 0, eps, out_dtype)
+    return _nodes().norm(x, scale, shift, True, False, eps, out_dtype)
 
 
 def rms_norm_func(x: torch.Tensor, weight: torch.Tensor = None, *, eps: float = 1e-6, out_dtype: torch.dtype = None) -> torch.Tensor:
@@ -318,7 +216,7 @@ def rms_norm_func(x: torch.Tensor, weight: torch.Tensor = None, *, eps: float = 
     rounded once, to ``out_dtype`` (default x's type)."""
     dim, eps, out_dtype = _check_norm(x, out_dtype, eps, weight)
     _require(weight is None or weight.shape == (dim,), f"weight must be [{dim}]")
-    return _norm(x, weight, None, 0, 1, eps, out_dtype)
+    return _nodes().norm(x, weight, None, False, True, eps, out_dtype)
 
 
 # ------------------------------------------------------------------------------------------
@@ -355,52 +253,6 @@ def rotary_table(positions: int, rotary_dim: int, theta: float = 10000.0, *, sca
     return (torch.cos(ang) * gain).float(), (torch.sin(ang) * gain).float()
 
 
-def _rotate(q, k, cos, sin, positions, sections, interleaved, backward):
-    """Both tensors turned (k may be None), new and contiguous."""
-    dev = q.device
-    B, S, _, D = q.shape
-    ys = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k)]
-    args = []
-    for t, y in zip((q, k), ys):
-        args += (0, 0, 0, 0, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:3], t.shape[2], y.data_ptr())
-    axes, sec = 1, None
-    if sections is not None:
-        axes = len(sections)
-        sec = ctypes.cast((ctypes.c_int32 * axes)(*sections), ctypes.c_void_p)
-    pos_sb = positions.stride(0) if positions.dim() == (2 if sections is None else 3) else 0
-    with on_device(dev):
-        rc = _lib.lib().icsa_rotary(*args, _FLOATS[q.dtype], B, S, D, 2 * cos.shape[1], interleaved, backward,
-                                    positions.data_ptr(), pos_sb, axes, sec, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-                                    stream_ptr(dev))
-    _lib.check("icsa_rotary", rc)
-    return ys
-
-
-def _unit_last(t):
-    return t if t is None or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, sections, interleaved):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(cos, sin, positions)
-        ctx.how = sections, interleaved
-        out = _rotate(q, k, cos, sin, positions, sections, interleaved, 0)
-        return out[0] if k is None else tuple(out)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk=None):
-        cos, sin, positions = ctx.saved_tensors
-        dq, dk = (_unit_last(t) if need else None for t, need in zip((dq, dk), ctx.needs_input_grad))
-        if dq is None and dk is not None:
-            dk = _rotate(dk, None, cos, sin, positions, *ctx.how, 1)[0]
-        elif dq is not None:
-            dq, dk = _rotate(dq, dk, cos, sin, positions, *ctx.how, 1)
-        return dq, dk, None, None, None, None, None
-
-
 def rotary_func(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, *,
                 sections=None, interleaved: bool = True):
     """q [B, S, H, D] and k [B, S, Hk, D] (or None), bfloat16 or float32, turned by their tokens' angles in one launch, with
@@ -423,7 +275,7 @@ def rotary_func(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.
         raise IcsaArgumentError("cos and sin must be float32 [P, R / 2] on the GPU of q")
     if not 1 <= cos.shape[1] <= D // 2:
         raise IcsaArgumentError(f"the tables' R / 2 columns must be 1 to {D // 2}")
-    if _wants_grad(cos, sin):
+    if (cos.requires_grad or sin.requires_grad) and torch.is_grad_enabled():
         raise IcsaArgumentError("the tables have no gradient")
     want = (S,)
     if sections is not None:
@@ -433,10 +285,7 @@ def rotary_func(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.
         want = (S, len(sections))
     if positions.dtype != torch.int32 or positions.device != dev or positions.shape not in (want, (B, *want)):
         raise IcsaArgumentError(f"positions must be int32 {[*want]} or {[B, *want]} on the GPU of q")
-    cos, sin, positions = cos.contiguous(), sin.contiguous(), positions.contiguous()
-    if _wants_grad(q, k):
-        return _Rotary.apply(_unit_last(q), _unit_last(k), cos, sin, positions, sections, int(interleaved))
-    out = _rotate(_unit_last(q), _unit_last(k), cos, sin, positions, sections, int(interleaved), 0)
+    out = _nodes().rotary(q, k, cos, sin, positions, sections or (), bool(interleaved))
     return out[0] if k is None else tuple(out)
 
 

@@ -175,7 +175,7 @@ def test_the_attentions_pair_in_a_graph(gpu):
     """Parts joined (few queries over many keys, few keys under many queries)."""
     for Sq, Sk in ((3, 2500), (2500, 3)):
         q, k, v, do = (torch.randn(1, n, 4, 64, device=gpu).to(BF) for n in (Sq, Sk, Sk, Sq))
-        run = lambda: (lambda o, l: (o, *cross_attn_bwd_hip(do, q, k, v, o, l)))(*cross_attn_fwd_hip(q, k, v))
+        run = lambda: (lambda o, *s: (o, *cross_attn_bwd_hip(do, q, k, v, o, *s)))(*cross_attn_fwd_hip(q, k, v))
         run()
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())

@@ -16,7 +16,7 @@ EIN, EUN, EWS = _lib.EINVAL, _lib.EUNSUPPORTED, _lib.EWORKSPACE
 
 def _fwd(**kw):
     a = dict(q=PTR, q_sb=0, q_ss=128, q_sh=128, k=PTR, k_sb=0, k_ss=128, k_sh=128, v=PTR, v_sb=0, v_ss=128, v_sh=128,
-             B=1, Sq=8, Sk=8, H=1, Hk=1, D=128, qst=0, kst=0, docs=1, scale=0.1, out=PTR, o_sb=0, o_ss=128, o_sh=128, lse=PTR,
+             B=1, Sq=8, Sk=8, H=1, Hk=1, D=128, qst=0, kst=0, docs=1, scale=0.1, out=PTR, o_sb=0, o_ss=128, o_sh=128, lse=PTR, rest=PTR,
              ws=0, wsb=0, stream=0)
     a.update(kw)
     return _lib.lib().icsa_cross_attn_fwd(*a.values())
@@ -24,7 +24,7 @@ def _fwd(**kw):
 
 def _bwd(**kw):
     a = dict(do=PTR, do_sb=0, do_ss=128, do_sh=128, q=PTR, q_sb=0, q_ss=128, q_sh=128, k=PTR, k_sb=0, k_ss=128, k_sh=128,
-             v=PTR, v_sb=0, v_ss=128, v_sh=128, out=PTR, o_sb=0, o_ss=128, o_sh=128, lse=PTR,
+             v=PTR, v_sb=0, v_ss=128, v_sh=128, out=PTR, o_sb=0, o_ss=128, o_sh=128, lse=PTR, rest=PTR,
              B=1, Sq=8, Sk=8, H=1, Hk=1, D=128, qst=0, kst=0, docs=1, scale=0.1, gd=_lib.BF16,
              dq=PTR, dq_sb=0, dq_ss=128, dq_sh=128, dk=PTR, dk_sb=0, dk_ss=128, dk_sh=128, dv=PTR, dv_sb=0, dv_ss=128, dv_sh=128,
              ws=PTR, wsb=1 << 30, stream=0)
@@ -35,7 +35,7 @@ def _bwd(**kw):
 @pytest.mark.parametrize("kw,code", [
     (dict(B=0), EIN), (dict(H=3, Hk=2), EIN), (dict(D=96), EUN), (dict(docs=0), EIN), (dict(docs=2), EIN), (dict(qst=PTR), EIN),
     (dict(scale=0.0), EIN), (dict(scale=float("nan")), EIN), (dict(q=0), EIN), (dict(k=0), EIN), (dict(q=PTR + 2), EIN),
-    (dict(k_ss=129), EIN), (dict(Sk=(1 << 30) + 1), EUN), (dict(Sq=(1 << 30) + 1), EUN),
+    (dict(k_ss=129), EIN), (dict(rest=PTR + 8), EIN), (dict(Sk=(1 << 30) + 1), EUN), (dict(Sq=(1 << 30) + 1), EUN),
 ])
 def test_cross_attention_refuses(kw, code):
     assert _fwd(**kw) == code and _lib.lib().icsa_last_error()
