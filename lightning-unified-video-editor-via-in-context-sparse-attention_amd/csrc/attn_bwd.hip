@@ -118,15 +118,21 @@ __global__ void __launch_bounds__(AB_THREADS, 2) icsa_attn_bwd_kernel(AttnBwdPar
   if constexpr (!KV) {                                                    // D = rowsum(dO * O), f32
     const bf16* so = p.o + row_at(p.o_sb, p.o_ss, p.o_sh, b, hk, p.by_g, rc) + 8 * hl;
     lse = p.lse[(int64_t)bh * n_q + rc];
-    const unsigned char* sr = p.rest == nullptr ? nullptr
-        : p.rest + row_at((int64_t)p.Sq * p.H * D, (int64_t)p.H * D, D, b, hk, p.by_g, rc) + 8 * hl;
+    u32x4 rest[kSteps / 2];                                               // 16 bytes: two steps' (rest_at)
+    if (p.rest != nullptr) {
+      const unsigned char* sr = p.rest + row_at((int64_t)p.Sq * p.H * D, (int64_t)p.H * D, D, b, hk, p.by_g, rc) + hl * (D / 2);
+#pragma unroll
+      for (int i = 0; i < kSteps / 2; ++i) rest[i] = *reinterpret_cast<const u32x4*>(sr + 16 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSteps / 2; ++i) rest[i] = u32x4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+    }
 #pragma unroll
     for (int kk = 0; kk < kSteps; ++kk) {
       const bf16x8 o = *reinterpret_cast<const bf16x8*>(so + 16 * kk);
-      u32x2 w = {0x80808080u, 0x80808080u};                               // nothing
-      if (sr != nullptr) w = *reinterpret_cast<const u32x2*>(sr + 16 * kk);
+      const int at = (kk & 1) * (kSteps / 2) + (kk >> 1);                 // its eight bytes
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dd = fmaf((float)b2[kk][e], with_rest(o[e], w[e >> 2], e & 3), dd);
+      for (int e = 0; e < 8; ++e) dd = fmaf((float)b2[kk][e], with_rest(o[e], rest[at >> 1][2 * (at & 1) + (e >> 2)], e & 3), dd);
     }
     dd = xhalf_sum(dd);
     if (split == 0 && hl == 0 && r < n_st) {                              // what the key-major kernel's accumulators start with

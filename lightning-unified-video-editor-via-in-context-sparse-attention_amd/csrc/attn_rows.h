@@ -121,40 +121,31 @@ __device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? I
 // from both: from the rounded O alone D's error, a row's common shift of dP, is as large as dS's own rounding where a row's weight
 // lies on few keys (77 keys: dq 0.0026 from the exact one in the 2-norm, 0.0024 with the byte, 0.0017 is the results' rounding alone; 8 keys:
 // 0.0029 and 0.0025; 3 keys: 0.0036 and 0.0025).
-__device__ __forceinline__ unsigned rest_byte(float o, bf16 b) {
-  const float f = (float)b;
-  const int e = (int)(__float_as_uint(f) >> 23 & 255u);
-  return (unsigned)((int)__builtin_rintf(fminf(fmaxf(__builtin_amdgcn_ldexpf(o - f, 142 - e), -127.f), 127.f)) + 128);
-}
+// A row's bytes lie in the order in which the backward's lanes read them: rest_at of a dim.
 __device__ __forceinline__ unsigned rest_bytes(const float o[4]) {
   unsigned w = 0u;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) w |= rest_byte(o[e], (bf16)o[e]) << (8 * e);
+  for (int e = 0; e < 4; ++e) {
+    const float f = (float)(bf16)o[e];
+    // 2^15 over f's power of two; what this is not for (values under 2^-112, infinities) has a byte that moves nothing
+    const float up = __uint_as_float(0x86800000u - (__float_as_uint(f) & 0x7f800000u));
+    w = __builtin_amdgcn_cvt_pk_u8_f32(fmaf(o[e] - f, up, 128.f), e, w);  // to a whole number, 0 to 255
+  }
   return w;
 }
 // and back: byte e of w beside b
 __device__ __forceinline__ float with_rest(bf16 b, unsigned w, int e) {
-  const float f = (float)b;
-  const int x = (int)(__float_as_uint(f) >> 23 & 255u) - 15;              // a 256th of the last place is 2^(x - 127)
-  const float step = x > 0 ? __uint_as_float((unsigned)x << 23) : 0.f;
-  return fmaf((float)((w >> (8 * e)) & 255u) - 128.f, step, f);
+  const float f = (float)b, power = __uint_as_float(__float_as_uint(f) & 0x7f800000u), t = (float)((w >> (8 * e)) & 255u);
+  return fmaf(fmaf(t, 0x1p-15f, -0x1p-8f), power, f);
+}
+template <int D> __device__ __forceinline__ int rest_at(int dim) {
+  return ((dim >> 3) & 1) * (D / 2) + ((dim >> 4) & 1) * (D / 4) + (dim >> 5) * 8 + (dim & 7);
 }
 
 // element offset of row r (query r / G, head hk G + r % G) in a [B, S, H, D] tensor
 __device__ __forceinline__ int64_t row_at(int64_t sb, int64_t ss, int64_t sh, int b, int hk, const FastDiv& g, int r) {
   const unsigned i = g.d == 1 ? r : g.div(r);
   return (int64_t)b * sb + (int64_t)i * ss + (int64_t)(hk * g.d + r - i * g.d) * sh;
-}
-
-// The rest bytes of one wave's 32 rows of 32 dims: dims 16 hl .. + 15 of row li in one store (v as in store_dims32)
-__device__ __forceinline__ void store_rest32(const float v[16], int rows_valid, unsigned char* row) {
-  const int lane = threadIdx.x & 63, li = lane & 31, hl = lane >> 5;
-  unsigned w[4];
-#pragma unroll
-  for (int g = 0; g < 4; ++g) w[g] = rest_bytes(v + 4 * g);
-  const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
-  const auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
-  if (li < rows_valid) *reinterpret_cast<u32x4*>(row + 16 * hl) = u32x4{a[0], a[1], b[0], b[1]};
 }
 
 // rest: [B, S, H, D] bytes like a contiguous output, or null
@@ -172,10 +163,32 @@ __device__ __forceinline__ void store_wave(const OutView& out, const FastDiv& by
     float v[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = o[ds][e] * inv_l;
-    if (rest != nullptr)
-      store_rest32(v, rows_valid, rest + row_at((int64_t)Sq * H * D, (int64_t)H * D, D, b, hk, by_g, r0 + li) + 32 * ds);
     if (out.dtype == ICSA_DT_BF16) store_dims32<1>(stage, v, rows_valid, off, own, out.p, 32 * ds);
     else store_dims32<0>(stage, v, rows_valid, off, own, out.p, 32 * ds);
+  }
+  if (rest == nullptr) return;
+  // dims 32 ds + 16 hl .. + 15 of row li in a lane: eight bytes for either half of the backward's lanes
+  const int hl = lane >> 5;
+  u32x2 first[D / 32], second[D / 32];
+#pragma unroll
+  for (int ds = 0; ds < D / 32; ++ds) {
+    unsigned w[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float v[4] = {o[ds][4 * g] * inv_l, o[ds][4 * g + 1] * inv_l, o[ds][4 * g + 2] * inv_l, o[ds][4 * g + 3] * inv_l};
+      w[g] = rest_bytes(v);
+    }
+    const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    first[ds] = u32x2{x[0], x[1]};
+    second[ds] = u32x2{y[0], y[1]};
+  }
+  if (li >= rows_valid) return;
+  unsigned char* dst = rest + row_at((int64_t)Sq * H * D, (int64_t)H * D, D, b, hk, by_g, r0 + li) + hl * (D / 4);
+#pragma unroll
+  for (int ds = 0; ds < D / 32; ds += 2) {
+    *reinterpret_cast<u32x4*>(dst + 8 * ds) = u32x4{first[ds][0], first[ds][1], first[ds + 1][0], first[ds + 1][1]};
+    *reinterpret_cast<u32x4*>(dst + D / 2 + 8 * ds) = u32x4{second[ds][0], second[ds][1], second[ds + 1][0], second[ds + 1][1]};
   }
 }
 

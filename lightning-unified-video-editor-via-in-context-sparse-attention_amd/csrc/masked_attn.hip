@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(256) icsa_masked_combine_kernel(MaskedAttnPara
   if (p.rest != nullptr) {
     const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
     *reinterpret_cast<unsigned*>(p.rest + row_at((int64_t)p.Sq * p.H * D, (int64_t)p.H * D, D, p.by_hk.div(bh), p.by_hk.mod(bh), p.by_g, r) +
-                                 4 * t) = rest_bytes(v);
+                                 rest_at<D>(4 * t)) = rest_bytes(v);
   }
   if (p.out.dtype == ICSA_DT_BF16) {
     bf16x4 y;
