@@ -35,7 +35,7 @@
 #define AB_WAVES 4
 #define AB_ROWS (32 * AB_WAVES)                         // held by a workgroup
 #define AB_AHEAD 3                                    // operands read ahead of their products
-#define AB_SCRATCH_WAVE 3072                          // staged output rows, at most 2 KB; in the loop: ranges, operands
+#define AB_SCRATCH_WAVE (3 * 1024)                    // staged output rows, at most 2 KB; in the loop: ranges, operands
 #define AB_CTL_BYTES 256
 #define AB_LOG2E 1.4426950408889634f
 
@@ -76,8 +76,9 @@ template <int D> constexpr int ab_lds() { return 4 * BTile<D>::kBytes + 2 * 512 
 
 }  // namespace
 
-template <int D, bool KV>
-__global__ void __launch_bounds__(AB_THREADS, 2) icsa_attn_bwd_kernel(AttnBwdParams p) {
+// FINE: P and dS as two bf16 each, where the queries are one tile
+template <int D, bool KV, bool FINE>
+__global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : 2) icsa_attn_bwd_kernel(AttnBwdParams p) {
   typedef BTile<D> T;
   constexpr int kSteps = D / 16, kSub = D / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(AB_THREADS, 2) icsa_attn_bwd_kernel(AttnBwdPar
   if constexpr (!KV) asm volatile("" : "+v"(lse), "+v"(dd));
   // Key-major with 128 dims the registers are two operands short; what the compiler spills it reloads behind a wait for all loads
   // in flight, the next tile's too.  Both sides' first operand lies in the wave's LDS instead.
-  constexpr bool kLent = KV && D == 128;
+  constexpr bool kLent = KV && D == 128 && !FINE;
   bf16x8* const lent = reinterpret_cast<bf16x8*>(scratch_all + wave * AB_SCRATCH_WAVE + 1024) + lane;
   if constexpr (kLent) { lent[0] = b1[0]; lent[64] = b2[0]; }
   if (t0 < t1) load_tile(t0);
@@ -302,6 +303,7 @@ __global__ void __launch_bounds__(AB_THREADS, 2) icsa_attn_bwd_kernel(AttnBwdPar
     floatx16 s[2], dp[2];
     bf16x8 first[2], second[2];
     bf16x8 pf[2][2], df[2][2];
+    bf16x8 pl[2][2], dl[2][2];                                            // FINE: what the roundings leave
     bf16x8 a[kOps];
     auto op = [&](int x) __attribute__((always_inline)) {
       const int what = kWhat[x / kSteps], sub = kOf[x / kSteps], i = x % kSteps;
@@ -316,13 +318,20 @@ __global__ void __launch_bounds__(AB_THREADS, 2) icsa_attn_bwd_kernel(AttnBwdPar
         a[x] = __builtin_bit_cast(bf16x8, a8);
       }
     };
-    // P and dS rounded to bf16, the matrix instruction's type (2^-8 of a weight at most), as in the forward
+    // P and dS rounded to bf16, the matrix instruction's type (2^-8 of a weight at most), as in the forward: over many queries
+    // that is as much again as the results' own rounding leaves.  Over a few, one weight's error can be most of a
+    // result's, and the products are no time at all: FINE adds what the rounding left.
     auto weights = [&](int sub, int e) __attribute__((always_inline)) {
       s[sub][e] = __builtin_amdgcn_exp2f(KV ? s[sub][e] * c : fmaf(s[sub][e], c, -lse));
-      if constexpr (KV) pf[sub][e >> 3][e & 7] = (bf16)s[sub][e];
+      if constexpr (KV) {
+        pf[sub][e >> 3][e & 7] = (bf16)s[sub][e];
+        if constexpr (FINE) pl[sub][e >> 3][e & 7] = (bf16)(s[sub][e] - (float)pf[sub][e >> 3][e & 7]);
+      }
     };
     auto slopes = [&](int sub, int e) __attribute__((always_inline)) {
-      df[sub][e >> 3][e & 7] = (bf16)(s[sub][e] * (KV ? dp[sub][e] : dp[sub][e] - dd));
+      const float x = s[sub][e] * (KV ? dp[sub][e] : dp[sub][e] - dd);
+      df[sub][e >> 3][e & 7] = (bf16)x;
+      if constexpr (FINE) dl[sub][e >> 3][e & 7] = (bf16)(x - (float)df[sub][e >> 3][e & 7]);
     };
     auto clear = [&](bf16x8 (&w)[2], int sub) __attribute__((always_inline)) {
       const int wd = (int)(unsigned)((visible() & ~cleared()) >> (32 * sub + 4 * hl));
@@ -363,6 +372,10 @@ __global__ void __launch_bounds__(AB_THREADS, 2) icsa_attn_bwd_kernel(AttnBwdPar
       else if (what == 1) dp[sub] = mfma32x32x16(a[x], i == 0 ? second[sub] : b2[i], dp[sub]);
       else if (what == 2) acc2[i % kSub] = mfma32x32x16(a[x], pf[sub][i / kSub], acc2[i % kSub]);
       else acc1[i % kSub] = mfma32x32x16(a[x], df[sub][i / kSub], acc1[i % kSub]);
+      if constexpr (FINE) {
+        if (what == 2) acc2[i % kSub] = mfma32x32x16(a[x], pl[sub][i / kSub], acc2[i % kSub]);
+        if (what == 3) acc1[i % kSub] = mfma32x32x16(a[x], dl[sub][i / kSub], acc1[i % kSub]);
+      }
 #pragma unroll
       for (int e = i * kEl; e < (i + 1) * kEl; ++e) {
         if (KV) {
@@ -383,9 +396,11 @@ __global__ void __launch_bounds__(AB_THREADS, 2) icsa_attn_bwd_kernel(AttnBwdPar
         if (KV) {
           if (what == 1) clear(pf[sub], sub);
           if (what == (kSpread ? 2 : 1)) clear(df[sub], sub);
+          if (FINE && what == 1) clear(pl[sub], sub);
+          if (FINE && what == (kSpread ? 2 : 1)) clear(dl[sub], sub);
         } else {
-          if (ph == 2) clear(df[0], 0);
-          else if (ph == 4) clear(df[1], 1);
+          if (ph == 2 || ph == 4) clear(df[ph / 4], ph / 4);
+          if (FINE && (ph == 2 || ph == 4)) clear(dl[ph / 4], ph / 4);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -459,6 +474,7 @@ __global__ void __launch_bounds__(256) icsa_attn_bwd_join_kernel(AttnBwdParams p
 
 #define AB_SLOTS 512                                  // workgroups that the chip holds: two a CU
 #define AB_MAX_SPLIT 64
+#define AB_FINE 64                                    // queries (of a key head's group) up to which P and dS are two bf16
 #define AB_MIN_TILES 8                                // of the walked side that a part is worth
 
 namespace {
@@ -481,12 +497,12 @@ int parts(int64_t items, int64_t tiles, int docs, int slots) {
 
 int64_t blocks(int64_t rows) { return (rows + AB_ROWS - 1) / AB_ROWS; }
 
-template <int D>
+template <int D, bool FINE>
 hipError_t run_bwd(const AttnBwdParams& p, hipStream_t stream) {
   static std::atomic<unsigned> set_q{0u}, set_k{0u};
-  hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(icsa_attn_bwd_kernel<D, false>), ab_lds<D>(), &set_q);
+  hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(icsa_attn_bwd_kernel<D, false, FINE>), ab_lds<D>(), &set_q);
   if (e != hipSuccess) return e;
-  e = ensure_lds_limit(reinterpret_cast<const void*>(icsa_attn_bwd_kernel<D, true>), ab_lds<D>(), &set_k);
+  e = ensure_lds_limit(reinterpret_cast<const void*>(icsa_attn_bwd_kernel<D, true, FINE>), ab_lds<D>(), &set_k);
   if (e != hipSuccess) return e;
   const int64_t BH = (int64_t)p.B * p.Hk, n_q = (int64_t)p.Sq * (p.H / p.Hk);
   const int64_t wq = BH * blocks(n_q) * p.q_split, wk = BH * blocks(p.Sk) * p.k_split;
@@ -494,7 +510,7 @@ hipError_t run_bwd(const AttnBwdParams& p, hipStream_t stream) {
   if (wq > 0x3fffffffLL || wk > 0x3fffffffLL || (p.q_split > 1 && jq > 0x7fffffffLL) || (p.k_split > 1 && jk > 0x7fffffffLL))
     return hipErrorInvalidValue;
   if (wq > 0) {                                       // without queries dk and dv are zeros, which the key-major kernel writes
-    hipLaunchKernelGGL((icsa_attn_bwd_kernel<D, false>), dim3(xcd_grid((int)wq)), dim3(AB_THREADS), ab_lds<D>(), stream, p);
+    hipLaunchKernelGGL((icsa_attn_bwd_kernel<D, false, FINE>), dim3(xcd_grid((int)wq)), dim3(AB_THREADS), ab_lds<D>(), stream, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (p.q_split > 1 && p.dq.p != nullptr) {
@@ -502,7 +518,7 @@ hipError_t run_bwd(const AttnBwdParams& p, hipStream_t stream) {
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (p.dk.p == nullptr && p.dv.p == nullptr) return hipSuccess;
-  hipLaunchKernelGGL((icsa_attn_bwd_kernel<D, true>), dim3(xcd_grid((int)wk)), dim3(AB_THREADS), ab_lds<D>(), stream, p);
+  hipLaunchKernelGGL((icsa_attn_bwd_kernel<D, true, FINE>), dim3(xcd_grid((int)wk)), dim3(AB_THREADS), ab_lds<D>(), stream, p);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   if (p.k_split > 1) hipLaunchKernelGGL((icsa_attn_bwd_join_kernel<D, true>), dim3((unsigned)jk, 2), dim3(256), 0, stream, p);
   return hipGetLastError();
@@ -522,5 +538,6 @@ hipError_t launch_attn_bwd(AttnBwdParams p, hipStream_t stream) {
   p.by_hk = fast_div(p.Hk);
   p.by_qblk = fast_div((unsigned)std::max<int64_t>(1, blocks((int64_t)p.Sq * G)));
   p.by_kblk = fast_div((unsigned)std::max<int64_t>(1, blocks(p.Sk)));
-  return p.D == 128 ? run_bwd<128>(p, stream) : run_bwd<64>(p, stream);
+  if ((int64_t)p.Sq * G <= AB_FINE) return p.D == 128 ? run_bwd<128, true>(p, stream) : run_bwd<64, true>(p, stream);
+  return p.D == 128 ? run_bwd<128, false>(p, stream) : run_bwd<64, false>(p, stream);
 }

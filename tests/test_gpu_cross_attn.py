@@ -225,6 +225,46 @@ def test_few_keys_and_what_the_rounding_left(gpu, D):
     assert torch.equal(out, v.expand_as(out)) and (rest == 128).all()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq,H,Hk", [(1, 3, 3), (64, 2, 2), (21, 6, 2)])
+def test_few_queries_keep_the_weights(gpu, Sq, H, Hk, D):
+    """Up to 64 rows of a key head take P and dS as two bf16.  What is left of their rounding is in the forward's totals and results:
+    over 600 keys with scores of deviation 1.5, sqrt(sum p^2) is about sqrt(e^2.25 / 600) = 0.13, so of a half step of
+    2^-8 (2^-8 / sqrt 3 of a deviation) 0.13 or 3e-4 reaches a row's total and as much its D; one bf16 would leave 1.7e-3 (2-norms)."""
+    x = _inputs(1, Sq, 600, H, Hk, D, Sq)
+    got = _check(gpu, *x, grad_dtype=torch.float32)
+    val, _ = O.cross_attention(*x)
+    for n, a in zip(NAMES[1:], got[1:]):
+        assert (a.double().cpu() - val[n]).norm() < 2.0 ** -10 * val[n].norm(), n
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [1, 3])
+@pytest.mark.parametrize("qs,ks", [([[0, 5, 5, 19]], [[0, 80, 90, 200]]), ([[2, 7, 15]], [[3, 90, 170]]), ([[0, 21], [0, 1], [0, 0]], [[0, 77], [0, 210], [0, 210]])])
+def test_documents_of_few_queries(gpu, qs, ks, G, D):
+    _check(gpu, *_inputs(len(qs), 21, 210, 2 * G, 2, D, G), _i32(qs), _i32(ks))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_few_queries_and_what_is_not_finite(gpu, bad, D):
+    """As with many: outside the documents it reaches nothing, inside one it stays there."""
+    qs, ks = _i32([[2, 20, 40]]), _i32([[3, 70, 140]])
+    x = _inputs(1, 44, 150, 2, 2, D)
+    clean = _run(gpu, *x, qs, ks)
+    q, k, v, do = (t.clone() for t in x)
+    for t, lo, hi in ((q, 2, 40), (k, 3, 140), (v, 3, 140), (do, 2, 40)):
+        t[:, :lo], t[:, hi:] = bad, bad
+    assert all(torch.equal(a, b) for a, b in zip(clean, _run(gpu, q, k, v, do, qs, ks)))
+    do[0, 30, 1, 5] = bad                                    # document 1, head 1
+    dirty = _run(gpu, q, k, v, do, qs, ks)
+    for n, a, b in zip(NAMES, clean, dirty):
+        assert torch.equal(a[:, :, 0], b[:, :, 0]), n
+        end = 20 if n in ("out", "dq") else 70
+        assert torch.equal(a[:, :end], b[:, :end]), n
+    assert dirty[1][0, 30, 1].isnan().all() and dirty[2][0, 70:140, 1].isnan().all() and not dirty[3][0, 70:140, 1, 5].isfinite().any()
+
+
 def test_autograd(gpu):
     """Shared key heads, a key tensor broadcast over the batch (its gradient is the sum), a query that needs none, and the
     forward's value, which is masked_attn_func's."""
