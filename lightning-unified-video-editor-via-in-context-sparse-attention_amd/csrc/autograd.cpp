@@ -27,6 +27,7 @@ struct Api {
   decltype(&icsa_last_error) last_error = nullptr;
   decltype(&icsa_cross_attn_workspace_size) attn_workspace;
   decltype(&icsa_cross_attn_fwd) attn_fwd;
+  decltype(&icsa_cross_attn_wants_rest) attn_wants_rest;
   decltype(&icsa_cross_attn_bwd_workspace_size) attn_bwd_workspace;
   decltype(&icsa_cross_attn_bwd) attn_bwd;
   decltype(&icsa_norm_fwd) norm_fwd;
@@ -45,6 +46,7 @@ void bind(const std::string& path, py::object error) {
   };
   get(api.attn_workspace, "icsa_cross_attn_workspace_size");
   get(api.attn_fwd, "icsa_cross_attn_fwd");
+  get(api.attn_wants_rest, "icsa_cross_attn_wants_rest");
   get(api.attn_bwd_workspace, "icsa_cross_attn_bwd_workspace_size");
   get(api.attn_bwd, "icsa_cross_attn_bwd");
   get(api.norm_fwd, "icsa_norm_fwd");
@@ -127,7 +129,7 @@ Tensor attn_forward(const Rows& q, const Rows& k, const Rows& v, const Tensor& q
   Tensor out = at::empty({z.B, z.Sq, z.H, z.D}, q.t.options());
   if (lse != nullptr) {
     *lse = at::empty({z.B, z.Hk, z.Sq, z.H / z.Hk}, q.t.options().dtype(at::kFloat));
-    *rest = at::empty({z.B, z.Sq, z.H, z.D}, q.t.options().dtype(at::kByte));
+    if (api.attn_wants_rest(z.Sq, z.Sk, z.H, z.Hk, qs.defined())) *rest = at::empty({z.B, z.Sq, z.H, z.D}, q.t.options().dtype(at::kByte));
   }
   const int64_t bytes = api.attn_workspace(z.B, z.Sq, z.Sk, z.H, z.Hk, z.D, (int)docs);
   check("icsa_cross_attn_workspace_size", bytes);
@@ -136,7 +138,7 @@ Tensor attn_forward(const Rows& q, const Rows& k, const Rows& v, const Tensor& q
         api.attn_fwd(q.p, q.sb, q.ss, q.sh, k.p, k.sb, k.ss, k.sh, v.p, v.sb, v.ss, v.sh, z.B, z.Sq, z.Sk, z.H, z.Hk, z.D,
                      (const int32_t*)at_or_null(qs), (const int32_t*)at_or_null(ks), (int)docs, (float)scale, out.data_ptr(),
                      (int64_t)z.Sq * z.H * z.D, (int64_t)z.H * z.D, z.D, lse ? (float*)lse->data_ptr() : nullptr,
-                     rest ? rest->data_ptr() : nullptr, at_or_null(ws), bytes, stream_of(out)));
+                     rest ? at_or_null(*rest) : nullptr, at_or_null(ws), bytes, stream_of(out)));
   return out;
 }
 
@@ -159,7 +161,7 @@ struct CrossAttn : public torch::autograd::Function<CrossAttn> {
       at::NoGradGuard none;
       c10::DeviceGuard guard(grads[0].device());
       const Rows g = rows16(grads[0]), q = rows16(s[0]), k = rows16(s[1]), v = rows16(s[2]), o = rows16(s[5]);
-      const Tensor lse = s[6].contiguous(), rest = s[7].contiguous(), qs = s[3].defined() ? s[3].contiguous() : s[3],
+      const Tensor lse = s[6].contiguous(), rest = s[7].defined() ? s[7].contiguous() : s[7], qs = s[3].defined() ? s[3].contiguous() : s[3],
                    ks = s[4].defined() ? s[4].contiguous() : s[4];
       const AttnSizes z = attn_sizes(q.t, k.t);
       const int docs = (int)ctx->saved_data["docs"].toInt();
@@ -173,7 +175,7 @@ struct CrossAttn : public torch::autograd::Function<CrossAttn> {
       const int64_t qss = (int64_t)z.H * z.D, kss = (int64_t)z.Hk * z.D;
       check("icsa_cross_attn_bwd",
             api.attn_bwd(g.p, g.sb, g.ss, g.sh, q.p, q.sb, q.ss, q.sh, k.p, k.sb, k.ss, k.sh, v.p, v.sb, v.ss, v.sh, o.p, o.sb, o.ss, o.sh,
-                         (const float*)lse.data_ptr(), rest.data_ptr(), z.B, z.Sq, z.Sk, z.H, z.Hk, z.D,
+                         (const float*)lse.data_ptr(), at_or_null(rest), z.B, z.Sq, z.Sk, z.H, z.Hk, z.D,
                          (const int32_t*)at_or_null(qs), (const int32_t*)at_or_null(ks), docs,
                          (float)ctx->saved_data["scale"].toDouble(), ICSA_BF16, at_or_null(res[0]), z.Sq * qss, qss, z.D,
                          at_or_null(res[1]), z.Sk * kss, kss, z.D, at_or_null(res[2]), z.Sk * kss, kss, z.D, at_or_null(ws), bytes,

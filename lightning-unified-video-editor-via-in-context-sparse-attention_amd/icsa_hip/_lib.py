@@ -51,7 +51,8 @@ EXPORTS = [
     "icsa_mx_codes_size", "icsa_mx_scales_size", "icsa_mx_quantize", "icsa_mx_dequantize",
     "icsa_mx_linear_workspace_size", "icsa_mx_linear",
     "icsa_masked_attn_workspace_size", "icsa_masked_attn",
-    "icsa_cross_attn_workspace_size", "icsa_cross_attn_fwd", "icsa_cross_attn_bwd_workspace_size", "icsa_cross_attn_bwd",
+    "icsa_cross_attn_workspace_size", "icsa_cross_attn_fwd", "icsa_cross_attn_wants_rest",
+    "icsa_cross_attn_bwd_workspace_size", "icsa_cross_attn_bwd",
     "icsa_norm_fwd", "icsa_norm_bwd_workspace_size", "icsa_norm_bwd", "icsa_rotary",
 ]
 
@@ -204,6 +205,7 @@ _SIGNATURES = {
         _p, _p, _i, _f,
         _p, _l, _l, _l, _p, _p,
         _p, _l, _p]),
+    "icsa_cross_attn_wants_rest": (_i, [_i, _i, _i, _i, _i]),
     "icsa_cross_attn_bwd_workspace_size": (_l, [_i, _i, _i, _i, _i, _i, _i]),
     "icsa_cross_attn_bwd": (_i, [
         _p, _l, _l, _l,

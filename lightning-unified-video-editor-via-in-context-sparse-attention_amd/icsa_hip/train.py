@@ -79,17 +79,18 @@ def _check_attn(q, k, v, q_starts, k_starts, softmax_scale):
 @torch.no_grad()
 def cross_attn_fwd_hip(q, k, v, q_starts=None, k_starts=None, softmax_scale=None):
     """``(out, lse, rest)`` of :func:`cross_attn_func`'s forward: out bfloat16 like q; lse float32 [B, Hk, Sq, H / Hk], log2 of each
-    row's sum of ``2 ** (score * log2 e)``, +inf for a row that sees nothing; rest uint8 like out, what its rounding left."""
+    row's sum of ``2 ** (score * log2 e)``, +inf for a row that sees nothing; rest uint8 like out, what its rounding
+    left, or None where that does not show in a gradient (over 256 keys without documents, and over 64 queries)."""
     sizes, docs, scale, q_starts, k_starts = _check_attn(q, k, v, q_starts, k_starts, softmax_scale)
-    B, Sq, _, H, Hk, D = sizes
+    B, Sq, Sk, H, Hk, D = sizes
     dev = q.device
     q, qa = _rows16(q)
     k, ka = _rows16(k)
     v, va = _rows16(v)
     out = torch.empty(B, Sq, H, D, dtype=_BF, device=dev)
-    rest = torch.empty(B, Sq, H, D, dtype=torch.uint8, device=dev)
     lse = torch.empty(B, Hk, Sq, H // Hk, dtype=torch.float32, device=dev)
     L = _lib.lib()
+    rest = torch.empty(B, Sq, H, D, dtype=torch.uint8, device=dev) if L.icsa_cross_attn_wants_rest(Sq, Sk, H, Hk, q_starts is not None) else None
     wsp, ws_bytes = 0, L.icsa_cross_attn_workspace_size(*sizes, docs)
     if ws_bytes:
         if ws_bytes < 0:
@@ -98,7 +99,7 @@ def cross_attn_fwd_hip(q, k, v, q_starts=None, k_starts=None, softmax_scale=None
         wsp = ws.data_ptr()
     with on_device(dev):
         rc = L.icsa_cross_attn_fwd(*qa, *ka, *va, *sizes, ptr(q_starts), ptr(k_starts), docs, scale, out.data_ptr(), Sq * H * D, H * D, D,
-                                   lse.data_ptr(), rest.data_ptr(), wsp, ws_bytes, stream_ptr(dev))
+                                   lse.data_ptr(), ptr(rest), wsp, ws_bytes, stream_ptr(dev))
     _lib.check("icsa_cross_attn_fwd", rc)
     return out, lse, rest
 

@@ -19,14 +19,14 @@ def documents(B, Sq, Sk, q_starts=None, k_starts=None):
                 yield b, i0, i1, j0, j1
 
 
-def cross_attention(q, k, v, dout, *, q_starts=None, k_starts=None, scale=None):
+def cross_attention(q, k, v, dout, *, q_starts=None, k_starts=None, scale=None, rest=True):
     """({name: value}, {name: bound}) for out, dq, dk, dv, float64.
 
     Bounds, element by element, for f32 scores and sums, P and dS rounded to bf16 (W each), and a total of rounded weights.  A score is off by e <= 2 U (D sum |q k| scale + 8 |s| + 8), so
     exp(score) by a factor 1 + 2 e; the total by W more, so a weight of the backward by f = 4 e + 1.01 W of itself, and its
     rounded form by f + W.
       out   1.01 (2.5 e sum p |v| + W sum p |v - o|), as in masked attention; D reads it with a byte of what its rounding left, in
-            256ths of the last place (2^-7 of a value at most), clamped by one: 2^-15 |o|
+            256ths of the last place (2^-7 of a value at most), clamped by one: 2^-15 |o|; without that byte (rest) rounded: W |o|
       D     sum |dout| (o's) + 2 U D sum |dout o|
       dP    2 U D sum |dout v|
       dS    p (f |dP - D| + (1 + f) (dP's + D's)), and W of |dS| + that
@@ -58,7 +58,7 @@ def cross_attention(q, k, v, dout, *, q_starts=None, k_starts=None, scale=None):
             em = e.amax(1, keepdim=True)
             f = 4 * em + 1.01 * W
             to = 1.01 * (2.5 * em * (p @ V.abs()) + W * (p @ V.abs() + o.abs()))
-            tD = (dO.abs() * (to + 2.0 ** -15 * (o.abs() + to))).sum(1, keepdim=True) + 2 * U * D * (dO * o).abs().sum(1, keepdim=True)
+            tD = (dO.abs() * (to + (2.0 ** -15 if rest else W) * (o.abs() + to))).sum(1, keepdim=True) + 2 * U * D * (dO * o).abs().sum(1, keepdim=True)
             tP = 2 * U * D * dO.abs() @ V.abs().t()
             tS = p * (f * (dP - Dr).abs() + (1 + f) * (tP + tD))
             tS = tS + W * (dS.abs() + tS)

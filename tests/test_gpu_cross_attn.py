@@ -41,7 +41,8 @@ def _compare(got, val, tol, own=(2.0 ** -8,) * 4, where=None):
 
 
 def _check(gpu, q, k, v, do, qs=None, ks=None, scale=None, grad_dtype=BF):
-    val, tol = O.cross_attention(q, k, v, do, q_starts=qs, k_starts=ks, scale=scale)
+    keeps = qs is not None or k.shape[1] <= 256 or q.shape[1] * (q.shape[2] // k.shape[2]) <= 64
+    val, tol = O.cross_attention(q, k, v, do, q_starts=qs, k_starts=ks, scale=scale, rest=keeps)
     got = _run(gpu, q, k, v, do, qs, ks, scale, grad_dtype)
     assert all(x.dtype == (BF if i == 0 else grad_dtype) for i, x in enumerate(got))
     _compare(got, val, tol, (2.0 ** -8,) + ((2.0 ** -8 if grad_dtype == BF else 2.0 ** -22),) * 3)
@@ -263,6 +264,21 @@ def test_few_queries_and_what_is_not_finite(gpu, bad, D):
         end = 20 if n in ("out", "dq") else 70
         assert torch.equal(a[:, :end], b[:, :end]), n
     assert dirty[1][0, 30, 1].isnan().all() and dirty[2][0, 70:140, 1].isnan().all() and not dirty[3][0, 70:140, 1, 5].isfinite().any()
+
+
+def test_where_the_rounding_is_kept(gpu):
+    """By keys, documents, or where the queries are few; the node keeps the same: a hook sees it or not."""
+    def kept(Sq, Sk, H, Hk, docs=0):
+        q, k, v, _ = (t.to(gpu) for t in _inputs(1, Sq, Sk, H, Hk, 64))
+        st = [None, None] if not docs else [torch.linspace(0, n, docs + 1).int()[None].to(gpu) for n in (Sq, Sk)]
+        pair = cross_attn_fwd_hip(q, k, v, *st)[2] is not None
+        seen = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.dtype) or t, lambda t: t):
+            cross_attn_func(q.requires_grad_(True), k, v, q_starts=st[0], k_starts=st[1])
+        assert (torch.uint8 in seen) == pair
+        return pair
+    assert [kept(*x) for x in ((65, 256, 2, 2), (65, 257, 2, 2), (64, 257, 2, 2), (33, 257, 4, 2), (100, 512, 2, 1, 1), (100, 513, 2, 1, 2))] == \
+        [True, False, True, False, True, True]
 
 
 def test_autograd(gpu):
