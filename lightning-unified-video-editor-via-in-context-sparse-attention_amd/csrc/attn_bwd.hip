@@ -479,11 +479,13 @@ __global__ void __launch_bounds__(256) icsa_attn_bwd_join_kernel(AttnBwdParams p
 
 namespace {
 
-// Parts of an item's walk (tiles, over all documents): as many as make the rounds of workgroups come out shortest, beside the parts' sums
-// on their way through memory: 256 KB written and read an item and part at some 4.5 TB/s, in the time of an item's tiles at 3.8 us
-// (65,520 queries over 512 keys of 40 heads: 160 items, 3 parts).  Documents differ in length, and blocks with rows of two walk
-// both: four parts at least where rounds are few (4 clips of 1,500 to 17,600 tokens over 320 to 370 keys, 440 items: dk and dv with their sums
-// 1,274 us in one part, 878 in two, 766 in four, 762 in eight; of 8,190 tokens each 794, 700, 698 in one, two, four).
+// Parts of an item's walk (tiles, over all documents): as many as make the rounds of workgroups come out shortest, beside the parts'
+// sums on their way through memory: 256 KB written and read an item and part at some 4.5 TB/s, in the time of an item's tiles at
+// 3.8 us (65,520 queries over 512 keys of 40 heads: 160 items, 3 parts).  Documents differ in length, and blocks with rows of two
+// walk both: there, where rounds are few, four parts at least and two rounds of workgroups (dk and dv: 4 clips of 1,500 to 17,600
+// tokens over 320 to 370 keys, 440 items, 1,274 us in one part, 878 in two, 766 in four, 762 in eight; of 8,190 tokens each 794, 700,
+// 698 in one, two, four; 5 of 30,000 tokens together over 512 keys, 160 items, 624 in four, 531 in seven; 2 of 20,000 over 1,000,
+// 96 items, 251 in four, 229 in eleven).
 int parts(int64_t items, int64_t tiles, int docs, int slots) {
   int best = 1;
   double time = 0.;
@@ -492,7 +494,9 @@ int parts(int64_t items, int64_t tiles, int docs, int slots) {
     const double t = (double)((items * n + slots - 1) / slots) / n + (n > 1 ? items * n / (65. * walk) : 0.);
     if (n == 1 || t < time) { time = t; best = n; }
   }
-  return best < 4 && docs > 1 && items <= 2 * slots && walk >= 4 * AB_MIN_TILES ? 4 : best;
+  if (docs > 1 && items <= 2 * slots)
+    best = std::max(best, (int)std::min<int64_t>({AB_MAX_SPLIT, walk / AB_MIN_TILES, std::max<int64_t>(4, (2 * slots + items - 1) / items)}));
+  return best;
 }
 
 int64_t blocks(int64_t rows) { return (rows + AB_ROWS - 1) / AB_ROWS; }
