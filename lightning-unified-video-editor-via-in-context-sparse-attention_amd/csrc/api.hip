@@ -707,8 +707,8 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
   if (rc || (rc = check_dtype(grad_dtype, "gradients"))) return rc;
   if (!q_starts != !k_starts) return fail(ICSA_EINVAL, "q_starts and k_starts must be both given or both NULL");
   if (docs < 1 || (!q_starts && docs != 1)) return fail(ICSA_EINVAL, "docs=%d without document starts", docs);
-  if (!std::isfinite(scale) || scale <= 0.f || !std::isfinite(2.f * scale))
-    return fail(ICSA_EINVAL, "scale must be positive and finite");
+  if (!std::isfinite(2.f * scale) || scale < 0x1p-96f)   // the row sums are held as -lse / scale
+    return fail(ICSA_EINVAL, "scale must be finite and 2^-96 or more");
   if (Sq > 0 && (!dout || !q || !out || !lse)) return fail(ICSA_EINVAL, "null pointer argument");
   if (Sk > 0 && (!k || !v)) return fail(ICSA_EINVAL, "null pointer argument");
   if (rest && !aligned16(rest)) return fail(ICSA_EINVAL, "rest must be 16-byte aligned");

@@ -13,6 +13,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
+#include <algorithm>
 
 #include "../../include/icsa.h"
 
@@ -214,7 +215,7 @@ Params params(const Tensor& gain, const Tensor& shift) {
     p.gain = p.gain.contiguous();
     p.shift = p.shift.contiguous();
   }
-  p.groups = (int)p.gain.size(0);
+  p.groups = std::max(1, (int)p.gain.size(0));          // without batch rows there are no rows either
   p.code = code_of(gain.scalar_type());
   p.stride = p.gain.stride(0);
   return p;

@@ -1,8 +1,8 @@
 // Rotary positions: the pair j of a head's first R dims is turned by its token's angle,
 //   (x0, x1) -> (x0 c - x1 s, x0 s + x1 c),  c = cos[pos][j], s = sin[pos][j],
 // and back (the transposed matrix, s -> -s) for gradients.  Pair j is dims 2 j, 2 j + 1 (interleaved) or j, j + R / 2 (halves); dims from R on
-// are copied.  Up to four axes: consecutive runs of pairs turn by positions of their own (frames, rows, columns).  A position
-// outside the table turns nothing.  Tables are f32 from angles in 64 bits, the products f32, rounded once.
+// are copied.  Up to four axes: consecutive runs of pairs turn by positions of their own (frames, rows, columns).  Pairs whose position
+// is outside the table are copied, whatever they hold.  Tables are f32 from angles in 64 bits, the products f32, rounded once.
 //
 // A wave takes one token, or part of its heads where tokens are few: a lane keeps its pairs' cos and sin over the heads, so that
 // tables are read once a token, and what bounds the kernel is x in and y out.  Two tensors (q and k) go in one launch.
@@ -56,9 +56,8 @@ __global__ void __launch_bounds__(RO_THREADS) icsa_rotary_kernel(RotaryParams p)
   const bool on = h0 < heads, turn = u < turned;
   const int first = HALF ? (turn ? 8 * u : p.R + 8 * (u - turned)) : 8 * u;    // the unit's first dim
   const int half = HALF && turn ? p.R / 2 : 0;
-  float c[kPairs], sn[kPairs];
-#pragma unroll
-  for (int e = 0; e < kPairs; ++e) { c[e] = 1.f; sn[e] = 0.f; }
+  float c[kPairs] = {}, sn[kPairs] = {};
+  unsigned still = 0u;                                // pairs that are copied: 0 times an infinity would not be
   if (on && turn) {
     const int* pos = p.pos + (int64_t)b * p.pos_sb + (int64_t)s * p.axes;
     const int np = p.R / 2, j0 = kPairs * u;
@@ -75,12 +74,15 @@ __global__ void __launch_bounds__(RO_THREADS) icsa_rotary_kernel(RotaryParams p)
 #pragma unroll
           for (int x = 0; x < 4; ++x) { c[e + x] = c4[x]; sn[e + x] = s4[x]; }
         }
+      } else {
+        still = ~0u;
       }
     } else {
 #pragma unroll
       for (int e = 0; e < kPairs; ++e) {
         const int at = pair_pos(p, pos, j0 + e);
         if (at >= 0) { c[e] = p.cos[(int64_t)at * np + j0 + e]; sn[e] = p.sin[(int64_t)at * np + j0 + e]; }
+        else still |= 1u << e;
       }
     }
     if (p.back) {
@@ -116,6 +118,7 @@ __global__ void __launch_bounds__(RO_THREADS) icsa_rotary_kernel(RotaryParams p)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float a = v[k].at(e), d = w[k].at(e);
+              if (still >> e & 1u) continue;
               v[k].set(e, fmaf(a, c[e], -d * sn[e]));
               w[k].set(e, fmaf(a, sn[e], d * c[e]));
             }
@@ -124,6 +127,7 @@ __global__ void __launch_bounds__(RO_THREADS) icsa_rotary_kernel(RotaryParams p)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float a = v[k].at(2 * e), d = v[k].at(2 * e + 1);
+              if (still >> e & 1u) continue;
               v[k].set(2 * e, fmaf(a, c[e], -d * sn[e]));
               v[k].set(2 * e + 1, fmaf(a, sn[e], d * c[e]));
             }
@@ -158,9 +162,12 @@ __global__ void __launch_bounds__(RO_THREADS) icsa_rotary_any_kernel(RotaryParam
         continue;
       }
       const int ps = pair_pos(p, pos, u), d0 = p.halves ? u : 2 * u, d1 = p.halves ? u + np : 2 * u + 1;
-      float c = 1.f, sn = 0.f;
-      if (ps >= 0) { c = p.cos[(int64_t)ps * np + u]; sn = p.sin[(int64_t)ps * np + u]; }
-      if (p.back) sn = -sn;
+      if (ps < 0) {                                   // copied
+        yh[d0] = xh[d0];
+        yh[d1] = xh[d1];
+        continue;
+      }
+      const float c = p.cos[(int64_t)ps * np + u], sn = p.back ? -p.sin[(int64_t)ps * np + u] : p.sin[(int64_t)ps * np + u];
       const float a = (float)xh[d0], d = (float)xh[d1];
       yh[d0] = (T)fmaf(a, c, -d * sn);
       yh[d1] = (T)fmaf(a, sn, d * c);

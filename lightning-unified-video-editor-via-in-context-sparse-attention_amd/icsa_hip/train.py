@@ -71,8 +71,8 @@ def _check_attn(q, k, v, q_starts, k_starts, softmax_scale):
         docs = q_starts.shape[1] - 1
         q_starts, k_starts = q_starts.contiguous(), k_starts.contiguous()
     scale = D ** -0.5 if softmax_scale is None else float(softmax_scale)
-    if not scale > 0:
-        raise IcsaArgumentError("softmax_scale must be positive")
+    if not scale >= 2.0 ** -96:
+        raise IcsaArgumentError("softmax_scale must be positive, 2 ** -96 or more")
     return (B, Sq, Sk, H, Hk, D), docs, scale, q_starts, k_starts
 
 
@@ -153,7 +153,7 @@ def cross_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_star
     ``q_starts``, ``k_starts``: int32 [B, N + 1] on the GPU, not decreasing, as in ``masked_attn_func``: document n of
     batch row b has queries ``q_starts[b, n] .. q_starts[b, n + 1] - 1`` and keys likewise, and sees its own keys alone
     (a batch row whose text has ``n`` real tokens is one document, ``[0, Sq]`` and ``[0, n]``).  Values past the lengths
-    are clamped on the GPU.  ``softmax_scale``: positive, default ``D ** -0.5``.
+    are clamped on the GPU.  ``softmax_scale``: 2 ** -96 or more, default ``D ** -0.5``.
 
     A query that sees nothing gets zeros; it, keys outside every document and padding take no part in any gradient and
     get zeros, whatever they and their ``dout`` hold.  A NaN or an infinity inside a document makes gradients of that

@@ -313,6 +313,7 @@ def test_refusals(gpu):
                  lambda: cross_attn_func(q, k, v, q_starts=s), lambda: cross_attn_func(q, k, v, q_starts=s, k_starts=s[:1]),
                  lambda: cross_attn_func(q, k, v, q_starts=s.long(), k_starts=s.long()),
                  lambda: cross_attn_func(q, k, v, q_starts=s.cpu(), k_starts=s.cpu()), lambda: cross_attn_func(q, k, v, softmax_scale=-1.0),
+                 lambda: cross_attn_func(q, k, v, softmax_scale=1e-30),
                  lambda: cross_attn_func(q, k.cpu(), v.cpu()), lambda: cross_attn_bwd_hip(do[:, :3], q, k, v, out, lse, rest),
                  lambda: cross_attn_bwd_hip(do.float(), q, k, v, out, lse, rest), lambda: cross_attn_bwd_hip(do, q, k, v, out, lse[:, :1], rest),
                  lambda: cross_attn_bwd_hip(do, q, k, v, out, lse, rest[:, :3]), lambda: cross_attn_bwd_hip(do, q, k, v, out, lse, rest.char()),

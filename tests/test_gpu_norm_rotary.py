@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from icsa_hip import layer_norm_func, rms_norm_func, rotary_func, rotary_table
+from icsa_hip._lib import IcsaError
 from icsa_hip.hip_host import IcsaArgumentError
 from oracle import norm_rotary as O
 
@@ -142,6 +143,11 @@ def test_norm_partial_needs_and_empty(gpu):
     y = layer_norm_func(none, w, c)
     gx, gw, gb = torch.autograd.grad(y, (none, w, c), torch.zeros_like(y))
     assert y.shape == gx.shape == (1, 0, 64) and not gw.any() and not gb.any()
+    none = torch.zeros(0, 5, 64, device=gpu).requires_grad_()              # no batch rows, so no scales either
+    s = torch.zeros(0, 64, device=gpu).requires_grad_()
+    y = layer_norm_func(none, scale=s, shift=s.detach())
+    gx, gs = torch.autograd.grad(y, (none, s), torch.zeros_like(y))
+    assert y.shape == gx.shape == (0, 5, 64) and gs.shape == (0, 64)
     X = torch.full((2, 64), 3.0, device=gpu).requires_grad_()              # rows of one value: a variance of 0
     y = layer_norm_func(X, w, c)
     assert torch.equal(y[0], c.detach())
@@ -174,6 +180,9 @@ def test_norm_refusals(gpu):
                  lambda: rms_norm_func(torch.zeros(1, 8193, device=gpu)), lambda: rms_norm_func(torch.zeros(2, 0, device=gpu))):
         with pytest.raises(IcsaArgumentError):
             call()
+    many = torch.zeros(70000, 1, 8, device=gpu, requires_grad=True)          # what the library refuses, a node raises
+    with pytest.raises(IcsaError, match="icsa_norm_fwd"):
+        layer_norm_func(many, scale=many.detach(), shift=many.detach())
 
 
 # ------------------------------------------------------------------------------------------
@@ -208,6 +217,32 @@ def test_rotary(gpu, B, S, H, Hk, D, R, sections, dt, interleaved):
     with torch.no_grad():
         alone = rotary_func(Q, None, *args, sections=sections, interleaved=interleaved)
         assert torch.equal(alone, got[0]) and alone.data_ptr() != Q.data_ptr()
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("D,R,sections", [(64, 64, None), (128, 128, (22, 21, 21)), (128, 32, None), (80, 80, (14, 13, 13)), (10, 6, None)])
+def test_what_is_not_turned_is_copied(gpu, D, R, sections, interleaved):
+    """Pairs whose position is outside the table are the same bits in either direction, infinities and negative zeros too."""
+    q, _, dq, _ = _turn_inputs(1, 6, 3, 1, D, BF)
+    A = 1 if sections is None else len(sections)
+    pos = torch.arange(6, dtype=torch.int32)[None, :, None].repeat(1, 1, A)
+    pos[0, 2] = -1
+    pos[0, 4, -1] = 50                                       # the last axis alone
+    last = (sections or (R // 2,))[-1]
+    still = torch.zeros(1, 6, 3, D, dtype=torch.bool)
+    still[0, 2] = True
+    j = torch.arange(R // 2 - last, R // 2)
+    still[0, 4][:, torch.cat([2 * j, 2 * j + 1] if interleaved else [j, j + R // 2])] = True
+    hard = torch.tensor([float("inf"), 1.0, -0.0, float("nan"), float("-inf"), 0.0, -0.0, 5.0], dtype=BF)
+    for t in (q, dq):
+        t[still] = hard.repeat(still.sum() // 8 + 1)[:still.sum()]
+    cos, sin = rotary_table(50, R)
+    Q = q.to(gpu).requires_grad_()
+    y = rotary_func(Q, None, cos, sin, (pos[..., 0] if sections is None else pos).to(gpu), sections=sections, interleaved=interleaved)
+    g, = torch.autograd.grad(y, Q, dq.to(gpu))
+    bits = lambda t: t.detach().cpu().view(torch.int16)
+    for a, b in ((y, q), (g, dq)):
+        assert torch.equal(bits(a)[still], bits(b)[still]) and a.detach().cpu()[~still].isfinite().all()
 
 
 def test_rotary_layouts_and_needs(gpu):

@@ -46,7 +46,7 @@ def test_cross_attention_refuses(kw, code):
     (dict(gd=7), EIN), (dict(do=0), EIN), (dict(out=0), EIN), (dict(lse=0), EIN), (dict(dq=PTR + 8), EIN), (dict(dk_ss=4), EIN),
     (dict(ws=0), EWS), (dict(wsb=8), EWS), (dict(ws=PTR + 8), EWS), (dict(k_ss=-128), EIN), (dict(q_ss=-128), EIN),
     (dict(k_ss=1 << 28), EUN), (dict(q_ss=1 << 28), EUN), (dict(do_ss=1 << 28), EUN), (dict(H=8, q_sh=1 << 28), EUN),
-    (dict(H=8, do_sh=-128), EIN),
+    (dict(H=8, do_sh=-128), EIN), (dict(scale=1e-30), EIN),
 ])
 def test_cross_attention_backward_refuses(kw, code):
     assert _bwd(**kw) == code and _lib.lib().icsa_last_error()
