@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/variable.h>
 #include <dlfcn.h>
 #include <algorithm>
 
@@ -74,6 +75,27 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// A captured backward must not meet a node that an eager graph has made on another stream, a leaf's accumulation among them, as
+// long as that graph lives: the engine would have the one wait for the other, which a capture does not allow, and the process
+// ends.  Refused while nothing of it is captured.
+void refuse_capture(std::initializer_list<const Tensor*> ts) {
+  auto capturing = [](hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return s != nullptr && hipStreamIsCapturing(s, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+  };
+  const auto now = c10::hip::getCurrentHIPStream((*ts.begin())->device().index());
+  if (!capturing(now.stream())) return;
+  for (const Tensor* t : ts) {
+    if (!t->defined() || !t->requires_grad()) continue;
+    const std::shared_ptr<torch::autograd::Node> node = t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto of = node ? node->stream() : std::nullopt;
+    if (!of || of->id() == now.id()) continue;
+    if (!capturing(c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, *of).stream()))
+      throw Failure("under capture an input has a node of an eager graph: drop that graph, or detach the input, before a backward is captured "
+                    "(torch.no_grad() for a forward alone)");
+  }
 }
 
 // An absent tensor is no input of a node, and needs_input_grad does not count it: only the last ones are absent here.
@@ -188,7 +210,10 @@ struct CrossAttn : public torch::autograd::Function<CrossAttn> {
 
 Tensor cross_attn(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& qs, const MaybeTensor& ks, int64_t docs,
                   double scale) {
-  if (wants_grad({&q, &k, &v})) return CrossAttn::apply(q, k, v, qs, ks, docs, scale);
+  if (wants_grad({&q, &k, &v})) {
+    refuse_capture({&q, &k, &v});
+    return CrossAttn::apply(q, k, v, qs, ks, docs, scale);
+  }
   return attn_forward(rows16(q), rows16(k), rows16(v), get(qs), get(ks), docs, scale, nullptr, nullptr);
 }
 
@@ -283,7 +308,10 @@ struct Norm : public torch::autograd::Function<Norm> {
 
 Tensor norm(const Tensor& x, const MaybeTensor& gain_, const MaybeTensor& shift_, bool plus_one, bool rms, double eps, at::ScalarType out) {
   const Tensor gain = get(gain_), shift = get(shift_);
-  if (wants_grad({&x, &gain, &shift})) return Norm::apply(x, gain_, shift_, plus_one, rms, eps, (int64_t)out);
+  if (wants_grad({&x, &gain, &shift})) {
+    refuse_capture({&x, &gain, &shift});
+    return Norm::apply(x, gain_, shift_, plus_one, rms, eps, (int64_t)out);
+  }
   return norm_forward(x, rows(x), gain, shift, plus_one, rms, eps, out, nullptr, nullptr);
 }
 
@@ -351,7 +379,10 @@ struct Rotary : public torch::autograd::Function<Rotary> {
 variable_list rotary(const Tensor& q, const MaybeTensor& k_, const Tensor& cos, const Tensor& sin, const Tensor& pos,
                      std::vector<int64_t> sections, bool interleaved) {
   const Tensor k = get(k_), c = cos.contiguous(), s = sin.contiguous(), p = pos.contiguous();
-  if (wants_grad({&q, &k})) return Rotary::apply(q, k_, c, s, p, std::move(sections), interleaved);
+  if (wants_grad({&q, &k})) {
+    refuse_capture({&q, &k});
+    return Rotary::apply(q, k_, c, s, p, std::move(sections), interleaved);
+  }
   auto y = rotate(q, k, c, s, p, sections, interleaved, false);
   return k.defined() ? variable_list{y.first, y.second} : variable_list{y.first};
 }

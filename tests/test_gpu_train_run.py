@@ -5,6 +5,7 @@ import torch
 
 from icsa_hip import (SparsePiecewiseAttn1stIntervalsFunction, cross_attn_bwd_hip, cross_attn_func, cross_attn_fwd_hip,
                       layer_norm_func, rms_norm_func, rotary_func, rotary_table, wan)
+from icsa_hip._lib import IcsaError
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -169,6 +170,48 @@ def test_two_captured_graphs(gpu):
             kept = [o.clone() for o in out]
             for a, b in zip(kept, _step(t)):
                 assert torch.equal(a, b), turn
+
+
+def test_a_capture_with_an_eager_graph_alive_is_refused(gpu):
+    """Nodes of an eager graph that lives, a leaf's and another's; without it, from the capture's own stream, and without
+    gradients the same calls are captured."""
+    x = torch.randn(2, 9, 128, device=gpu, requires_grad=True)
+    q = torch.randn(1, 9, 2, 64, device=gpu).to(BF).requires_grad_()
+    table, pos = rotary_table(9, 64), torch.arange(9, dtype=torch.int32, device=gpu)
+    calls = [lambda: layer_norm_func(x), lambda: rms_norm_func(x), lambda: cross_attn_func(q, q, q), lambda: rotary_func(q, None, *table, pos)]
+    for call in calls:
+        call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def captured(call, refused):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            if refused:
+                with pytest.raises(IcsaError, match="eager graph"):
+                    call()
+            else:
+                call()
+            torch.zeros(1, device=gpu)                       # something to capture
+        g.replay()
+        torch.cuda.synchronize()
+
+    held = [x * 2, q * 2]
+    for call in calls:
+        captured(call, True)
+        with torch.no_grad():
+            captured(call, False)
+    h = held[0]
+    captured(lambda: layer_norm_func(h), True)               # no leaf: its own node
+    captured(lambda: layer_norm_func(h.detach().requires_grad_()), False)
+    del held, h
+    for call in calls:
+        captured(call, False)
+    with torch.cuda.stream(side):
+        held = [x * 2, q * 2]
+    for call in calls:
+        captured(call, False)
+    torch.cuda.current_stream().wait_stream(side)
 
 
 def test_the_attentions_pair_in_a_graph(gpu):
