@@ -5,7 +5,8 @@
 // is outside the table are copied, whatever they hold.  Tables are f32 from angles in 64 bits, the products f32, rounded once.
 //
 // A wave takes one token, or part of its heads where tokens are few: a lane keeps its pairs' cos and sin over the heads, so that
-// tables are read once a token, and what bounds the kernel is x in and y out.  Two tensors (q and k) go in one launch.
+// tables are read once a token, and what bounds the kernel is x in and y out: q and k of 65,520 tokens, 40 heads of 128 each, take 496 us
+// for 2.7 GB (5.4 TB/s).  Two tensors (q and k) go in one launch; 8 tokens of 40 and 8 heads take 4.6 us, most of it launch.
 #include "icsa_kernels.h"
 
 #define RO_THREADS 256
