@@ -1,18 +1,20 @@
 // Autograd nodes of the training operators (icsa_hip/train.py) over the C ABI of libicsa.so.
 //
 // A Python autograd function runs its backward on a thread of autograd's own, which waits for the interpreter and finds its objects
-// in another core's cache: a layer norm of six rows, forward and backward, took 130 us in Python and 72 here, where the
+// in another core's cache: a layer norm of six rows, forward and backward, took 130 us in Python and 63 here, where the
 // backward never enters the interpreter.
 //
 // Arguments have been checked in Python.  The library is the one that the package has loaded, found by its path.  What the
 // backward reads is taken from the saved tensors, not remembered by address: hooks may have moved it.
 #include <torch/extension.h>
 #include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/variable.h>
 #include <dlfcn.h>
 #include <algorithm>
 
@@ -21,7 +23,7 @@
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 typedef c10::optional<Tensor> MaybeTensor;
 
@@ -71,10 +73,19 @@ void check(const char* fn, int64_t code) {
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
-  if (!c10::GradMode::is_enabled()) return false;
+  bool some = false;
   for (const Tensor* t : ts)
-    if (t->defined() && t->requires_grad()) return true;
-  return false;
+    if (t->defined()) {
+      TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "icsa_hip's training operators have no forward-mode derivative");
+      some = some || t->requires_grad();
+    }
+  return some && c10::GradMode::is_enabled();
+}
+
+template <class N, class... T> std::shared_ptr<N> make_node(const T&... inputs) {
+  std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+  return node;
 }
 
 // A captured backward must not meet a node that an eager graph has made on another stream, a leaf's accumulation among them, as
@@ -98,7 +109,6 @@ void refuse_capture(std::initializer_list<const Tensor*> ts) {
   }
 }
 
-// An absent tensor is no input of a node, and needs_input_grad does not count it: only the last ones are absent here.
 Tensor get(const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); }
 void* at_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 int code_of(at::ScalarType t) { return t == at::kBFloat16 ? ICSA_BF16 : ICSA_F32; }
@@ -137,6 +147,12 @@ Rows rows16(const Tensor& t) {
 }
 
 // ------------------------------------------------------------------------------------------ cross attention
+// a saved tensor, contiguous as it was (hooks may have changed its strides), or none
+Tensor whole(SavedVariable& s) {
+  const Tensor t = s.unpack();
+  return t.defined() ? t.contiguous() : t;
+}
+
 struct AttnSizes {
   int B, Sq, Sk, H, Hk, D;
 };
@@ -165,33 +181,32 @@ Tensor attn_forward(const Rows& q, const Rows& k, const Rows& v, const Tensor& q
   return out;
 }
 
-struct CrossAttn : public torch::autograd::Function<CrossAttn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const MaybeTensor& qs_,
-                        const MaybeTensor& ks_, int64_t docs, double scale) {
-    const Tensor qs = get(qs_), ks = get(ks_);
-    const Rows q = rows16(q_), k = rows16(k_), v = rows16(v_);
-    Tensor lse, rest, out = attn_forward(q, k, v, qs, ks, docs, scale, &lse, &rest);
-    ctx->save_for_backward({q.t, k.t, v.t, qs, ks, out, lse, rest});
-    ctx->saved_data["docs"] = docs;
-    ctx->saved_data["scale"] = scale;
-    return out;
+struct CrossAttnBackward : public torch::autograd::Node {
+  SavedVariable q, k, v, qs, ks, out, lse, rest;
+  int docs = 1;
+  double scale = 1.;
+  std::string name() const override { return "CrossAttnBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* s : {&q, &k, &v, &qs, &ks, &out, &lse, &rest}) s->reset_data();
   }
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const variable_list s = ctx->get_saved_variables();
-    variable_list res(7);
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list res(3);
+    if (!grads[0].defined()) return res;
+    const Tensor sq = q.unpack(), sk = k.unpack(), sv = v.unpack(), so = out.unpack(shared_from_this());
     {
-      at::NoGradGuard none;
+      at::AutoDispatchBelowADInplaceOrView below;
       c10::DeviceGuard guard(grads[0].device());
-      const Rows g = rows16(grads[0]), q = rows16(s[0]), k = rows16(s[1]), v = rows16(s[2]), o = rows16(s[5]);
-      const Tensor lse = s[6].contiguous(), rest = s[7].defined() ? s[7].contiguous() : s[7], qs = s[3].defined() ? s[3].contiguous() : s[3],
-                   ks = s[4].defined() ? s[4].contiguous() : s[4];
+      const Rows g = rows16(grads[0]), q = rows16(sq), k = rows16(sk), v = rows16(sv), o = rows16(so);
+      const Tensor lse = whole(this->lse), rest = whole(this->rest), qs = whole(this->qs), ks = whole(this->ks);
       const AttnSizes z = attn_sizes(q.t, k.t);
-      const int docs = (int)ctx->saved_data["docs"].toInt();
       const auto opt = q.t.options();
-      if (ctx->needs_input_grad(0)) res[0] = at::empty({z.B, z.Sq, z.H, z.D}, opt);
-      if (ctx->needs_input_grad(1)) res[1] = at::empty({z.B, z.Sk, z.Hk, z.D}, opt);
-      if (ctx->needs_input_grad(2)) res[2] = at::empty({z.B, z.Sk, z.Hk, z.D}, opt);
+      if (task_should_compute_output(0)) res[0] = at::empty({z.B, z.Sq, z.H, z.D}, opt);
+      if (task_should_compute_output(1)) res[1] = at::empty({z.B, z.Sk, z.Hk, z.D}, opt);
+      if (task_should_compute_output(2)) res[2] = at::empty({z.B, z.Sk, z.Hk, z.D}, opt);
       const int64_t bytes = api.attn_bwd_workspace(z.B, z.Sq, z.Sk, z.H, z.Hk, z.D, docs);
       check("icsa_cross_attn_bwd_workspace_size", bytes);
       const Tensor ws = workspace(bytes, q.t);
@@ -199,22 +214,45 @@ struct CrossAttn : public torch::autograd::Function<CrossAttn> {
       check("icsa_cross_attn_bwd",
             api.attn_bwd(g.p, g.sb, g.ss, g.sh, q.p, q.sb, q.ss, q.sh, k.p, k.sb, k.ss, k.sh, v.p, v.sb, v.ss, v.sh, o.p, o.sb, o.ss, o.sh,
                          (const float*)lse.data_ptr(), at_or_null(rest), z.B, z.Sq, z.Sk, z.H, z.Hk, z.D,
-                         (const int32_t*)at_or_null(qs), (const int32_t*)at_or_null(ks), docs,
-                         (float)ctx->saved_data["scale"].toDouble(), ICSA_BF16, at_or_null(res[0]), z.Sq * qss, qss, z.D,
-                         at_or_null(res[1]), z.Sk * kss, kss, z.D, at_or_null(res[2]), z.Sk * kss, kss, z.D, at_or_null(ws), bytes,
-                         stream_of(q.t)));
+                         (const int32_t*)at_or_null(qs), (const int32_t*)at_or_null(ks), docs, (float)scale, ICSA_BF16,
+                         at_or_null(res[0]), z.Sq * qss, qss, z.D, at_or_null(res[1]), z.Sk * kss, kss, z.D,
+                         at_or_null(res[2]), z.Sk * kss, kss, z.D, at_or_null(ws), bytes, stream_of(q.t)));
     }
     return once(std::move(res));
   }
 };
 
-Tensor cross_attn(const Tensor& q, const Tensor& k, const Tensor& v, const MaybeTensor& qs, const MaybeTensor& ks, int64_t docs,
+Tensor cross_attn(const Tensor& q_, const Tensor& k_, const Tensor& v_, const MaybeTensor& qs_, const MaybeTensor& ks_, int64_t docs,
                   double scale) {
-  if (wants_grad({&q, &k, &v})) {
-    refuse_capture({&q, &k, &v});
-    return CrossAttn::apply(q, k, v, qs, ks, docs, scale);
+  const Tensor qs = get(qs_), ks = get(ks_);
+  std::shared_ptr<CrossAttnBackward> node;
+  if (wants_grad({&q_, &k_, &v_})) {
+    refuse_capture({&q_, &k_, &v_});
+    node = make_node<CrossAttnBackward>(q_, k_, v_);
   }
-  return attn_forward(rows16(q), rows16(k), rows16(v), get(qs), get(ks), docs, scale, nullptr, nullptr);
+  Tensor out, lse, rest;
+  Rows q, k, v;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    q = rows16(q_);
+    k = rows16(k_);
+    v = rows16(v_);
+    out = attn_forward(q, k, v, qs, ks, docs, scale, node ? &lse : nullptr, node ? &rest : nullptr);
+  }
+  if (node) {
+    torch::autograd::set_history(out, node);
+    node->q = SavedVariable(q.t, false);
+    node->k = SavedVariable(k.t, false);
+    node->v = SavedVariable(v.t, false);
+    node->qs = SavedVariable(qs, false);
+    node->ks = SavedVariable(ks, false);
+    node->out = SavedVariable(out, true);
+    node->lse = SavedVariable(lse, false);
+    node->rest = SavedVariable(rest, false);
+    node->docs = (int)docs;
+    node->scale = scale;
+  }
+  return out;
 }
 
 // ------------------------------------------------------------------------------------------ layer norm, RMS norm
@@ -247,59 +285,57 @@ Params params(const Tensor& gain, const Tensor& shift) {
 }
 
 Tensor norm_forward(const Tensor& x, const Tensor& r, const Tensor& gain, const Tensor& shift, bool plus_one, bool rms, double eps,
-                    at::ScalarType out, Tensor* mean, Tensor* rstd) {
+                    at::ScalarType out, Tensor* stats) {
   c10::DeviceGuard guard(x.device());
   const Params p = params(gain, shift);
   const int64_t n = r.size(0), dim = r.size(1);
   Tensor y = at::empty(x.sizes(), x.options().dtype(out));
-  if (rstd != nullptr) {
-    *rstd = at::empty({n}, x.options().dtype(at::kFloat));
-    if (!rms) *mean = at::empty({n}, x.options().dtype(at::kFloat));
+  float* rstd = nullptr;
+  if (stats != nullptr) {                              // [1 / deviation, mean] of each row
+    *stats = at::empty({rms ? 1 : 2, n}, x.options().dtype(at::kFloat));
+    rstd = (float*)stats->data_ptr();
   }
   check("icsa_norm_fwd", api.norm_fwd(r.data_ptr(), code_of(r.scalar_type()), row_stride(r), n / p.groups, p.groups, (int)dim,
                                       at_or_null(p.gain), at_or_null(p.shift), p.code, p.stride, plus_one, rms, (float)eps, y.data_ptr(),
-                                      code_of(out), dim, mean ? (float*)at_or_null(*mean) : nullptr,
-                                      rstd ? (float*)rstd->data_ptr() : nullptr, stream_of(x)));
+                                      code_of(out), dim, rstd && !rms ? rstd + n : nullptr, rstd, stream_of(x)));
   return y;
 }
 
-struct Norm : public torch::autograd::Function<Norm> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const MaybeTensor& gain_, const MaybeTensor& shift_, bool plus_one,
-                        bool rms, double eps, int64_t out) {
-    const Tensor gain = get(gain_), shift = get(shift_);
-    const Tensor r = rows(x);
-    Tensor mean, rstd, y = norm_forward(x, r, gain, shift, plus_one, rms, eps, (at::ScalarType)out, &mean, &rstd);
-    ctx->save_for_backward({r, gain, mean, rstd});
-    ctx->saved_data["how"] = (int64_t)(plus_one | rms << 1);
-    ctx->saved_data["x"] = x.sizes();
-    if (shift.defined()) ctx->saved_data["shift"] = shift.sizes();
-    return y;
+struct NormBackward : public torch::autograd::Node {
+  SavedVariable x, gain, stats;
+  std::vector<int64_t> x_sizes, shift_sizes;
+  bool plus_one = false, rms = false, shifted = false;
+  std::string name() const override { return rms ? "RmsNormBackward" : "LayerNormBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* s : {&x, &gain, &stats}) s->reset_data();
   }
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const variable_list s = ctx->get_saved_variables();
-    variable_list res(7);
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list res(3);
+    if (!grads[0].defined()) return res;
+    const Tensor sx = x.unpack(), sg = gain.unpack();
     {
-      at::NoGradGuard none;
+      at::AutoDispatchBelowADInplaceOrView below;
       c10::DeviceGuard guard(grads[0].device());
-      const Tensor d = rows(grads[0]), r = rows(s[0]), mean = s[2], rstd = s[3];
-      const Params p = params(s[1], Tensor());
-      const int64_t how = ctx->saved_data["how"].toInt(), n = r.size(0), dim = r.size(1);
-      const bool need_gain = s[1].defined() && ctx->needs_input_grad(1);
-      const bool need_shift = ctx->saved_data.count("shift") != 0 && ctx->needs_input_grad(2), sums = need_gain || need_shift;
-      if (ctx->needs_input_grad(0)) res[0] = at::empty(ctx->saved_data["x"].toIntVector(), r.options());
-      auto make = [&](at::IntArrayRef size) { return n > 0 ? at::empty(size, s[1].options()) : at::zeros(size, s[1].options()); };
-      if (need_gain) res[1] = make(s[1].sizes());
-      if (need_shift) res[2] = make(ctx->saved_data["shift"].toIntVector());
+      const Tensor d = rows(grads[0]), r = rows(sx), stats = whole(this->stats);
+      const Params p = params(sg, Tensor());
+      const int64_t n = r.size(0), dim = r.size(1);
+      const bool need_gain = sg.defined() && task_should_compute_output(1), need_shift = shifted && task_should_compute_output(2);
+      if (task_should_compute_output(0)) res[0] = at::empty(x_sizes, r.options());
+      auto make = [&](at::IntArrayRef size) { return n > 0 ? at::empty(size, sg.options()) : at::zeros(size, sg.options()); };
+      if (need_gain) res[1] = make(sg.sizes());
+      if (need_shift) res[2] = make(shift_sizes);
       if (n > 0) {
-        const int64_t bytes = sums ? api.norm_workspace(n / p.groups, p.groups, (int)dim) : 0;
+        const int64_t bytes = need_gain || need_shift ? api.norm_workspace(n / p.groups, p.groups, (int)dim) : 0;
         check("icsa_norm_bwd_workspace_size", bytes);
         const Tensor ws = workspace(bytes, r);
         check("icsa_norm_bwd", api.norm_bwd(d.data_ptr(), code_of(d.scalar_type()), row_stride(d), r.data_ptr(), code_of(r.scalar_type()),
-                                            row_stride(r), n / p.groups, p.groups, (int)dim, at_or_null(p.gain), p.code, p.stride,
-                                            (int)(how & 1), (int)(how >> 1), (const float*)at_or_null(mean), (const float*)rstd.data_ptr(),
-                                            at_or_null(res[0]), dim, at_or_null(res[1]), at_or_null(res[2]), at_or_null(ws), bytes,
-                                            stream_of(r)));
+                                            row_stride(r), n / p.groups, p.groups, (int)dim, at_or_null(p.gain), p.code, p.stride, plus_one,
+                                            rms, rms ? nullptr : (const float*)stats.data_ptr() + n, (const float*)stats.data_ptr(),
+                                            at_or_null(res[0]), dim, at_or_null(res[1]), at_or_null(res[2]), at_or_null(ws), bytes, stream_of(r)));
       }
     }
     return once(std::move(res));
@@ -308,11 +344,29 @@ struct Norm : public torch::autograd::Function<Norm> {
 
 Tensor norm(const Tensor& x, const MaybeTensor& gain_, const MaybeTensor& shift_, bool plus_one, bool rms, double eps, at::ScalarType out) {
   const Tensor gain = get(gain_), shift = get(shift_);
+  std::shared_ptr<NormBackward> node;
   if (wants_grad({&x, &gain, &shift})) {
     refuse_capture({&x, &gain, &shift});
-    return Norm::apply(x, gain_, shift_, plus_one, rms, eps, (int64_t)out);
+    node = make_node<NormBackward>(x, gain, shift);
   }
-  return norm_forward(x, rows(x), gain, shift, plus_one, rms, eps, out, nullptr, nullptr);
+  Tensor r, y, stats;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    r = rows(x);
+    y = norm_forward(x, r, gain, shift, plus_one, rms, eps, out, node ? &stats : nullptr);
+  }
+  if (node) {
+    torch::autograd::set_history(y, node);
+    node->x = SavedVariable(r.is_alias_of(x) ? x : r, false);            // x itself: its changes in place are seen
+    node->gain = SavedVariable(gain, false);
+    node->stats = SavedVariable(stats, false);
+    node->x_sizes = x.sizes().vec();
+    node->plus_one = plus_one;
+    node->rms = rms;
+    node->shifted = shift.defined();
+    if (shift.defined()) node->shift_sizes = shift.sizes().vec();
+  }
+  return y;
 }
 
 // ------------------------------------------------------------------------------------------ rotary positions
@@ -348,29 +402,26 @@ std::pair<Tensor, Tensor> rotate(const Tensor& q_, const Tensor& k_, const Tenso
   return {y[0], y[1]};
 }
 
-struct Rotary : public torch::autograd::Function<Rotary> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& q, const MaybeTensor& k_, const Tensor& cos, const Tensor& sin,
-                               const Tensor& pos, std::vector<int64_t> sections, bool interleaved) {
-    const Tensor k = get(k_);
-    ctx->set_materialize_grads(false);
-    ctx->save_for_backward({cos, sin, pos});
-    auto y = rotate(q, k, cos, sin, pos, sections, interleaved, false);
-    ctx->saved_data["sections"] = std::move(sections);
-    ctx->saved_data["interleaved"] = interleaved;
-    if (!k.defined()) return {y.first};
-    return {y.first, y.second};
+struct RotaryBackward : public torch::autograd::Node {
+  SavedVariable cos, sin, pos;
+  std::vector<int64_t> sections;
+  bool interleaved = true;
+  std::string name() const override { return "RotaryBackward"; }
+
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (SavedVariable* s : {&cos, &sin, &pos}) s->reset_data();
   }
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const variable_list s = ctx->get_saved_variables();
-    variable_list res(7);
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    variable_list res(2);
     {
-      at::NoGradGuard none;
-      const Tensor dq = ctx->needs_input_grad(0) ? grads[0] : Tensor();
-      const Tensor dk = grads.size() > 1 && ctx->needs_input_grad(1) ? grads[1] : Tensor();
-      if (dq.defined() || dk.defined())
-        std::tie(res[0], res[1]) = rotate(dq, dk, s[0].contiguous(), s[1].contiguous(), s[2].contiguous(),
-                                          ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), true);
+      at::AutoDispatchBelowADInplaceOrView below;
+      const Tensor c = whole(cos), s = whole(sin), p = whole(pos);
+      const Tensor dq = task_should_compute_output(0) ? grads[0] : Tensor();
+      const Tensor dk = grads.size() > 1 && task_should_compute_output(1) ? grads[1] : Tensor();
+      if (dq.defined() || dk.defined()) std::tie(res[0], res[1]) = rotate(dq, dk, c, s, p, sections, interleaved, true);
     }
     return once(std::move(res));
   }
@@ -379,12 +430,27 @@ struct Rotary : public torch::autograd::Function<Rotary> {
 variable_list rotary(const Tensor& q, const MaybeTensor& k_, const Tensor& cos, const Tensor& sin, const Tensor& pos,
                      std::vector<int64_t> sections, bool interleaved) {
   const Tensor k = get(k_), c = cos.contiguous(), s = sin.contiguous(), p = pos.contiguous();
+  std::shared_ptr<RotaryBackward> node;
   if (wants_grad({&q, &k})) {
     refuse_capture({&q, &k});
-    return Rotary::apply(q, k_, c, s, p, std::move(sections), interleaved);
+    node = make_node<RotaryBackward>(q, k);
   }
-  auto y = rotate(q, k, c, s, p, sections, interleaved, false);
-  return k.defined() ? variable_list{y.first, y.second} : variable_list{y.first};
+  variable_list out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto y = rotate(q, k, c, s, p, sections, interleaved, false);
+    out.push_back(y.first);
+    if (k.defined()) out.push_back(y.second);
+  }
+  if (node) {
+    torch::autograd::set_history(out, node);
+    node->cos = SavedVariable(c, false);
+    node->sin = SavedVariable(s, false);
+    node->pos = SavedVariable(p, false);
+    node->sections = std::move(sections);
+    node->interleaved = interleaved;
+  }
+  return out;
 }
 
 }  // namespace

@@ -12,7 +12,7 @@
 //
 // What bounds it: the bytes.  65,520 f32 rows of 5,120 into bf16 take 380 us (2.0 GB, 5.3 TB/s) and back 597 (3.4 GB, 5.6; a large copy
 // reaches 4.9, its half of reads less); 28,080 bf16 rows with a scale and shift 110 and 184; 9,373 of 1,536 15.5 and 20.5.  6 rows: 5.3, and 6.2
-// and 5.6 for the two kernels back, which is launch and two trips to memory; the call is the host's 70 us.
+// and 5.6 for the two kernels back, which is launch and two trips to memory; the call is the host's 63 us.
 #include "icsa_kernels.h"
 
 #define NM_THREADS 256

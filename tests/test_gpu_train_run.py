@@ -260,6 +260,51 @@ def test_saved_tensors_moved_and_changed(gpu):
         y.float().sum().backward()
 
 
+class _Nothing(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return x * 1
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+def test_the_graphs_rules(gpu):
+    """A graph used twice, a result changed in place, no gradient for a result, views of it, forward-mode derivatives."""
+    x = torch.randn(2, 9, 128, device=gpu, requires_grad=True)
+    q = torch.randn(1, 9, 2, 64, device=gpu).to(BF).requires_grad_()
+    table, pos = rotary_table(9, 64), torch.arange(9, dtype=torch.int32, device=gpu)
+    calls = [(x, lambda t: layer_norm_func(t)), (x, lambda t: rms_norm_func(t)), (q, lambda t: cross_attn_func(t, t, t)),
+             (q, lambda t: rotary_func(t, None, *table, pos))]
+    for t, f in calls:
+        y = f(t)
+        dy = torch.randn_like(y)
+        assert y.requires_grad and y.is_leaf is False and not f(t.detach()).requires_grad
+        want, = torch.autograd.grad(y, t, dy, retain_graph=True)
+        assert torch.equal(torch.autograd.grad(y, t, dy)[0], want)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, t, dy)
+        got, = torch.autograd.grad(_Nothing.apply(f(t)), t, dy, allow_unused=True)
+        assert got is None
+        part, = torch.autograd.grad(f(t)[:, :4], t, dy[:, :4])
+        assert torch.equal(part, torch.autograd.grad(f(t), t, torch.cat([dy[:, :4], torch.zeros_like(dy[:, 4:])], 1))[0])
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(NotImplementedError):
+                f(torch.autograd.forward_ad.make_dual(t.detach(), dy.to(t.dtype)))
+    y = cross_attn_func(q, q, q)                            # its backward reads the result
+    with torch.no_grad():
+        y.mul_(2)
+    with pytest.raises(RuntimeError):
+        y.float().sum().backward()
+    u = x * 1
+    y = layer_norm_func(u.view(18, 128))                    # saved by a view
+    with torch.no_grad():
+        u.add_(1)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
 def test_backward_into_grads_and_accumulation(gpu):
     t = _tensors(gpu, 4)
     want = _step(t)[1:]
