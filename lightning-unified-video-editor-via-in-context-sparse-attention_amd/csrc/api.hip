@@ -689,7 +689,7 @@ AttnBwdLayout attn_bwd_layout(int B, int Sq, int Sk, int H, int Hk, int D, AttnB
 int64_t icsa_cross_attn_bwd_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs) {
   if (check_masked_sizes(B, Sq, Sk, H, Hk, D)) return -1;
   if (docs < 1) return fail(ICSA_EINVAL, "docs=%d", docs), -1;
-  return attn_bwd_layout(B, Sq, Sk, H, Hk, D, attn_bwd_plan(B, Sq, Sk, H, Hk, docs)).total;
+  return attn_bwd_layout(B, Sq, Sk, H, Hk, D, attn_bwd_plan(B, Sq, Sk, H, Hk, D, docs)).total;
 }
 
 int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t do_sh,
@@ -729,7 +729,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
   auto far = [&](int64_t ss, int64_t sh) { return ss > most / 65 || (G > 1 && sh > (most - 65 * ss) / G); };
   if (k_ss > most / 65 || v_ss > most / 65 || far(q_ss, q_sh) || far(do_ss, do_sh))
     return fail(ICSA_EUNSUPPORTED, "64 rows of q, dout, k and v must lie within 2 GiB");
-  const AttnBwdPlan plan = attn_bwd_plan(B, Sq, Sk, H, Hk, docs);
+  const AttnBwdPlan plan = attn_bwd_plan(B, Sq, Sk, H, Hk, D, docs);
   const AttnBwdLayout L = attn_bwd_layout(B, Sq, Sk, H, Hk, D, plan);
   if (L.total > 0 && (!workspace || workspace_bytes < L.total || !aligned16(workspace)))
     return fail(ICSA_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)L.total);

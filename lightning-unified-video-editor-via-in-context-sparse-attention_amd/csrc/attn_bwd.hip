@@ -5,7 +5,7 @@
 // Two kernels of one body, without atomics, so that the same inputs give the same bits: query-major (dq, and D on the way)
 // and key-major (dk, dv), which compute S and dP each.  A workgroup of 4 waves holds 128 rows of one side in registers, 32 a
 // wave (queries with dO, or keys with values), and walks the other side in tiles of 64 rows, whose two row-major arrays arrive by
-// direct global->LDS loads, two buffers, one barrier a tile; two workgroups share a CU.  Products by v_mfma_f32_32x32x16_bf16: S
+// direct global->LDS loads, two buffers, one barrier a tile; two workgroups share a CU, three with heads of 64.  Products by v_mfma_f32_32x32x16_bf16: S
 // and dP with the tile's rows as the first operand and the held rows as the second, so that a lane holds one of its wave's rows; P
 // and dS go from there to the second products, whose first operand is read transposed from the same tile.  Where few blocks of a
 // side exist, the walk is cut in parts, whose f32 sums a third kernel joins.
@@ -34,7 +34,6 @@
 #define AB_THREADS 256
 #define AB_WAVES 4
 #define AB_ROWS (32 * AB_WAVES)                         // held by a workgroup
-#define AB_AHEAD 3                                    // operands read ahead of their products
 #define AB_SCRATCH_WAVE (3 * 1024)                    // staged output rows, at most 2 KB; in the loop: ranges, operands
 #define AB_CTL_BYTES 256
 #define AB_LOG2E 1.4426950408889634f
@@ -78,7 +77,7 @@ template <int D> constexpr int ab_lds() { return 4 * BTile<D>::kBytes + 2 * 512 
 
 // FINE: P and dS as two bf16 each, where the queries are one tile
 template <int D, bool KV, bool FINE>
-__global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : 2) icsa_attn_bwd_kernel(AttnBwdParams p) {
+__global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : D == 64 ? 3 : 2) icsa_attn_bwd_kernel(AttnBwdParams p) {
   typedef BTile<D> T;
   constexpr int kSteps = D / 16, kSub = D / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -292,11 +291,13 @@ __global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : 2) icsa_attn_bwd_kernel
         }
       }
     }
-    // The tile's products in one stream of phases of kSteps each, an operand read AB_AHEAD products ahead of its use, the
-    // elementwise work of one phase between the products of the next:
-    //   key-major     S, dP | P, dv | dS, dk of either 32 rows in turn
+    // The tile's products in one stream of phases of kSteps each, an operand read kAhead products ahead of its use; query-major, the
+    // elementwise work of one phase between the products of the next (key-major has no registers for that):
+    //   key-major     S, dP | P, dS | dv, dk of either 32 rows in turn
     //   query-major   S0, dP0 | P0, S1 | dS0, dP1 | P1, dq0 | dS1, dq1
-    constexpr bool kSpread = !KV || D == 64;
+    // Key-major with 64 dims: spread out too, and operands three ahead, it takes 184 registers instead of 168, and a third workgroup on
+    // the CU is worth more (65,520 queries over 512 keys, 40 heads: 693 us, 682 with three, 649 with parts for three).
+    constexpr int kAhead = KV && D == 64 ? 2 : 3;
     constexpr int kPhases = KV ? 8 : 6, kOps = kPhases * kSteps, kEl = 16 / kSteps;
     static constexpr int kWhat[8] = {0, 1, KV ? 2 : 0, KV ? 3 : 1, KV ? 0 : 3, KV ? 1 : 3, 2, 3};      // S, dP, dv, dk (dq)
     static constexpr int kOf[8] = {0, 0, KV ? 0 : 1, KV ? 0 : 1, KV ? 1 : 0, 1, 1, 1};                  // which 32 rows
@@ -362,12 +363,12 @@ __global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : 2) icsa_attn_bwd_kernel
     start(0);
     if (!KV) start(1);
 #pragma unroll
-    for (int x = 0; x < AB_AHEAD; ++x) op(x);
+    for (int x = 0; x < kAhead; ++x) op(x);
     each(std::make_integer_sequence<int, kOps>{}, [&](auto number) __attribute__((always_inline)) {
       constexpr int x = decltype(number)::value, ph = x / kSteps, what = kWhat[ph], sub = kOf[ph], i = x % kSteps;
       if (KV && x == 4 * kSteps) start(1);
-      if (x + AB_AHEAD < kOps) op(x + AB_AHEAD);
-      if (what == 0 && i == kSteps - AB_AHEAD) second[sub] = kLent ? lent[64] : b2[0];
+      if (x + kAhead < kOps) op(x + kAhead);
+      if (what == 0 && i == kSteps - kAhead) second[sub] = kLent ? lent[64] : b2[0];
       if (what == 0) s[sub] = mfma32x32x16(a[x], i == 0 ? first[sub] : b1[i], s[sub]);
       else if (what == 1) dp[sub] = mfma32x32x16(a[x], i == 0 ? second[sub] : b2[i], dp[sub]);
       else if (what == 2) acc2[i % kSub] = mfma32x32x16(a[x], pf[sub][i / kSub], acc2[i % kSub]);
@@ -376,31 +377,27 @@ __global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : 2) icsa_attn_bwd_kernel
         if (what == 2) acc2[i % kSub] = mfma32x32x16(a[x], pl[sub][i / kSub], acc2[i % kSub]);
         if (what == 3) acc1[i % kSub] = mfma32x32x16(a[x], dl[sub][i / kSub], acc1[i % kSub]);
       }
+      if constexpr (KV) {
+        if (what == 1 && i == kSteps - 1) {
 #pragma unroll
-      for (int e = i * kEl; e < (i + 1) * kEl; ++e) {
-        if (KV) {
-          if (kSpread && what == 1) weights(sub, e);
-          else if (kSpread && what == 2) slopes(sub, e);
-        } else {
+          for (int e = 0; e < 16; ++e) { weights(sub, e); slopes(sub, e); }
+          if (partial) {
+            clear(pf[sub], sub);
+            clear(df[sub], sub);
+            if (FINE) { clear(pl[sub], sub); clear(dl[sub], sub); }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = i * kEl; e < (i + 1) * kEl; ++e) {
           if (ph == 1) weights(0, e);
           else if (ph == 2) slopes(0, e);
           else if (ph == 3) weights(1, e);
           else if (ph == 4) slopes(1, e);
         }
-      }
-      if (!kSpread && i == kSteps - 1 && what == 1) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) { weights(sub, e); slopes(sub, e); }
-      }
-      if (i == kSteps - 1 && partial) {
-        if (KV) {
-          if (what == 1) clear(pf[sub], sub);
-          if (what == (kSpread ? 2 : 1)) clear(df[sub], sub);
-          if (FINE && what == 1) clear(pl[sub], sub);
-          if (FINE && what == (kSpread ? 2 : 1)) clear(dl[sub], sub);
-        } else {
-          if (ph == 2 || ph == 4) clear(df[ph / 4], ph / 4);
-          if (FINE && (ph == 2 || ph == 4)) clear(dl[ph / 4], ph / 4);
+        if (i == kSteps - 1 && partial && (ph == 2 || ph == 4)) {
+          clear(df[ph / 4], ph / 4);
+          if (FINE) clear(dl[ph / 4], ph / 4);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -472,7 +469,7 @@ __global__ void __launch_bounds__(256) icsa_attn_bwd_join_kernel(AttnBwdParams p
   }
 }
 
-#define AB_SLOTS 512                                  // workgroups that the chip holds: two a CU
+#define AB_CUS 256
 #define AB_MAX_SPLIT 64
 #define AB_FINE 64                                    // queries (of a key head's group) up to which P and dS are two bf16
 #define AB_MIN_TILES 8                                // of the walked side that a part is worth
@@ -485,13 +482,20 @@ namespace {
 // walk both: there, where rounds are few, four parts at least and two rounds of workgroups (dk and dv: 4 clips of 1,500 to 17,600
 // tokens over 320 to 370 keys, 440 items, 1,274 us in one part, 878 in two, 766 in four, 762 in eight; of 8,190 tokens each 794, 700,
 // 698 in one, two, four; 5 of 30,000 tokens together over 512 keys, 160 items, 624 in four, 531 in seven; 2 of 20,000 over 1,000,
-// 96 items, 251 in four, 229 in eleven).
-int parts(int64_t items, int64_t tiles, int docs, int slots) {
+// 96 items, 251 in four, 229 in eleven).  With heads of 64 a CU holds three workgroups, of which one alone makes about 0.6 of the
+// rate and two 0.93: a round of one or two a CU takes that much less time (8,192 x 8,192, 8 heads: 270 in one part, 282 in three;
+// 65,520 over 512, 40 heads: 889 in eight, 907 in nine, 935 in three, with the row sums' 260).
+int parts(int64_t items, int64_t tiles, int docs, int D) {
+  const int slots = AB_CUS * (D == 64 ? 3 : 2);
+  auto rounds = [&](int64_t n) {
+    const int64_t last = n % slots, cu = (last + AB_CUS - 1) / AB_CUS;
+    return (double)(n / slots) + (cu == 0 ? 0. : D != 64 || cu == 3 ? 1. : cu == 2 ? 0.72 : 0.56);
+  };
   int best = 1;
   double time = 0.;
   const int64_t walk = tiles / docs > 0 ? tiles / docs : 1;
   for (int n = 1; n <= AB_MAX_SPLIT && (n == 1 || walk / n >= AB_MIN_TILES); ++n) {
-    const double t = (double)((items * n + slots - 1) / slots) / n + (n > 1 ? items * n / (65. * walk) : 0.);
+    const double t = rounds(items * n) / n + (n > 1 ? items * n / (65. * walk) : 0.);
     if (n == 1 || t < time) { time = t; best = n; }
   }
   if (docs > 1 && items <= 2 * slots)
@@ -530,10 +534,10 @@ hipError_t run_bwd(const AttnBwdParams& p, hipStream_t stream) {
 
 }  // namespace
 
-AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, int docs) {
+AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, int D, int docs) {
   const int64_t BH = (int64_t)B * Hk, n_q = (int64_t)Sq * (H / Hk);
-  return AttnBwdPlan{parts(BH * blocks(n_q), (Sk + ATT_BN - 1) / ATT_BN, docs, AB_SLOTS),
-                     parts(BH * blocks(Sk), (n_q + ATT_BN - 1) / ATT_BN, docs, AB_SLOTS)};
+  return AttnBwdPlan{parts(BH * blocks(n_q), (Sk + ATT_BN - 1) / ATT_BN, docs, D),
+                     parts(BH * blocks(Sk), (n_q + ATT_BN - 1) / ATT_BN, docs, D)};
 }
 
 hipError_t launch_attn_bwd(AttnBwdParams p, hipStream_t stream) {

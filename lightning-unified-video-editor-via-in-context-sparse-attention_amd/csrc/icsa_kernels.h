@@ -319,7 +319,7 @@ struct AttnBwdParams {
 };
 // parts that a query block's keys and a key block's rows are cut into
 struct AttnBwdPlan { int q_split, k_split; };
-AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, int docs);
+AttnBwdPlan attn_bwd_plan(int B, int Sq, int Sk, int H, int Hk, int D, int docs);
 hipError_t launch_attn_bwd(AttnBwdParams p, hipStream_t stream);
 
 // ---------------------------------------------------------------- layer norm, RMS norm (norm.hip)
