@@ -797,7 +797,7 @@ int icsa_norm_fwd(const void* x, int x_dtype, int64_t x_ss, int64_t rows, int gr
 
 int64_t icsa_norm_bwd_workspace_size(int64_t rows, int groups, int dim) {
   if (check_norm(ICSA_F32, ICSA_F32, rows, groups, dim, nullptr, nullptr, ICSA_F32)) return -1;
-  if (rows == 0) return 0;
+  if (rows == 0 || norm_bwd_few(rows, groups)) return 0;
   return align256((int64_t)groups * norm_bwd_workgroups(rows, dim, groups) * 2 * ((dim + 3) & ~3) * 4);
 }
 
@@ -823,7 +823,7 @@ int icsa_norm_bwd(const void* dy, int dy_dtype, int64_t dy_ss, const void* x, in
   p.gain = gain; p.p_dtype = p_dtype; p.p_sg = p_sg; p.plus_one = plus_one != 0; p.rms = rms != 0;
   p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
   p.dy = dy; p.y_dtype = dy_dtype; p.dy_ss = dy_ss; p.dx = dx; p.dx_ss = dx_ss; p.dgain = dgain; p.dshift = dshift;
-  p.part = sums ? reinterpret_cast<float*>(workspace) : nullptr;
+  p.part = need > 0 ? reinterpret_cast<float*>(workspace) : nullptr;
   p.vec_x = whole_chunks(x, x_ss, rows * groups, dim, elsize(x_dtype));
   p.vec_y = whole_chunks(dy, dy_ss, rows * groups, dim, elsize(dy_dtype));
   p.vec_dx = whole_chunks(dx, dx_ss, rows * groups, dim, elsize(x_dtype));

@@ -341,6 +341,7 @@ struct NormParams {
   int n_wg;                                       // workgroups a group (set by the launch)
   int vec_x, vec_y, vec_dx, vec_p;                // rows of whole, aligned 8-element chunks (p: gain and shift)
 };
+bool norm_bwd_few(int64_t rows, int groups);          // no workspace
 int norm_bwd_workgroups(int64_t rows, int dim, int groups);
 hipError_t launch_norm_fwd(NormParams p, hipStream_t stream);
 hipError_t launch_norm_bwd(NormParams p, hipStream_t stream);

@@ -11,14 +11,16 @@
 // kernel adds them in a fixed order (the same inputs give the same bits).
 //
 // What bounds it: the bytes.  65,520 f32 rows of 5,120 into bf16 take 380 us (2.0 GB, 5.3 TB/s) and back 597 (3.4 GB, 5.6; a large copy
-// reaches 4.9, its half of reads less); 28,080 bf16 rows with a scale and shift 110 and 184; 9,373 of 1,536 15.5 and 20.5.  6 rows: 5.3, and 6.2
-// and 5.6 for the two kernels back, which is launch and two trips to memory; the call is the host's 63 us.
+// reaches 4.9, its half of reads less); 28,080 bf16 rows with a scale and shift 110 and 184; 9,373 of 1,536 15.5 and 20.5.  6 rows: 5.3 and
+// 9.7, launch and two trips to memory; the call is the host's.
 #include "icsa_kernels.h"
 
 #define NM_THREADS 256
 #define NM_MAX_THREADS 512                            // 8,192 elements, two chunks of 8 a thread
 #define NM_WAVES 1024                                 // one a SIMD
-#define NM_FEW_ROWS 2                                 // one workgroup a group: 6 rows of 5,120 took it 18 us, six and the second kernel 14
+#define NM_FEW_ROWS 2                                 // of a group: one workgroup, which needs no second kernel
+#define NM_FEW_TOTAL 8                                // rows of all groups, back: columns instead of rows to workgroups, in one launch
+#define NM_FEW_COLS 512
 
 namespace {
 
@@ -316,6 +318,70 @@ __global__ void __launch_bounds__(LPR == 0 ? NM_MAX_THREADS : NM_THREADS) icsa_n
   }
 }
 
+// Backward of few rows in one launch: a workgroup takes NM_FEW_COLS columns of a group's rows, the sums over whole rows for itself, a
+// row a wave, and adds its columns' da and db over the rows in their order.  One launch and no workspace, 4 us of the host's time, against the two
+// kernels' time: 8 rows of 5,120 f32 elements 10.4 us and 8.4 with a launch between them, of 1,536 6.4 and 6.6, of 128 4.9 and 5.0; 16 rows
+// of 5,120 16.3 and 8.6.
+template <typename TX, typename TY, bool RMS>
+__global__ void __launch_bounds__(NM_FEW_COLS) icsa_norm_bwd_few_kernel(NormParams p) {
+  __shared__ float sums[NM_FEW_TOTAL][2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = blockIdx.y, rows = (int)p.rows;
+  const int64_t row0 = (int64_t)g * p.rows;
+  const TX* x = reinterpret_cast<const TX*>(p.x) + row0 * p.x_ss;
+  const TY* dy = reinterpret_cast<const TY*>(p.dy) + row0 * p.dy_ss;
+  if (p.dx != nullptr) {
+    for (int r = wave; r < rows; r += NM_FEW_COLS / 64) {
+      const float mean = RMS ? 0.f : p.mean[row0 + r], rstd = p.rstd[row0 + r];
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll 4
+      for (int d = 8 * lane; d < p.dim; d += 512) {
+        const int n[1] = {p.dim - d};
+        Raw8<TX> vx;
+        Raw8<TY> vy;
+        float a[1][8];
+        vx.load(x + r * p.x_ss + d, n[0], p.vec_x);
+        vy.load(dy + r * p.dy_ss + d, n[0], p.vec_y);
+        load_params<1>(p, p.gain, g * p.p_sg + d, 0, 0, a, n, 1.f, p.plus_one ? 1.f : 0.f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float u = vy.at(e) * a[0][e];         // 0 past the row's end
+          s0 = fmaf(u, e < n[0] ? (vx.at(e) - mean) * rstd : 0.f, s0);
+          s1 += u;
+        }
+      }
+      s0 = lanes_sum<64>(s0);
+      s1 = lanes_sum<64>(s1);
+      if (lane == 0) { sums[r][0] = s0; sums[r][1] = s1; }
+    }
+    __syncthreads();
+  }
+  const int d = blockIdx.x * NM_FEW_COLS + threadIdx.x;
+  if (d >= p.dim) return;
+  const float inv_n = 1.f / (float)p.dim;
+  const int64_t at = g * p.p_sg + d;
+  const float a = p.gain == nullptr ? 1.f : (p.plus_one ? 1.f : 0.f) + (p.p_dtype == ICSA_DT_F32 ? reinterpret_cast<const float*>(p.gain)[at] :
+                                                                        (float)reinterpret_cast<const bf16*>(p.gain)[at]);
+  float da = 0.f, db = 0.f;
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    const float mean = RMS ? 0.f : p.mean[row0 + r], rstd = p.rstd[row0 + r];
+    const float v = (float)dy[r * p.dy_ss + d], xh = ((float)x[r * p.x_ss + d] - mean) * rstd;
+    da = fmaf(v, xh, da);
+    db += v;
+    if (p.dx != nullptr) {
+      const float m1 = sums[r][0] * inv_n, m0 = RMS ? 0.f : sums[r][1] * inv_n;
+      reinterpret_cast<TX*>(p.dx)[(row0 + r) * p.dx_ss + d] = (TX)(rstd * (v * a - m0 - xh * m1));
+    }
+  }
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    void* const out = which ? p.dshift : p.dgain;
+    if (out == nullptr) continue;
+    if (p.p_dtype == ICSA_DT_F32) reinterpret_cast<float*>(out)[(int64_t)g * p.dim + d] = which ? db : da;
+    else reinterpret_cast<bf16*>(out)[(int64_t)g * p.dim + d] = (bf16)(which ? db : da);
+  }
+}
+
 // da and db of a group from its workgroups' sums: 64 columns a workgroup, 16 threads of 4 columns by 16 shares of the parts
 __global__ void __launch_bounds__(256) icsa_norm_join_kernel(NormParams p) {
   __shared__ __attribute__((aligned(16))) float all[16][64];
@@ -354,7 +420,7 @@ int threads_of(int dim) { return dim <= 256 ? 16 : dim <= 1024 ? 64 : dim <= 614
 // Workgroups that a group of rows is dealt to, over all groups, as few as leave no round incomplete by much: three waves a SIMD
 // forward (5,120 f32 elements, 65,520 rows: 394 us, with four 414; 1,000 bf16 elements, 40,000 rows: 40 and 44), four where a row
 // takes eight waves (8,192 elements: 134 us, with three 155); four back, two where their registers leave no more (28,080
-// rows of 5,120: 185, with one and a half 214).  Few rows back: one workgroup, which needs no second kernel for the parameters' gradients.
+// rows of 5,120: 185, with one and a half 214).  Few rows of a group back: one workgroup, which needs no second kernel for the parameters' gradients (2 rows of 1,536: 4.9 us).
 int workgroups(int64_t rows, int dim, int groups, bool back) {
   const int t = threads_of(dim), waves = t <= 64 ? 4 : t / 64;
   const int64_t per = t <= 64 ? NM_THREADS / t : 1, n = (rows + per - 1) / per;
@@ -374,7 +440,9 @@ void go(const NormParams& p, bool back, hipStream_t stream) {
 template <typename TX, typename TY, bool RMS>
 void by_size(const NormParams& p, bool back, hipStream_t stream) {
   const int n = p.dim;
-  if (n <= 128) go<TX, TY, RMS, 16, 1>(p, back, stream);
+  if (back && norm_bwd_few(p.rows, p.groups))
+    hipLaunchKernelGGL((icsa_norm_bwd_few_kernel<TX, TY, RMS>), dim3((n + NM_FEW_COLS - 1) / NM_FEW_COLS, p.groups), dim3(NM_FEW_COLS), 0, stream, p);
+  else if (n <= 128) go<TX, TY, RMS, 16, 1>(p, back, stream);
   else if (n <= 256) go<TX, TY, RMS, 16, 2>(p, back, stream);
   else if (n <= 512) go<TX, TY, RMS, 64, 1>(p, back, stream);
   else if (n <= 1024) go<TX, TY, RMS, 64, 2>(p, back, stream);
@@ -398,6 +466,8 @@ hipError_t run_norm(const NormParams& p, bool back, hipStream_t stream) {
 
 }  // namespace
 
+bool norm_bwd_few(int64_t rows, int groups) { return rows * groups <= NM_FEW_TOTAL; }
+
 int norm_bwd_workgroups(int64_t rows, int dim, int groups) { return workgroups(rows, dim, groups, true); }
 
 hipError_t launch_norm_fwd(NormParams p, hipStream_t stream) {
@@ -407,6 +477,7 @@ hipError_t launch_norm_fwd(NormParams p, hipStream_t stream) {
 
 hipError_t launch_norm_bwd(NormParams p, hipStream_t stream) {
   p.n_wg = norm_bwd_workgroups(p.rows, p.dim, p.groups);
+  if (norm_bwd_few(p.rows, p.groups)) p.part = nullptr;
   if (p.n_wg == 1 && threads_of(p.dim) > 64) p.part = nullptr;      // written by the workgroup itself
   const hipError_t e = run_norm(p, true, stream);
   if (e != hipSuccess || p.part == nullptr) return e;

@@ -66,6 +66,34 @@ def test_norms(gpu, form, i, dim):
         assert torch.equal(fn(X, *(() if kw else leaves[1:]), **kw, eps=1e-5, out_dtype=yt), y)
 
 
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("G,rows,dim,i", [(1, 8, 5120, 0), (1, 9, 5120, 1), (4, 2, 513, 2), (3, 3, 513, 3), (8, 1, 8192, 0), (9, 1, 8192, 1),
+                                          (2, 4, 77, 2), (2, 4, 1, 1), (1, 1, 7, 0), (3, 30, 1536, 3), (2, 40, 100, 0), (5, 3, 2, 1), (300, 2, 512, 2), (40, 2, 2048, 3)])
+def test_few_rows_and_many_groups(gpu, G, rows, dim, i, rms):
+    """On either side of where columns instead of rows are dealt to workgroups, and of one workgroup a group; strided rows."""
+    xt, yt, pt = TYPES[i]
+    x, dy, a, b = _norm_inputs(G, rows, dim, xt, yt, pt, 5)
+    if rms:
+        x, dy, a = x.reshape(1, G * rows, dim), dy.reshape(1, G * rows, dim), a[:1]
+        val, tol = O.norm(x, dy, a, None, rms=True)
+    else:
+        val, tol = O.norm(x, dy, 1 + a.double(), b)
+    wide = torch.zeros(*x.shape[:-1], dim + 3, dtype=xt, device=gpu)
+    wide[..., 3:] = x.to(gpu)
+    X, A, B = wide[..., 3:].requires_grad_(), a.to(gpu).requires_grad_(), b.to(gpu).requires_grad_()
+    if rms:
+        w = A.detach()[0].clone().requires_grad_()
+        y, leaves = rms_norm_func(X, w, out_dtype=yt), (X, w)
+    else:
+        y, leaves = layer_norm_func(X, scale=A, shift=B, out_dtype=yt), (X, A, B)
+    d = dy.to(gpu)
+    grads = torch.autograd.grad(y, leaves, d, retain_graph=True)
+    for n, got in zip(("y", "dx", "da", "db"), (y.detach(), *grads)):
+        _close(n, got, val[n], tol[n])
+    for n in range(len(leaves)):                             # one at a time
+        assert torch.equal(torch.autograd.grad(y, leaves[n], d, retain_graph=True)[0], grads[n])
+
+
 @pytest.mark.parametrize("rows,dim", [(4000, 64), (2500, 640), (3121, 1536), (1, 8192), (700, 5120)])
 def test_sums_over_many_rows(gpu, rows, dim):
     x, dy, a, b = _norm_inputs(1, rows, dim, BF, BF, F32)

@@ -86,11 +86,11 @@ def test_norms_refuse(back, kw, code):
 def test_norms_refuse_more():
     assert _norm(False, eps=-1.0) == _norm(False, eps=float("nan")) == _norm(False, y=0) == EIN
     assert _norm(True, dy=0) == _norm(True, rstd=0) == _norm(True, rows=0) == EIN
-    assert _norm(True, ws=0) == _norm(True, wsb=4) == _norm(True, ws=PTR + 4) == EWS
+    assert _norm(True, rows=40, ws=0) == _norm(True, rows=40, wsb=4) == _norm(True, rows=40, ws=PTR + 4) == EWS
     assert _norm(False, rows=0, x=0, y=0) == _norm(True, rows=0, dgain=0, dshift=0) == _norm(True, dx=0, dgain=0, dshift=0) == _lib.OK
     L = _lib.lib()
-    assert L.icsa_norm_bwd_workspace_size(1, 1, 5) >= 2 * 8 * 4 and L.icsa_norm_bwd_workspace_size(4, 0, 8) == -1
-    assert L.icsa_norm_bwd_workspace_size(0, 1, 8) == 0
+    assert L.icsa_norm_bwd_workspace_size(9, 1, 5) >= 2 * 8 * 4 and L.icsa_norm_bwd_workspace_size(4, 0, 8) == -1
+    assert L.icsa_norm_bwd_workspace_size(0, 1, 8) == L.icsa_norm_bwd_workspace_size(2, 4, 8192) == 0
 
 
 def _rotary(sections=None, **kw):
