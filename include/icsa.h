@@ -447,7 +447,7 @@ int icsa_cross_attn_fwd(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                         void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Whether rest is worth keeping for the backward: 1 or 0.  documents: q_starts and k_starts are given. */
-int icsa_cross_attn_wants_rest(int Sq, int Sk, int H, int Hk, int documents);
+int icsa_cross_attn_wants_rest(int Sq, int Sk, int H, int Hk, int D, int documents);
 
 /* Workspace bytes of icsa_cross_attn_bwd (rows' sums; sums of parts where a side has few rows). */
 int64_t icsa_cross_attn_bwd_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs);

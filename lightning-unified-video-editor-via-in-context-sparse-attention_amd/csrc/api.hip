@@ -664,11 +664,11 @@ int icsa_cross_attn_fwd(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
 }
 
 // The error of a rounded out reaches dq and dk through rowsum(dout out), the less the more keys share a row's weight: scores of deviation
-// 1.5, dq from the exact one (2-norm), with rest and without: 0.0025, 0.0034 over 4 keys, 0.0024, 0.0026 over 32, 0.0024, 0.0025 over 192,
-// the same from 256 on.  Documents' lengths are on the GPU: with documents it is kept.  It costs a byte of memory a value; 65,520 queries of 40 heads 0.10 ms forward, 0.03 to 0.06 backward
+// 1.5, dq from the exact one (2-norm, in f32 beside the result's own rounding), with rest and without: 0.0019, 0.0030 over 4 keys, 0.00172,
+// 0.0020 over 32, 0.00173, 0.00178 over 226 of 128 dims, where its own roundings leave 0.00166; heads of 64 0.00178 and 0.00185 over 300 to 500.  Documents' lengths are on the GPU: with documents it is kept.  It costs a byte of memory a value; 65,520 queries of 40 heads 0.10 ms forward, 0.03 to 0.06 backward
 // (0.36 and 0.75 over 77 keys, 0.82 and 1.23 over 512).
-int icsa_cross_attn_wants_rest(int Sq, int Sk, int H, int Hk, int documents) {
-  return documents != 0 || Sk <= 256 || (Hk > 0 && (int64_t)Sq * (H / Hk) <= 64);
+int icsa_cross_attn_wants_rest(int Sq, int Sk, int H, int Hk, int D, int documents) {
+  return documents != 0 || Sk <= (D == 64 ? 1024 : 256) || (Hk > 0 && (int64_t)Sq * (H / Hk) <= 128);
 }
 
 namespace {

@@ -75,7 +75,7 @@ template <int D> constexpr int ab_lds() { return 4 * BTile<D>::kBytes + 2 * 512 
 
 }  // namespace
 
-// FINE: P and dS as two bf16 each, where the queries are one tile
+// FINE: P and dS as two bf16 each, where the queries are one block
 template <int D, bool KV, bool FINE>
 __global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : D == 64 ? 3 : 2) icsa_attn_bwd_kernel(AttnBwdParams p) {
   typedef BTile<D> T;
@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : D == 64 ? 3 : 2) icsa_a
   const float c = p.scale * AB_LOG2E;
   floatx16 acc1[kSub] = {};                                               // dq or dk
   floatx16 acc2[KV ? kSub : 1] = {};                                      // dv
+  float total[2] = {};                                                    // query-major: of the row's P
 
   for (int t = t0; t < t1; ++t) {
     const int j0 = u_lo + t * ATT_BN;
@@ -395,6 +396,16 @@ __global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : D == 64 ? 3 : 2) icsa_a
           else if (ph == 3) weights(1, e);
           else if (ph == 4) slopes(1, e);
         }
+        if (i == kSteps - 1 && (ph == 1 || ph == 3)) {
+          const int wd = partial ? (int)(unsigned)((visible() & ~cleared()) >> (16 * (ph - 1) + 4 * hl)) : -1;
+          if (partial) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) total[e & 1] += wd >> (8 * (e >> 2) + (e & 3)) & 1 ? s[ph / 2][e] : 0.f;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) total[e & 1] += s[ph / 2][e];
+          }
+        }
         if (i == kSteps - 1 && partial && (ph == 2 || ph == 4)) {
           clear(df[ph / 4], ph / 4);
           if (FINE) clear(dl[ph / 4], ph / 4);
@@ -418,6 +429,11 @@ __global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : D == 64 ? 3 : 2) icsa_a
     if (seen[128] != 0) f1 = f2 = NAN;
   } else if (lse != lse || !__builtin_isfinite(dd)) {
     f1 = NAN;
+  } else if (n_split == 1) {
+    // lse is the forward's total of rounded weights; P sums to 1 but for that.  It would be a third of what dq is off beside its own roundings
+    // (f32 dq over 226 keys 0.00179 from the exact one, so 0.00173); the sums cost 3 % (65,520 over 512: 1,226 and 1,258 us)
+    const float sum = xhalf_sum(total[0] + total[1]);
+    if (sum > 0.5f && sum < 2.f) f1 /= sum;
   }
   auto finish = [&](const floatx16* acc, float f, const OutView& out, float* part) {
     if (n_split == 1) {
@@ -471,7 +487,7 @@ __global__ void __launch_bounds__(256) icsa_attn_bwd_join_kernel(AttnBwdParams p
 
 #define AB_CUS 256
 #define AB_MAX_SPLIT 64
-#define AB_FINE 64                                    // queries (of a key head's group) up to which P and dS are two bf16
+#define AB_FINE AB_ROWS                               // queries (of a key head's group) up to which P and dS are two bf16
 #define AB_MIN_TILES 8                                // of the walked side that a part is worth
 
 namespace {

@@ -168,7 +168,7 @@ Tensor attn_forward(const Rows& q, const Rows& k, const Rows& v, const Tensor& q
   Tensor out = at::empty({z.B, z.Sq, z.H, z.D}, q.t.options());
   if (lse != nullptr) {
     *lse = at::empty({z.B, z.Hk, z.Sq, z.H / z.Hk}, q.t.options().dtype(at::kFloat));
-    if (api.attn_wants_rest(z.Sq, z.Sk, z.H, z.Hk, qs.defined())) *rest = at::empty({z.B, z.Sq, z.H, z.D}, q.t.options().dtype(at::kByte));
+    if (api.attn_wants_rest(z.Sq, z.Sk, z.H, z.Hk, z.D, qs.defined())) *rest = at::empty({z.B, z.Sq, z.H, z.D}, q.t.options().dtype(at::kByte));
   }
   const int64_t bytes = api.attn_workspace(z.B, z.Sq, z.Sk, z.H, z.Hk, z.D, (int)docs);
   check("icsa_cross_attn_workspace_size", bytes);

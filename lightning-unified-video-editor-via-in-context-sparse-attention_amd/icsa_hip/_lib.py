@@ -205,7 +205,7 @@ _SIGNATURES = {
         _p, _p, _i, _f,
         _p, _l, _l, _l, _p, _p,
         _p, _l, _p]),
-    "icsa_cross_attn_wants_rest": (_i, [_i, _i, _i, _i, _i]),
+    "icsa_cross_attn_wants_rest": (_i, [_i, _i, _i, _i, _i, _i]),
     "icsa_cross_attn_bwd_workspace_size": (_l, [_i, _i, _i, _i, _i, _i, _i]),
     "icsa_cross_attn_bwd": (_i, [
         _p, _l, _l, _l,

@@ -80,7 +80,7 @@ def _check_attn(q, k, v, q_starts, k_starts, softmax_scale):
 def cross_attn_fwd_hip(q, k, v, q_starts=None, k_starts=None, softmax_scale=None):
     """``(out, lse, rest)`` of :func:`cross_attn_func`'s forward: out bfloat16 like q; lse float32 [B, Hk, Sq, H / Hk], log2 of each
     row's sum of ``2 ** (score * log2 e)``, +inf for a row that sees nothing; rest uint8 like out, what its rounding
-    left, or None where that does not show in a gradient (over 256 keys without documents, and over 64 queries)."""
+    left, or None where that does not show in a gradient (without documents: over 256 keys, with heads of 64 over 1,024, and over 128 queries)."""
     sizes, docs, scale, q_starts, k_starts = _check_attn(q, k, v, q_starts, k_starts, softmax_scale)
     B, Sq, Sk, H, Hk, D = sizes
     dev = q.device
@@ -90,7 +90,7 @@ def cross_attn_fwd_hip(q, k, v, q_starts=None, k_starts=None, softmax_scale=None
     out = torch.empty(B, Sq, H, D, dtype=_BF, device=dev)
     lse = torch.empty(B, Hk, Sq, H // Hk, dtype=torch.float32, device=dev)
     L = _lib.lib()
-    rest = torch.empty(B, Sq, H, D, dtype=torch.uint8, device=dev) if L.icsa_cross_attn_wants_rest(Sq, Sk, H, Hk, q_starts is not None) else None
+    rest = torch.empty(B, Sq, H, D, dtype=torch.uint8, device=dev) if L.icsa_cross_attn_wants_rest(Sq, Sk, H, Hk, D, q_starts is not None) else None
     wsp, ws_bytes = 0, L.icsa_cross_attn_workspace_size(*sizes, docs)
     if ws_bytes:
         if ws_bytes < 0:
