@@ -75,9 +75,9 @@ template <int D> constexpr int ab_lds() { return 4 * BTile<D>::kBytes + 2 * 512 
 
 }  // namespace
 
-// FINE: P and dS as two bf16 each, where the queries are one block
+// FINE: P and dS as two bf16 each, where the queries are one block or the keys a few
 template <int D, bool KV, bool FINE>
-__global__ void __launch_bounds__(AB_THREADS, FINE ? 1 : D == 64 ? 3 : 2) icsa_attn_bwd_kernel(AttnBwdParams p) {
+__global__ void __launch_bounds__(AB_THREADS, FINE ? (D == 64 && !KV ? 2 : 1) : D == 64 ? 3 : 2) icsa_attn_bwd_kernel(AttnBwdParams p) {
   typedef BTile<D> T;
   constexpr int kSteps = D / 16, kSub = D / 32;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
@@ -487,7 +487,11 @@ __global__ void __launch_bounds__(256) icsa_attn_bwd_join_kernel(AttnBwdParams p
 
 #define AB_CUS 256
 #define AB_MAX_SPLIT 64
-#define AB_FINE AB_ROWS                               // queries (of a key head's group) up to which P and dS are two bf16
+// P and dS as two bf16 (FINE): up to this many queries of a key head's group, where a call is all start and end; and this many keys,
+// where the one bf16's error shows beside the result's own rounding (600 queries over 2 to 8: dq 1.47 to 1.54 of that rounding, dk 1.49 to 1.57;
+// FINE 1.07 to 1.14 and 1.09 to 1.17) at a price where queries are many (65,520 of 40 heads: dq 785 us and 1,020, dk and dv 288 and 585).
+#define AB_FINE AB_ROWS
+#define AB_FINE_KEYS 8
 #define AB_MIN_TILES 8                                // of the walked side that a part is worth
 
 namespace {
@@ -562,6 +566,6 @@ hipError_t launch_attn_bwd(AttnBwdParams p, hipStream_t stream) {
   p.by_hk = fast_div(p.Hk);
   p.by_qblk = fast_div((unsigned)std::max<int64_t>(1, blocks((int64_t)p.Sq * G)));
   p.by_kblk = fast_div((unsigned)std::max<int64_t>(1, blocks(p.Sk)));
-  if ((int64_t)p.Sq * G <= AB_FINE) return p.D == 128 ? run_bwd<128, true>(p, stream) : run_bwd<64, true>(p, stream);
+  if ((int64_t)p.Sq * G <= AB_FINE || p.Sk <= AB_FINE_KEYS) return p.D == 128 ? run_bwd<128, true>(p, stream) : run_bwd<64, true>(p, stream);
   return p.D == 128 ? run_bwd<128, false>(p, stream) : run_bwd<64, false>(p, stream);
 }

@@ -240,9 +240,9 @@ def test_few_queries_keep_the_weights(gpu, Sq, H, Hk, D):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("Sq,H,Hk,Sk", [(128, 2, 2, 600), (128, 2, 2, 100), (42, 6, 2, 300)])
+@pytest.mark.parametrize("Sq,H,Hk,Sk", [(128, 2, 2, 600), (128, 2, 2, 100), (42, 6, 2, 300), (700, 2, 2, 8), (700, 4, 2, 3)])
 def test_a_block_of_queries_keeps_the_weights(gpu, Sq, H, Hk, Sk, D):
-    """What the forward's rounded weights leave, row by row.  bf16 rounds a weight m 2^e by 2^-8 / (m sqrt 3) of it (deviation), over
+    """And up to 8 keys.  What the forward's rounded weights leave, row by row.  bf16 rounds a weight m 2^e by 2^-8 / (m sqrt 3) of it (deviation), over
     log-uniform m u = 2^-8 sqrt((1 - 1/4) / (2 ln 2) / 3) = 0.00166.  Its total is off by u |p| of itself, which scales the row's P (not
     in dq, which divides by its own total), and D by u |p (dP - D)|.  Rows are independent: 1.5 deviations of their sum, and
     2^-14 for the rest.  One bf16 would add u |dS| to every row."""
