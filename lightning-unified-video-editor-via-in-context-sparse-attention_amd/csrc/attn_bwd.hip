@@ -19,12 +19,13 @@
 // from a NaN of lse or a D that is not finite, which every such row has unless its weight there is 0.
 //
 // What bounds it: the matrix pipe, the elementwise work (an exponential, a multiplication or two and two conversions a pair), the
-// operands' way from LDS and the clock, side by side: 8,192 x 8,192 rows of 8 heads of 128 take 352 us (dq, 1.17 PFLOP/s of its three
-// products) and 455 (dk and dv, 1.21 of four); the same without exponentials 342, without operand reads 299, with neither 274, without
+// operands' way from LDS and the clock, side by side: 8,192 x 8,192 rows of 8 heads of 128 take 372 us (dq, 1.11 PFLOP/s of its three
+// products; 354 without the rows' totals) and 455 (dk and dv, 1.21 of four); the same without exponentials 342, without operand reads 299, with neither 274, without
 // the tiles' loads 327 (dq).  Short walks add a workgroup's start and end: over 512 keys (eight tiles) dq of 65,520 queries of 40 heads
-// takes 1.20 ms (0.86), 0.60 of it for the rows' bytes alone, which the other workgroup of the CU does not hide whole; dk and dv 1.24
-// (1.10; the matrix pipe busy 64 % at 1.6 GHz, in dq 44 % at 1.9).  Tried: 64 held rows a wave, whose operands serve two products (one wave a SIMD, accumulators moved between register
-// files: dq 8,192 x 8,192 402, dk and dv spill); elementwise work between the products of key-major 128 dims (registers); the first tile
+// takes 1.25 ms (0.82), 0.60 of it for the rows' bytes alone, which the other workgroup of the CU does not hide whole; dk and dv 1.24
+// (1.10; the matrix pipe busy 64 % at 1.6 GHz, in dq 44 % at 1.9).  Tried: 64 held rows a wave, whose operands serve two products (one
+// wave a SIMD, accumulators moved between register files: dq 8,192 x 8,192 402, dk and dv spill); elementwise work between the
+// products of key-major 128 dims (registers); the first tile
 // requested before the held rows, starts staggered, the next workgroup's lines requested ahead: no change, or slower.
 #include <algorithm>
 #include <utility>
