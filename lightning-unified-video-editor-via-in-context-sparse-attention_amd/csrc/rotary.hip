@@ -96,8 +96,9 @@ __global__ void __launch_bounds__(RO_THREADS) icsa_rotary_kernel(RotaryParams p)
   for (int i = 0; i < 2; ++i) {
     const int H = p.H[i];
     if (H == 0) continue;
-    // this share's heads, whole passes
-    const int passes = (H + heads - 1) / heads, h_lo = passes * share / p.shares * heads, h_hi = min(H, passes * (share + 1) / p.shares * heads);
+    // this share's heads, whole passes: 2^20 passes by 2^11 shares at most, without a sign in 32 bits
+    const unsigned passes = (unsigned)(H + heads - 1) / heads;
+    const int h_lo = (int)(passes * share / p.shares) * heads, h_hi = min(H, (int)(passes * (share + 1) / p.shares) * heads);
     const T* x = reinterpret_cast<const T*>(p.x[i]) + (int64_t)b * p.sb[i] + (int64_t)s * p.ss[i] + first;
     T* y = reinterpret_cast<T*>(p.y[i]) + (tok * H) * p.D + first;
     for (int hh = h_lo + h0; hh < h_hi; hh += RO_UNROLL * heads) {
