@@ -72,13 +72,18 @@ void check(const char* fn, int64_t code) {
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
-bool wants_grad(std::initializer_list<const Tensor*> ts) {
+// constants: inputs without a gradient, which may have no tangent either
+bool wants_grad(std::initializer_list<const Tensor*> ts, std::initializer_list<const Tensor*> constants = {}) {
+  auto no_tangent = [](const Tensor& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "icsa_hip's training operators have no forward-mode derivative");
+  };
   bool some = false;
   for (const Tensor* t : ts)
     if (t->defined()) {
-      TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "icsa_hip's training operators have no forward-mode derivative");
+      no_tangent(*t);
       some = some || t->requires_grad();
     }
+  for (const Tensor* t : constants) no_tangent(*t);
   return some && c10::GradMode::is_enabled();
 }
 
@@ -429,9 +434,11 @@ struct RotaryBackward : public torch::autograd::Node {
 
 variable_list rotary(const Tensor& q, const MaybeTensor& k_, const Tensor& cos, const Tensor& sin, const Tensor& pos,
                      std::vector<int64_t> sections, bool interleaved) {
-  const Tensor k = get(k_), c = cos.contiguous(), s = sin.contiguous(), p = pos.contiguous();
+  const Tensor k = get(k_);
+  const bool grad = wants_grad({&q, &k}, {&cos, &sin});
+  const Tensor c = cos.contiguous(), s = sin.contiguous(), p = pos.contiguous();
   std::shared_ptr<RotaryBackward> node;
-  if (wants_grad({&q, &k})) {
+  if (grad) {
     refuse_capture({&q, &k});
     node = make_node<RotaryBackward>(q, k);
   }

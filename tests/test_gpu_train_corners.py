@@ -23,3 +23,16 @@ def test_rotary_of_one_token_with_as_many_heads_as_there_may_be(gpu, H):
     del fill
     y = rotary_func(x.expand(1, 1, H, 512), None, cos, sin, pos)
     assert bool((y == want).all())
+
+
+def test_rotary_tables_with_a_tangent_are_refused(gpu):
+    """Forward mode, as with q and k."""
+    q = torch.randn(1, 5, 2, 64, device=gpu)
+    cos, sin = rotary_table(5, 64)
+    pos = torch.arange(5, dtype=torch.int32, device=gpu)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual
+        for c, s in ((dual(cos, -sin), sin), (cos, dual(sin, cos))):
+            for grad in (False, True):
+                with pytest.raises(NotImplementedError), torch.set_grad_enabled(grad):
+                    rotary_func(q, None, c, s, pos)
