@@ -147,25 +147,40 @@ def wan_qk_prologue(yq: torch.Tensor, yk, norm_q_weight: torch.Tensor, norm_k_we
 
 def rope_positions(grid_sizes, source_video_grid_sizes, TAG: int, B: int, S: int, device) -> torch.Tensor:
     """int32 [B, S, 3]: each token's frame, row and column on the target grid, then (TAG 1) on the source grid from 0 again, and
-    -1 for those that rope_apply leaves unrotated (model.py:69-95)."""
+    -1 for those that rope_apply leaves unrotated (model.py:69-95).  The tensor's ``rope_rows`` is the longest axis of all grids,
+    which :func:`wan_qk_trainable` holds against its table."""
+    _require(TAG in (0, 1), "TAG must be 0 or 1")
     pos = torch.full((B, S, 3), -1, dtype=torch.int32)
+    rows = 0
     for b in range(B):
-        at = 0
-        for f, h, w in (_grid(grid_sizes[b]), _grid(source_video_grid_sizes[b]))[:2 if TAG == 1 else 1]:
+        at, grids = 0, (_grid(grid_sizes[b]), _grid(source_video_grid_sizes[b]))
+        for n, grid in enumerate(grids):
+            _require(len(grid) == 3 and min(grid) >= 0, "grid sizes are (frames, rows, columns), not negative")
+            rows = max(rows, *grid)
+            if n > TAG:
+                continue
+            f, h, w = grid
             i = torch.arange(min(f * h * w, S - at), dtype=torch.int32)
             pos[b, at:at + len(i)] = torch.stack([i // (h * w), i // w % h, i % w], 1)
             at += len(i)
-    return pos.to(device)
+    pos = pos.to(device)
+    pos.rope_rows = rows
+    return pos
 
 
 def wan_qk_trainable(yq: torch.Tensor, yk: torch.Tensor, norm_q_weight: torch.Tensor, norm_k_weight: torch.Tensor,
                      positions: torch.Tensor, freqs: torch.Tensor, num_heads: int, eps: float = 1e-6):
     """q and k of WanSelfAttention.forward from the projections yq, yk [B, S, dim], bf16 [B, S, H, D] as
     :func:`wan_qk_prologue` makes them, with gradients to the projections and both norm weights: RMS norm over all heads, then the
-    three-axis rotation at ``positions`` (:func:`rope_positions`).  The normalised row is rounded to bf16 once, after its weight."""
+    three-axis rotation at ``positions`` (:func:`rope_positions`).  The normalised row is rounded to bf16 once, after its weight.
+
+    A grid longer than ``freqs`` has rows is refused, as there.  Positions that come from elsewhere, or as a new tensor made of
+    those, carry no ``rope_rows`` and are on the GPU: a row past the table leaves its pairs as they are (:func:`rotary_func`)."""
     B, S, dim = yq.shape
     _require(yk.shape == yq.shape and dim % num_heads == 0, "yq and yk must be [B, S, dim], dim a multiple of num_heads")
     D = dim // num_heads
+    rows = getattr(positions, "rope_rows", 0)
+    _require(rows <= freqs.shape[0], f"a grid axis of {rows} is longer than the table of {freqs.shape[0]} rows")
     cos, sin = rope_tables(freqs, yq.device)
     third = D // 6
     q, k = (rms_norm_func(y, w, eps=eps, out_dtype=torch.bfloat16).view(B, S, num_heads, D)

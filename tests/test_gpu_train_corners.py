@@ -3,7 +3,9 @@ host does during a call, and results that must not depend on how a launch is div
 import pytest
 import torch
 
-from icsa_hip import rotary_func, rotary_table
+from icsa_hip import rotary_func, rotary_table, wan
+from icsa_hip._lib import IcsaError
+from icsa_hip.hip_host import IcsaArgumentError
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -36,3 +38,21 @@ def test_rotary_tables_with_a_tangent_are_refused(gpu):
             for grad in (False, True):
                 with pytest.raises(NotImplementedError), torch.set_grad_enabled(grad):
                     rotary_func(q, None, c, s, pos)
+
+
+# ------------------------------------------------------------------------------------------
+# the producer in front of the sparse attention
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("grid,src,tag,rows", [((2, 5, 6), (1, 5, 6), 1, 5), ((9, 2, 3), (1, 2, 3), 0, 8), ((1, 2, 3), (1, 2, 9), 1, 8),
+                                               ((1, -2, 3), (1, 2, 3), 0, 64), ((1, 2, 3), (1, 2, 3), 2, 64),
+                                               ((2, 3), (2, 3), 1, 64)])
+def test_grids_that_the_prologue_refuses(gpu, grid, src, tag, rows):
+    """An axis longer than the table, a negative one, another TAG, two entries: neither way turns some tokens and not others."""
+    B, S, H, D = 1, 128, 2, 64
+    yq, yk = (torch.randn(B, S, H * D, device=gpu).to(BF) for _ in range(2))
+    w = torch.ones(H * D, device=gpu)
+    freqs = wan.wan_freqs(D, rows)
+    for call in (lambda: wan.wan_qk_prologue(yq, yk, w, w, [grid], [src], tag, freqs, H),
+                 lambda: wan.wan_qk_trainable(yq, yk, w, w, wan.rope_positions([grid], [src], tag, B, S, gpu), freqs, H)):
+        with pytest.raises((IcsaError, IcsaArgumentError)):
+            call()

@@ -1,0 +1,32 @@
+"""Corners of the training operators that need no GPU."""
+import pytest
+import torch
+
+from icsa_hip import wan
+from icsa_hip.hip_host import IcsaArgumentError
+
+pytestmark = pytest.mark.cpu
+
+
+def test_rope_positions():
+    """Target, then source from 0 again; tokens behind both, and all of a grid of nothing, stay; the longest axis of either."""
+    pos = wan.rope_positions([(2, 1, 2), (1, 2, 1)], [(1, 1, 3), (0, 5, 6)], 1, 2, 8, "cpu")
+    assert pos.dtype == torch.int32 and pos.rope_rows == 6
+    assert pos[0].tolist() == [[0, 0, 0], [0, 0, 1], [1, 0, 0], [1, 0, 1], [0, 0, 0], [0, 0, 1], [0, 0, 2], [-1, -1, -1]]
+    assert pos[1].tolist() == [[0, 0, 0], [0, 1, 0]] + [[-1, -1, -1]] * 6
+    assert wan.rope_positions(torch.tensor([[2, 1, 2]]), torch.tensor([[1, 1, 3]]), 0, 1, 6, "cpu")[0, 4:].tolist() == [[-1, -1, -1]] * 2
+    assert wan.rope_positions([(9, 9, 9)], [(1, 1, 1)], 1, 1, 4, "cpu")[0].tolist() == [[0, 0, i] for i in range(4)]   # cut at S
+
+
+@pytest.mark.parametrize("grid,src,tag", [((1, 2), (1, 2, 3), 0), ((1, 2, 3), (1, 2, 3, 4), 0), ((1, -2, 3), (1, 2, 3), 1), ((1, 2, 3), (1, 2, -3), 0),
+                                          ((1, 2, 3), (1, 2, 3), 2), ((1, 2, 3), (1, 2, 3), -1)])
+def test_rope_positions_refuse(grid, src, tag):
+    with pytest.raises(IcsaArgumentError):
+        wan.rope_positions([grid], [src], tag, 1, 8, "cpu")
+
+
+@pytest.mark.parametrize("grid,src,tag", [((6, 2, 3), (1, 2, 3), 0), ((1, 2, 3), (1, 2, 9), 1), ((1, 2, 3), (1, 9, 3), 0)])
+def test_a_grid_longer_than_the_table_is_refused(grid, src, tag):
+    y, w, freqs = torch.zeros(1, 64, 64), torch.ones(64), wan.wan_freqs(64, 5)
+    with pytest.raises(IcsaArgumentError, match="longer than the table"):
+        wan.wan_qk_trainable(y, y, w, w, wan.rope_positions([grid], [src], tag, 1, 64, "cpu"), freqs, 1)
