@@ -475,7 +475,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
 /* y = (x - mean) rstd a + b over rows of dim values, rstd = 1 / sqrt(mean((x - mean)^2) + eps); rms: mean = 0.  x, y
  * [groups * rows, dim] bf16 or f32, row strides x_ss, y_ss, any alignment; a = gain (1 + gain with plus_one; NULL: 1) and
  * b = shift (NULL: 0) [groups, dim] of p_dtype, group stride p_sg.  mean, rstd: f32 [groups * rows] for the backward (NULL: not
- * wanted; rms has no mean).  dim <= ICSA_NORM_MAX_DIM. */
+ * wanted; without rms an rstd needs its mean beside it; with rms mean is not written).  dim <= ICSA_NORM_MAX_DIM. */
 int icsa_norm_fwd(const void* x, int x_dtype, int64_t x_ss, int64_t rows, int groups, int dim,
                   const void* gain, const void* shift, int p_dtype, int64_t p_sg, int plus_one, int rms, float eps,
                   void* y, int y_dtype, int64_t y_ss, float* mean, float* rstd, void* stream);

@@ -195,9 +195,9 @@ __global__ void __launch_bounds__(LPR == 0 ? NM_MAX_THREADS : NM_THREADS) icsa_n
       for (int e = 0; e < 8; ++e) o[e] = fmaf(v[u][e] * rstd, a[u][e], b[u][e]);
       store8(dst + 8 * u * lanes, o, n[u], vy);
     }
-    if (t == 0 && p.rstd != nullptr) {
-      p.rstd[row0 + r] = rstd;
-      if (!RMS) p.mean[row0 + r] = mean;
+    if (t == 0) {
+      if (p.rstd != nullptr) p.rstd[row0 + r] = rstd;
+      if (!RMS && p.mean != nullptr) p.mean[row0 + r] = mean;
     }
   }
 }

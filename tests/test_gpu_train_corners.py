@@ -3,7 +3,7 @@ host does during a call, and results that must not depend on how a launch is div
 import pytest
 import torch
 
-from icsa_hip import rotary_func, rotary_table, wan
+from icsa_hip import _lib, rotary_func, rotary_table, wan
 from icsa_hip._lib import IcsaError
 from icsa_hip.hip_host import IcsaArgumentError
 
@@ -56,3 +56,22 @@ def test_grids_that_the_prologue_refuses(gpu, grid, src, tag, rows):
                  lambda: wan.wan_qk_trainable(yq, yk, w, w, wan.rope_positions([grid], [src], tag, B, S, gpu), freqs, H)):
         with pytest.raises((IcsaError, IcsaArgumentError)):
             call()
+
+
+# ------------------------------------------------------------------------------------------
+# norms
+# ------------------------------------------------------------------------------------------
+def test_norm_means_alone(gpu):
+    """Of the C entry point: mean and rstd are optional each."""
+    x = torch.randn(7, 640, device=gpu) + 3
+    y = torch.empty_like(x)
+    both = [torch.full((7,), float("nan"), device=gpu) for _ in range(2)]
+    alone = torch.full((7,), float("nan"), device=gpu)
+
+    def run(mean, rstd):
+        ptr = lambda t: 0 if t is None else t.data_ptr()
+        return _lib.lib().icsa_norm_fwd(x.data_ptr(), _lib.F32, 640, 7, 1, 640, 0, 0, _lib.F32, 0, 0, 0, 1e-6, y.data_ptr(), _lib.F32, 640,
+                                        ptr(mean), ptr(rstd), torch.cuda.current_stream().cuda_stream)
+    assert run(*both) == run(alone, None) == _lib.OK
+    torch.cuda.synchronize()
+    assert both[0].isfinite().all() and torch.equal(alone, both[0])
