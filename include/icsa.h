@@ -437,7 +437,8 @@ int64_t icsa_cross_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, int
 /* Attention of q [B, Sq, H, D] over k, v [B, Sk, Hk, D], all bf16, D 64 or 128: icsa_masked_attn with documents alone, and
  * for the backward lse f32 [B, Hk, Sq, H / Hk] (NULL: not wanted): log2 of a row's sum of 2^(score log2 e), +inf for a row that
  * sees nothing, and rest u8 [B, Sq, H, D] (contiguous; NULL: not wanted): what rounding out to bf16 left, in 1/256 of its last
- * place, + 128, a row's bytes in an order of the library's. */
+ * place, + 128, a row's bytes in an order of the library's.  With lse it refuses what the backward would: scales under 2^-96, and
+ * q, k or v of which 64 rows (of q: with the heads of a group) do not lie within 2 GiB. */
 int icsa_cross_attn_fwd(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                         const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
                         const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,

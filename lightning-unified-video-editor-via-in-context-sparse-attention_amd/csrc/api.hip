@@ -646,6 +646,24 @@ int icsa_masked_attn(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
 }
 
 // ---- cross attention with its backward ----
+namespace {
+// The backward's limits, which the forward that keeps its state refuses by too: row sums are held as -lse / scale, and 64 rows of what a
+// walk reads, with a group's heads, lie within 32-bit offsets.
+int check_back_scale(float scale) {
+  if (!std::isfinite(2.f * scale) || scale < 0x1p-96f) return fail(ICSA_EINVAL, "scale must be finite and 2^-96 or more");
+  return ICSA_OK;
+}
+int check_walked(int64_t ss, int64_t sh, int n, int H, int G) {
+  const int64_t most = 0x3fffffffLL;                   // elements
+  if (n <= 1) ss = 0;                                  // strides over one element do not count
+  if (H == 1) sh = 0;
+  if (ss < 0 || sh < 0) return fail(ICSA_EINVAL, "negative strides");
+  if (ss > most / 65 || (G > 1 && sh > (most - 65 * ss) / G))
+    return fail(ICSA_EUNSUPPORTED, "64 rows of q, dout, k and v must lie within 2 GiB");
+  return ICSA_OK;
+}
+}  // namespace
+
 int64_t icsa_cross_attn_workspace_size(int B, int Sq, int Sk, int H, int Hk, int D, int docs) {
   return icsa_masked_attn_workspace_size(B, Sq, Sk, H, Hk, D, docs, 0);
 }
@@ -658,6 +676,11 @@ int icsa_cross_attn_fwd(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh,
                         void* out, int64_t o_sb, int64_t o_ss, int64_t o_sh, float* lse, void* rest,
                         void* workspace, int64_t workspace_bytes, void* stream_) {
   if (rest && !aligned16(rest)) return fail(ICSA_EINVAL, "rest must be 16-byte aligned");
+  int rc = check_masked_sizes(B, Sq, Sk, H, Hk, D);
+  if (!rc && lse && !(rc = check_back_scale(scale)) && !(rc = check_walked(q_ss, q_sh, Sq, H, H / Hk)) &&
+      !(rc = check_walked(k_ss, 0, Sk, 1, 1)))
+    rc = check_walked(v_ss, 0, Sk, 1, 1);
+  if (rc) return rc;
   return masked_attn(q, q_sb, q_ss, q_sh, k, k_sb, k_ss, k_sh, v, v_sb, v_ss, v_sh, B, Sq, Sk, H, Hk, D, q_starts, k_starts, docs,
                      0, nullptr, scale, 0.f, nullptr, 0, out, ICSA_BF16, o_sb, o_ss, o_sh, lse,
                      reinterpret_cast<unsigned char*>(rest), workspace, workspace_bytes, stream_);
@@ -707,8 +730,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
   if (rc || (rc = check_dtype(grad_dtype, "gradients"))) return rc;
   if (!q_starts != !k_starts) return fail(ICSA_EINVAL, "q_starts and k_starts must be both given or both NULL");
   if (docs < 1 || (!q_starts && docs != 1)) return fail(ICSA_EINVAL, "docs=%d without document starts", docs);
-  if (!std::isfinite(2.f * scale) || scale < 0x1p-96f)   // the row sums are held as -lse / scale
-    return fail(ICSA_EINVAL, "scale must be finite and 2^-96 or more");
+  if ((rc = check_back_scale(scale))) return rc;
   if (Sq > 0 && (!dout || !q || !out || !lse)) return fail(ICSA_EINVAL, "null pointer argument");
   if (Sk > 0 && (!k || !v)) return fail(ICSA_EINVAL, "null pointer argument");
   if (rest && !aligned16(rest)) return fail(ICSA_EINVAL, "rest must be 16-byte aligned");
@@ -720,15 +742,13 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
       !ok(v, Sk, ICSA_BF16, v_sb, v_ss, v_sh) || !ok(dq, Sq, grad_dtype, dq_sb, dq_ss, dq_sh) ||
       !ok(dk, Sk, grad_dtype, dk_sb, dk_ss, dk_sh) || !ok(dv, Sk, grad_dtype, dv_sb, dv_ss, dv_sh))
     return fail(ICSA_EINVAL, "rows must be 16-byte aligned (pointers and strides)");
-  if (Sq <= 1) q_ss = do_ss = o_ss = 0;                // strides over one element do not count
+  const int G = H / Hk;
+  if ((rc = check_walked(q_ss, q_sh, Sq, H, G)) || (rc = check_walked(do_ss, do_sh, Sq, H, G)) ||
+      (rc = check_walked(k_ss, 0, Sk, 1, 1)) || (rc = check_walked(v_ss, 0, Sk, 1, 1)))
+    return rc;
+  if (Sq <= 1) q_ss = do_ss = o_ss = 0;
   if (Sk <= 1) k_ss = v_ss = 0;
   if (H == 1) q_sh = do_sh = 0;
-  if (k_ss < 0 || v_ss < 0 || q_ss < 0 || do_ss < 0 || q_sh < 0 || do_sh < 0)
-    return fail(ICSA_EINVAL, "negative strides");
-  const int64_t most = 0x3fffffffLL, G = H / Hk;       // elements
-  auto far = [&](int64_t ss, int64_t sh) { return ss > most / 65 || (G > 1 && sh > (most - 65 * ss) / G); };
-  if (k_ss > most / 65 || v_ss > most / 65 || far(q_ss, q_sh) || far(do_ss, do_sh))
-    return fail(ICSA_EUNSUPPORTED, "64 rows of q, dout, k and v must lie within 2 GiB");
   const AttnBwdPlan plan = attn_bwd_plan(B, Sq, Sk, H, Hk, D, docs);
   const AttnBwdLayout L = attn_bwd_layout(B, Sq, Sk, H, Hk, D, plan);
   if (L.total > 0 && (!workspace || workspace_bytes < L.total || !aligned16(workspace)))

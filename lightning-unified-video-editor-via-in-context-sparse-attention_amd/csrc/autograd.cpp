@@ -131,24 +131,27 @@ variable_list once(variable_list grads) {
   return error.apply(std::move(in));
 }
 
-// t [B, S, H, D] with a unit stride in each row and rows on 16 bytes (itself where they are), its address and strides
+// t [B, S, H, D] with a unit stride in each row and rows on 16 bytes (itself where they are), its address and strides.  group: of
+// heads (1 for k, v) where 64 rows with a group's heads have to lie within 2 GiB, as the backward reads them; 0: they need not.
 struct Rows {
   Tensor t;
   void* p;
   int64_t sb, ss, sh;
 };
-Rows rows16(const Tensor& t) {
+Rows rows16(const Tensor& t, int64_t group) {
   auto of = [](const Tensor& x) {
     Rows r{x, x.data_ptr(), x.size(0) > 1 ? x.stride(0) : 0, x.size(1) > 1 ? x.stride(1) : 0, x.size(2) > 1 ? x.stride(2) : 0};
     return r;
   };
-  auto ok = [](const Rows& r) {
-    return r.t.stride(3) == 1 && ((reinterpret_cast<uintptr_t>(r.p) | (uintptr_t)((r.sb | r.ss | r.sh) * 2)) & 15) == 0;
+  auto ok = [group](const Rows& r) {
+    const int64_t most = 0x3fffffff;
+    return r.t.stride(3) == 1 && ((reinterpret_cast<uintptr_t>(r.p) | (uintptr_t)((r.sb | r.ss | r.sh) * 2)) & 15) == 0 &&
+           (group == 0 || (r.ss <= most / 65 && (group == 1 || r.sh <= (most - 65 * r.ss) / group)));
   };
   Rows r = of(t);
   if (ok(r)) return r;
   r = of(t.contiguous());
-  return ok(r) ? r : of(t.clone(at::MemoryFormat::Contiguous));
+  return ok(r) || !t.is_contiguous() ? r : of(t.clone(at::MemoryFormat::Contiguous));
 }
 
 // ------------------------------------------------------------------------------------------ cross attention
@@ -205,7 +208,8 @@ struct CrossAttnBackward : public torch::autograd::Node {
     {
       at::AutoDispatchBelowADInplaceOrView below;
       c10::DeviceGuard guard(grads[0].device());
-      const Rows g = rows16(grads[0]), q = rows16(sq), k = rows16(sk), v = rows16(sv), o = rows16(so);
+      const int64_t G = sq.size(2) / sk.size(2);
+      const Rows g = rows16(grads[0], G), q = rows16(sq, G), k = rows16(sk, 1), v = rows16(sv, 1), o = rows16(so, 0);
       const Tensor lse = whole(this->lse), rest = whole(this->rest), qs = whole(this->qs), ks = whole(this->ks);
       const AttnSizes z = attn_sizes(q.t, k.t);
       const auto opt = q.t.options();
@@ -239,9 +243,9 @@ Tensor cross_attn(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Ma
   Rows q, k, v;
   {
     at::AutoDispatchBelowADInplaceOrView below;
-    q = rows16(q_);
-    k = rows16(k_);
-    v = rows16(v_);
+    q = rows16(q_, node ? q_.size(2) / k_.size(2) : 0);
+    k = rows16(k_, node ? 1 : 0);
+    v = rows16(v_, node ? 1 : 0);
     out = attn_forward(q, k, v, qs, ks, docs, scale, node ? &lse : nullptr, node ? &rest : nullptr);
   }
   if (node) {

@@ -23,6 +23,7 @@ from .hip_host import IcsaArgumentError, _require, _rows16, on_device, ptr, stre
 _BF = torch.bfloat16
 _FLOATS = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
 NORM_MAX_DIM = 8192
+_WALK = 0x3fffffff           # elements within 32-bit byte offsets
 
 
 _native = None
@@ -76,6 +77,17 @@ def _check_attn(q, k, v, q_starts, k_starts, softmax_scale):
     return (B, Sq, Sk, H, Hk, D), docs, scale, q_starts, k_starts
 
 
+def _near16(t, group=1):
+    """:func:`_rows16`, and 64 rows with the heads of a group within 2 GiB, as the backward reads them."""
+    t, a = _rows16(t)
+    _, n1, n2, n3 = t.shape
+    ss, sh = a[2] if n1 > 1 else 0, a[3] if n2 > 1 else 0
+    if ss > _WALK // 65 or (group > 1 and sh > (_WALK - 65 * ss) // group):
+        t = t.contiguous()
+        a = (t.data_ptr(), n1 * n2 * n3, n2 * n3, n3)
+    return t, a
+
+
 @torch.no_grad()
 def cross_attn_fwd_hip(q, k, v, q_starts=None, k_starts=None, softmax_scale=None):
     """``(out, lse, rest)`` of :func:`cross_attn_func`'s forward: out bfloat16 like q; lse float32 [B, Hk, Sq, H / Hk], log2 of each
@@ -84,9 +96,9 @@ def cross_attn_fwd_hip(q, k, v, q_starts=None, k_starts=None, softmax_scale=None
     sizes, docs, scale, q_starts, k_starts = _check_attn(q, k, v, q_starts, k_starts, softmax_scale)
     B, Sq, Sk, H, Hk, D = sizes
     dev = q.device
-    q, qa = _rows16(q)
-    k, ka = _rows16(k)
-    v, va = _rows16(v)
+    q, qa = _near16(q, H // Hk)
+    k, ka = _near16(k)
+    v, va = _near16(v)
     out = torch.empty(B, Sq, H, D, dtype=_BF, device=dev)
     lse = torch.empty(B, Hk, Sq, H // Hk, dtype=torch.float32, device=dev)
     L = _lib.lib()
@@ -123,10 +135,10 @@ def cross_attn_bwd_hip(dout, q, k, v, out, lse, rest=None, q_starts=None, k_star
         raise IcsaArgumentError("dout, out, lse and rest must be on the GPU of q")
     if grad_dtype not in _FLOATS:
         raise IcsaArgumentError("grad_dtype must be bfloat16 or float32")
-    dout, da = _rows16(dout)
-    q, qa = _rows16(q)
-    k, ka = _rows16(k)
-    v, va = _rows16(v)
+    dout, da = _near16(dout, H // Hk)
+    q, qa = _near16(q, H // Hk)
+    k, ka = _near16(k)
+    v, va = _near16(v)
     out, oa = _rows16(out)
     L = _lib.lib()
     ws_bytes = L.icsa_cross_attn_bwd_workspace_size(*sizes, docs)
@@ -154,6 +166,7 @@ def cross_attn_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, q_star
     batch row b has queries ``q_starts[b, n] .. q_starts[b, n + 1] - 1`` and keys likewise, and sees its own keys alone
     (a batch row whose text has ``n`` real tokens is one document, ``[0, Sq]`` and ``[0, n]``).  Values past the lengths
     are clamped on the GPU.  ``softmax_scale``: 2 ** -96 or more, default ``D ** -0.5``.
+    With gradients, a tensor of which 64 rows (of q: with the heads of a group) do not lie within 2 GiB is copied.
 
     A query that sees nothing gets zeros; it, keys outside every document and padding take no part in any gradient and
     get zeros, whatever they and their ``dout`` hold.  A NaN or an infinity inside a document makes gradients of that

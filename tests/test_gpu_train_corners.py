@@ -3,7 +3,7 @@ host does during a call, and results that must not depend on how a launch is div
 import pytest
 import torch
 
-from icsa_hip import _lib, rotary_func, rotary_table, wan
+from icsa_hip import _lib, cross_attn_bwd_hip, cross_attn_func, cross_attn_fwd_hip, rotary_func, rotary_table, wan
 from icsa_hip._lib import IcsaError
 from icsa_hip.hip_host import IcsaArgumentError
 
@@ -75,3 +75,36 @@ def test_norm_means_alone(gpu):
     assert run(*both) == run(alone, None) == _lib.OK
     torch.cuda.synchronize()
     assert both[0].isfinite().all() and torch.equal(alone, both[0])
+
+
+# ------------------------------------------------------------------------------------------
+# cross attention
+# ------------------------------------------------------------------------------------------
+def _far(t, step, dim):
+    """t's values with `step` elements between neighbours of one dim."""
+    strides = list(t.contiguous().stride())
+    strides[dim] = step
+    span = sum((n - 1) * s for n, s in zip(t.shape, strides)) + 1
+    view = torch.empty(span, dtype=t.dtype, device=t.device).as_strided(t.shape, strides)
+    return view.copy_(t)
+
+
+@pytest.mark.parametrize("far", ["q rows", "k rows", "v rows", "dout rows", "q heads"])
+def test_what_the_forward_takes_the_backward_takes(gpu, far):
+    """64 rows, with the heads of a group, over more than 2 GiB (heads first in memory, of long sequences): gradients, and the
+    same bits as from contiguous tensors."""
+    torch.manual_seed(0)
+    Sq, Sk, H, Hk = 70, 66, 6, 2
+    x = dict(q=torch.randn(1, Sq, H, 64), k=torch.randn(1, Sk, Hk, 64), v=torch.randn(1, Sk, Hk, 64), dout=torch.randn(1, Sq, H, 64))
+    x = {n: t.to(gpu, BF) for n, t in x.items()}
+    run = lambda q, k, v, dout: (lambda o: (o.detach(), *torch.autograd.grad(o, (q, k, v), dout)))(cross_attn_func(q, k, v))
+    leaf = lambda y: [y[n].detach().requires_grad_(n != "dout") for n in ("q", "k", "v", "dout")]
+    want = run(*leaf(x))
+    name, which = far.split()
+    y = dict(x)
+    y[name] = _far(x[name], (1 << 28) + (1 << 27) if which == "heads" else (1 << 24) - 64, 2 if which == "heads" else 1)
+    for a, b in zip(want, run(*leaf(y))):
+        assert torch.equal(a, b)
+    out, lse, rest = cross_attn_fwd_hip(y["q"], y["k"], y["v"])
+    for a, b in zip(want, (out, *cross_attn_bwd_hip(y["dout"], y["q"], y["k"], y["v"], out, lse, rest))):
+        assert torch.equal(a, b)

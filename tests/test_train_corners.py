@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from icsa_hip import wan
+from icsa_hip import _lib, wan
 from icsa_hip.hip_host import IcsaArgumentError
 
 pytestmark = pytest.mark.cpu
@@ -30,3 +30,16 @@ def test_a_grid_longer_than_the_table_is_refused(grid, src, tag):
     y, w, freqs = torch.zeros(1, 64, 64), torch.ones(64), wan.wan_freqs(64, 5)
     with pytest.raises(IcsaArgumentError, match="longer than the table"):
         wan.wan_qk_trainable(y, y, w, w, wan.rope_positions([grid], [src], tag, 1, 64, "cpu"), freqs, 1)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(scale=1e-30), _lib.EINVAL), (dict(q_ss=1 << 28), _lib.EUNSUPPORTED), (dict(H=8, q_sh=1 << 28), _lib.EUNSUPPORTED),
+    (dict(k_ss=(1 << 24) - 64), _lib.EUNSUPPORTED), (dict(v_ss=(1 << 24) - 64), _lib.EUNSUPPORTED), (dict(q_ss=-128), _lib.EINVAL),
+])
+def test_the_forward_that_keeps_its_state_refuses_what_the_backward_would(kw, code):
+    """At the forward's call, not after it."""
+    at = 1 << 20
+    a = dict(q=at, q_sb=0, q_ss=128, q_sh=128, k=at, k_sb=0, k_ss=128, k_sh=128, v=at, v_sb=0, v_ss=128, v_sh=128, B=1, Sq=8, Sk=8, H=1, Hk=1,
+             D=128, qst=0, kst=0, docs=1, scale=0.1, out=at, o_sb=0, o_ss=128, o_sh=128, lse=at, rest=at, ws=0, wsb=0, stream=0)
+    a.update(kw)
+    assert _lib.lib().icsa_cross_attn_fwd(*a.values()) == code and _lib.lib().icsa_last_error()
