@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
@@ -71,6 +72,18 @@ void check(const char* fn, int64_t code) {
 }
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+// Inputs with memory of their own, in a call that is not traced.  A batched, lifted or functional tensor has none; a null address (of a
+// wrapper, or a tensor of zeros that is none) would read as an operand that is not given; and a trace would hold the results'
+// allocation without what fills it.
+void require_plain(std::initializer_list<const Tensor*> ts) {
+  bool plain = !torch::jit::tracer::isTracing();
+  for (const Tensor* t : ts)
+    plain = plain && (!t->defined() || (t->has_storage() && !t->key_set().has(c10::DispatchKey::Functionalize) &&
+                                        (t->numel() == 0 || t->data_ptr() != nullptr)));
+  TORCH_CHECK_NOT_IMPLEMENTED(plain, "icsa_hip's training operators take tensors with memory of their own: not under vmap, torch.func, "
+                                     "batched gradients or tracing");
+}
 
 // constants: inputs without a gradient, which may have no tangent either
 bool wants_grad(std::initializer_list<const Tensor*> ts, std::initializer_list<const Tensor*> constants = {}) {
@@ -204,6 +217,7 @@ struct CrossAttnBackward : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list res(3);
     if (!grads[0].defined()) return res;
+    require_plain({&grads[0]});
     const Tensor sq = q.unpack(), sk = k.unpack(), sv = v.unpack(), so = out.unpack(shared_from_this());
     {
       at::AutoDispatchBelowADInplaceOrView below;
@@ -234,6 +248,7 @@ struct CrossAttnBackward : public torch::autograd::Node {
 Tensor cross_attn(const Tensor& q_, const Tensor& k_, const Tensor& v_, const MaybeTensor& qs_, const MaybeTensor& ks_, int64_t docs,
                   double scale) {
   const Tensor qs = get(qs_), ks = get(ks_);
+  require_plain({&q_, &k_, &v_, &qs, &ks});
   std::shared_ptr<CrossAttnBackward> node;
   if (wants_grad({&q_, &k_, &v_})) {
     refuse_capture({&q_, &k_, &v_});
@@ -325,6 +340,7 @@ struct NormBackward : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list res(3);
     if (!grads[0].defined()) return res;
+    require_plain({&grads[0]});
     const Tensor sx = x.unpack(), sg = gain.unpack();
     {
       at::AutoDispatchBelowADInplaceOrView below;
@@ -353,6 +369,7 @@ struct NormBackward : public torch::autograd::Node {
 
 Tensor norm(const Tensor& x, const MaybeTensor& gain_, const MaybeTensor& shift_, bool plus_one, bool rms, double eps, at::ScalarType out) {
   const Tensor gain = get(gain_), shift = get(shift_);
+  require_plain({&x, &gain, &shift});
   std::shared_ptr<NormBackward> node;
   if (wants_grad({&x, &gain, &shift})) {
     refuse_capture({&x, &gain, &shift});
@@ -379,7 +396,7 @@ Tensor norm(const Tensor& x, const MaybeTensor& gain_, const MaybeTensor& shift_
 }
 
 // ------------------------------------------------------------------------------------------ rotary positions
-Tensor unit_last(const Tensor& t) { return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor unit_last(const Tensor& t) { return !t.defined() ? t : t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
 // Both turned (either may be undefined), new and contiguous.  axes 0: one axis without sections.
 std::pair<Tensor, Tensor> rotate(const Tensor& q_, const Tensor& k_, const Tensor& cos, const Tensor& sin, const Tensor& pos,
@@ -430,6 +447,7 @@ struct RotaryBackward : public torch::autograd::Node {
       const Tensor c = whole(cos), s = whole(sin), p = whole(pos);
       const Tensor dq = task_should_compute_output(0) ? grads[0] : Tensor();
       const Tensor dk = grads.size() > 1 && task_should_compute_output(1) ? grads[1] : Tensor();
+      require_plain({&dq, &dk});
       if (dq.defined() || dk.defined()) std::tie(res[0], res[1]) = rotate(dq, dk, c, s, p, sections, interleaved, true);
     }
     return once(std::move(res));
@@ -439,8 +457,9 @@ struct RotaryBackward : public torch::autograd::Node {
 variable_list rotary(const Tensor& q, const MaybeTensor& k_, const Tensor& cos, const Tensor& sin, const Tensor& pos,
                      std::vector<int64_t> sections, bool interleaved) {
   const Tensor k = get(k_);
+  require_plain({&q, &k, &cos, &sin, &pos});
   const bool grad = wants_grad({&q, &k}, {&cos, &sin});
-  const Tensor c = cos.contiguous(), s = sin.contiguous(), p = pos.contiguous();
+  const Tensor c = cos.contiguous(), s = sin.contiguous().resolve_neg(), p = pos.contiguous();
   std::shared_ptr<RotaryBackward> node;
   if (grad) {
     refuse_capture({&q, &k});

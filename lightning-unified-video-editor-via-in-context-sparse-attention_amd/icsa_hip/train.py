@@ -77,6 +77,12 @@ def _check_attn(q, k, v, q_starts, k_starts, softmax_scale):
     return (B, Sq, Sk, H, Hk, D), docs, scale, q_starts, k_starts
 
 
+def _require_plain(*ts):
+    """As the autograd nodes do of their inputs."""
+    if torch._C._get_tracing_state() is not None or not all(t is None or torch._C._has_storage(t) for t in ts):
+        raise NotImplementedError("icsa_hip's training operators take tensors with memory of their own: not under vmap, torch.func or tracing")
+
+
 def _near16(t, group=1):
     """:func:`_rows16`, and 64 rows with the heads of a group within 2 GiB, as the backward reads them."""
     t, a = _rows16(t)
@@ -93,6 +99,7 @@ def cross_attn_fwd_hip(q, k, v, q_starts=None, k_starts=None, softmax_scale=None
     """``(out, lse, rest)`` of :func:`cross_attn_func`'s forward: out bfloat16 like q; lse float32 [B, Hk, Sq, H / Hk], log2 of each
     row's sum of ``2 ** (score * log2 e)``, +inf for a row that sees nothing; rest uint8 like out, what its rounding
     left, or None where that does not show in a gradient (without documents: over 256 keys, with heads of 64 over 1,024, and over 128 queries)."""
+    _require_plain(q, k, v, q_starts, k_starts)
     sizes, docs, scale, q_starts, k_starts = _check_attn(q, k, v, q_starts, k_starts, softmax_scale)
     B, Sq, Sk, H, Hk, D = sizes
     dev = q.device
@@ -122,6 +129,7 @@ def cross_attn_bwd_hip(dout, q, k, v, out, lse, rest=None, q_starts=None, k_star
     """Gradients ``(dq, dk, dv)`` (bfloat16 or float32 by ``grad_dtype``; None where ``need`` is false) from the forward's
     inputs and results.  Without ``rest`` rowsum(dout * out) comes from the rounded out alone, whose error shows in dq and
     dk where rows see few keys."""
+    _require_plain(dout, q, k, v, out, lse, rest, q_starts, k_starts)
     sizes, docs, scale, q_starts, k_starts = _check_attn(q, k, v, q_starts, k_starts, softmax_scale)
     B, Sq, Sk, H, Hk, D = sizes
     dev = q.device

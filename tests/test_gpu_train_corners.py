@@ -3,7 +3,8 @@ host does during a call, and results that must not depend on how a launch is div
 import pytest
 import torch
 
-from icsa_hip import _lib, cross_attn_bwd_hip, cross_attn_func, cross_attn_fwd_hip, rotary_func, rotary_table, wan
+from icsa_hip import (_lib, cross_attn_bwd_hip, cross_attn_func, cross_attn_fwd_hip, layer_norm_func, rms_norm_func, rotary_func,
+                      rotary_table, wan)
 from icsa_hip._lib import IcsaError
 from icsa_hip.hip_host import IcsaArgumentError
 
@@ -108,3 +109,53 @@ def test_what_the_forward_takes_the_backward_takes(gpu, far):
     out, lse, rest = cross_attn_fwd_hip(y["q"], y["k"], y["v"])
     for a, b in zip(want, (out, *cross_attn_bwd_hip(y["dout"], y["q"], y["k"], y["v"], out, lse, rest))):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------
+# transforms
+# ------------------------------------------------------------------------------------------
+def _calls(gpu):
+    """(an input, the operator of it) for each."""
+    torch.manual_seed(2)
+    x, q = torch.randn(3, 2, 9, 128, device=gpu), torch.randn(3, 1, 9, 2, 64, device=gpu).to(BF)
+    table, pos = rotary_table(9, 64), torch.arange(9, dtype=torch.int32, device=gpu)
+    return [(x, lambda t: layer_norm_func(t)), (x, lambda t: rms_norm_func(t)), (q, lambda t: cross_attn_func(t, t, t)),
+            (q, lambda t: rotary_func(t, None, *table, pos)), (q, lambda t: cross_attn_fwd_hip(t, t, t)[0])]
+
+
+def test_transforms_are_refused(gpu):
+    """vmap, torch.func, batched gradients, tracing (whose result would be memory that nothing fills) and tensors without memory."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    for x, f in _calls(gpu):
+        for transformed in (lambda: torch.func.vmap(f)(x), lambda: torch.func.grad(lambda t: f(t).float().sum())(x[0]),
+                            lambda: torch.func.functionalize(f)(x[0])):
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                transformed()
+        with pytest.raises(NotImplementedError, match="memory of their own"):
+            torch.jit.trace(f, (x[0],))
+        with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            with pytest.raises((NotImplementedError, RuntimeError)):
+                f(mode.from_tensor(x[0]))
+    for x, f in _calls(gpu)[:4]:
+        with pytest.raises(NotImplementedError, match="memory of their own"):
+            torch.func.vmap(f)(x)
+        leaf = x[0].requires_grad_()
+        y = f(leaf)
+        with pytest.raises(NotImplementedError, match="memory of their own"):
+            torch.autograd.grad(y, leaf, torch.ones(2, *y.shape, dtype=y.dtype, device=gpu), is_grads_batched=True)
+    x, w = torch.randn(4, 16, device=gpu), torch._efficientzerotensor(16, device=gpu)
+    with pytest.raises(NotImplementedError, match="memory of their own"):
+        layer_norm_func(x, w)                                # its address is null, as that of no weight
+
+
+def test_checkpointed(gpu):
+    """Recomputed in the backward: the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+    for x, f in _calls(gpu)[:4]:
+        leaf = x[0].clone().requires_grad_()
+        dy = torch.randn_like(f(x[0]))
+        want, = torch.autograd.grad(f(leaf), leaf, dy)
+        for reentrant in (False, True):
+            leaf.grad = None
+            checkpoint(f, leaf, use_reentrant=reentrant).backward(dy)
+            assert torch.equal(leaf.grad, want)
