@@ -282,7 +282,7 @@ Tensor cross_attn(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Ma
 // ------------------------------------------------------------------------------------------ layer norm, RMS norm
 // t [..., dim] as [rows, dim] with a unit stride in each row
 Tensor rows(const Tensor& t) {
-  const Tensor x = t.size(-1) != 1 && t.stride(-1) != 1 ? t.contiguous() : t;
+  const Tensor x = t.size(-1) != 1 && t.stride(-1) != 1 ? t.contiguous() : t.resolve_neg();
   return x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
 }
 int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
@@ -396,7 +396,7 @@ Tensor norm(const Tensor& x, const MaybeTensor& gain_, const MaybeTensor& shift_
 }
 
 // ------------------------------------------------------------------------------------------ rotary positions
-Tensor unit_last(const Tensor& t) { return !t.defined() ? t : t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor unit_last(const Tensor& t) { return !t.defined() ? t : t.size(-1) == 1 || t.stride(-1) == 1 ? t.resolve_neg() : t.contiguous(); }
 
 // Both turned (either may be undefined), new and contiguous.  axes 0: one axis without sections.
 std::pair<Tensor, Tensor> rotate(const Tensor& q_, const Tensor& k_, const Tensor& cos, const Tensor& sin, const Tensor& pos,
@@ -459,7 +459,7 @@ variable_list rotary(const Tensor& q, const MaybeTensor& k_, const Tensor& cos, 
   const Tensor k = get(k_);
   require_plain({&q, &k, &cos, &sin, &pos});
   const bool grad = wants_grad({&q, &k}, {&cos, &sin});
-  const Tensor c = cos.contiguous(), s = sin.contiguous().resolve_neg(), p = pos.contiguous();
+  const Tensor c = cos.contiguous().resolve_neg(), s = sin.contiguous().resolve_neg(), p = pos.contiguous();
   std::shared_ptr<RotaryBackward> node;
   if (grad) {
     refuse_capture({&q, &k});

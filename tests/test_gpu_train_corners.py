@@ -148,6 +148,24 @@ def test_transforms_are_refused(gpu):
         layer_norm_func(x, w)                                # its address is null, as that of no weight
 
 
+def test_views_with_a_sign(gpu):
+    """What a conjugate's imaginary part is: values of the other sign than memory's."""
+    x, w = torch.randn(6, 64, device=gpu), torch.randn(64, device=gpu)
+    neg = torch._neg_view
+    assert torch.equal(layer_norm_func(neg(x), neg(w)), layer_norm_func(-x, -w))
+    assert torch.equal(rms_norm_func(neg(x)), rms_norm_func(-x))
+    q = torch.randn(1, 6, 2, 64, device=gpu)
+    cos, sin = rotary_table(6, 64)
+    pos = torch.arange(6, dtype=torch.int32, device=gpu)
+    want = rotary_func(-q, None, cos, -sin, pos)
+    assert torch.equal(rotary_func(neg(q), None, cos, neg(sin), pos), want)
+    assert torch.equal(rotary_func(-q, None, cos, torch.complex(cos, sin).conj().imag, pos), want)
+    leaf = x.clone().requires_grad_()
+    a, = torch.autograd.grad(layer_norm_func(leaf), leaf, neg(x))
+    b, = torch.autograd.grad(layer_norm_func(leaf), leaf, -x)
+    assert torch.equal(a, b)
+
+
 def test_checkpointed(gpu):
     """Recomputed in the backward: the same gradients."""
     from torch.utils.checkpoint import checkpoint
