@@ -485,9 +485,10 @@ variable_list rotary(const Tensor& q, const MaybeTensor& k_, const Tensor& cos, 
 
 }  // namespace
 
+// Without the interpreter's lock, as torch's own operators and the package's calls of the library: allocations and launches may wait.
 PYBIND11_MODULE(_autograd, m) {
   m.def("bind", torch::wrap_pybind_function(bind));
-  m.def("cross_attn", torch::wrap_pybind_function(cross_attn));
-  m.def("norm", torch::wrap_pybind_function(norm));
-  m.def("rotary", torch::wrap_pybind_function(rotary));
+  m.def("cross_attn", torch::wrap_pybind_function_no_gil(cross_attn));
+  m.def("norm", torch::wrap_pybind_function_no_gil(norm));
+  m.def("rotary", torch::wrap_pybind_function_no_gil(rotary));
 }

@@ -1,5 +1,9 @@
 """Corners of the training operators: sizes at the ends of their ranges, layouts and transforms outside the usual ones, what the
 host does during a call, and results that must not depend on how a launch is divided."""
+import sys
+import threading
+import time
+
 import pytest
 import torch
 
@@ -109,6 +113,49 @@ def test_what_the_forward_takes_the_backward_takes(gpu, far):
     out, lse, rest = cross_attn_fwd_hip(y["q"], y["k"], y["v"])
     for a, b in zip(want, (out, *cross_attn_bwd_hip(y["dout"], y["q"], y["k"], y["v"], out, lse, rest))):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------
+# the host
+# ------------------------------------------------------------------------------------------
+def test_other_threads_run_during_a_call(gpu):
+    """The operators leave the interpreter to others while they allocate and launch.  The other thread counts; the interpreter is not
+    taken from this one by time (the switch interval), so that it counts only where a call lets go of it.  Results of 1 GiB of new
+    memory each make the calls long enough."""
+    x = torch.zeros(1 << 17, 4096, dtype=BF, device=gpu)
+    q = torch.zeros(1, 1 << 16, 64, 128, dtype=BF, device=gpu)
+    k = torch.zeros(1, 1, 64, 128, dtype=BF, device=gpu)
+    table, pos = rotary_table(1, 128), torch.zeros(1 << 16, dtype=torch.int32, device=gpu)
+    calls = [lambda: rms_norm_func(x), lambda: rotary_func(q, None, *table, pos), lambda: cross_attn_func(q, k, k)]
+    for call in calls:
+        call()
+    torch.cuda.synchronize()
+    counted, stop = [0], threading.Event()
+
+    def count():
+        while not stop.is_set():
+            counted[0] += 1
+            time.sleep(0)
+    other = threading.Thread(target=count)
+    interval = sys.getswitchinterval()
+    other.start()
+    try:
+        sys.setswitchinterval(30.0)
+        for call in calls:
+            moved = False
+            for _ in range(60):
+                torch.cuda.empty_cache()
+                before = counted[0]
+                y = call()
+                moved = moved or counted[0] > before
+                del y
+                if moved:
+                    break
+            assert moved
+    finally:
+        sys.setswitchinterval(interval)
+        stop.set()
+        other.join()
 
 
 # ------------------------------------------------------------------------------------------
