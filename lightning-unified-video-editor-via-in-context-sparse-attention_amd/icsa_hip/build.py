@@ -4,7 +4,8 @@ Every HIP source is compiled to an object in ``csrc/_build`` (in parallel), then
 into ``icsa_hip/libicsa.so`` next to this file.  The link goes to a
 temporary name first and is renamed into place, so a concurrent loader never sees a
 half-written library.  ``_autograd.so`` (the autograd nodes of ``train.py``) is built beside it against the
-installed torch.  Run ``python -m icsa_hip.build`` or call :func:`build_library`.
+installed torch.  Where that cannot be (no g++, no headers) the command fails, after ``libicsa.so`` is in place: the C library needs hipcc alone.
+Run ``python -m icsa_hip.build`` or call :func:`build_library`.
 """
 from __future__ import annotations
 
@@ -92,10 +93,10 @@ def build_library(verbose: bool = False, jobs: int = 8) -> str:
     with ThreadPoolExecutor(max_workers=max(1, min(jobs, len(SOURCES) + 1))) as ex:
         nodes = ex.submit(_build_nodes, verbose)          # the longest one first
         objs = list(ex.map(compile_one, SOURCES))
-        nodes.result()
-    tmp = LIB_PATH + f".tmp{os.getpid()}"
-    _run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs], verbose)
-    os.replace(tmp, LIB_PATH)
+        tmp = LIB_PATH + f".tmp{os.getpid()}"
+        _run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs], verbose)
+        os.replace(tmp, LIB_PATH)
+        nodes.result()                                    # the library is in place, whatever the host compiler says
     return LIB_PATH
 
 

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from icsa_hip import _lib, wan
+from icsa_hip import _lib, build, wan
 from icsa_hip.hip_host import IcsaArgumentError
 
 pytestmark = pytest.mark.cpu
@@ -43,3 +43,23 @@ def test_the_forward_that_keeps_its_state_refuses_what_the_backward_would(kw, co
              D=128, qst=0, kst=0, docs=1, scale=0.1, out=at, o_sb=0, o_ss=128, o_sh=128, lse=at, rest=at, ws=0, wsb=0, stream=0)
     a.update(kw)
     assert _lib.lib().icsa_cross_attn_fwd(*a.values()) == code and _lib.lib().icsa_last_error()
+
+
+def test_the_library_is_built_where_the_nodes_cannot_be(monkeypatch, tmp_path):
+    """Without a host compiler: hipcc's part is linked and in place, and the failure is reported."""
+    steps = []
+
+    def run(cmd, verbose):
+        steps.append(cmd)
+        if cmd[0] == "no-such-compiler":
+            raise RuntimeError("command failed: no-such-compiler")
+        open(cmd[cmd.index("-o") + 1], "w").close()
+    monkeypatch.setenv("CXX", "no-such-compiler")
+    monkeypatch.setattr(build, "_run", run)
+    monkeypatch.setattr(build, "BUILD_DIR", str(tmp_path / "objects"))
+    monkeypatch.setattr(build, "LIB_PATH", str(tmp_path / "libicsa.so"))
+    monkeypatch.setattr(build, "NODES_PATH", str(tmp_path / "_autograd.so"))
+    with pytest.raises(RuntimeError, match="no-such-compiler"):
+        build.build_library()
+    assert (tmp_path / "libicsa.so").exists() and not (tmp_path / "_autograd.so").exists()
+    assert sum("-shared" in cmd for cmd in steps) == 2 and len(steps) == len(build.SOURCES) + 2
