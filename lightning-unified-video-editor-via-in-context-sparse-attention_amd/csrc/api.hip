@@ -701,7 +701,7 @@ AttnBwdLayout attn_bwd_layout(int B, int Sq, int Sk, int H, int Hk, int D, AttnB
   AttnBwdLayout L;
   L.rowv = 0;
   L.dq = align256(2 * q_rows * 4);
-  L.dk = L.dq + (f.q_split > 1 ? align256(f.q_split * q_rows * D * 4) : 0);
+  L.dk = L.dq + (f.q_split > 1 ? align256(f.q_split * q_rows * (D + 1) * 4) : 0);
   const int64_t k_part = f.k_split > 1 ? align256(f.k_split * k_rows * D * 4) : 0;
   L.dv = L.dk + k_part;
   L.total = L.dv + k_part;
@@ -766,6 +766,7 @@ int icsa_cross_attn_bwd(const void* dout, int64_t do_sb, int64_t do_ss, int64_t 
   p.q_starts = q_starts; p.k_starts = k_starts; p.docs = docs; p.scale = scale;
   p.rowv = reinterpret_cast<float*>(ws + L.rowv);
   p.dq_part = reinterpret_cast<float*>(ws + L.dq);
+  p.dq_total = p.dq_part + (int64_t)plan.q_split * B * Sq * H * D;
   p.dk_part = reinterpret_cast<float*>(ws + L.dk);
   p.dv_part = reinterpret_cast<float*>(ws + L.dv);
   p.q_split = plan.q_split; p.k_split = plan.k_split;

@@ -72,6 +72,11 @@ struct DocView {
   static constexpr const int* prefix = nullptr;
 };
 
+// What dq is divided by for its row's total of P.  lse is the forward's total of rounded weights; P sums to 1 but for that.  It would
+// be a third of what dq is off beside its own roundings (f32 dq over 226 keys 0.00179 from the exact one, so 0.00173); the sums cost 3 % (65,520
+// over 512: 1,226 and 1,258 us).  A total far from 1 is no rounding's: a row of nothing, or of what is not finite.
+__device__ __forceinline__ float row_total(float sum) { return sum > 0.5f && sum < 2.f ? sum : 1.f; }
+
 template <int D> constexpr int ab_lds() { return 4 * BTile<D>::kBytes + 2 * 512 + AB_WAVES * AB_SCRATCH_WAVE + AB_CTL_BYTES; }
 
 }  // namespace
@@ -431,10 +436,13 @@ __global__ void __launch_bounds__(AB_THREADS, FINE ? (D == 64 && !KV ? 2 : 1) : 
   } else if (lse != lse || !__builtin_isfinite(dd)) {
     f1 = NAN;
   } else if (n_split == 1) {
-    // lse is the forward's total of rounded weights; P sums to 1 but for that.  It would be a third of what dq is off beside its own roundings
-    // (f32 dq over 226 keys 0.00179 from the exact one, so 0.00173); the sums cost 3 % (65,520 over 512: 1,226 and 1,258 us)
-    const float sum = xhalf_sum(total[0] + total[1]);
-    if (sum > 0.5f && sum < 2.f) f1 /= sum;
+    f1 /= row_total(xhalf_sum(total[0] + total[1]));
+  }
+  if constexpr (!KV) {                                                    // of parts: divided by where they are joined
+    if (n_split > 1) {
+      const float sum = xhalf_sum(total[0] + total[1]);
+      if (hl == 0 && li < rows_valid) p.dq_total[((int64_t)split * BH + bh) * n_st + r] = sum;
+    }
   }
   auto finish = [&](const floatx16* acc, float f, const OutView& out, float* part) {
     if (n_split == 1) {
@@ -468,11 +476,18 @@ __global__ void __launch_bounds__(256) icsa_attn_bwd_join_kernel(AttnBwdParams p
   const int d = threadIdx.x % kPer * 4;
   const float* src = (!KV ? p.dq_part : blockIdx.y ? p.dv_part : p.dk_part) + row * D + d;
   floatx4 s = *reinterpret_cast<const floatx4*>(src);
+  float total = KV ? 1.f : p.dq_total[row];
 #pragma unroll 4
   for (int i = 1; i < n_split; ++i) {
     const floatx4 v = *reinterpret_cast<const floatx4*>(src + (int64_t)i * rows * D);
+    if constexpr (!KV) total += p.dq_total[i * rows + row];
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] += v[e];
+  }
+  if constexpr (!KV) {
+    total = row_total(total);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] /= total;
   }
   const int bh = (int)((unsigned)row / (unsigned)n_st), r = (int)row - bh * n_st;         // rows: under 2^28, check_masked_sizes
   const int64_t off = row_at(out.sb, out.ss, out.sh, p.by_hk.div(bh), p.by_hk.mod(bh), KV ? FastDiv{1u, 0u, 1u, 0u} : p.by_g, r) + d;

@@ -315,6 +315,7 @@ struct AttnBwdParams {
   OutView dq, dk, dv;                             // p null: not wanted
   int q_split, k_split;                           // AttnBwdPlan
   float* dq_part; float* dk_part; float* dv_part; // the parts' sums, [part][B Hk][row][D]
+  float* dq_total;                                // and of the rows' P, [part][B Hk][row]
   FastDiv by_g, by_hk, by_qblk, by_kblk;          // set by the launch
 };
 // parts that a query block's keys and a key block's rows are cut into

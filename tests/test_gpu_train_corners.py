@@ -115,6 +115,36 @@ def test_what_the_forward_takes_the_backward_takes(gpu, far):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_dq_does_not_depend_on_the_number_of_parts(gpu, D):
+    """The same rows by themselves (their keys cut in parts) and beside many others (in one): each dq is divided by its row's total of P
+    either way.  A row whose weight lies on few keys would be off by most of a bf16 rounding, 2^-9 or so, without; the order of the
+    sums, of at most n float32 terms, moves an element by n 2^-24 of its terms' absolute sum, scale sum |dS k|, where |dS| <= p (|dP| + |D|)."""
+    torch.manual_seed(1)
+    Sq, Sk, many = 200, 2000, 400
+    q, k, v, do = (torch.randn(1, n, 2, D, device=gpu).to(BF) for n in (Sq, Sk, Sk, Sq))
+    q = (4 * q).to(BF)                                       # scores of deviation 4: few keys carry a row
+    st = lambda n, B: torch.tensor([[0, n]] * B, dtype=torch.int32, device=gpu)
+
+    def dq(B):
+        y = [t.expand(B, -1, -1, -1) for t in (q, k, v, do)]
+        out, lse, rest = cross_attn_fwd_hip(*y[:3], st(Sq, B), st(Sk, B))
+        # its forward's own parts differ too: state of the rows by themselves for both
+        return (out, lse, rest), lambda s: cross_attn_bwd_hip(y[3], *y[:3], *s, st(Sq, B), st(Sk, B), grad_dtype=torch.float32,
+                                                              need=(True, False, False))[0]
+    size = lambda B: _lib.lib().icsa_cross_attn_bwd_workspace_size(B, Sq, Sk, 2, 2, D, 1)
+    assert size(1) > 4 * Sq * 2 * D * 2 and size(many) < 4 * many * Sq * 2 * D      # parts, none
+    state, one = dq(1)
+    _, all_of_them = dq(many)
+    a = one(state)[0].double()
+    b = all_of_them([t.expand(many, *t.shape[1:]).contiguous() for t in state])[-1].double()
+    p = torch.softmax(D ** -0.5 * torch.einsum("qhd,khd->hqk", q[0].float(), k[0].float()), -1)
+    dP = torch.einsum("qhd,khd->hqk", do[0].float(), v[0].float())
+    dS = p * (dP.abs() + (p * dP).sum(-1, keepdim=True).abs())
+    terms = D ** -0.5 * torch.einsum("hqk,khd->qhd", dS, k[0].float().abs())
+    assert ((a - b).abs() <= 1.1 * (Sk + 64) * 2.0 ** -24 * terms.double()).all(), ((a - b).norm() / b.norm()).item()
+
+
 # ------------------------------------------------------------------------------------------
 # the host
 # ------------------------------------------------------------------------------------------
