@@ -254,3 +254,43 @@ def test_checkpointed(gpu):
             leaf.grad = None
             checkpoint(f, leaf, use_reentrant=reentrant).backward(dy)
             assert torch.equal(leaf.grad, want)
+
+
+# ------------------------------------------------------------------------------------------
+# the cross attention's sublayer
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("lens", [None, [50, 7]])
+def test_the_key_bias_has_its_gradient(gpu, lens):
+    """A bias of the keys shifts all scores of a row alike but for the norm behind it; over text tokens of different sizes its gradient is
+    several times the tokens' terms.  These are of at most 16 roundings to bf16, 2^-8 of a tensor's 2-norm each (norm, q and k, their norms,
+    P, out, o's input and result, and back), and a sum of n rows is off by sqrt(n) times their error's 2-norm at most.  The gradient
+    is over twice that bound, so that a missing one, off by all of it, fails."""
+    torch.manual_seed(0)
+    dim, H, B, S, T = 256, 2, 2, 70, 60
+    att = wan.WanT2VCrossAttention(dim, H, trainable=True).to(gpu, BF)
+    with torch.no_grad():
+        for n in (att.norm_q, att.norm_k):
+            n.weight.copy_(0.5 + 0.1 * torch.randn(dim))
+    x = torch.randn(B, S, dim, device=gpu).to(BF)
+    text = (torch.randn(B, T, dim, device=gpu) * torch.exp(torch.randn(B, T, 1, device=gpu))).to(BF)
+    dy = torch.randn(B, S, dim, device=gpu).to(BF)
+    got, = torch.autograd.grad(att(x, text, lens), att.k.bias, dy)
+
+    P = {n: p.detach().double() for n, p in att.named_parameters() if "alpha" not in n}
+    lin = lambda v, n: v @ P[n + ".weight"].t() + P[n + ".bias"]
+    rms = lambda v, g: v * torch.rsqrt(v.square().mean(-1, keepdim=True) + att.eps) * g
+    C = text.double()
+    yk = lin(C, "k").requires_grad_()
+    q, k = rms(lin(x.double(), "q"), P["norm_q.weight"]), rms(yk, P["norm_k.weight"])
+    q, k, v = (t.unflatten(2, (H, dim // H)).transpose(1, 2).contiguous() for t in (q, k, lin(C, "v")))
+    s = torch.matmul(q, k.transpose(2, 3).contiguous()) * (dim // H) ** -0.5
+    if lens is not None:
+        see = torch.arange(T, device=gpu)[None] < torch.tensor(lens, device=gpu)[:, None]
+        s = s.masked_fill(~see[:, None, None], float("-inf"))
+    y = lin(torch.matmul(torch.softmax(s, -1), v).transpose(1, 2).flatten(2), "o")
+    terms, = torch.autograd.grad(y, yk, dy.double())
+    want = terms.sum((0, 1))
+    n = B * T if lens is None else sum(lens)                # padding has no terms
+    bound = 16 * 2.0 ** -8 * n ** 0.5 * terms.norm()
+    assert want.norm() > 2 * bound
+    assert (got.double() - want).norm() <= bound, ((got.double() - want).norm() / bound).item()
