@@ -23,7 +23,8 @@
 // products; 354 without the rows' totals) and 455 (dk and dv, 1.21 of four); the same without exponentials 342, without operand reads 299, with neither 274, without
 // the tiles' loads 327 (dq).  Short walks add a workgroup's start and end: over 512 keys (eight tiles) dq of 65,520 queries of 40 heads
 // takes 1.25 ms (0.82), 0.60 of it for the rows' bytes alone, which the other workgroup of the CU does not hide whole; dk and dv 1.24
-// (1.10; the matrix pipe busy 64 % at 1.6 GHz, in dq 44 % at 1.9).  Tried: 64 held rows a wave, whose operands serve two products (one
+// (1.10; the matrix pipe busy 64 % at 1.6 GHz, in dq 43 % at 1.9).  Heads of 64 halve the products of a pair and none of its elementwise work:
+// 2 x 9,373 queries of 24 heads on 8, padded prompts, dq 155 us with vector instructions active 73 % of the time, at heads of 128 49 %.  Tried: 64 held rows a wave, whose operands serve two products (one
 // wave a SIMD, accumulators moved between register files: dq 8,192 x 8,192 402, dk and dv spill); elementwise work between the
 // products of key-major 128 dims (registers); the first tile
 // requested before the held rows, starts staggered, the next workgroup's lines requested ahead: no change, or slower.
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(256) icsa_attn_bwd_join_kernel(AttnBwdParams p
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] /= total;
   }
-  const int bh = (int)((unsigned)row / (unsigned)n_st), r = (int)row - bh * n_st;         // rows: under 2^28, check_masked_sizes
+  const int bh = (int)((unsigned)row / (unsigned)n_st), r = (int)row - bh * n_st;   // query rows: under 2^28 (check_masked_sizes); key rows: 2^32 of dk are 512 GiB
   const int64_t off = row_at(out.sb, out.ss, out.sh, p.by_hk.div(bh), p.by_hk.mod(bh), KV ? FastDiv{1u, 0u, 1u, 0u} : p.by_g, r) + d;
   if (out.dtype == ICSA_DT_BF16) {
     bf16x4 y;

@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(RO_THREADS) icsa_rotary_kernel(RotaryParams p)
   }
 }
 
-// Any sizes, strides and alignment: a lane takes a pair, or a dim past R, at a time.
+// Any sizes, strides and alignment: a lane takes a pair, or a dim past R, at a time, in elements: 65,520 tokens, 12 + 12 heads of 80 with 20 dims
+// turned 365 us, 40 in halves 323 (105 by their bytes; the kernel above, 40 interleaved, 92).
 template <typename T>
 __global__ void __launch_bounds__(RO_THREADS) icsa_rotary_any_kernel(RotaryParams p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;

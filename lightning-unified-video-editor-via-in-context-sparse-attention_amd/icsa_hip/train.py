@@ -8,7 +8,8 @@
 
 Each is an autograd node over a pair of library calls (csrc/autograd.cpp); without an enabled grad mode, or inputs
 that require gradients, the forward alone runs and keeps nothing.  Gradients are sums in a fixed order: the same
-inputs give the same bits.  There is no second derivative.  :func:`cross_attn_fwd_hip` and
+inputs give the same bits.  There is no second derivative and none of forward mode; inputs are tensors with memory of their
+own (vmap, ``torch.func``, batched gradients and tracing are refused).  :func:`cross_attn_fwd_hip` and
 :func:`cross_attn_bwd_hip` are the attention's pair by itself, for callers with their own graph.
 """
 from __future__ import annotations
